@@ -33,6 +33,7 @@ extern "C" {
 
 #define LKV_DTYPE_F32 0
 #define LKV_DTYPE_F16 1
+#define LKV_DTYPE_BF16 2 /* the lkv_kv8_* entry points only */
 
 /* Library version (major*10000 + minor*100 + patch) and last error text. */
 int lkv_version(void);
@@ -650,6 +651,89 @@ int lkv_decode_layer_step_f16kv(const lkv_decode_dims* dims, const lkv_decode_la
 int lkv_decode_head(const lkv_decode_dims* dims, const void* final_norm, const void* lm_head, const void* x,
                     void* logits, int64_t* tok, int64_t* pos, int64_t* tok_history, int64_t history_len,
                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* 8-bit block-scaled KV cache (no reference counterpart)                    */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * One layer's keys and values of `batch` sequences, `kv_heads` heads of 128
+ * dims, `blocks` blocks of 64 tokens each.  Every finished block of a head is
+ * held in 8 bits with one scale for its keys and one for its values:
+ *   scale = amax / 127, code = rint(x * (127 / amax)), value = code * scale
+ * (fp32, amax over the block's 64 x 128 fp16 numbers; a zero block has scale
+ * 0); the unfinished last block of a sequence is fp16.  What is stored is
+ * finite: inputs are rounded to fp16, numbers beyond +-65504 and infinities
+ * become +-65504, a NaN becomes 0.  All buffers are 16-byte aligned device
+ * memory of the caller, cleared once before the first use.  A code is stored
+ * as the byte code + 128; values lie by dim, at position 16 g + 8 k + 4 t + i
+ * of a dim's 64 bytes (or fp16 numbers) token 32 k + 16 t + 4 g + i.
+ * A sequence's length lives with the caller, in int32 device memory.
+ */
+typedef struct lkv_kv8_store {
+  void* k_codes; /* uint8 [batch][kv_heads][blocks][64][128]              */
+  void* v_codes; /* uint8 [batch][kv_heads][blocks][128][64]              */
+  void* scales;  /* fp32  [batch][kv_heads][blocks][2]: key, value        */
+  void* ranges;  /* int8  [batch][kv_heads][blocks][2][128]: lowest and
+                    highest key code of each dim                          */
+  void* k_tail;  /* fp16  [batch][kv_heads][64][128]                      */
+  void* v_tail;  /* fp16  [batch][kv_heads][128][64]                      */
+  int64_t batch, kv_heads, blocks;
+} lkv_kv8_store;
+
+/*
+ * Stores S new tokens of every sequence: k and v are [batch][kv_heads][S][128]
+ * of `dtype` (LKV_DTYPE_*), each with its three strides in elements (rows
+ * dense and 16-byte aligned).  Sequence b's tokens go to positions pos[b] ..;
+ * pos[b] must be what it holds.  n_new (optional) gives how many of the S
+ * tokens are the sequence's (a padded batch: the rest is not read).  Tokens
+ * past the store are dropped, a position outside it stores nothing.
+ */
+int lkv_kv8_update(const lkv_kv8_store* store, const void* k, const int64_t* k_strides, const void* v,
+                   const int64_t* v_strides, int dtype, int64_t S, const int32_t* pos, const int32_t* n_new,
+                   void* stream);
+
+/* k, v = fp16 [batch][kv_heads][n][128]: tokens first .. first + n - 1 of every
+ * sequence as attention sees them, zeros past its length lens[b]. */
+int lkv_kv8_read(const lkv_kv8_store* store, const int32_t* lens, int64_t first, int64_t n, void* k, void* v,
+                 void* stream);
+
+/*
+ * Softmax attention of the S newest tokens' queries q [batch][Hq][S][128] over
+ * the store (Hq a multiple of kv_heads; query head h reads kv head h /
+ * (Hq / kv_heads)): out = softmax(scale * q K^T) V in the type of q.  Query i
+ * of sequence b, which has q_lens[b] of them (null: S; at most lens[b]), sees tokens
+ * 0 .. lens[b] - q_lens[b] + i; rows from q_lens[b] on, and rows that see no
+ * token, are zeros.  max_len is the caller's bound on lens (the work is split
+ * for it); what a longer sequence holds past it is not read.
+ * index (optional, S = 1): int32 [batch][kv_heads][n_index], the finished
+ * blocks that a kv head's queries read (entries outside the finished blocks
+ * are skipped) next to the unfinished block, which they always read.
+ * Scores and sums are fp32 of fp16 queries and whole-number codes; the weights
+ * are rounded to fp16 for the value product.
+ */
+size_t lkv_kv8_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t S, int64_t max_len, int64_t n_index);
+int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int64_t* q_strides, int dtype, int64_t Hq, int64_t S,
+                 const int32_t* lens, const int32_t* q_lens, int64_t max_len, const int32_t* index, int64_t n_index,
+                 float scale, void* out, const int64_t* out_strides, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/*
+ * index [batch][kv_heads][n]: for the newest token's queries q [batch][Hq][128]
+ * (strides of batch and head; a third is not used) the n finished blocks with the highest
+ * score, ascending, -1 where there are fewer.  The first `sink` and the last
+ * `recent` finished blocks are always among them; of equal scores the lower
+ * index wins.  The score of a block is
+ *   max over the kv head's queries of (float(dot) * qscale), times kscale,
+ *   dot = sum_d max(q8_d lo_d, q8_d hi_d)
+ * with q8 = rint(q * (127 / amax|q|)), qscale = amax|q| / 127 of the fp16
+ * query and lo, hi the lowest and highest key codes: an upper bound (up to the
+ * query's rounding) of every product of the block, in two fp32 roundings.
+ */
+size_t lkv_kv8_select_workspace_bytes(int64_t B, int64_t Hkv, int64_t max_len);
+int lkv_kv8_select_blocks(const lkv_kv8_store* store, const void* q, const int64_t* q_strides, int dtype, int64_t Hq,
+                          const int32_t* lens, int64_t max_len, int64_t n, int64_t sink, int64_t recent,
+                          int32_t* index, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

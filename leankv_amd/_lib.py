@@ -21,6 +21,7 @@ from .build import LIB_PATH
 LKV_OK = 0
 LKV_DTYPE_F32 = 0
 LKV_DTYPE_F16 = 1
+LKV_DTYPE_BF16 = 2  # lkv_kv8_* only
 
 _c_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -88,6 +89,14 @@ SIGNATURES = {
     "lkv_decode_evict": (_int, [_c_p, _c_p, ctypes.c_int64, _c_p, _sz, _c_p]),
     "lkv_decode_layer_step": (_int, [_c_p, _c_p, _c_p, _c_p, _sz, _c_p]),
     "lkv_decode_layer_step_f16kv": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _sz, _c_p]),
+    "lkv_kv8_update": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _int, _i64, _c_p, _c_p, _c_p]),
+    "lkv_kv8_read": (_int, [_c_p, _c_p, _i64, _i64, _c_p, _c_p, _c_p]),
+    "lkv_kv8_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "lkv_kv8_attn": (_int, [_c_p, _c_p, _c_p, _int, _i64, _i64, _c_p, _c_p, _i64, _c_p, _i64, _f32, _c_p, _c_p, _c_p,
+                            _sz, _c_p]),
+    "lkv_kv8_select_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "lkv_kv8_select_blocks": (_int, [_c_p, _c_p, _c_p, _int, _i64, _c_p, _i64, _i64, _i64, _i64, _c_p, _c_p, _sz,
+                                     _c_p]),
     "lkv_decode_head": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p, _sz, _c_p]),
 }
 
@@ -122,6 +131,14 @@ class DecodeLayout(ctypes.Structure):
         ("chunks_qkv", ctypes.c_int32), ("chunks_o", ctypes.c_int32), ("chunks_gateup", ctypes.c_int32),
         ("chunks_down", ctypes.c_int32), ("chunks_lm", ctypes.c_int32),
     ]
+
+
+
+class KV8StoreStruct(ctypes.Structure):
+    """lkv_kv8_store (include/leankv_amd.h)."""
+
+    _fields_ = [("k_codes", _c_p), ("v_codes", _c_p), ("scales", _c_p), ("ranges", _c_p), ("k_tail", _c_p),
+                ("v_tail", _c_p), ("batch", _i64), ("kv_heads", _i64), ("blocks", _i64)]
 
 
 _lib = None

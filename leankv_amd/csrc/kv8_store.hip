@@ -1,0 +1,393 @@
+// 8-bit block-scaled KV cache: storing tokens and reading them back (layout in kv8_common.h).
+//
+// lkv_kv8_update, one launch, one workgroup of 256 threads for each (key or value, sequence, kv head, touched block).
+// A block that the new tokens finish is quantized from the unfinished block's fp16 tokens and the new ones: its 64 x 128
+// values lie in registers (a thread has 8 dims of 4 consecutive tokens, read in 16-byte rows), one max over the
+// workgroup gives the scale, and the codes go out in 8-byte pieces (keys) or through LDS as [dim][position] rows
+// (values: the 4 tokens of a thread's dim are one dword of the row, so the transpose is dword moves).  Tokens that
+// finish no block go to the fp16 tail.  The workgroup of the first touched block also writes the new tail, after its
+// own reads of the old one, so no other workgroup touches the tail.
+// Bound by memory: a value is read once (2 bytes) and written once (1 byte).
+#include "kv8_common.h"
+
+namespace lkv {
+namespace kv8 {
+namespace {
+
+constexpr int kThr = 256;
+constexpr int kVRow = 17;  // dwords of a staged value row: 16 and one of padding
+
+__device__ __forceinline__ uint32_t xg_min(uint32_t v) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  auto mn = [](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+  };
+  auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = mn(a[0], a[1]);
+  a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return mn(a[0], a[1]);
+}
+
+struct UpdateArgs {
+  Store st;
+  const void* x[2];           // keys, values
+  int64_t sb[2], sh[2], ss[2];  // strides in elements
+  const int* pos;             // [B] tokens held before
+  const int* n_new;           // [B] or null
+  int S;
+};
+
+// thread: dims 8 c .. 8 c + 7 of tokens 4 a .. 4 a + 3 of the block
+template <int DT>
+__global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
+  __shared__ float s_max[4];
+  __shared__ uint32_t s_rng[4][2][64];
+  __shared__ uint32_t s_v[kD * kVRow];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c = tid & 15, a = tid >> 4;
+  const int which = blockIdx.y & 1;  // 0 keys, 1 values
+  const int h = blockIdx.y >> 1, b = blockIdx.z;
+  const Store& st = P.st;
+  // the sequence's tokens [p0, p1); a position outside the store stores nothing, tokens past it are dropped
+  const int64_t cap = static_cast<int64_t>(st.blocks) * kBlk;
+  const int64_t p0 = P.pos[b];
+  if (p0 < 0 || p0 >= cap) return;
+  int64_t n = P.n_new ? P.n_new[b] : P.S;
+  n = min(n, static_cast<int64_t>(P.S));
+  if (n <= 0) return;
+  const int64_t p1 = min(p0 + n, cap);
+  const int64_t blk = p0 / kBlk + blockIdx.x;
+  const int64_t t0 = blk * kBlk;  // first token of this block
+  if (t0 >= p1) return;
+  const bool first = blockIdx.x == 0;
+  const bool done = t0 + kBlk <= p1;
+  if (!done && !first) return;  // the unfinished block is the first workgroup's
+
+  const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
+  const void* x = P.x[which];
+  const int64_t xrow = b * P.sb[which] + h * P.sh[which];
+  uint16_t* tail = (which ? st.v_tail : st.k_tail) + bh * kBlkBytes;
+
+  if (done) {
+    float v[4][8];
+    // tokens from the old tail: those before p0 (none but in the first block)
+    const int old = first ? static_cast<int>(p0 - t0) : 0;
+    uint2 vt[8];
+    if (which && 4 * a < old) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vt[j] = *reinterpret_cast<const uint2*>(tail + (8 * c + j) * kBlk + 4 * v_dword(a));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * a + i;
+      if (t >= old) {
+        load8<DT>(x, xrow + (t0 + t - p0) * P.ss[which] + 8 * c, v[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = h2f(f2h(clamp_kv(v[i][j])));
+      } else if (!which) {
+        load8<LKV_DTYPE_F16>(tail, t * kD + 8 * c, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w = i < 2 ? vt[j].x : vt[j].y;
+          v[i][j] = h2f(static_cast<uint16_t>((i & 1) ? w >> 16 : w & 0xffffu));
+        }
+      }
+    }
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[i][j]));
+    m = wave_max(m);
+    if (lane == 0) s_max[wave] = m;
+    __syncthreads();
+    const float amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const float inv = amax > 0.f ? 127.f / amax : 0.f;
+    // codes, rounded to nearest even; |x * inv| <= 127 (1 + 2^-23) rounds to 127 at most
+    int code[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) code[i][j] = static_cast<int>(rintf(v[i][j] * inv));
+    const int64_t at = bh * st.blocks + blk;
+    if (tid == 0) st.scales[2 * at + which] = amax / 127.f;
+    if (!which) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          w[k] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[k] |= static_cast<uint32_t>(code[i][4 * k + j] + 128) << (8 * j);
+        }
+        *reinterpret_cast<uint2*>(st.k_codes + at * kBlkBytes + (4 * a + i) * kD + 8 * c) = uint2{w[0], w[1]};
+      }
+      // lowest and highest code of every dim: over the thread's 4 tokens, the wave's 16, the block's 64 (the highest as
+      // the negated lowest of the negated codes)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        auto lowest = [&](int sign) {
+          int l[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            l[k] = sign * code[0][2 * j + k];
+#pragma unroll
+            for (int i = 1; i < 4; ++i) l[k] = min(l[k], sign * code[i][2 * j + k]);
+          }
+          return xg_min((static_cast<uint32_t>(l[0]) & 0xffffu) | (static_cast<uint32_t>(l[1]) << 16));
+        };
+        const uint32_t lo = lowest(1), hi = lowest(-1);
+        if (lane < 16) {
+          s_rng[wave][0][4 * c + j] = lo;
+          s_rng[wave][1][4 * c + j] = hi;
+        }
+      }
+      __syncthreads();
+      // dims 2 d2, 2 d2 + 1
+      if (tid < 128) {
+        const int d2 = tid & 63, hi = tid >> 6;
+        int r0 = 127, r1 = 127;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t u = s_rng[w][hi][d2];
+          r0 = min(r0, static_cast<int>(static_cast<int16_t>(u & 0xffffu)));
+          r1 = min(r1, static_cast<int>(static_cast<int16_t>(u >> 16)));
+        }
+        if (hi) r0 = -r0, r1 = -r1;
+        reinterpret_cast<uint16_t*>(st.ranges + at * 2 * kD + hi * kD)[d2] =
+            static_cast<uint16_t>((r0 & 0xff) | ((r1 & 0xff) << 8));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= static_cast<uint32_t>(code[i][j] + 128) << (8 * i);
+        s_v[(8 * c + j) * kVRow + v_dword(a)] = w;
+      }
+      __syncthreads();
+      // two 16-byte pieces a thread
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int piece = k * kThr + tid, d = piece >> 2, q = 4 * (piece & 3);
+        const uint32_t* s = s_v + d * kVRow + q;
+        *reinterpret_cast<u32x4*>(st.v_codes + at * kBlkBytes + d * kBlk + 4 * q) = u32x4{s[0], s[1], s[2], s[3]};
+      }
+    }
+  }
+  if (!first) return;
+  // the new tail: the tokens of the unfinished last block, in its slots
+  __syncthreads();  // (every read of the old tail is done)
+  const int64_t tt = p1 / kBlk * kBlk;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int slot = 4 * a + i;
+    const int64_t t = tt + slot;
+    if (t < p0 || t >= p1) continue;
+    float y[8];
+    load8<DT>(x, xrow + (t - p0) * P.ss[which] + 8 * c, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = clamp_kv(y[j]);
+    if (!which) {
+      *reinterpret_cast<u32x4*>(tail + slot * kD + 8 * c) =
+          u32x4{pk2(y[0], y[1]), pk2(y[2], y[3]), pk2(y[4], y[5]), pk2(y[6], y[7])};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) tail[(8 * c + j) * kBlk + v_pos(slot)] = f2h(y[j]);
+    }
+  }
+}
+
+struct ReadArgs {
+  Store st;
+  const int* lens;
+  uint16_t* out[2];  // keys, values: fp16 [B][Hkv][n][128]
+  int64_t first, n;  // tokens first .. first + n - 1
+};
+
+// One workgroup per (key or value, sequence, kv head, block of 64 tokens): codes in 16-byte pieces, values through LDS
+// back to rows, fp16 rows out in 16-byte pieces.  Bound by memory.
+__global__ __launch_bounds__(kThr) void read_kernel(ReadArgs P) {
+  __shared__ uint32_t s_v[kD * kVRow];
+  const int tid = threadIdx.x;
+  const int c = tid & 15, a = tid >> 4;
+  const int which = blockIdx.y & 1, h = blockIdx.y >> 1, b = blockIdx.z;
+  const Store& st = P.st;
+  const int64_t cap = static_cast<int64_t>(st.blocks) * kBlk;
+  const int64_t len = min(max(static_cast<int64_t>(P.lens[b]), static_cast<int64_t>(0)), cap);
+  const int64_t blk = P.first / kBlk + blockIdx.x, t0 = blk * kBlk;
+  const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
+  const bool done = t0 + kBlk <= len;
+  const int64_t at = bh * st.blocks + blk;
+  uint32_t w[4][4];  // token 4 a + i, dims 8 c .. as fp16 pairs
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[i][j] = 0;
+  if (done) {
+    const float scale = st.scales[2 * at + which];
+    auto val = [&](uint32_t byte) { return static_cast<float>(static_cast<int>(byte) - 128) * scale; };
+    if (!which) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint2 u = *reinterpret_cast<const uint2*>(st.k_codes + at * kBlkBytes + (4 * a + i) * kD + 8 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x = (j < 2 ? u.x : u.y) >> (16 * (j & 1));
+          w[i][j] = pk2(val(x & 0xffu), val((x >> 8) & 0xffu));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int piece = k * kThr + tid, d = piece >> 2, q = 4 * (piece & 3);
+        const u32x4 u = *reinterpret_cast<const u32x4*>(st.v_codes + at * kBlkBytes + d * kBlk + 4 * q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_v[d * kVRow + q + j] = u[j];
+      }
+      __syncthreads();
+      uint32_t u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = s_v[(8 * c + j) * kVRow + v_dword(a)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[i][j] = pk2(val((u[2 * j] >> (8 * i)) & 0xffu), val((u[2 * j + 1] >> (8 * i)) & 0xffu));
+    }
+  } else if (t0 < len) {
+    const uint16_t* tail = (which ? st.v_tail : st.k_tail) + bh * kBlkBytes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * a + i;
+      if (t0 + t >= len) continue;
+      if (!which) {
+        const u32x4 u = *reinterpret_cast<const u32x4*>(tail + t * kD + 8 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[i][j] = u[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[i][j] = static_cast<uint32_t>(tail[(8 * c + 2 * j) * kBlk + v_pos(t)]) |
+                    (static_cast<uint32_t>(tail[(8 * c + 2 * j + 1) * kBlk + v_pos(t)]) << 16);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t t = t0 + 4 * a + i - P.first;
+    if (t < 0 || t >= P.n) continue;
+    *reinterpret_cast<u32x4*>(P.out[which] + (bh * P.n + t) * kD + 8 * c) = u32x4{w[i][0], w[i][1], w[i][2], w[i][3]};
+  }
+}
+
+}  // namespace
+}  // namespace kv8
+}  // namespace lkv
+
+using namespace lkv;
+using namespace lkv::kv8;
+
+namespace lkv {
+namespace kv8 {
+
+int check_store(const lkv_kv8_store* s, const char* what) {
+  LKV_REQUIRE(s, "%s: null store", what);
+  LKV_REQUIRE(s->batch >= 0 && s->batch < 65536 && s->kv_heads > 0 && s->kv_heads < 32768 && s->blocks > 0 &&
+                  s->blocks < (1ll << 24),
+              "%s: store of %lld sequences, %lld kv heads, %lld blocks out of range", what, (long long)s->batch,
+              (long long)s->kv_heads, (long long)s->blocks);
+  LKV_REQUIRE(s->batch == 0 || (s->k_codes && s->v_codes && s->scales && s->ranges && s->k_tail && s->v_tail),
+              "%s: null pointer in the store", what);
+  LKV_REQUIRE(aligned16(s->k_codes) && aligned16(s->v_codes) && aligned16(s->scales) && aligned16(s->ranges) &&
+                  aligned16(s->k_tail) && aligned16(s->v_tail),
+              "%s: the store's buffers must be 16-byte aligned", what);
+  return LKV_OK;
+}
+
+Store device_store(const lkv_kv8_store* s) {
+  Store d;
+  d.k_codes = static_cast<uint8_t*>(s->k_codes);
+  d.v_codes = static_cast<uint8_t*>(s->v_codes);
+  d.scales = static_cast<float*>(s->scales);
+  d.ranges = static_cast<int8_t*>(s->ranges);
+  d.k_tail = static_cast<uint16_t*>(s->k_tail);
+  d.v_tail = static_cast<uint16_t*>(s->v_tail);
+  d.Hkv = static_cast<int>(s->kv_heads);
+  d.blocks = static_cast<int>(s->blocks);
+  return d;
+}
+
+int check_rows(const void* x, const int64_t* strides, int dtype, const char* what, const char* name) {
+  const int64_t unit = dtype == LKV_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+  LKV_REQUIRE(aligned16(x) && strides && strides[0] % unit == 0 && strides[1] % unit == 0 && strides[2] % unit == 0,
+              "%s: rows of %s must be 16-byte aligned", what, name);
+  return LKV_OK;
+}
+
+}  // namespace kv8
+}  // namespace lkv
+
+extern "C" int lkv_kv8_update(const lkv_kv8_store* store, const void* k, const int64_t* k_strides, const void* v,
+                              const int64_t* v_strides, int dtype, int64_t S, const int32_t* pos, const int32_t* n_new,
+                              void* stream) {
+  if (int rc = check_store(store, "kv8_update")) return rc;
+  LKV_REQUIRE(dtype == LKV_DTYPE_F32 || dtype == LKV_DTYPE_F16 || dtype == LKV_DTYPE_BF16, "kv8_update: dtype %d", dtype);
+  LKV_REQUIRE(S >= 0 && S < (1ll << 30), "kv8_update: S=%lld out of range", (long long)S);
+  if (store->batch == 0 || S == 0) return LKV_OK;
+  LKV_REQUIRE(k && v && pos, "kv8_update: null pointer");
+  if (int rc = check_rows(k, k_strides, dtype, "kv8_update", "k")) return rc;
+  if (int rc = check_rows(v, v_strides, dtype, "kv8_update", "v")) return rc;
+  UpdateArgs P;
+  P.st = device_store(store);
+  P.x[0] = k;
+  P.x[1] = v;
+  for (int w = 0; w < 2; ++w) {
+    const int64_t* s = w ? v_strides : k_strides;
+    P.sb[w] = s[0];
+    P.sh[w] = s[1];
+    P.ss[w] = s[2];
+  }
+  P.pos = pos;
+  P.n_new = n_new;
+  P.S = static_cast<int>(S);
+  // blocks that S tokens from any position touch
+  const dim3 grid(static_cast<unsigned>((S + kBlk - 2) / kBlk + 1), static_cast<unsigned>(2 * store->kv_heads),
+                  static_cast<unsigned>(store->batch));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == LKV_DTYPE_F32)
+    hipLaunchKernelGGL(update_kernel<LKV_DTYPE_F32>, grid, dim3(kThr), 0, st, P);
+  else if (dtype == LKV_DTYPE_F16)
+    hipLaunchKernelGGL(update_kernel<LKV_DTYPE_F16>, grid, dim3(kThr), 0, st, P);
+  else
+    hipLaunchKernelGGL(update_kernel<LKV_DTYPE_BF16>, grid, dim3(kThr), 0, st, P);
+  LKV_LAUNCH_CHECK("kv8_update");
+  return LKV_OK;
+}
+
+extern "C" int lkv_kv8_read(const lkv_kv8_store* store, const int32_t* lens, int64_t first, int64_t n, void* k, void* v,
+                            void* stream) {
+  if (int rc = check_store(store, "kv8_read")) return rc;
+  const int64_t cap = store->blocks * kBlk;
+  LKV_REQUIRE(first >= 0 && first <= cap && n >= 0 && n <= cap - first,
+              "kv8_read: %lld tokens from %lld on outside a store of %lld", (long long)n, (long long)first,
+              (long long)cap);
+  if (store->batch == 0 || n == 0) return LKV_OK;
+  LKV_REQUIRE(lens && k && v, "kv8_read: null pointer");
+  LKV_REQUIRE(aligned16(k) && aligned16(v), "kv8_read: outputs must be 16-byte aligned");
+  ReadArgs P;
+  P.st = device_store(store);
+  P.lens = lens;
+  P.out[0] = static_cast<uint16_t*>(k);
+  P.out[1] = static_cast<uint16_t*>(v);
+  P.first = first;
+  P.n = n;
+  const int64_t nb = (first + n - 1) / kBlk - first / kBlk + 1;
+  hipLaunchKernelGGL(read_kernel, dim3(static_cast<unsigned>(nb), static_cast<unsigned>(2 * store->kv_heads),
+                                       static_cast<unsigned>(store->batch)),
+                     dim3(kThr), 0, static_cast<hipStream_t>(stream), P);
+  LKV_LAUNCH_CHECK("kv8_read");
+  return LKV_OK;
+}

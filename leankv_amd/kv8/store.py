@@ -1,0 +1,254 @@
+"""One layer's keys and values in 8 bits, and the attention that reads them (lkv_kv8_* in include/leankv_amd.h).
+
+Every finished block of 64 tokens of a kv head is held as one byte a number with one fp32 scale for its keys and one
+for its values (amax / 127; no rotation, no codebook); the unfinished last block of a sequence is fp16.  A stored token
+costs 256 bytes a kv head instead of 512, and a number is off by at most half a code, amax / 254.  For each finished
+block the store also keeps the lowest and the highest key code of every dim, from which the sparse decode attention
+finds the blocks worth reading.
+
+The store does not know its sequences' lengths: they live with the caller, as int32 device tensors that every call
+takes, so that a decode step can be captured into a HIP graph and replayed with other lengths.  Nothing here
+synchronises, and every workspace is allocated for its call on the current stream.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from .. import _lib
+from .._lib import LeanKVError, check
+
+HEAD_DIM = 128
+BLOCK = 64
+_DTYPES = {torch.float32: _lib.LKV_DTYPE_F32, torch.float16: _lib.LKV_DTYPE_F16, torch.bfloat16: _lib.LKV_DTYPE_BF16}
+_I64x3 = ctypes.c_int64 * 3
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
+
+
+def _dtype(t: torch.Tensor, what: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise LeanKVError("%s: float16, bfloat16 or float32 expected, got %s" % (what, t.dtype))
+    return code
+
+
+def _rows(t: torch.Tensor):
+    """(t, its strides of batch, head and token in elements): t itself where its rows of 128 are dense and 16-byte
+    aligned, else a copy.  t is [B, H, S, 128]; strides of single sizes are 0 (torch leaves them free)."""
+    b, h, s = t.stride()[:3]
+    n = t.shape
+    strides = (b if n[0] > 1 else 0, h if n[1] > 1 else 0, s if n[2] > 1 else 0)
+    unit = 16 // t.element_size()
+    if t.stride(3) == 1 and not (strides[0] % unit or strides[1] % unit or strides[2] % unit) \
+            and t.data_ptr() % 16 == 0:
+        return t, _I64x3(*strides)
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, _I64x3(*t.stride()[:3])
+
+
+class KV8Store:
+    """Keys and values of `batch` sequences x `kv_heads` heads of 128 dims, up to `capacity` tokens each (rounded up to
+    whole blocks of 64), in 8 bits with a scale for each block and head.
+
+        store = KV8Store(batch, kv_heads, capacity, device="cuda")
+        store.update(k, v, pos)                        # S new tokens of every sequence, at positions pos[b] ..
+        out = store.prefill_attention(q, lens)         # their queries, causal over everything stored
+        out = store.decode_attention(q1, lens)         # one new token's queries
+        out, index = store.sparse_decode_attention(q1, lens, blocks=64)
+        k, v = store.read(lens, n)                     # the K / V that attention sees, fp16
+
+    pos, lens, n_new and q_lens are int32 device tensors [batch]; lens counts every stored token, the queries' own among
+    them, and may not pass the capacity.  Inputs are float16, bfloat16 or float32 of any strides; they are rounded to
+    float16 first (infinities and larger numbers to +-65504; a NaN key or value is stored as 0).  There is no gradient."""
+
+    def __init__(self, batch: int, kv_heads: int, capacity: int, device="cuda"):
+        if batch < 1 or kv_heads < 1 or capacity < 1:
+            raise ValueError("KV8Store: batch, kv_heads and capacity must be at least 1, got %d, %d, %d"
+                             % (batch, kv_heads, capacity))
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise LeanKVError("leankv_amd kernels run on the GPU only; got device %s" % self.device)
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.batch, self.kv_heads = int(batch), int(kv_heads)
+        self.blocks = -(-int(capacity) // BLOCK)
+        rows = (self.batch, self.kv_heads)
+
+        def zeros(*shape, dtype):
+            return torch.zeros(*rows, *shape, dtype=dtype, device=self.device)
+
+        self.k_codes = zeros(self.blocks, BLOCK, HEAD_DIM, dtype=torch.uint8)
+        self.v_codes = zeros(self.blocks, HEAD_DIM, BLOCK, dtype=torch.uint8)
+        self.scales = zeros(self.blocks, 2, dtype=torch.float32)
+        self.ranges = zeros(self.blocks, 2, HEAD_DIM, dtype=torch.int8)
+        self.k_tail = zeros(BLOCK, HEAD_DIM, dtype=torch.float16)
+        self.v_tail = zeros(HEAD_DIM, BLOCK, dtype=torch.float16)
+        self._struct = _lib.KV8StoreStruct(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.scales.data_ptr(),
+                                           self.ranges.data_ptr(), self.k_tail.data_ptr(), self.v_tail.data_ptr(),
+                                           self.batch, self.kv_heads, self.blocks)
+        self._ref = ctypes.byref(self._struct)
+        self._lib = _lib.load()
+
+    @property
+    def capacity(self) -> int:
+        return self.blocks * BLOCK
+
+    def nbytes(self) -> int:
+        """Device bytes of the store."""
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.scales, self.ranges,
+                                                          self.k_tail, self.v_tail))
+
+    # ------------------------------------------------------------------------------------------------ checks
+    def _call(self, name: str, *args):
+        """One C entry on the store's device and that device's current stream."""
+        idx = self.device.index
+        if torch.cuda.current_device() == idx:
+            rc = getattr(self._lib, name)(self._ref, *args, torch._C._cuda_getCurrentRawStream(idx))
+        else:
+            with torch.cuda.device(self.device):
+                rc = getattr(self._lib, name)(self._ref, *args, torch._C._cuda_getCurrentRawStream(idx))
+        if rc:
+            check(rc, name)
+
+    def _ints(self, t, what: str, name: str):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device \
+                or t.numel() != self.batch or not t.is_contiguous():
+            raise LeanKVError("%s: %s must be a contiguous int32 tensor of %d entries on %s"
+                              % (what, name, self.batch, self.device))
+        return t.data_ptr()
+
+    def _queries(self, q, dims: int, what: str):
+        if q.dim() != dims or q.shape[0] != self.batch or q.shape[-1] != HEAD_DIM or q.shape[1] % self.kv_heads \
+                or not q.shape[1] or q.device != self.device:
+            raise LeanKVError("%s: q must be [%d, heads, %s%d] on %s with a multiple of %d heads, got %s on %s"
+                              % (what, self.batch, "S, " if dims == 4 else "", HEAD_DIM, self.device, self.kv_heads,
+                                 tuple(q.shape), q.device))
+        return _dtype(q, what)
+
+    def _bound(self, max_len, what: str) -> int:
+        if max_len is None:
+            return self.blocks * BLOCK
+        if not 0 <= int(max_len) <= self.blocks * BLOCK:
+            raise LeanKVError("%s: max_len=%d outside a store of %d tokens" % (what, max_len, self.blocks * BLOCK))
+        return int(max_len)
+
+    def _workspace(self, nbytes: int):
+        """Allocated for its call on the current stream: calls on several streams and captured graphs share none."""
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+
+    # ------------------------------------------------------------------------------------------------ storing
+    def update(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, n_new: torch.Tensor | None = None) -> None:
+        """Store S new tokens of every sequence: k, v [batch, kv_heads, S, 128], sequence b's at positions pos[b] .. (what
+        it holds already).  n_new: how many of the S are sequence b's (a padded batch; the rest is not read).  Tokens
+        past the capacity are dropped.  One launch; blocks that become whole are quantized."""
+        what = "KV8Store.update"
+        for t, name in ((k, "k"), (v, "v")):
+            if t.dim() != 4 or t.shape[0] != self.batch or t.shape[1] != self.kv_heads or t.shape[3] != HEAD_DIM \
+                    or t.device != self.device:
+                raise LeanKVError("%s: %s must be [%d, %d, S, %d] on %s, got %s on %s"
+                                  % (what, name, self.batch, self.kv_heads, HEAD_DIM, self.device, tuple(t.shape),
+                                     t.device))
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise LeanKVError("%s: k and v must be alike, got %s %s and %s %s"
+                              % (what, k.dtype, tuple(k.shape), v.dtype, tuple(v.shape)))
+        dtype = _dtype(k, what)
+        p = self._ints(pos, what, "pos")
+        m = None if n_new is None else self._ints(n_new, what, "n_new")
+        (k, ks), (v, vs) = _rows(k.detach()), _rows(v.detach())
+        self._call("lkv_kv8_update", k.data_ptr(), ks, v.data_ptr(), vs, dtype, k.shape[2], p, m)
+
+    def read(self, lens: torch.Tensor, n: int, first: int = 0):
+        """(K, V) float16 [batch, kv_heads, n - first, 128]: tokens first .. n - 1 of every sequence as attention sees
+        them, zeros past its length."""
+        what = "KV8Store.read"
+        if not 0 <= first <= n <= self.blocks * BLOCK:
+            raise LeanKVError("%s: tokens %d .. %d outside a store of %d" % (what, first, n, self.blocks * BLOCK))
+        p = self._ints(lens, what, "lens")
+        k = torch.empty(self.batch, self.kv_heads, n - first, HEAD_DIM, dtype=torch.float16, device=self.device)
+        v = torch.empty_like(k)
+        self._call("lkv_kv8_read", p, first, n - first, k.data_ptr(), v.data_ptr())
+        return k, v
+
+    # ---------------------------------------------------------------------------------------------- attention
+    def _out(self, q: torch.Tensor, out: torch.Tensor | None, what: str):
+        """The output for q [B, Hq, S, 128] and its strides; a fresh one is laid out token by token (what the output
+        projection reads)."""
+        if out is None:
+            B, Hq, S, _ = q.shape
+            out = torch.empty(B, S, Hq, HEAD_DIM, dtype=q.dtype, device=q.device).transpose(1, 2)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            raise LeanKVError("%s: out must be like q, %s %s on %s" % (what, q.dtype, tuple(q.shape), q.device))
+        rows, strides = _rows(out)
+        if rows is not out:
+            raise LeanKVError("%s: rows of out must be dense and 16-byte aligned" % what)
+        return out, strides
+
+    def _attend(self, q, dtype, lens, q_lens, max_len, index, scale, out, what):
+        p = self._ints(lens, what, "lens")
+        m = None if q_lens is None else self._ints(q_lens, what, "q_lens")
+        L = self._bound(max_len, what)
+        out, os = self._out(q, out, what)
+        q, qs = _rows(q.detach())
+        Hq, S = q.shape[1], q.shape[2]
+        n = 0 if index is None else index.shape[2]
+        nbytes = self._lib.lkv_kv8_attn_workspace_bytes(self.batch, Hq, self.kv_heads, S, L, n)
+        ws = self._workspace(nbytes) if nbytes else None
+        self._call("lkv_kv8_attn", q.data_ptr(), qs, dtype, Hq, S, p, m, L, None if index is None else index.data_ptr(),
+                   n, _SCALE if scale is None else float(scale), out.data_ptr(), os,
+                   None if ws is None else ws.data_ptr(), nbytes)
+        return out
+
+    def decode_attention(self, q: torch.Tensor, lens: torch.Tensor, max_len: int | None = None,
+                         scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of one query per sequence and head, q [batch, heads, 128], over everything stored (its own token
+        among it): [batch, heads, 128] in q's type.  A sequence of length 0 gives zeros.  max_len: the caller's bound on
+        lens (default the capacity), which the work is split for.  scale: 1 / sqrt(128) by default."""
+        what = "KV8Store.decode_attention"
+        dtype = self._queries(q, 3, what)
+        o = self._attend(q.unsqueeze(2), dtype, lens, None, max_len, None, scale,
+                         None if out is None else out.unsqueeze(2), what)
+        return o.squeeze(2) if out is None else out
+
+    def prefill_attention(self, q: torch.Tensor, lens: torch.Tensor, q_lens: torch.Tensor | None = None,
+                          max_len: int | None = None, scale: float | None = None,
+                          out: torch.Tensor | None = None) -> torch.Tensor:
+        """Causal attention of the S newest tokens' queries q [batch, heads, S, 128] (after their update): query i of a
+        sequence with q_lens[b] of them (default S) sees tokens 0 .. lens[b] - q_lens[b] + i.  Rows from q_lens[b] on
+        are zeros.  Returns [batch, heads, S, 128] in q's type, laid out [batch, S, heads, 128]."""
+        what = "KV8Store.prefill_attention"
+        dtype = self._queries(q, 4, what)
+        return self._attend(q, dtype, lens, q_lens, max_len, None, scale, out, what)
+
+    # ------------------------------------------------------------------------------------------------- sparse
+    def select_blocks(self, q: torch.Tensor, lens: torch.Tensor, blocks: int, sink: int = 1, recent: int = 1,
+                      max_len: int | None = None) -> torch.Tensor:
+        """int32 [batch, kv_heads, blocks]: for one query per sequence, q [batch, heads, 128], the finished blocks with
+        the highest upper bound of q.k (over the kv head's queries), ascending, -1 where a sequence has fewer.  The first
+        `sink` and the last `recent` finished blocks are always among them; of equal scores the lower index wins."""
+        what = "KV8Store.select_blocks"
+        dtype = self._queries(q, 3, what)
+        p = self._ints(lens, what, "lens")
+        L = self._bound(max_len, what)
+        blocks, sink, recent = int(blocks), int(sink), int(recent)
+        if blocks < 1 or sink < 0 or recent < 0 or sink + recent > blocks:
+            raise LeanKVError("%s: %d blocks with the first %d and the last %d among them" % (what, blocks, sink, recent))
+        q, qs = _rows(q.detach().unsqueeze(2))
+        index = torch.empty(self.batch, self.kv_heads, blocks, dtype=torch.int32, device=self.device)
+        nbytes = self._lib.lkv_kv8_select_workspace_bytes(self.batch, self.kv_heads, L)
+        ws = self._workspace(nbytes)
+        self._call("lkv_kv8_select_blocks", q.data_ptr(), qs, dtype, q.shape[1], p, L, blocks, sink, recent,
+                   index.data_ptr(), ws.data_ptr(), nbytes)
+        return index
+
+    def sparse_decode_attention(self, q: torch.Tensor, lens: torch.Tensor, blocks: int, sink: int = 1, recent: int = 1,
+                                max_len: int | None = None, scale: float | None = None):
+        """decode_attention over the blocks that select_blocks chooses and the unfinished block: (out [batch, heads, 128],
+        index)."""
+        what = "KV8Store.sparse_decode_attention"
+        dtype = self._queries(q, 3, what)
+        index = self.select_blocks(q, lens, blocks, sink, recent, max_len)
+        out = self._attend(q.unsqueeze(2), dtype, lens, None, max_len, index, scale, None, what)
+        return out.squeeze(2), index
