@@ -660,9 +660,9 @@ int lkv_decode_head(const lkv_decode_dims* dims, const void* final_norm, const v
  * One layer's keys and values of `batch` sequences, `kv_heads` heads of 128
  * dims, `blocks` blocks of 64 tokens each.  Every finished block of a head is
  * held in 8 bits with one scale for its keys and one for its values:
- *   scale = amax / 127, code = rint(x * (127 / amax)), value = code * scale
- * (fp32, amax over the block's 64 x 128 fp16 numbers; a zero block has scale
- * 0); the unfinished last block of a sequence is fp16.  What is stored is
+ *   scale = amax * s, code = rint(x * (127 * (1 / amax))), value = code * scale
+ * (fp32, each operation rounded; s = fp32(1 / 127), amax over the block's
+ * 64 x 128 fp16 numbers; a zero block has scale 0 and codes 0); the unfinished last block of a sequence is fp16.  What is stored is
  * finite: inputs are rounded to fp16, numbers beyond +-65504 and infinities
  * become +-65504, a NaN becomes 0.  All buffers are 16-byte aligned device
  * memory of the caller, cleared once before the first use.  A code is stored
@@ -726,8 +726,7 @@ int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int64_t* q_str
  * index wins.  The score of a block is
  *   max over the kv head's queries of (float(dot) * qscale), times kscale,
  *   dot = sum_d max(q8_d lo_d, q8_d hi_d)
- * with q8 = rint(q * (127 / amax|q|)), qscale = amax|q| / 127 of the fp16
- * query and lo, hi the lowest and highest key codes: an upper bound (up to the
+ * with q8 and qscale the codes and scale of the fp16 query, as a block's and lo, hi the lowest and highest key codes: an upper bound (up to the
  * query's rounding) of every product of the block, in two fp32 roundings.
  */
 size_t lkv_kv8_select_workspace_bytes(int64_t B, int64_t Hkv, int64_t max_len);

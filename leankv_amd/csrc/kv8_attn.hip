@@ -398,7 +398,7 @@ __global__ __launch_bounds__(kThr) void score_kernel(SelectArgs P) {
         }
       }
       amax = groups_max(amax);
-      const float inv = amax > 0.f ? 127.f / amax : 0.f, qs = amax / 127.f;
+      const float inv = code_factor(amax), qs = amax * kStep;
       i32x4 neg[2], pos[2];
 #pragma unroll
       for (int w = 0; w < 8; ++w) {

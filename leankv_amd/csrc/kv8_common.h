@@ -1,8 +1,8 @@
 // Layout and device helpers of the 8-bit block-scaled KV cache (kv8_store.hip, kv8_attn.hip, kv8_prefill.hip).
 //
 // A finished block is 64 tokens of one kv head.  Its 64 x 128 keys share one scale, so do its values:
-//   scale = amax / 127, code = rint(x * (127 / amax)) in -127 .. 127, value = code * scale,
-// and a code is stored as the byte code + 128.  Keys lie [token][dim].  Values lie [dim][position], so that the value
+//   scale = amax / 127, code = rint(x * (127 / amax)) in -127 .. 127, value = code * scale
+// (in fp32 with the roundings of amax * fp32(1 / 127) and x * (127 * (1 / amax))), and a code is stored as the byte code + 128.  Keys lie [token][dim].  Values lie [dim][position], so that the value
 // product reads its operand (8 tokens of one dim per lane) as it lies in memory, with no transpose in the attention
 // kernels; position 16 g + 8 ks + 4 t + i holds token 32 ks + 16 t + 4 g + i: the tokens whose weights lane group g of
 // a wave has after the 16-row score products 2 ks and 2 ks + 1.  The unfinished block of a head is fp16 in the same
@@ -21,6 +21,10 @@ constexpr float kF16Max = 65504.f;
 constexpr float kLog2e = 1.4426950408889634f;
 // Values of a block enter the softmax weights as a power of two (see kv8_attn.hip); a block of zeros takes this one.
 constexpr float kMinScale = 4.656612873077393e-10f;  // 2^-31, below 2^-24 / 127, the smallest scale of a nonzero block
+
+constexpr float kStep = 1.f / 127.f;
+// What numbers with the largest magnitude amax are multiplied by before they are rounded to codes.
+__device__ __forceinline__ float code_factor(float amax) { return amax > 0.f ? (1.f / amax) * 127.f : 0.f; }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

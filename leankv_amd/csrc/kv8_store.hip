@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
     if (lane == 0) s_max[wave] = m;
     __syncthreads();
     const float amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    const float inv = amax > 0.f ? 127.f / amax : 0.f;
+    const float inv = code_factor(amax);
     // codes, rounded to nearest even; |x * inv| <= 127 (1 + 2^-23) rounds to 127 at most
     int code[4][8];
 #pragma unroll
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) code[i][j] = static_cast<int>(rintf(v[i][j] * inv));
     const int64_t at = bh * st.blocks + blk;
-    if (tid == 0) st.scales[2 * at + which] = amax / 127.f;
+    if (tid == 0) st.scales[2 * at + which] = amax * kStep;
     if (!which) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

@@ -16,12 +16,18 @@ def query(x):
     return x.double().clamp(-65504.0, 65504.0).half()
 
 
+STEP = torch.tensor(1.0) / torch.tensor(127.0)  # fp32
+
+
+def factor(amax):
+    return torch.where(amax > 0, (torch.ones_like(amax) / amax) * 127.0, torch.zeros_like(amax))
+
+
 def quantize(blocks):
     """(codes int, scale fp32) of fp16 blocks [..., 64, 128]."""
     x = blocks.float()
     amax = x.abs().amax((-2, -1))
-    inv = torch.where(amax > 0, torch.tensor(127.0) / amax, torch.zeros_like(amax))
-    return torch.round(x * inv[..., None, None]).to(torch.int64), amax / torch.tensor(127.0)
+    return torch.round(x * factor(amax)[..., None, None]).to(torch.int64), amax * STEP
 
 
 class Ref:
@@ -79,10 +85,9 @@ def choose(ref, q, n, sink, recent):
     best = None
     for row in stored(q):
         amax = row.float().abs().max()
-        q8 = torch.round(row.float() * (torch.tensor(127.0) / amax)).to(torch.int64) if amax > 0 else torch.zeros(
-            D, dtype=torch.int64)
+        q8 = torch.round(row.float() * factor(amax)).to(torch.int64)
         dot = torch.maximum(q8 * lo, q8 * hi).sum(1)
-        sc = dot.float() * (amax / torch.tensor(127.0))
+        sc = dot.float() * (amax * STEP)
         best = sc if best is None else torch.maximum(best, sc)
     score = (best * ref.scales["k"] + 0.0).tolist()
     forced = set(range(min(sink, nb))) | set(range(max(0, nb - recent), nb))

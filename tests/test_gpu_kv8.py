@@ -2,7 +2,7 @@
 same in 64 bits, with the bounds that its documented roundings give (kv8_ref.Ref.attend)."""
 import pytest
 import torch
-from kv8_ref import BLOCK, SCALE, D, Ref, choose, query, stored, v_tokens
+from kv8_ref import BLOCK, SCALE, STEP, D, Ref, choose, factor, query, stored, v_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -315,8 +315,8 @@ def test_sparse_many_blocks(cuda):
     best = None
     for row in q[0].float():
         a = row.abs().max()
-        q8 = torch.round(row * (127.0 / a)).double()
-        sc = torch.maximum(q8 * lo, q8 * hi).sum(1).float() * (a / 127.0)
+        q8 = torch.round(row * factor(a)).double()
+        sc = torch.maximum(q8 * lo, q8 * hi).sum(1).float() * (a * STEP.to(cuda))
         best = sc if best is None else torch.maximum(best, sc)
     score = best * store.scales[0, 0, :, 0]
     score[0] = score[-1] = float("inf")
