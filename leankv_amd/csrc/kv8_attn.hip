@@ -35,6 +35,8 @@ namespace {
 
 constexpr int kThr = 256;
 constexpr int kWaves = 4;
+constexpr int kManyCols = 256;  // columns of a workgroup of the many-row kernel
+constexpr int kManyChunk = 8;   // and the fewest blocks that a split of it gets
 // Offset kept above the largest log2 weight seen, so that most blocks need no new one.
 constexpr float kHeadroom = 4.f;
 
@@ -80,9 +82,14 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
   const int nlist = P.index ? P.n_index : nfull;
   const int units = nlist + (rest ? 1 : 0);
   const int u0 = blockIdx.x * P.chunk;
-  if (P.splits > 1 && u0 >= units) return;
-  const int u1 = min(u0 + P.chunk, units);
   const int col0 = group * 16 * NT;
+  if (P.splits > 1 && u0 >= units) {  // nothing to do: an empty record
+    const int col = col0 + tid;
+    if (tid < 16 * NT && col < r.cols)
+      *reinterpret_cast<float2*>(P.part_ml + 2 * ((bh * r.cols + col) * P.splits + blockIdx.x)) = float2{-INFINITY, 0.f};
+    return;
+  }
+  const int u1 = min(u0 + P.chunk, units);
 
   // ---- query rows: lane: column c16, dims 64 (ks / 2) + 16 g + 8 (ks % 2) + j
   f16x8 qf[NT][4];
@@ -276,16 +283,19 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
         acc[0] += a * *reinterpret_cast<const f32x4*>(&s_o[w][row][d]);
         acc[1] += a * *reinterpret_cast<const f32x4*>(&s_o[w][row][64 + d]);
       }
+      const bool row_ok = col / r.G < qlen;
       if (P.splits == 1) {
-        const float inv = col / r.G < qlen && L != 0.f ? 1.f / L : 0.f;  // no token: zeros
-        if (inv == 0.f) acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const bool some = row_ok && L != 0.f;  // no such row, or no token: zeros
+        const float inv = some ? 1.f / L : 0.f;
+        if (!some) acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
         store_row<DT>(r, b, h, col, d, acc[0] * inv);
         store_row<DT>(r, b, h, col, 64 + d, acc[1] * inv);
       } else {
         const int64_t at = ((bh * r.cols + col) * P.splits + blockIdx.x);
         *reinterpret_cast<f32x4*>(P.part_o + at * kD + d) = acc[0];
         *reinterpret_cast<f32x4*>(P.part_o + at * kD + 64 + d) = acc[1];
-        if ((tid & 15) == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = float2{M, L};
+        if ((tid & 15) == 0)
+          *reinterpret_cast<float2*>(P.part_ml + 2 * at) = row_ok ? float2{M, L} : float2{-INFINITY, 0.f};
       }
     }
   }
@@ -295,24 +305,21 @@ struct CombineArgs {
   Rows r;
   const float* part_o;
   const float* part_ml;
-  int Hkv, n_index, sparse, chunk, splits;
+  int Hkv, splits;
 };
 
-// One workgroup per row: 8 groups of 32 lanes, each every 8th split, 4 dims a lane.
+// One workgroup per row: 8 groups of 32 lanes, each every 8th split, 4 dims a lane.  A split without a token for the row
+// has offset -inf (and wrote no sums).
 template <int DT>
 __global__ __launch_bounds__(kThr) void combine_kernel(CombineArgs P) {
   __shared__ __align__(16) float s_o[8][kD];
   __shared__ float s_l[8];
   const Rows& r = P.r;
   const int tid = threadIdx.x, d = 4 * (tid & 31), part = tid >> 5;
-  const int col = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int len = min(max(r.lens[b], 0), r.max_len);
-  const int qlen = min(r.q_lens ? min(max(r.q_lens[b], 0), r.S) : r.S, len);
-  const int units = (P.sparse ? P.n_index : len / kBlk) + (len % kBlk ? 1 : 0);
-  const int n = col / r.G < qlen ? min((units + P.chunk - 1) / P.chunk, P.splits) : 0;
-  const int64_t row = (static_cast<int64_t>(b) * P.Hkv + h) * r.cols + col;
-  const float* ml = P.part_ml + row * P.splits * 2;
-  const float* po = P.part_o + row * P.splits * kD + d;
+  const int64_t row = blockIdx.x;  // ((sequence, kv head), column)
+  const int n = P.splits;
+  const float* ml = P.part_ml + row * n * 2;
+  const float* po = P.part_o + row * n * kD + d;
   float M = -INFINITY;
   for (int i = tid & 63; i < n; i += 64) M = fmaxf(M, ml[2 * i]);  // every wave for itself
   M = wave_max(M);
@@ -322,9 +329,12 @@ __global__ __launch_bounds__(kThr) void combine_kernel(CombineArgs P) {
 #pragma unroll 4
   for (int i = part; i < n; i += 8) {
     const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
-    const float a = exp2_(x.x - mu);
-    L += a * x.y;
-    acc += a * *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * kD);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * kD);
+    if (x.x != -INFINITY) {
+      const float a = exp2_(x.x - mu);
+      L += a * x.y;
+      acc += a * v;
+    }
   }
   *reinterpret_cast<f32x4*>(&s_o[part][d]) = acc;
   if ((tid & 31) == 0) s_l[part] = L;
@@ -336,8 +346,10 @@ __global__ __launch_bounds__(kThr) void combine_kernel(CombineArgs P) {
       L += s_l[p];
     }
     const float inv = L != 0.f ? 1.f / L : 0.f;
-    if (inv == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    store_row<DT>(r, b, h, col, d, acc * inv);
+    if (L == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t bh = row / r.cols;
+    store_row<DT>(r, static_cast<int>(bh / P.Hkv), static_cast<int>(bh % P.Hkv), static_cast<int>(row - bh * r.cols), d,
+                  acc * inv);
   }
 }
 
@@ -523,17 +535,19 @@ __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
 Plan make_plan(int64_t B, int64_t Hkv, int64_t cols, int64_t units) {
   Plan p;
   if (units < 1) units = 1;
-  p.nt = cols <= 16 ? 1 : 2;
-  p.groups = static_cast<int>((cols + 16 * p.nt - 1) / (16 * p.nt));
-  {
-    const int64_t items = B * Hkv * p.groups;
-    const int64_t target = 2 * device_cu_count();  // workgroups resident at once
-    int64_t want = (target + items - 1) / items;
-    int64_t chunk = (units + want - 1) / want;
-    chunk = (chunk + kWaves - 1) / kWaves * kWaves;
-    p.chunk = static_cast<int>(chunk);
-    p.splits = static_cast<int>((units + chunk - 1) / chunk);
-  }
+  const int64_t cus = device_cu_count();
+  p.nt = cols <= 16 ? 1 : cols <= 64 ? 2 : 0;
+  const int64_t wide = p.nt ? 16 * p.nt : kManyCols;
+  p.groups = static_cast<int>((cols + wide - 1) / wide);
+  const int64_t items = B * Hkv * p.groups;
+  // workgroups resident at once: two of the few-row kernel on a CU, one of the other
+  int64_t want = ((p.nt ? 2 : 1) * cus + items - 1) / items;
+  int64_t chunk = (units + want - 1) / want;
+  const int64_t unit = p.nt ? kWaves : 2;  // a block for every wave, or a pair of blocks
+  chunk = (chunk + unit - 1) / unit * unit;
+  if (!p.nt && chunk < kManyChunk) chunk = kManyChunk;
+  p.chunk = static_cast<int>(chunk);
+  p.splits = static_cast<int>((units + chunk - 1) / chunk);
   return p;
 }
 
@@ -591,6 +605,7 @@ extern "C" int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int
               "kv8_attn: a list of %lld blocks", (long long)n_index);
   LKV_REQUIRE(!index || S == 1, "kv8_attn: a block list is for one query per sequence");
   const int64_t B = store->batch, Hkv = store->kv_heads, G = Hq / Hkv, cols = G * S;
+  LKV_REQUIRE(B * Hkv * cols < (1ll << 31), "kv8_attn: %lld query rows", (long long)(B * Hkv * cols));
   if (B == 0 || S == 0) return LKV_OK;
   LKV_REQUIRE(q && out && lens, "kv8_attn: null pointer");
   if (int rc = check_rows(q, q_strides, dtype, "kv8_attn", "q")) return rc;
@@ -619,16 +634,20 @@ extern "C" int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int
   float* part_o = static_cast<float*>(workspace);
   float* part_ml = part_o + static_cast<size_t>(B * Hkv * cols) * p.splits * kD;
   SplitArgs A{device_store(store), r, index, static_cast<int>(n_index), p.groups, p.chunk, p.splits, part_o, part_ml};
-  if (dtype == LKV_DTYPE_F32)
-    launch_split<LKV_DTYPE_F32>(A, p.nt, B, st);
-  else if (dtype == LKV_DTYPE_F16)
-    launch_split<LKV_DTYPE_F16>(A, p.nt, B, st);
-  else
-    launch_split<LKV_DTYPE_BF16>(A, p.nt, B, st);
-  LKV_LAUNCH_CHECK("kv8_attn split");
+  if (!p.nt) {
+    if (int rc = launch_prefill(A.st, r, p, dtype, B, part_o, part_ml, st)) return rc;
+  } else {
+    if (dtype == LKV_DTYPE_F32)
+      launch_split<LKV_DTYPE_F32>(A, p.nt, B, st);
+    else if (dtype == LKV_DTYPE_F16)
+      launch_split<LKV_DTYPE_F16>(A, p.nt, B, st);
+    else
+      launch_split<LKV_DTYPE_BF16>(A, p.nt, B, st);
+    LKV_LAUNCH_CHECK("kv8_attn split");
+  }
   if (p.splits > 1) {
-    const CombineArgs C{r, part_o, part_ml, static_cast<int>(Hkv), static_cast<int>(n_index), index != nullptr, p.chunk, p.splits};
-    const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>(Hkv), static_cast<unsigned>(B));
+    const CombineArgs C{r, part_o, part_ml, static_cast<int>(Hkv), p.splits};
+    const dim3 grid(static_cast<unsigned>(B * Hkv * cols));
     if (dtype == LKV_DTYPE_F32)
       hipLaunchKernelGGL(combine_kernel<LKV_DTYPE_F32>, grid, dim3(kThr), 0, st, C);
     else if (dtype == LKV_DTYPE_F16)

@@ -14,6 +14,7 @@ synchronises, and every workspace is allocated for its call on the current strea
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -28,6 +29,16 @@ _I64x3 = ctypes.c_int64 * 3
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
+@functools.lru_cache(maxsize=256)
+def _strides3(b: int, h: int, s: int):
+    return _I64x3(b, h, s)
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_bytes(batch: int, heads: int, kv_heads: int, S: int, max_len: int, n_index: int) -> int:
+    return _lib.load().lkv_kv8_attn_workspace_bytes(batch, heads, kv_heads, S, max_len, n_index)
+
+
 def _dtype(t: torch.Tensor, what: str) -> int:
     code = _DTYPES.get(t.dtype)
     if code is None:
@@ -35,18 +46,34 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return code
 
 
+def _in_place(shape, strides, t: torch.Tensor):
+    """The strides of batch, head and token of t [B, H, S, 128] as the kernels take them, None where its rows are not
+    dense or not 16-byte aligned.  Strides of single sizes count as 0 (torch leaves them free)."""
+    b = strides[0] if shape[0] > 1 else 0
+    h = strides[1] if shape[1] > 1 else 0
+    s = strides[2] if shape[2] > 1 else 0
+    if strides[3] != 1 or (b | h | s) % (16 // t.element_size()) or t.data_ptr() % 16:
+        return None
+    return _strides3(b, h, s)
+
+
 def _rows(t: torch.Tensor):
-    """(t, its strides of batch, head and token in elements): t itself where its rows of 128 are dense and 16-byte
-    aligned, else a copy.  t is [B, H, S, 128]; strides of single sizes are 0 (torch leaves them free)."""
-    b, h, s = t.stride()[:3]
-    n = t.shape
-    strides = (b if n[0] > 1 else 0, h if n[1] > 1 else 0, s if n[2] > 1 else 0)
-    unit = 16 // t.element_size()
-    if t.stride(3) == 1 and not (strides[0] % unit or strides[1] % unit or strides[2] % unit) \
-            and t.data_ptr() % 16 == 0:
-        return t, _I64x3(*strides)
-    t = t.clone(memory_format=torch.contiguous_format)
-    return t, _I64x3(*t.stride()[:3])
+    """(t or a copy of it, strides) for t [B, H, S, 128] that is read."""
+    strides = _in_place(t.shape, t.stride(), t)
+    if strides is None:
+        t = t.detach().clone(memory_format=torch.contiguous_format)
+        strides = _in_place(t.shape, t.stride(), t)
+    return t, strides
+
+
+def _query_rows(q: torch.Tensor):
+    """The same for q [B, H, 128]: one token a sequence."""
+    b, h, d = q.stride()
+    strides = _in_place((q.shape[0], q.shape[1], 1), (b, h, 0, d), q)
+    if strides is None:
+        q = q.detach().clone(memory_format=torch.contiguous_format)
+        strides = _strides3(q.stride(0), q.stride(1), 0)
+    return q, strides
 
 
 class KV8Store:
@@ -90,6 +117,7 @@ class KV8Store:
                                            self.ranges.data_ptr(), self.k_tail.data_ptr(), self.v_tail.data_ptr(),
                                            self.batch, self.kv_heads, self.blocks)
         self._ref = ctypes.byref(self._struct)
+        self._index = self.device.index
         self._lib = _lib.load()
 
     @property
@@ -104,29 +132,31 @@ class KV8Store:
     # ------------------------------------------------------------------------------------------------ checks
     def _call(self, name: str, *args):
         """One C entry on the store's device and that device's current stream."""
-        idx = self.device.index
-        if torch.cuda.current_device() == idx:
+        idx = self._index
+        if torch._C._cuda_getDevice() == idx:
             rc = getattr(self._lib, name)(self._ref, *args, torch._C._cuda_getCurrentRawStream(idx))
         else:
-            with torch.cuda.device(self.device):
+            with torch.cuda.device(idx):
                 rc = getattr(self._lib, name)(self._ref, *args, torch._C._cuda_getCurrentRawStream(idx))
         if rc:
             check(rc, name)
 
     def _ints(self, t, what: str, name: str):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device \
-                or t.numel() != self.batch or not t.is_contiguous():
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or not t.is_cuda \
+                or t.get_device() != self._index or t.numel() != self.batch or not t.is_contiguous():
             raise LeanKVError("%s: %s must be a contiguous int32 tensor of %d entries on %s"
                               % (what, name, self.batch, self.device))
         return t.data_ptr()
 
     def _queries(self, q, dims: int, what: str):
-        if q.dim() != dims or q.shape[0] != self.batch or q.shape[-1] != HEAD_DIM or q.shape[1] % self.kv_heads \
-                or not q.shape[1] or q.device != self.device:
+        """Heads of q [batch, heads(, S), 128] and its dtype code."""
+        n = q.shape
+        if len(n) != dims or n[0] != self.batch or n[-1] != HEAD_DIM or n[1] % self.kv_heads or not n[1] \
+                or not q.is_cuda or q.get_device() != self._index:
             raise LeanKVError("%s: q must be [%d, heads, %s%d] on %s with a multiple of %d heads, got %s on %s"
                               % (what, self.batch, "S, " if dims == 4 else "", HEAD_DIM, self.device, self.kv_heads,
-                                 tuple(q.shape), q.device))
-        return _dtype(q, what)
+                                 tuple(n), q.device))
+        return n[1], _dtype(q, what)
 
     def _bound(self, max_len, what: str) -> int:
         if max_len is None:
@@ -135,9 +165,10 @@ class KV8Store:
             raise LeanKVError("%s: max_len=%d outside a store of %d tokens" % (what, max_len, self.blocks * BLOCK))
         return int(max_len)
 
-    def _workspace(self, nbytes: int):
-        """Allocated for its call on the current stream: calls on several streams and captured graphs share none."""
-        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+    def _empty(self, shape, dtype):
+        """Workspaces too are allocated for their call, on the current stream: calls on several streams and captured
+        graphs share none."""
+        return torch.empty(shape, dtype=dtype, device=self.device)
 
     # ------------------------------------------------------------------------------------------------ storing
     def update(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, n_new: torch.Tensor | None = None) -> None:
@@ -145,20 +176,20 @@ class KV8Store:
         it holds already).  n_new: how many of the S are sequence b's (a padded batch; the rest is not read).  Tokens
         past the capacity are dropped.  One launch; blocks that become whole are quantized."""
         what = "KV8Store.update"
-        for t, name in ((k, "k"), (v, "v")):
-            if t.dim() != 4 or t.shape[0] != self.batch or t.shape[1] != self.kv_heads or t.shape[3] != HEAD_DIM \
-                    or t.device != self.device:
+        nk, nv = k.shape, v.shape
+        for t, n, name in ((k, nk, "k"), (v, nv, "v")):
+            if len(n) != 4 or n[0] != self.batch or n[1] != self.kv_heads or n[3] != HEAD_DIM or not t.is_cuda \
+                    or t.get_device() != self._index:
                 raise LeanKVError("%s: %s must be [%d, %d, S, %d] on %s, got %s on %s"
-                                  % (what, name, self.batch, self.kv_heads, HEAD_DIM, self.device, tuple(t.shape),
-                                     t.device))
-        if k.shape != v.shape or k.dtype != v.dtype:
+                                  % (what, name, self.batch, self.kv_heads, HEAD_DIM, self.device, tuple(n), t.device))
+        if nk != nv or k.dtype != v.dtype:
             raise LeanKVError("%s: k and v must be alike, got %s %s and %s %s"
-                              % (what, k.dtype, tuple(k.shape), v.dtype, tuple(v.shape)))
+                              % (what, k.dtype, tuple(nk), v.dtype, tuple(nv)))
         dtype = _dtype(k, what)
         p = self._ints(pos, what, "pos")
         m = None if n_new is None else self._ints(n_new, what, "n_new")
-        (k, ks), (v, vs) = _rows(k.detach()), _rows(v.detach())
-        self._call("lkv_kv8_update", k.data_ptr(), ks, v.data_ptr(), vs, dtype, k.shape[2], p, m)
+        (k, ks), (v, vs) = _rows(k), _rows(v)
+        self._call("lkv_kv8_update", k.data_ptr(), ks, v.data_ptr(), vs, dtype, nk[2], p, m)
 
     def read(self, lens: torch.Tensor, n: int, first: int = 0):
         """(K, V) float16 [batch, kv_heads, n - first, 128]: tokens first .. n - 1 of every sequence as attention sees
@@ -167,38 +198,19 @@ class KV8Store:
         if not 0 <= first <= n <= self.blocks * BLOCK:
             raise LeanKVError("%s: tokens %d .. %d outside a store of %d" % (what, first, n, self.blocks * BLOCK))
         p = self._ints(lens, what, "lens")
-        k = torch.empty(self.batch, self.kv_heads, n - first, HEAD_DIM, dtype=torch.float16, device=self.device)
-        v = torch.empty_like(k)
+        k, v = self._empty((2, self.batch, self.kv_heads, n - first, HEAD_DIM), torch.float16).unbind(0)
         self._call("lkv_kv8_read", p, first, n - first, k.data_ptr(), v.data_ptr())
         return k, v
 
     # ---------------------------------------------------------------------------------------------- attention
-    def _out(self, q: torch.Tensor, out: torch.Tensor | None, what: str):
-        """The output for q [B, Hq, S, 128] and its strides; a fresh one is laid out token by token (what the output
-        projection reads)."""
-        if out is None:
-            B, Hq, S, _ = q.shape
-            out = torch.empty(B, S, Hq, HEAD_DIM, dtype=q.dtype, device=q.device).transpose(1, 2)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-            raise LeanKVError("%s: out must be like q, %s %s on %s" % (what, q.dtype, tuple(q.shape), q.device))
-        rows, strides = _rows(out)
-        if rows is not out:
-            raise LeanKVError("%s: rows of out must be dense and 16-byte aligned" % what)
-        return out, strides
-
-    def _attend(self, q, dtype, lens, q_lens, max_len, index, scale, out, what):
-        p = self._ints(lens, what, "lens")
-        m = None if q_lens is None else self._ints(q_lens, what, "q_lens")
-        L = self._bound(max_len, what)
-        out, os = self._out(q, out, what)
-        q, qs = _rows(q.detach())
-        Hq, S = q.shape[1], q.shape[2]
-        n = 0 if index is None else index.shape[2]
-        nbytes = self._lib.lkv_kv8_attn_workspace_bytes(self.batch, Hq, self.kv_heads, S, L, n)
-        ws = self._workspace(nbytes) if nbytes else None
-        self._call("lkv_kv8_attn", q.data_ptr(), qs, dtype, Hq, S, p, m, L, None if index is None else index.data_ptr(),
-                   n, _SCALE if scale is None else float(scale), out.data_ptr(), os,
-                   None if ws is None else ws.data_ptr(), nbytes)
+    def _decode(self, q, heads, dtype, p, L, index, n, scale, out):
+        """One query a sequence; out [batch, heads, 128] with dense, aligned rows."""
+        q, qs = _query_rows(q)
+        os = _strides3(out.stride(0), out.stride(1), 0)
+        nbytes = _attn_bytes(self.batch, heads, self.kv_heads, 1, L, n)
+        ws = self._empty(nbytes, torch.uint8) if nbytes else None
+        self._call("lkv_kv8_attn", q.data_ptr(), qs, dtype, heads, 1, p, None, L, index, n,
+                   _SCALE if scale is None else scale, out.data_ptr(), os, None if ws is None else ws.data_ptr(), nbytes)
         return out
 
     def decode_attention(self, q: torch.Tensor, lens: torch.Tensor, max_len: int | None = None,
@@ -207,48 +219,70 @@ class KV8Store:
         among it): [batch, heads, 128] in q's type.  A sequence of length 0 gives zeros.  max_len: the caller's bound on
         lens (default the capacity), which the work is split for.  scale: 1 / sqrt(128) by default."""
         what = "KV8Store.decode_attention"
-        dtype = self._queries(q, 3, what)
-        o = self._attend(q.unsqueeze(2), dtype, lens, None, max_len, None, scale,
-                         None if out is None else out.unsqueeze(2), what)
-        return o.squeeze(2) if out is None else out
+        heads, dtype = self._queries(q, 3, what)
+        p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
+        if out is None:
+            out = self._empty((self.batch, heads, HEAD_DIM), q.dtype)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device \
+                or _in_place((self.batch, heads, 1), (*out.stride()[:2], 0, out.stride(2)), out) is None:
+            raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
+                              % (what, q.dtype, tuple(q.shape), q.device))
+        return self._decode(q, heads, dtype, p, L, None, 0, scale, out)
 
     def prefill_attention(self, q: torch.Tensor, lens: torch.Tensor, q_lens: torch.Tensor | None = None,
                           max_len: int | None = None, scale: float | None = None,
                           out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention of the S newest tokens' queries q [batch, heads, S, 128] (after their update): query i of a
-        sequence with q_lens[b] of them (default S) sees tokens 0 .. lens[b] - q_lens[b] + i.  Rows from q_lens[b] on
-        are zeros.  Returns [batch, heads, S, 128] in q's type, laid out [batch, S, heads, 128]."""
+        sequence with q_lens[b] of them (default S, at most its length) sees tokens 0 .. lens[b] - q_lens[b] + i.  Rows
+        from q_lens[b] on are zeros.  Returns [batch, heads, S, 128] in q's type, laid out [batch, S, heads, 128]."""
         what = "KV8Store.prefill_attention"
-        dtype = self._queries(q, 4, what)
-        return self._attend(q, dtype, lens, q_lens, max_len, None, scale, out, what)
+        heads, dtype = self._queries(q, 4, what)
+        p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
+        m = None if q_lens is None else self._ints(q_lens, what, "q_lens")
+        S = q.shape[2]
+        if out is None:  # laid out token by token, as an output projection reads it
+            out = self._empty((self.batch, S, heads, HEAD_DIM), q.dtype).transpose(1, 2)
+        os = _in_place(q.shape, out.stride(), out) if out.dim() == 4 else None
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or os is None:
+            raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
+                              % (what, q.dtype, tuple(q.shape), q.device))
+        q, qs = _rows(q)
+        nbytes = _attn_bytes(self.batch, heads, self.kv_heads, S, L, 0)
+        ws = self._empty(nbytes, torch.uint8) if nbytes else None
+        self._call("lkv_kv8_attn", q.data_ptr(), qs, dtype, heads, S, p, m, L, None, 0,
+                   _SCALE if scale is None else scale, out.data_ptr(), os, None if ws is None else ws.data_ptr(), nbytes)
+        return out
 
     # ------------------------------------------------------------------------------------------------- sparse
+    def _select(self, q, heads, dtype, p, L, blocks, sink, recent, what):
+        blocks, sink, recent = int(blocks), int(sink), int(recent)
+        if blocks < 1 or sink < 0 or recent < 0 or sink + recent > blocks:
+            raise LeanKVError("%s: %d blocks with the first %d and the last %d among them" % (what, blocks, sink, recent))
+        q, qs = _query_rows(q)
+        index = self._empty((self.batch, self.kv_heads, blocks), torch.int32)
+        nbytes = self.batch * self.kv_heads * (L // BLOCK) * 4
+        ws = self._empty(nbytes, torch.uint8)
+        self._call("lkv_kv8_select_blocks", q.data_ptr(), qs, dtype, heads, p, L, blocks, sink, recent,
+                   index.data_ptr(), ws.data_ptr(), nbytes)
+        return index
+
     def select_blocks(self, q: torch.Tensor, lens: torch.Tensor, blocks: int, sink: int = 1, recent: int = 1,
                       max_len: int | None = None) -> torch.Tensor:
         """int32 [batch, kv_heads, blocks]: for one query per sequence, q [batch, heads, 128], the finished blocks with
         the highest upper bound of q.k (over the kv head's queries), ascending, -1 where a sequence has fewer.  The first
         `sink` and the last `recent` finished blocks are always among them; of equal scores the lower index wins."""
         what = "KV8Store.select_blocks"
-        dtype = self._queries(q, 3, what)
-        p = self._ints(lens, what, "lens")
-        L = self._bound(max_len, what)
-        blocks, sink, recent = int(blocks), int(sink), int(recent)
-        if blocks < 1 or sink < 0 or recent < 0 or sink + recent > blocks:
-            raise LeanKVError("%s: %d blocks with the first %d and the last %d among them" % (what, blocks, sink, recent))
-        q, qs = _rows(q.detach().unsqueeze(2))
-        index = torch.empty(self.batch, self.kv_heads, blocks, dtype=torch.int32, device=self.device)
-        nbytes = self._lib.lkv_kv8_select_workspace_bytes(self.batch, self.kv_heads, L)
-        ws = self._workspace(nbytes)
-        self._call("lkv_kv8_select_blocks", q.data_ptr(), qs, dtype, q.shape[1], p, L, blocks, sink, recent,
-                   index.data_ptr(), ws.data_ptr(), nbytes)
-        return index
+        heads, dtype = self._queries(q, 3, what)
+        p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
+        return self._select(q, heads, dtype, p, L, blocks, sink, recent, what)
 
     def sparse_decode_attention(self, q: torch.Tensor, lens: torch.Tensor, blocks: int, sink: int = 1, recent: int = 1,
                                 max_len: int | None = None, scale: float | None = None):
         """decode_attention over the blocks that select_blocks chooses and the unfinished block: (out [batch, heads, 128],
         index)."""
         what = "KV8Store.sparse_decode_attention"
-        dtype = self._queries(q, 3, what)
-        index = self.select_blocks(q, lens, blocks, sink, recent, max_len)
-        out = self._attend(q.unsqueeze(2), dtype, lens, None, max_len, index, scale, None, what)
-        return out.squeeze(2), index
+        heads, dtype = self._queries(q, 3, what)
+        p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
+        index = self._select(q, heads, dtype, p, L, blocks, sink, recent, what)
+        out = self._empty((self.batch, heads, HEAD_DIM), q.dtype)
+        return self._decode(q, heads, dtype, p, L, index.data_ptr(), index.shape[2], scale, out), index
