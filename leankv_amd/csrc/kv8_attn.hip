@@ -37,8 +37,6 @@ constexpr int kThr = 256;
 constexpr int kWaves = 4;
 constexpr int kManyCols = 256;  // columns of a workgroup of the many-row kernel
 constexpr int kManyChunk = 8;   // and the fewest blocks that a split of it gets
-// Offset kept above the largest log2 weight seen, so that most blocks need no new one.
-constexpr float kHeadroom = 4.f;
 
 __device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -145,7 +143,7 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
         s[e] = fmaf(sc[n][e >> 2][e & 3], kc, lv - m[n]);
         mx = fmaxf(mx, s[e]);
       }
-      if (t0 + kBlk > lim_min || wave_ballot(mx > 0.f) != 0) {  // uniform
+      if (t0 + kBlk > lim_min || wave_ballot(mx > kMaxWeight) != 0) {  // uniform
         const int left = lim[n] - t0 - 4 * g;  // the lane's token 16 T + i is visible below this
         mx = -INFINITY;
 #pragma unroll
@@ -155,7 +153,7 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
           mx = fmaxf(mx, s[e]);
         }
         mx = groups_max(mx);
-        const float mn = mx > m[n] ? mx + kHeadroom : m[n];
+        const float mn = mx - m[n] > kMaxWeight ? mx - kTopWeight : m[n];
         const float mu = mn == -INFINITY ? 0.f : mn;
         const float alpha = exp2_(m[n] - mu);
         m[n] = mn;

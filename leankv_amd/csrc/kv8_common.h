@@ -22,6 +22,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Values of a block enter the softmax weights as a power of two (see kv8_attn.hip); a block of zeros takes this one.
 constexpr float kMinScale = 4.656612873077393e-10f;  // 2^-31, below 2^-24 / 127, the smallest scale of a nonzero block
 
+// log2 of the softmax weights as fp16 holds them: a new offset puts the largest at 2^6, and there is none until a weight
+// passes 2^15, so that most blocks need no max over lanes and no rescaled sums.  A weight keeps fp16's 11 bits down to
+// 2^-20 of the largest.
+constexpr float kTopWeight = 6.f, kMaxWeight = 15.f;
+
 constexpr float kStep = 1.f / 127.f;
 // What numbers with the largest magnitude amax are multiplied by before they are rounded to codes.
 __device__ __forceinline__ float code_factor(float amax) { return amax > 0.f ? (1.f / amax) * 127.f : 0.f; }
@@ -46,7 +51,7 @@ __host__ __device__ __forceinline__ constexpr int v_pos(int t) { return 4 * v_dw
 static_assert(v_pos(0) == 0 && v_pos(4) == 16 && v_pos(16) == 4 && v_pos(32) == 8 && v_pos(63) == 63, "value order");
 
 __device__ __forceinline__ uint32_t pk2(float lo, float hi) {
-  return static_cast<uint32_t>(f2h(lo)) | (static_cast<uint32_t>(f2h(hi)) << 16);
+  return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
 }
 __device__ __forceinline__ float bf2f(uint32_t h) { return __uint_as_float(h << 16); }
 
@@ -95,13 +100,26 @@ __device__ __forceinline__ float clamp_kv(float x) {
   const float c = fminf(fmaxf(x, -kF16Max), kF16Max);
   return x != x ? 0.f : c;
 }
+// The same for two fp16 numbers: an infinity (0x7c00 without its sign) becomes the number before it.
+__device__ __forceinline__ uint32_t clamp_q2(uint32_t u) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  const u16x2 x = __builtin_bit_cast(u16x2, u), one = u16x2{1, 1};
+  const u16x2 t = (x & u16x2{0x7fff, 0x7fff}) - u16x2{0x7c00, 0x7c00};
+  return __builtin_bit_cast(uint32_t, static_cast<u16x2>(x + (__builtin_elementwise_min(t, one) - one)));
+}
 template <int DT>
 __device__ __forceinline__ f16x8 load_q8(const void* base, int64_t at) {
-  float x[8];
-  load8<DT>(base, at, x);
   u32x4 r;
+  if constexpr (DT == LKV_DTYPE_F16) {
+    r = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + at);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) r[j] = pk2(clamp_q(x[2 * j]), clamp_q(x[2 * j + 1]));
+    for (int j = 0; j < 4; ++j) r[j] = clamp_q2(r[j]);
+  } else {
+    float x[8];
+    load8<DT>(base, at, x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = pk2(clamp_q(x[2 * j]), clamp_q(x[2 * j + 1]));
+  }
   return __builtin_bit_cast(f16x8, r);
 }
 

@@ -11,8 +11,6 @@
 //   out^T (32 dims x 32 columns) += A = values from LDS, B = the weights from the lane's own registers (the values' token
 //   order in LDS is the order in which a lane holds its scores).
 // Scales and the running offset are those of kv8_attn.hip; most blocks need no max over lanes and no rescale.
-// Two blocks per barrier and two pairs of LDS buffers in turn; waves 4-7 fill the next pair before they compute, waves
-// 0-3 after, so that the two waves of a SIMD are out of step.
 #include "kv8_common.h"
 
 namespace lkv {
@@ -25,9 +23,7 @@ constexpr int kCols = 32 * kWaves;
 constexpr int kKRow = kD + 8;    // fp16 numbers of a staged key row
 constexpr int kVRow = kBlk + 8;  // and of a value row
 constexpr int kKBuf = kBlk * kKRow, kVBuf = kD * kVRow;
-constexpr int kBufs = 4;
 constexpr int kXcds = 8;
-constexpr float kHeadroom = 4.f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -43,157 +39,156 @@ __device__ __forceinline__ float half_sum(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
-__device__ __forceinline__ uint32_t cvt2(float a, float b) {
-  return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
-}
-
 struct PrefillArgs {
   Store st;
   Rows r;
   int tiles;   // column tiles per (sequence, kv head)
   int chunk, splits;
+  int items;   // (sequence, kv head) pairs
+  int total;   // items * tiles * splits pieces of work
   float* part_o;
   float* part_ml;
 };
 
 template <int DT>
 __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
-  __shared__ __align__(16) uint16_t sK[kBufs * kKBuf];
-  __shared__ __align__(16) uint16_t sV[kBufs * kVBuf];
+  __shared__ __align__(16) uint16_t sK[2 * kKBuf];
+  __shared__ __align__(16) uint16_t sV[2 * kVBuf];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, hf = lane >> 5;
   const Store& st = P.st;
   const Rows& r = P.r;
-  // Workgroups go to the XCDs round-robin by linear id, and the tiles of one (sequence, kv head) read the same blocks:
-  // the items are placed XCD by XCD where their number allows it, the latest queries (the longest) first.
-  int tile, split, h, b;
-  {
-    const int per = P.tiles * P.splits;  // workgroups of an item
-    const int items = static_cast<int>(gridDim.x) / per;
-    const int p = static_cast<int>(blockIdx.x);
-    int item, t;
-    if (items % kXcds == 0) {
-      const int k = items / kXcds, s = p / kXcds;
-      item = p % kXcds + kXcds * (s % k);
-      t = s / k;
-    } else if (kXcds % items == 0 && per % (kXcds / items) == 0) {
-      const int k = kXcds / items, x = p % kXcds;
-      item = x % items;
-      t = (p / kXcds) * k + x / items;
-    } else {
-      item = p / per;
-      t = p % per;
-    }
-    // (divisions leave them in vector registers: made scalar again)
-    tile = __builtin_amdgcn_readfirstlane(P.tiles - 1 - t / P.splits);
-    split = __builtin_amdgcn_readfirstlane(t % P.splits);
-    h = __builtin_amdgcn_readfirstlane(item % st.Hkv);
-    b = __builtin_amdgcn_readfirstlane(item / st.Hkv);
-  }
-  const int len = min(max(r.lens[b], 0), r.max_len);
-  const int qlen = min(r.q_lens ? min(max(r.q_lens[b], 0), r.S) : r.S, len);
-  const int nfull = len / kBlk;
-  const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
-  const int col0 = tile * kCols;
-  // ---- the lane's column
-  const int col = col0 + 32 * wave + c32, qs = col / r.G, qh = col - qs * r.G;
-  const bool ok = col < r.cols && qs < qlen;
-  const int lim = ok ? len - qlen + qs + 1 : 0x7fffffff;  // tokens it sees
-  f16x8 qf[8];  // B: the column's row, dims 16 kb + 8 hf ..
-#pragma unroll
-  for (int kb = 0; kb < 8; ++kb) {
-    qf[kb] = f16x8{};
-    if (ok)
-      qf[kb] = load_q8<DT>(r.q, b * r.q_sb + static_cast<int64_t>(h * r.G + qh) * r.q_sh + qs * r.q_ss + 16 * kb + 8 * hf);
-  }
-  // blocks [blk0, blk1): what the workgroup's last column sees, of the split's
-  const int last = min((col0 + kCols - 1) / r.G, qlen - 1);  // its last query
-  const int kend = last >= col0 / r.G ? len - qlen + last + 1 : 0;
-  const int blk0 = split * P.chunk;
-  const int blk1 = min(blk0 + P.chunk, (kend + kBlk - 1) / kBlk);
-  // tokens that every column of the wave sees
-  const int wq = (col0 + 32 * wave) / r.G;
-  const int lim_min = wq < qlen ? len - qlen + wq + 1 : 0x7fffffff;
 
-  // ---- staging: waves 0-3: keys, token kk, dims 32 part ..; waves 4-7: values, dim vd, its tokens of half vh
+  // ---- staging: waves 0-3 keys (token kk, 32 dims), waves 4-7 values (dim vd, half of its tokens): 2 x 16 bytes of codes
+  // a thread, w0 and w1; 16-byte piece p of its four in LDS is dword p of each.  A piece of a key row is then dims
+  // 32 part + 4 p + i and 16 + that, and one of a value row tokens 16 p + 4 vh + i and 8 + that: the order of the query
+  // operand below, and of a lane's weights.
   const bool key_thr = wave < 4;
   const int kk = (tid & 255) >> 2, part = tid & 3;
   const int vd = (tid & 255) >> 1, vh = tid & 1;
-  const uint8_t* const src = (key_thr ? st.k_codes + kk * kD + 32 * part : st.v_codes + vd * kBlk + 16 * vh) +
-                             bh * st.blocks * kBlkBytes;
-  const int src2 = key_thr ? 16 : 32;  // the thread's second 16 bytes
-  uint16_t* const dst = key_thr ? sK + kk * kKRow + 32 * part : sV + vd * kVRow + 8 * vh;
-  u32x4 w[2][2];
-  auto load_tile = [&](int blk, int u) {
-    if (blk < min(blk1, nfull)) {  // uniform
-      const uint8_t* p = src + static_cast<int64_t>(blk) * kBlkBytes;
-      w[u][0] = *reinterpret_cast<const u32x4*>(p);
-      w[u][1] = *reinterpret_cast<const u32x4*>(p + src2);
-    }
-  };
-  auto stage_tile = [&](int blk, int u) {
-    const int buf = (blk - blk0) % kBufs;
-    uint16_t* d = dst + buf * (key_thr ? kKBuf : kVBuf);
-    if (blk < nfull) {
-      if (key_thr) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<f16x8*>(d + 8 * k) = codes8h(w[u][k >> 1][2 * (k & 1)], w[u][k >> 1][2 * (k & 1) + 1]);
-      } else {
-        // step ks of the value product: tokens 16 ks + 4 vh + i, then 16 ks + 8 + 4 vh + i
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) *reinterpret_cast<f16x8*>(d + 16 * ks) = codes8h(w[u][0][ks], w[u][1][ks]);
-      }
-    } else if (key_thr) {  // the unfinished block: fp16 as it is
-      const uint16_t* p = st.k_tail + bh * kBlkBytes + kk * kD + 32 * part;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x4*>(d + 8 * k) = *reinterpret_cast<const u32x4*>(p + 8 * k);
-    } else {
-      const uint16_t* p = st.v_tail + bh * kBlkBytes + vd * kBlk + 16 * vh;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const uint2 a = *reinterpret_cast<const uint2*>(p + 4 * ks), c = *reinterpret_cast<const uint2*>(p + 32 + 4 * ks);
-        *reinterpret_cast<u32x4*>(d + 16 * ks) = u32x4{a.x, a.y, c.x, c.y};
-      }
-    }
-  };
+  const int src_off = key_thr ? kk * kD + 32 * part : vd * kBlk + 16 * vh;
+  const int src2 = key_thr ? 16 : 32;  // the second 16 bytes
+  uint16_t* const dst = key_thr ? sK + kk * kKRow + 64 * (part >> 1) + 8 * (part & 1) : sV + vd * kVRow + 8 * vh;
+  const int dst_buf = key_thr ? kKBuf : kVBuf;
+  const int off = key_thr ? 1 : 0;  // keys are staged a tile further ahead than values
+  const uint16_t* const krow = sK + c32 * kKRow + 8 * hf;
+  const uint16_t* const vrow = sV + c32 * kVRow + 8 * hf;
 
-  float m = ok ? -INFINITY : 0.f, l = 0.f;  // a column that is no row keeps offset 0 over zero scores
-  f32x16 o[4];  // dims 32 db + 8 (i / 4) + 4 hf + i % 4
-#pragma unroll
-  for (int db = 0; db < 4; ++db) o[db] = f32x16{};
+  // The workgroups stay and take their pieces of work in turn, the longest first and the order reversed in every second
+  // round, so that each gets as much.  Workgroups go to the XCDs round-robin, and the column tiles of one (sequence, kv
+  // head) read the same blocks: where the numbers allow it they are all taken on one XCD.
+  const int G = r.G;
+  const int lanes = gridDim.x % kXcds == 0 && P.items % kXcds == 0 ? kXcds : 1;  // (XCDs apart or not)
+  const int width = static_cast<int>(gridDim.x) / lanes;
+  const int mine = static_cast<int>(blockIdx.x) / lanes, xcd = static_cast<int>(blockIdx.x) % lanes;
+  const int per_lane = P.total / lanes, item_step = P.items / lanes;
+#pragma unroll 1
+  for (int round = 0; round * width < per_lane; ++round) {
+    const int pos = round * width + ((round & 1) ? width - 1 - mine : mine);
+    if (pos >= per_lane) continue;  // uniform
+    // (divisions leave uniform values in vector registers: made scalar again)
+    const int piece = __builtin_amdgcn_readfirstlane(pos / item_step);
+    const int item = (pos - piece * item_step) * lanes + xcd;
+    const int tile = P.tiles - 1 - __builtin_amdgcn_readfirstlane(piece / P.splits);
+    const int split = piece - (P.tiles - 1 - tile) * P.splits;
+    const int b = __builtin_amdgcn_readfirstlane(item / st.Hkv), h = item - b * st.Hkv;
+    const int len = min(max(r.lens[b], 0), r.max_len);
+    const int qlen = min(r.q_lens ? min(max(r.q_lens[b], 0), r.S) : r.S, len);
+    const int nfull = len / kBlk;
+    const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
+    const int col0 = tile * kCols;
+    const int q_first = __builtin_amdgcn_readfirstlane(col0 / G);
+    // blocks [blk0, blk1): what the piece's last column sees, of the split's; nf of them finished
+    const int last = min(__builtin_amdgcn_readfirstlane((col0 + kCols - 1) / G), qlen - 1);  // its last query
+    const int kend = last >= q_first ? len - qlen + last + 1 : 0;
+    const int blk0 = split * P.chunk;
+    const int blk1 = min(blk0 + P.chunk, (kend + kBlk - 1) / kBlk);
+    const int nf = max(min(blk1, nfull) - blk0, 0);
+    const bool rest = blk1 > blk0 && blk1 > nfull;  // the unfinished block is the last of them
 
-  auto compute_tile = [&](int blk) {
-    const int buf = (blk - blk0) % kBufs, t0 = blk * kBlk;
-    const uint16_t* k = sK + buf * kKBuf + c32 * kKRow + 8 * hf;
-    const uint16_t* v = sV + buf * kVBuf + c32 * kVRow + 8 * hf;
+    // ---- loads that depend on nothing else, all on their way together
+    const uint8_t* const src = (key_thr ? st.k_codes : st.v_codes) + (bh * st.blocks + blk0) * kBlkBytes + src_off;
+    const float* const scales = st.scales + 2 * (bh * st.blocks + blk0);
+    u32x4 w0, w1;
+    auto load_tile = [&](int t) {  // (past the last: the last again, staged where nothing reads it)
+      const uint8_t* p = src + static_cast<int64_t>(min(t, nf - 1)) * kBlkBytes;
+      w0 = *reinterpret_cast<const u32x4*>(p);
+      w1 = *reinterpret_cast<const u32x4*>(p + src2);
+    };
+    auto load_scales = [&](int t) { return *reinterpret_cast<const float2*>(scales + 2 * min(t, nf - 1)); };
+    auto stage_piece = [&](int t, int p) {
+      *reinterpret_cast<f16x8*>(dst + (t & 1) * dst_buf + 16 * p) = codes8h(w0[p], w1[p]);
+    };
+    float2 scale = float2{1.f, 1.f}, scale0 = scale;
+    u32x4 x0, x1;
+    if (nf) {
+      load_tile(off);
+      x0 = w0;
+      x1 = w1;
+      load_tile(0);
+      scale0 = load_scales(0);
+      scale = load_scales(1);
+    }
+    // ---- the lane's column: query qs, head qh
+    const int col = col0 + 32 * wave + c32, qs = col / G, qh = col - qs * G;
+    const bool ok = col < r.cols && qs < qlen;
+    const int lim = ok ? len - qlen + qs + 1 : 0x7fffffff;  // tokens it sees
+    f16x8 qf[8];  // B: step kb: dims 64 (kb / 4) + 32 hf + 4 (kb % 4) + i and 16 + that
+    {
+      const int64_t at = b * r.q_sb + static_cast<int64_t>(h * G + qh) * r.q_sh + qs * r.q_ss + 32 * hf;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) qf[k] = f16x8{};
+      if (ok) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const f16x8 x[4] = {load_q8<DT>(r.q, at + 64 * k), load_q8<DT>(r.q, at + 64 * k + 8),
+                              load_q8<DT>(r.q, at + 64 * k + 16), load_q8<DT>(r.q, at + 64 * k + 24)};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f16x8 lo = x[j >> 1], hi = x[2 + (j >> 1)];
+            qf[4 * k + j] = (j & 1) ? __builtin_shufflevector(lo, hi, 4, 5, 6, 7, 12, 13, 14, 15)
+                                    : __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 8, 9, 10, 11);
+          }
+        }
+      }
+    }
+    // tokens that every column of the wave sees
+    const int wq = __builtin_amdgcn_readfirstlane((col0 + 32 * wave) / G);
+    const int lim_min = wq < qlen ? len - qlen + wq + 1 : 0x7fffffff;
+
+    float m = ok ? -INFINITY : 0.f, l = 0.f;  // a column that is no row keeps offset 0 over zero scores
+    f32x16 o[4];  // dims 32 db + 8 (i / 4) + 4 hf + i % 4
+#pragma unroll
+    for (int db = 0; db < 4; ++db) o[db] = f32x16{};
+    f32x16 sc[2];  // scores of tokens 32 kt + 8 (i / 4) + 4 hf + i % 4
+    float s[32];   // log2 weights of the present tile, relative to m
+    u32x4 pf[4];   // its weights
+    constexpr int kAhead = 4;  // operands on their way from LDS
+    f16x8 fr[kAhead];
+    // operand i of the 16 score products (tile t's keys) and of the 16 value products
+    auto key_op = [&](int i, int t) {
+      return *reinterpret_cast<const f16x8*>(krow + (t & 1) * kKBuf + 32 * (i & 1) * kKRow + 16 * (i >> 1));
+    };
+    auto value_op = [&](int i, int t) {
+      return *reinterpret_cast<const f16x8*>(vrow + (t & 1) * kVBuf + 32 * (i & 3) * kVRow + 16 * (i >> 2));
+    };
+    // a tile's factors: key scale * scale * log2(e), log2(value scale), 1 / value scale
     float kc = r.scale_log2, lv = 0.f, iv = 1.f;
-    if (blk < nfull) {  // uniform
-      const float2 sc = *reinterpret_cast<const float2*>(st.scales + 2 * (bh * st.blocks + blk));
-      const float vs = fmaxf(sc.y, kMinScale);
-      kc *= sc.x;
+    auto factors = [&](const float2& x) {
+      const float vs = fmaxf(x.y, kMinScale);
+      kc = r.scale_log2 * x.x;
       lv = __log2f(vs);
       iv = __builtin_amdgcn_rcpf(vs);
-    }
-    f32x16 sc[2];  // token 32 kt + 8 (i / 4) + 4 hf + i % 4
+    };
+    auto score_products = [&](int t) {
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      sc[kt] = f32x16{};
-#pragma unroll
-      for (int kb = 0; kb < 8; ++kb)
-        sc[kt] = mfma32(*reinterpret_cast<const f16x8*>(k + 32 * kt * kKRow + 16 * kb), qf[kb], sc[kt]);
-    }
-    float s[32];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      s[e] = fmaf(sc[e >> 4][e & 15], kc, lv - m);
-      mx = fmaxf(mx, s[e]);
-    }
-    if (t0 + kBlk > lim_min || wave_ballot(mx > 0.f) != 0) {  // uniform
-      const int left = lim - t0 - 4 * hf;
-      mx = -INFINITY;
+      for (int i = 0; i < 16; ++i) sc[i & 1] = mfma32(key_op(i, t), qf[i >> 1], i < 2 ? f32x16{} : sc[i & 1]);
+    };
+    // masks and a new offset, where a column of the wave needs one
+    auto general = [&](int t) {
+      const int left = lim - (blk0 + t) * kBlk - 4 * hf;
+      float mx = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
         const float x = fmaf(sc[e >> 4][e & 15], kc, lv);
@@ -201,7 +196,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
         mx = fmaxf(mx, s[e]);
       }
       mx = half_max(mx);
-      const float mn = mx > m ? mx + kHeadroom : m;
+      const float mn = mx - m > kMaxWeight ? mx - kTopWeight : m;
       const float mu = mn == -INFINITY ? 0.f : mn;
       const float alpha = exp2_(m - mu);
       m = mn;
@@ -210,79 +205,132 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
       for (int db = 0; db < 4; ++db) o[db] = o[db] * alpha;
 #pragma unroll
       for (int e = 0; e < 32; ++e) s[e] -= mu;
-    }
-    float ps[2] = {0.f, 0.f};
-    f16x8 pf[4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      u32x4 u;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = exp2_(s[8 * ks + 2 * j]), c = exp2_(s[8 * ks + 2 * j + 1]);
-        ps[0] += a;
-        ps[1] += c;
-        u[j] = cvt2(a, c);
-      }
-      pf[ks] = __builtin_bit_cast(f16x8, u);
-    }
-    l = fmaf(ps[0] + ps[1], iv, l);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int db = 0; db < 4; ++db)
-        o[db] = mfma32(*reinterpret_cast<const f16x8*>(v + 32 * db * kVRow + 16 * ks), pf[ks], o[db]);
-  };
+    };
+    // weights 2 i, 2 i + 1 of the present tile, into the value operand
+    float ps[2];
+    auto weights = [&](int i) {
+      const float a = exp2_(s[2 * i]), c = exp2_(s[2 * i + 1]);
+      ps[0] += a;
+      ps[1] += c;
+      uint32_t u = pk2(a, c);
+      __asm__ volatile("" : "+v"(u));  // (no instruction: keeps the work beside the product that it stands next to)
+      pf[i >> 2][i & 3] = u;
+    };
 
-  const int n = max(blk1 - blk0, 0), npair = (n + 1) / 2;
-  auto next_pair = [&](int it) {
-    const int blk = blk0 + 2 * it;
+    // ---- tile 0 (and the keys of tile 1)
+    __syncthreads();  // the buffers are free
+    if (nf) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (blk + u < blk1) stage_tile(blk + u, u);
+      for (int p = 0; p < 4; ++p) stage_piece(0, p);
+      if (key_thr) {
+        w0 = x0;
+        w1 = x1;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) load_tile(blk + 2 + u, u);
-  };
-  if (npair) {
-    load_tile(blk0, 0);
-    load_tile(blk0 + 1, 1);
-    next_pair(0);
-  }
-  __syncthreads();
-#pragma unroll 1
-  for (int it = 0; it < npair; ++it) {
-    if (!key_thr && it + 1 < npair) next_pair(it + 1);
-#pragma unroll 1
-    for (int blk = blk0 + 2 * it; blk < min(blk0 + 2 * it + 2, blk1); ++blk) compute_tile(blk);
-    if (key_thr && it + 1 < npair) next_pair(it + 1);
+        for (int p = 0; p < 4; ++p) stage_piece(1, p);
+      }
+      load_tile(1 + off);
+      factors(scale0);
+    }
     __syncthreads();
-  }
-
-  if (col >= r.cols) return;
-  l = half_sum(l);
-  if (P.splits == 1) {
-    const bool some = ok && l != 0.f;
-    const float inv = some ? 1.f / l : 0.f;
-    const int64_t at = b * r.o_sb + static_cast<int64_t>(h * r.G + qh) * r.o_sh + qs * r.o_ss + 4 * hf;
+    if (nf) {
+      score_products(0);
+      general(0);
+    }
+    __syncthreads();  // (the keys of tile 0 are overwritten next)
+    // ---- A tile is two stretches of 16 products, each with vector work between them: the scores of tile t + 1 beside
+    // the weights of tile t, then the values of tile t beside the offsets of tile t + 1 and the staging of the next
+    // tiles.  Keys and values have two buffers: what a tile overwrites was last read in the tile before.  (Past the last
+    // tile the scores are of what lies in LDS, unused.)
+#pragma unroll 1
+    for (int t = 0; t < nf; ++t) {
+      ps[0] = ps[1] = 0.f;
 #pragma unroll
-    for (int db = 0; db < 4; ++db)
+      for (int i = 0; i < kAhead; ++i) fr[i] = key_op(i, t + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = some ? o[db][4 * k + i] * inv : 0.f;
-        store4<DT>(r.out, at + 32 * db + 8 * k, x[0], x[1], x[2], x[3]);
+      for (int i = 0; i < 16; ++i) {
+        sc[i & 1] = mfma32(fr[i % kAhead], qf[i >> 1], i < 2 ? f32x16{} : sc[i & 1]);
+        fr[i % kAhead] = i + kAhead < 16 ? key_op(i + kAhead, t + 1) : value_op(i + kAhead - 16, t);
+        weights(i);
+        __builtin_amdgcn_sched_barrier(0);
       }
-  } else {
-    const int64_t at = (bh * r.cols + col) * P.splits + split;
-    const bool some = ok && n > 0;
-    if (hf == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = some ? float2{m, l} : float2{-INFINITY, 0.f};
-    if (some) {
+      l = fmaf(ps[0] + ps[1], iv, l);
+      factors(scale);
+      const float base = lv - m;
+      float mx = -INFINITY;
 #pragma unroll
-      for (int db = 0; db < 4; ++db)
+      for (int i = 0; i < 16; ++i) {
+        o[i & 3] = mfma32(fr[i % kAhead], __builtin_bit_cast(f16x8, pf[i >> 2]), o[i & 3]);
+        if (i + kAhead < 16) fr[i % kAhead] = value_op(i + kAhead, t);
+        if ((i & 3) == 0) stage_piece(t + 1 + off, i >> 2);
+        s[2 * i] = fmaf(sc[i >> 3][2 * i & 15], kc, base);
+        s[2 * i + 1] = fmaf(sc[i >> 3][(2 * i + 1) & 15], kc, base);
+        mx = fmaxf(fmaxf(mx, s[2 * i]), s[2 * i + 1]);
+      }
+      load_tile(t + 2 + off);
+      scale = load_scales(t + 2);
+      if (t + 1 < nf && ((blk0 + t + 2) * kBlk > lim_min || wave_ballot(mx > kMaxWeight) != 0)) general(t + 1);  // uniform
+      __syncthreads();
+    }
+    // ---- the unfinished block: fp16 as it is
+    if (rest) {
+      if (key_thr) {
+        const uint16_t* p = st.k_tail + bh * kBlkBytes + src_off;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<f32x4*>(P.part_o + at * kD + 32 * db + 8 * k + 4 * hf) =
-              f32x4{o[db][4 * k], o[db][4 * k + 1], o[db][4 * k + 2], o[db][4 * k + 3]};
+        for (int k = 0; k < 4; ++k) {
+          const uint2 a = *reinterpret_cast<const uint2*>(p + 4 * k), c = *reinterpret_cast<const uint2*>(p + 16 + 4 * k);
+          *reinterpret_cast<u32x4*>(dst + 16 * k) = u32x4{a.x, a.y, c.x, c.y};
+        }
+      } else {
+        const uint16_t* p = st.v_tail + bh * kBlkBytes + src_off;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint2 a = *reinterpret_cast<const uint2*>(p + 4 * k), c = *reinterpret_cast<const uint2*>(p + 32 + 4 * k);
+          *reinterpret_cast<u32x4*>(dst + 16 * k) = u32x4{a.x, a.y, c.x, c.y};
+        }
+      }
+      __syncthreads();
+      score_products(0);
+      kc = r.scale_log2;
+      lv = 0.f;
+      general(nf);
+      ps[0] = ps[1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) weights(i);
+      l += ps[0] + ps[1];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i & 3] = mfma32(value_op(i, 0), __builtin_bit_cast(f16x8, pf[i >> 2]), o[i & 3]);
+    }
+
+    // ---- out
+    l = half_sum(l);
+    if (col < r.cols) {
+      if (P.splits == 1) {
+        const bool some = ok && l != 0.f;
+        const float inv = some ? 1.f / l : 0.f;
+        const int64_t at = b * r.o_sb + static_cast<int64_t>(h * G + qh) * r.o_sh + qs * r.o_ss + 4 * hf;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = some ? o[db][4 * k + i] * inv : 0.f;
+            store4<DT>(r.out, at + 32 * db + 8 * k, x[0], x[1], x[2], x[3]);
+          }
+      } else {
+        const int64_t at = (bh * r.cols + col) * P.splits + split;
+        const bool some = ok && blk1 > blk0;
+        if (hf == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = some ? float2{m, l} : float2{-INFINITY, 0.f};
+        if (some) {
+#pragma unroll
+          for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<f32x4*>(P.part_o + at * kD + 32 * db + 8 * k + 4 * hf) =
+                  f32x4{o[db][4 * k], o[db][4 * k + 1], o[db][4 * k + 2], o[db][4 * k + 3]};
+        }
+      }
     }
   }
 }
@@ -291,10 +339,12 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
 
 int launch_prefill(const Store& store, const Rows& r, const Plan& p, int dtype, int64_t B, float* part_o,
                    float* part_ml, hipStream_t stream) {
-  const PrefillArgs A{store, r, p.groups, p.chunk, p.splits, part_o, part_ml};
-  const int64_t wgs = B * store.Hkv * p.groups * p.splits;
-  LKV_REQUIRE(wgs < (1ll << 31), "kv8_attn: %lld workgroups", (long long)wgs);
-  const dim3 grid(static_cast<unsigned>(wgs));
+  const int64_t items = B * store.Hkv, total = items * p.groups * p.splits;
+  LKV_REQUIRE(total < (1ll << 30), "kv8_attn: %lld pieces of work", (long long)total);
+  const PrefillArgs A{store, r, p.groups, p.chunk, p.splits, static_cast<int>(items), static_cast<int>(total), part_o,
+                      part_ml};
+  const int64_t cus = device_cu_count();
+  const dim3 grid(static_cast<unsigned>(total < cus ? total : cus));
   if (dtype == LKV_DTYPE_F32)
     hipLaunchKernelGGL(prefill_kernel<LKV_DTYPE_F32>, grid, dim3(kThr), 0, stream, A);
   else if (dtype == LKV_DTYPE_F16)
