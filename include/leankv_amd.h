@@ -734,6 +734,14 @@ int lkv_kv8_select_blocks(const lkv_kv8_store* store, const void* q, const int64
                           const int32_t* lens, int64_t max_len, int64_t n, int64_t sink, int64_t recent,
                           int32_t* index, void* workspace, size_t workspace_bytes, void* stream);
 
+/* lkv_kv8_select_blocks, then lkv_kv8_attn of the same queries over the blocks
+ * it chose (left in index), in one workspace. */
+size_t lkv_kv8_sparse_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_len, int64_t n);
+int lkv_kv8_sparse_attn(const lkv_kv8_store* store, const void* q, const int64_t* q_strides, int dtype, int64_t Hq,
+                        const int32_t* lens, int64_t max_len, int64_t n, int64_t sink, int64_t recent, float scale,
+                        int32_t* index, void* out, const int64_t* out_strides, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -97,6 +97,9 @@ SIGNATURES = {
     "lkv_kv8_select_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "lkv_kv8_select_blocks": (_int, [_c_p, _c_p, _c_p, _int, _i64, _c_p, _i64, _i64, _i64, _i64, _c_p, _c_p, _sz,
                                      _c_p]),
+    "lkv_kv8_sparse_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "lkv_kv8_sparse_attn": (_int, [_c_p, _c_p, _c_p, _int, _i64, _c_p, _i64, _i64, _i64, _i64, _f32, _c_p, _c_p, _c_p,
+                                   _c_p, _sz, _c_p]),
     "lkv_decode_head": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p, _sz, _c_p]),
 }
 

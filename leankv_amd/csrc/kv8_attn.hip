@@ -34,7 +34,7 @@ int check_rows(const void* x, const int64_t* strides, int dtype, const char* wha
 namespace {
 
 constexpr int kThr = 256;
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;  // of a split workgroup
 constexpr int kManyCols = 256;  // columns of a workgroup of the many-row kernel
 constexpr int kManyChunk = 8;   // and the fewest blocks that a split of it gets
 
@@ -72,6 +72,18 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
   const Store& st = P.st;
   const Rows& r = P.r;
   const int b = blockIdx.z, h = blockIdx.y / P.groups, group = blockIdx.y - h * P.groups;
+  // the columns' query rows, asked for first (a column that is no row reads the last one)
+  const int col0 = group * 16 * NT;
+  RawQ<DT> qraw[NT][4];
+  int qs[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = min(col0 + 16 * n + c16, r.cols - 1);
+    qs[n] = col / r.G;
+    const int64_t at = b * r.q_sb + static_cast<int64_t>(h * r.G + col - qs[n] * r.G) * r.q_sh + qs[n] * r.q_ss + 16 * g;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) qraw[n][ks] = load_raw_q8<DT>(r.q, at + 64 * (ks >> 1) + 8 * (ks & 1));
+  }
   const int len = min(max(r.lens[b], 0), r.max_len);
   const int qlen = min(r.q_lens ? min(max(r.q_lens[b], 0), r.S) : r.S, len);
   const int nfull = len / kBlk, rest = len - nfull * kBlk;
@@ -80,7 +92,6 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
   const int nlist = P.index ? P.n_index : nfull;
   const int units = nlist + (rest ? 1 : 0);
   const int u0 = blockIdx.x * P.chunk;
-  const int col0 = group * 16 * NT;
   if (P.splits > 1 && u0 >= units) {  // nothing to do: an empty record
     const int col = col0 + tid;
     if (tid < 16 * NT && col < r.cols)
@@ -89,22 +100,58 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
   }
   const int u1 = min(u0 + P.chunk, units);
 
-  // ---- query rows: lane: column c16, dims 64 (ks / 2) + 16 g + 8 (ks % 2) + j
+  // ---- the wave's units u0 + wave, + kWaves, ...: lane i holds number i's block and factors, 64 at a time
+  const int* list = P.index ? P.index + bh * P.n_index : nullptr;
+  const uint8_t* kbase = st.k_codes + bh * st.blocks * kBlkBytes + c16 * kD + 16 * g;
+  const uint8_t* vbase = st.v_codes + bh * st.blocks * kBlkBytes + c16 * kBlk + 16 * g;
+  u32x4 kr[8], vr[8];
+  auto load_k = [&](int blk) {
+    const uint8_t* p = kbase + static_cast<int64_t>(blk) * kBlkBytes;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) kr[j] = *reinterpret_cast<const u32x4*>(p + (j >> 1) * 16 * kD + (j & 1) * 64);
+  };
+  auto load_v = [&](int blk) {
+    const uint8_t* p = vbase + static_cast<int64_t>(blk) * kBlkBytes;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vr[j] = *reinterpret_cast<const u32x4*>(p + j * 16 * kBlk);
+  };
+  const int uend = min(u0 + P.chunk, nlist);
+  int ub = u0 + wave, i = 0, blk = 0;
+  uint64_t todo = 0;  // lanes whose blocks are still to do (skipped entries lie anywhere in a list)
+  int blk_l;
+  float2 scale_l;
+  // the next 64 units that hold a block; its first one's loads are on their way afterwards
+  auto next_units = [&]() {
+    for (; ub < uend && !todo; ub += 64 * kWaves) {
+      const int mine = ub + kWaves * lane;
+      blk_l = -1;
+      if (mine < uend) {
+        blk_l = list ? list[mine] : mine;
+        if (blk_l >= nfull) blk_l = -1;  // (no such block)
+      }
+      scale_l = float2{0.f, 0.f};
+      if (blk_l >= 0) scale_l = *reinterpret_cast<const float2*>(st.scales + 2 * (bh * st.blocks + blk_l));
+      todo = wave_ballot(blk_l >= 0);
+    }
+    if (todo) {
+      i = __builtin_ctzll(todo);
+      blk = lane_i(blk_l, i);
+      load_k(blk);
+      load_v(blk);
+    }
+  };
+  next_units();
+
+  // ---- the queries' rows: lane: column c16, dims 64 (ks / 2) + 16 g + 8 (ks % 2) + j
   f16x8 qf[NT][4];
   int lim[NT];  // tokens that the lane's column sees (all, if there is no such row)
   float m[NT], l[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int col = col0 + 16 * n + c16, s = col / r.G, hq = col - s * r.G;
-    const bool ok = col < r.cols && s < qlen;
+    const bool ok = col0 + 16 * n + c16 < r.cols && qs[n] < qlen;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      qf[n][ks] = f16x8{};
-      if (ok)
-        qf[n][ks] = load_q8<DT>(r.q, b * r.q_sb + static_cast<int64_t>(h * r.G + hq) * r.q_sh + s * r.q_ss +
-                                         64 * (ks >> 1) + 16 * g + 8 * (ks & 1));
-    }
-    lim[n] = ok ? len - qlen + s + 1 : 0x7fffffff;
+    for (int ks = 0; ks < 4; ++ks) qf[n][ks] = ok ? convert_q8<DT>(qraw[n][ks]) : f16x8{};
+    lim[n] = ok ? len - qlen + qs[n] + 1 : 0x7fffffff;
     m[n] = ok ? -INFINITY : 0.f;  // a column that is no row keeps offset 0 over zero scores
     l[n] = 0.f;
   }
@@ -185,43 +232,9 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
       }
   };
 
-  // ---- the wave's units u0 + wave, + kWaves, ...: lane i holds number i's block and scales, 64 at a time
-  const int* list = P.index ? P.index + bh * P.n_index : nullptr;
-  const uint8_t* kbase = st.k_codes + bh * st.blocks * kBlkBytes + c16 * kD + 16 * g;
-  const uint8_t* vbase = st.v_codes + bh * st.blocks * kBlkBytes + c16 * kBlk + 16 * g;
-  u32x4 kr[8], vr[8];
-  auto load_k = [&](int blk) {
-    const uint8_t* p = kbase + static_cast<int64_t>(blk) * kBlkBytes;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) kr[j] = *reinterpret_cast<const u32x4*>(p + (j >> 1) * 16 * kD + (j & 1) * 64);
-  };
-  auto load_v = [&](int blk) {
-    const uint8_t* p = vbase + static_cast<int64_t>(blk) * kBlkBytes;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) vr[j] = *reinterpret_cast<const u32x4*>(p + j * 16 * kBlk);
-  };
-  const int uend = min(u1, nlist);
-  for (int ub = u0 + wave; ub < uend; ub += 64 * kWaves) {
-    const int mine = ub + kWaves * lane;
-    int blk_l = -1;
-    if (mine < uend) {
-      blk_l = list ? list[mine] : mine;
-      if (blk_l >= nfull) blk_l = -1;  // (no such block: skipped)
-    }
-    float ks_l = 0.f, vs_l = kMinScale;
-    if (blk_l >= 0) {
-      const float2 sc = *reinterpret_cast<const float2*>(st.scales + 2 * (bh * st.blocks + blk_l));
-      ks_l = sc.x;
-      vs_l = fmaxf(sc.y, kMinScale);
-    }
-    const float kc_l = ks_l * r.scale_log2, lv_l = __log2f(vs_l), iv_l = 1.f / vs_l;
-    // skipped entries lie anywhere in a list: only those lanes that hold a block are walked
-    uint64_t todo = wave_ballot(blk_l >= 0);
-    if (!todo) continue;
-    int i = __builtin_ctzll(todo);
-    int blk = lane_i(blk_l, i);
-    load_k(blk);
-    load_v(blk);
+  while (todo) {
+    const float vs_l = fmaxf(scale_l.y, kMinScale);
+    const float kc_l = scale_l.x * r.scale_log2, lv_l = __log2f(vs_l), iv_l = 1.f / vs_l;
     while (true) {
       todo &= todo - 1;
       const float kc = lane_f(kc_l, i), lv = lane_f(lv_l, i), iv = lane_f(iv_l, i);
@@ -234,6 +247,7 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
       if (!more) break;
       load_v(blk);
     }
+    next_units();
   }
   // ---- the unfinished block, by the wave whose turn it is
   if (rest && u1 == units && (nlist - u0) % kWaves == wave) {
@@ -265,36 +279,39 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
 #pragma unroll
     for (int jt = 0; jt < 8; ++jt) *reinterpret_cast<f32x4*>(&s_o[wave][c16][16 * jt + 4 * g]) = o[n][jt];
     __syncthreads();
-    const int row = tid >> 4, d = 4 * (tid & 15);
+    // a row by kThr / 16 lanes, 4 dims each at a time
+    constexpr int kLanes = kThr / 16, kPieces = kD / 4 / kLanes;
+    const int row = tid / kLanes, d = 4 * (tid % kLanes);
     const int col = col0 + 16 * n + row;
     if (col < r.cols) {
       float M = s_m[0][16 * n + row];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][16 * n + row]);
       const float mu = M == -INFINITY ? 0.f : M;
-      f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      f32x4 acc[kPieces];
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
       float L = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float a = exp2_(s_m[w][16 * n + row] - mu);
         L += a * s_l[w][16 * n + row];
-        acc[0] += a * *reinterpret_cast<const f32x4*>(&s_o[w][row][d]);
-        acc[1] += a * *reinterpret_cast<const f32x4*>(&s_o[w][row][64 + d]);
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) acc[k] += a * *reinterpret_cast<const f32x4*>(&s_o[w][row][4 * kLanes * k + d]);
       }
       const bool row_ok = col / r.G < qlen;
-      if (P.splits == 1) {
-        const bool some = row_ok && L != 0.f;  // no such row, or no token: zeros
-        const float inv = some ? 1.f / L : 0.f;
-        if (!some) acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-        store_row<DT>(r, b, h, col, d, acc[0] * inv);
-        store_row<DT>(r, b, h, col, 64 + d, acc[1] * inv);
-      } else {
-        const int64_t at = ((bh * r.cols + col) * P.splits + blockIdx.x);
-        *reinterpret_cast<f32x4*>(P.part_o + at * kD + d) = acc[0];
-        *reinterpret_cast<f32x4*>(P.part_o + at * kD + 64 + d) = acc[1];
-        if ((tid & 15) == 0)
-          *reinterpret_cast<float2*>(P.part_ml + 2 * at) = row_ok ? float2{M, L} : float2{-INFINITY, 0.f};
+      const bool some = row_ok && L != 0.f;  // no such row, or no token: zeros
+      const float inv = some ? 1.f / L : 0.f;
+      const int64_t at = ((bh * r.cols + col) * P.splits + blockIdx.x);
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k) {
+        if (P.splits == 1)
+          store_row<DT>(r, b, h, col, 4 * kLanes * k + d, some ? acc[k] * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+        else
+          *reinterpret_cast<f32x4*>(P.part_o + at * kD + 4 * kLanes * k + d) = acc[k];
       }
+      if (P.splits > 1 && tid % kLanes == 0)
+        *reinterpret_cast<float2*>(P.part_ml + 2 * at) = row_ok ? float2{M, L} : float2{-INFINITY, 0.f};
     }
   }
 }
@@ -303,57 +320,86 @@ struct CombineArgs {
   Rows r;
   const float* part_o;
   const float* part_ml;
+  int64_t rows;
   int Hkv, splits;
 };
 
-// One workgroup per row: 8 groups of 32 lanes, each every 8th split, 4 dims a lane.  A split without a token for the row
-// has offset -inf (and wrote no sums).
-template <int DT>
+// A row by PARTS groups of 32 lanes, each every PARTS-th split, 4 dims a lane; a workgroup has 8 / PARTS rows.  A split
+// without a token for the row has offset -inf (and wrote no sums).  Bound by latency for few rows (8 groups: every load of
+// up to 64 splits is asked for before the first is used), by memory for many.
+template <int DT, int PARTS>
 __global__ __launch_bounds__(kThr) void combine_kernel(CombineArgs P) {
-  __shared__ __align__(16) float s_o[8][kD];
-  __shared__ float s_l[8];
+  __shared__ __align__(16) float s_o[PARTS][kD];
+  __shared__ float s_ml[PARTS][2];
   const Rows& r = P.r;
-  const int tid = threadIdx.x, d = 4 * (tid & 31), part = tid >> 5;
-  const int64_t row = blockIdx.x;  // ((sequence, kv head), column)
+  const int tid = threadIdx.x, d = 4 * (tid & 31), part = (tid >> 5) % PARTS;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (8 / PARTS) + (tid >> 5) / PARTS;  // ((sequence, kv head), column)
+  if (row >= P.rows) return;  // (PARTS 8: never)
   const int n = P.splits;
   const float* ml = P.part_ml + row * n * 2;
   const float* po = P.part_o + row * n * kD + d;
-  float M = -INFINITY;
-  for (int i = tid & 63; i < n; i += 64) M = fmaxf(M, ml[2 * i]);  // every wave for itself
-  M = wave_max(M);
-  const float mu = M == -INFINITY ? 0.f : M;
+  float M = -INFINITY, L = 0.f;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-#pragma unroll 4
-  for (int i = part; i < n; i += 8) {
-    const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
-    const f32x4 v = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * kD);
-    if (x.x != -INFINITY) {
-      const float a = exp2_(x.x - mu);
-      L += a * x.y;
-      acc += a * v;
-    }
-  }
-  *reinterpret_cast<f32x4*>(&s_o[part][d]) = acc;
-  if ((tid & 31) == 0) s_l[part] = L;
-  __syncthreads();
-  if (part == 0) {
+  for (int i0 = part; i0 < n; i0 += 8 * PARTS) {
+    float2 x[8];
+    f32x4 v[8];
 #pragma unroll
-    for (int p = 1; p < 8; ++p) {
-      acc += *reinterpret_cast<const f32x4*>(&s_o[p][d]);
-      L += s_l[p];
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + k * PARTS;
+      x[k] = float2{-INFINITY, 0.f};
+      if (i < n) {
+        x[k] = *reinterpret_cast<const float2*>(ml + 2 * i);
+        v[k] = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * kD);
+      }
     }
-    const float inv = L != 0.f ? 1.f / L : 0.f;
-    if (L == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int64_t bh = row / r.cols;
-    store_row<DT>(r, static_cast<int>(bh / P.Hkv), static_cast<int>(bh % P.Hkv), static_cast<int>(row - bh * r.cols), d,
-                  acc * inv);
+    float mx = M;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mx = fmaxf(mx, x[k].x);
+    if (mx == -INFINITY) continue;
+    const float a = exp2_(M - mx);
+    M = mx;
+    L *= a;
+    acc *= a;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (x[k].x != -INFINITY) {
+        const float w = exp2_(x[k].x - M);
+        L = fmaf(w, x[k].y, L);
+        acc += w * v[k];
+      }
   }
+  if constexpr (PARTS > 1) {
+    *reinterpret_cast<f32x4*>(&s_o[part][d]) = acc;
+    if ((tid & 31) == 0) {
+      s_ml[part][0] = M;
+      s_ml[part][1] = L;
+    }
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) M = fmaxf(M, s_ml[p][0]);
+    L = 0.f;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+      if (s_ml[p][0] != -INFINITY) {
+        const float w = exp2_(s_ml[p][0] - M);
+        L = fmaf(w, s_ml[p][1], L);
+        acc += w * *reinterpret_cast<const f32x4*>(&s_o[p][d]);
+      }
+  }
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  if (L == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t bh = row / r.cols;
+  store_row<DT>(r, static_cast<int>(bh / P.Hkv), static_cast<int>(bh % P.Hkv), static_cast<int>(row - bh * r.cols), d,
+                acc * inv);
 }
 
 // --------------------------------------------------------------------------------------------------- block selection
-constexpr int kSelThr = 256;
-constexpr int kLdsKeys = 8192;  // so many keys of a (sequence, kv head) stay in LDS, more are read again from memory
+constexpr int kSelThr = 512;
+constexpr int kSelWaves = kSelThr / 64;
+constexpr int kLdsKeys = 8192;     // so many keys of a (sequence, kv head) stay in LDS, more are read again from memory
+constexpr int kFusedBlocks = 512;  // up to so many blocks one workgroup scores and selects (2048: 36.6 us a call, apart 23.5)
 
 struct SelectArgs {
   Store st;
@@ -361,9 +407,9 @@ struct SelectArgs {
   int64_t q_sb, q_sh;
   const int* lens;
   int G, n, sink, recent;
-  int max_blocks;   // the grid's bound on finished blocks
-  uint32_t* keys;   // [B][Hkv][max_blocks]
-  int* index;       // [B][Hkv][n]
+  int max_len, max_blocks;  // bounds on the length and on the finished blocks
+  uint32_t* keys;           // [B][Hkv][max_blocks], or null: scored by the selecting workgroup
+  int* index;               // [B][Hkv][n]
 };
 
 // Order-preserving bits of a score (-0 made +0 before); larger is larger.
@@ -372,159 +418,322 @@ __device__ __forceinline__ uint32_t sort_bits(float f) {
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// Scores of 16 blocks per wave and step; a lane has column c16 = query head, k slots 16 g + j of a 64-dim step.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// 16 of a kv head's queries in 8 bits: min(q8, 0) and max(q8, 0) of every dim, and their scales.
+// By 512 threads: thread: query h0 + tid / 32, dims 4 (tid % 32) ..; into LDS, from where a wave reads its operands.
+struct QueryCodes {
+  uint32_t code[16][2][kD / 4];  // min(q8, 0), max(q8, 0)
+  float scale[16];
+};
 template <int DT>
-__global__ __launch_bounds__(kThr) void score_kernel(SelectArgs P) {
-  typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void query_codes(const float (&x)[4], bool ok, QueryCodes& s, int tid) {
+  float y[4], amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    y[j] = ok ? clamp_kv(x[j]) : 0.f;
+    if constexpr (DT != LKV_DTYPE_F16) y[j] = h2f(f2h(y[j]));
+    amax = fmaxf(amax, fabsf(y[j]));
+  }
+  amax = row16_max(amax);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(amax), __float_as_uint(amax), false, false);
+  amax = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const float inv = code_factor(amax);
+  uint32_t un[4], up[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // rint by 1.5 * 2^23: the sum's low byte is the code
+    const float t = y[j] * inv;
+    un[j] = __float_as_uint(fminf(t, 0.f) + 12582912.f);
+    up[j] = __float_as_uint(fmaxf(t, 0.f) + 12582912.f);
+  }
+  auto bytes = [](const uint32_t (&u)[4]) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u),
+                                 __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), 0x05040100u);
+  };
+  const int hh = (tid >> 5) & 15, d4 = tid & 31;
+  s.code[hh][0][d4] = bytes(un);
+  s.code[hh][1][d4] = bytes(up);
+  if (d4 == 0) s.scale[hh] = amax * kStep;
+}
+template <int DT>
+__device__ __forceinline__ void load_query4(const SelectArgs& P, int b, int h, int h0, int tid, float (&x)[4]) {
+  const int64_t at = b * P.q_sb + static_cast<int64_t>(h * P.G + min(h0 + ((tid >> 5) & 15), P.G - 1)) * P.q_sh + 4 * (tid & 31);
+  if constexpr (DT == LKV_DTYPE_F32) {
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(P.q) + at);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(P.q) + at);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = j < 2 ? v.x : v.y, u = (j & 1) ? w >> 16 : w & 0xffffu;
+      x[j] = DT == LKV_DTYPE_F16 ? h2f(static_cast<uint16_t>(u)) : bf2f(u);
+    }
+  }
+}
+// Operands: column c16 = query, k slots = 16 bytes at dim 64 ks + 16 g.
+__device__ __forceinline__ void query_operands(const QueryCodes& s, int c16, int g, i32x4 (&neg)[2], i32x4 (&pos)[2],
+                                               float& qs) {
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    neg[ks] = *reinterpret_cast<const i32x4*>(&s.code[c16][0][16 * ks + 4 * g]);
+    pos[ks] = *reinterpret_cast<const i32x4*>(&s.code[c16][1][16 * ks + 4 * g]);
+  }
+  qs = s.scale[c16];
+}
+
+// The lane's block row of a 16-block group: lowest codes, then highest ones.
+__device__ __forceinline__ void load_ranges(const int8_t* p, i32x4 (&a)[4]) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) a[ks] = *reinterpret_cast<const i32x4*>(p + 64 * ks);
+}
+
+// Largest scaled product of the 16 columns with blocks 4 g + i of the group: the lane with c16 = i % 4 gets block i's.
+__device__ __forceinline__ float group_best(const i32x4 (&a)[4], const i32x4 (&neg)[2], const i32x4 (&pos)[2], float qs,
+                                            bool ok, int c16) {
+  i32x4 d = i32x4{0, 0, 0, 0};
+  d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[0], neg[0], d, 0, 0, 0);
+  d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[1], neg[1], d, 0, 0, 0);
+  d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[2], pos[0], d, 0, 0, 0);
+  d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[3], pos[1], d, 0, 0, 0);
+  float best[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) best[i] = row16_max(ok ? static_cast<float>(d[i]) * qs : -INFINITY);
+  return (c16 & 2) ? ((c16 & 1) ? best[3] : best[2]) : ((c16 & 1) ? best[1] : best[0]);
+}
+
+// Keys of 16 blocks per wave, for contexts whose scores are worth more than one workgroup per (sequence, kv head).
+template <int DT>
+__global__ __launch_bounds__(kSelThr) void score_kernel(SelectArgs P) {
+  __shared__ __align__(16) QueryCodes s_q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const int h = blockIdx.y, b = blockIdx.z;
   const Store& st = P.st;
-  const int len = min(max(P.lens[b], 0), st.blocks * kBlk);
-  const int nfull = min(len / kBlk, P.max_blocks);
+  float x[4];
+  load_query4<DT>(P, b, h, 0, tid, x);
+  const int nfull = min(max(P.lens[b], 0), P.max_len) / kBlk;
   const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
-  const int step = gridDim.x * kWaves * 16;
-  for (int j0 = (blockIdx.x * kWaves + wave) * 16; j0 < nfull; j0 += step) {
-    const int jr = min(j0 + c16, nfull - 1);
-    i32x4 a[4];
-    const int8_t* p = st.ranges + (bh * st.blocks + jr) * 2 * kD + 16 * g;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) a[ks] = *reinterpret_cast<const i32x4*>(p + 64 * ks);
-    float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    for (int h0 = 0; h0 < P.G; h0 += 16) {
-      // the column's query in 8 bits: dims 16 g .. + 15 and 64 + 16 g .. + 15
-      const bool ok = h0 + c16 < P.G;
-      float x[4][8];
-      float amax = 0.f;
-      const int64_t at = b * P.q_sb + static_cast<int64_t>(h * P.G + (ok ? h0 + c16 : 0)) * P.q_sh + 16 * g;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        load8<DT>(P.q, at + 64 * (k >> 1) + 8 * (k & 1), x[k]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[k][j] = h2f(f2h(clamp_kv(x[k][j])));
-          amax = fmaxf(amax, fabsf(x[k][j]));
-        }
-      }
-      amax = groups_max(amax);
-      const float inv = code_factor(amax), qs = amax * kStep;
-      i32x4 neg[2], pos[2];
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        uint32_t un = 0, up = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int q8 = static_cast<int>(rintf(x[w >> 1][4 * (w & 1) + j] * inv));
-          un |= (static_cast<uint32_t>(min(q8, 0)) & 0xffu) << (8 * j);
-          up |= (static_cast<uint32_t>(max(q8, 0)) & 0xffu) << (8 * j);
-        }
-        neg[w >> 2][w & 3] = static_cast<int>(un);
-        pos[w >> 2][w & 3] = static_cast<int>(up);
-      }
-      i32x4 d = i32x4{0, 0, 0, 0};
-      d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[0], neg[0], d, 0, 0, 0);
-      d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[1], neg[1], d, 0, 0, 0);
-      d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[2], pos[0], d, 0, 0, 0);
-      d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[3], pos[1], d, 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) best[i] = fmaxf(best[i], row16_max(ok ? static_cast<float>(d[i]) * qs : -INFINITY));
+  const int j0 = (blockIdx.x * kSelWaves + wave) * 16;
+  if (static_cast<int>(blockIdx.x) * kSelWaves * 16 >= nfull) return;  // (the whole workgroup)
+  i32x4 a[4];
+  load_ranges(st.ranges + (bh * st.blocks + min(j0 + c16, nfull - 1)) * 2 * kD + 16 * g, a);
+  const int j = j0 + 4 * g + (c16 & 3);
+  const float ks = st.scales[2 * (bh * st.blocks + min(j, nfull - 1))];
+  float best = -INFINITY;
+  for (int h0 = 0; h0 < P.G; h0 += 16) {
+    if (h0) {
+      load_query4<DT>(P, b, h, h0, tid, x);
+      __syncthreads();
     }
-    // rows (blocks) j0 + 4 g + i; lane c16 = i writes it
-    const float mine = c16 == 0 ? best[0] : c16 == 1 ? best[1] : c16 == 2 ? best[2] : best[3];
-    const int j = j0 + 4 * g + c16;
-    if (c16 < 4 && j < nfull) {
-      uint32_t key = sort_bits(mine * st.scales[2 * (bh * st.blocks + j)]);
-      if (j < P.sink || j >= nfull - P.recent) key = 0xffffffffu;
-      P.keys[bh * P.max_blocks + j] = key;
-    }
+    query_codes<DT>(x, h0 + (tid >> 5) < P.G, s_q, tid);
+    __syncthreads();
+    i32x4 neg[2], pos[2];
+    float qs;
+    query_operands(s_q, c16, g, neg, pos, qs);
+    best = fmaxf(best, group_best(a, neg, pos, qs, h0 + c16 < P.G, c16));
   }
+  if (c16 < 4 && j < nfull) P.keys[bh * P.max_blocks + j] = sort_bits(best * ks);
+}
+
+// Over the wave: or, and, and the sum of the lanes up to this one (DPP, no LDS round trips).
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_or(uint32_t v) {
+  v |= dpp_u<0xB1>(v);
+  v |= dpp_u<0x4E>(v);
+  v |= dpp_u<0x141>(v);
+  v |= dpp_u<0x140>(v);
+  return static_cast<uint32_t>(lane_i(v, 0) | lane_i(v, 16) | lane_i(v, 32) | lane_i(v, 48));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += dpp_u<0x111>(v);  // row_shr:1, 2, 4, 8 (lanes shifted in from outside a row add 0)
+  v += dpp_u<0x112>(v);
+  v += dpp_u<0x114>(v);
+  v += dpp_u<0x118>(v);
+  const uint32_t r0 = lane_i(v, 15), r1 = lane_i(v, 31), r2 = lane_i(v, 47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return v + (row > 0 ? r0 : 0u) + (row > 1 ? r1 : 0u) + (row > 2 ? r2 : 0u);
 }
 
 // The n highest keys of a (sequence, kv head), equal ones by index, as ascending indices; the rest of the row is -1.
+// With P.keys null the workgroup computes them itself (every wave 16 blocks at a time, into LDS).  Bound by latency: one
+// barrier a radix pass (a histogram each, every wave finds the bin by itself).
+template <int DT>
 __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
   __shared__ uint32_t s_key[kLdsKeys];
-  __shared__ uint32_t s_hist[256];
-  __shared__ uint32_t s_pick[2];
-  __shared__ int s_cnt[2][kSelThr / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __align__(16) uint32_t s_hist[4][256];
+  __shared__ uint32_t s_or[kSelWaves], s_nor[kSelWaves];
+  __shared__ int s_cnt[2][2][kSelWaves];
+  __shared__ __align__(16) QueryCodes s_q;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = blockIdx.x, b = blockIdx.y;
   const Store& st = P.st;
-  const int len = min(max(P.lens[b], 0), st.blocks * kBlk);
-  const int nfull = min(len / kBlk, P.max_blocks);
+  float x[4];
+  if (!P.keys) load_query4<DT>(P, b, h, 0, tid, x);  // (beside the length)
+  const int nfull = min(max(P.lens[b], 0), P.max_len) / kBlk;
   const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
   int* out = P.index + bh * P.n;
   if (nfull <= P.n) {  // all of them
     for (int j = tid; j < P.n; j += kSelThr) out[j] = j < nfull ? j : -1;
     return;
   }
-  const uint32_t* keys = P.keys + bh * P.max_blocks;
+  for (int i = tid; i < 4 * 256; i += kSelThr) s_hist[0][i] = 0;
+  if (!P.keys) {
+    const int c16 = lane & 15, g = lane >> 4;
+    const int8_t* ranges = st.ranges + bh * st.blocks * 2 * kD + 16 * g;
+    const float* scales = st.scales + 2 * bh * st.blocks;
+    constexpr int kUn = 4;
+    i32x4 a[kUn][4];
+    float ks[kUn];
+    auto load_groups = [&](int j0) {
+#pragma unroll
+      for (int u = 0; u < kUn; ++u) {
+        const int jg = j0 + 16 * kSelWaves * u;
+        load_ranges(ranges + static_cast<int64_t>(min(jg + c16, nfull - 1)) * 2 * kD, a[u]);
+        ks[u] = scales[2 * min(jg + 4 * g + (c16 & 3), nfull - 1)];
+      }
+    };
+    load_groups(16 * wave);  // (on their way beside the queries' codes)
+    for (int h0 = 0; h0 < P.G; h0 += 16) {
+      if (h0) {
+        load_query4<DT>(P, b, h, h0, tid, x);
+        __syncthreads();
+      }
+      query_codes<DT>(x, h0 + (tid >> 5) < P.G, s_q, tid);
+      __syncthreads();
+      i32x4 neg[2], pos[2];
+      float qs;
+      query_operands(s_q, c16, g, neg, pos, qs);
+      const bool ok = h0 + c16 < P.G, end = h0 + 16 >= P.G;
+      for (int j0 = 16 * wave; j0 < nfull;) {
+        const int now = j0;
+        float best[kUn], kn[kUn];
+#pragma unroll
+        for (int u = 0; u < kUn; ++u) {
+          best[u] = group_best(a[u], neg, pos, qs, ok, c16);
+          kn[u] = ks[u];
+        }
+        j0 += 16 * kSelWaves * kUn;
+        if (j0 < nfull || !end) load_groups(j0 < nfull ? j0 : 16 * wave);
+#pragma unroll
+        for (int u = 0; u < kUn; ++u) {
+          const int j = now + 16 * kSelWaves * u + 4 * g + (c16 & 3);
+          if (c16 < 4 && j < nfull) {  // (a lane writes and reads back its own)
+            if (h0) best[u] = fmaxf(best[u], __uint_as_float(s_key[j]));
+            s_key[j] = end ? sort_bits(best[u] * kn[u]) : __float_as_uint(best[u]);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();  // (keys and cleared histograms)
+  const uint32_t* keys = P.keys ? P.keys + bh * P.max_blocks : nullptr;
   const bool in_lds = nfull <= kLdsKeys;
-  if (in_lds)
+  if (keys && in_lds)
     for (int j = tid; j < nfull; j += kSelThr) s_key[j] = keys[j];  // (a thread reads back its own)
   auto key_at = [&](int j) { return in_lds ? s_key[j] : keys[j]; };
-  // radix selection from the top byte down: the key of rank n is (prefix, low bits)
-  uint32_t prefix = 0;
-  int need = P.n;  // rank within the keys that share the prefix
-#pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    s_hist[tid] = 0;
-    __syncthreads();
-    const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int j = tid; j < nfull; j += kSelThr) {
-      const uint32_t k = key_at(j);
-      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+  constexpr int kReg = 4;  // keys of a thread in registers: j = tid + kSelThr i
+  const bool in_reg = nfull <= kReg * kSelThr;
+  uint32_t kr[kReg];
+#pragma unroll
+  for (int i = 0; i < kReg; ++i) kr[i] = in_reg && tid + kSelThr * i < nfull ? s_key[tid + kSelThr * i] : 0u;
+  // the first `sink` and the last `recent` blocks are in anyway: the others compete for the remaining places
+  const int lo = min(P.sink, nfull), hi = max(nfull - P.recent, lo);  // [lo, hi) compete
+  int need = P.n - (nfull - (hi - lo));
+  // f(key) for the thread's keys that compete
+  auto each_key = [&](auto f) {
+    if (in_reg) {
+#pragma unroll
+      for (int i = 0; i < kReg; ++i)
+        if (tid + kSelThr * i >= lo && tid + kSelThr * i < hi) f(kr[i]);
+    } else {
+      for (int j = tid; j < hi; j += kSelThr)
+        if (j >= lo) f(key_at(j));
     }
-    __syncthreads();
-    if (wave == 0) {
-      // lane: bins 4 lane .. + 3; counts above them
-      uint32_t c[4], sum = 0;
+  };
+  // bits in which the competing keys differ
+  uint32_t any = 0, none = 0;  // set in some key, clear in some key
+  each_key([&](uint32_t k) {
+    any |= k;
+    none |= ~k;
+  });
+  any = wave_or(any);
+  none = wave_or(none);
+  if (lane == 0) {
+    s_or[wave] = any;
+    s_nor[wave] = none;
+  }
+  __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = s_hist[4 * lane + i], sum += c[i];
-      uint32_t above = sum;  // inclusive sum from lane on, then exclusive
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t t = __shfl_down(above, off);
-        if (lane + off < 64) above += t;
-      }
-      above -= sum;
+  for (int w = 0; w < kSelWaves; ++w) {
+    any |= s_or[w];
+    none |= s_nor[w];
+  }
+  any = __builtin_amdgcn_readfirstlane(any);
+  const uint32_t diff = __builtin_amdgcn_readfirstlane(any & none);
+  // radix selection from the highest of them down, 8 bits a pass (scores lie close: from the top of the word the first
+  // pass would put nearly every key into one bin): the key of rank `need` is (prefix, lower bits)
+  uint32_t prefix = need > 0 ? any : 0xffffffffu;  // (no place left: no key is above it)
+  int top = diff ? 31 - __builtin_clz(diff) : -1;
+  if (top >= 0 && need > 0) {
+    prefix = top == 31 ? 0u : any & (0xffffffffu << (top + 1));
+#pragma unroll 1
+    for (int pass = 0; top >= 0; top -= 8, ++pass) {
+      const int shift = max(top - 7, 0);
+      const uint32_t mask = top == 31 ? 0u : 0xffffffffu << (top + 1), digit = (1u << (top - shift + 1)) - 1u;
+      each_key([&](uint32_t k) {
+        if ((k & mask) == prefix) atomicAdd(&s_hist[pass][(k >> shift) & digit], 1u);
+      });
+      __syncthreads();
+      // lane: bins 4 lane .. + 3, and the counts above them
+      const u32x4 c = *reinterpret_cast<const u32x4*>(&s_hist[pass][4 * lane]);
+      const uint32_t sum = c[0] + c[1] + c[2] + c[3], upto = wave_scan(sum);
+      uint32_t above = static_cast<uint32_t>(lane_i(static_cast<int>(upto), 63)) - upto;
+      uint32_t bin = 0, over = 0;
+      bool here = false;
 #pragma unroll
       for (int i = 3; i >= 0; --i) {
         if (above < static_cast<uint32_t>(need) && above + c[i] >= static_cast<uint32_t>(need)) {
-          s_pick[0] = 4 * lane + i;
-          s_pick[1] = above;
+          here = true;
+          bin = 4 * lane + i;
+          over = above;
         }
         above += c[i];
       }
+      const int who = __builtin_ctzll(wave_ballot(here));  // (one lane)
+      prefix |= static_cast<uint32_t>(lane_i(static_cast<int>(bin), who)) << shift;
+      need -= lane_i(static_cast<int>(over), who);
     }
-    __syncthreads();
-    prefix |= s_pick[0] << shift;
-    need -= static_cast<int>(s_pick[1]);
   }
-  // keys above `prefix` and the first `need` equal to it, in index order
+  // the first and last blocks, the keys above `prefix` and the first `need` equal to it, in index order
   int base_gt = 0, base_eq = 0;
-  for (int j0 = 0; j0 < nfull; j0 += kSelThr) {
+  for (int j0 = 0, it = 0; j0 < nfull; j0 += kSelThr, it ^= 1) {
     const int j = j0 + tid;
-    const uint32_t k = j < nfull ? key_at(j) : 0u;
-    const bool gt = j < nfull && k > prefix, eq = j < nfull && k == prefix;
+    const bool in = j >= lo && j < hi;
+    const uint32_t k = in ? key_at(j) : 0u;
+    const bool gt = j < nfull && (!in || k > prefix), eq = in && k == prefix;
     const uint64_t mg = wave_ballot(gt), me = wave_ballot(eq);
     if (lane == 0) {
-      s_cnt[0][wave] = __popcll(mg);
-      s_cnt[1][wave] = __popcll(me);
+      s_cnt[it][0][wave] = __popcll(mg);
+      s_cnt[it][1][wave] = __popcll(me);
     }
-    __syncthreads();
+    __syncthreads();  // (two sets of counts in turn: one barrier a round)
     int gt_before = base_gt + lane_prefix(mg), eq_before = base_eq + lane_prefix(me);
 #pragma unroll
-    for (int w = 0; w < kSelThr / 64; ++w) {
+    for (int w = 0; w < kSelWaves; ++w) {
+      const int cg = s_cnt[it][0][w], ce = s_cnt[it][1][w];
       if (w < wave) {
-        gt_before += s_cnt[0][w];
-        eq_before += s_cnt[1][w];
+        gt_before += cg;
+        eq_before += ce;
       }
-      base_gt += s_cnt[0][w];
-      base_eq += s_cnt[1][w];
+      base_gt += cg;
+      base_eq += ce;
     }
     if (gt || (eq && eq_before < need)) out[gt_before + min(eq_before, need)] = j;
-    __syncthreads();
   }
 }
 
@@ -538,8 +747,9 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t cols, int64_t units) {
   const int64_t wide = p.nt ? 16 * p.nt : kManyCols;
   p.groups = static_cast<int>((cols + wide - 1) / wide);
   const int64_t items = B * Hkv * p.groups;
-  // workgroups resident at once: two of the few-row kernel on a CU, one of the other
-  int64_t want = ((p.nt ? 2 : 1) * cus + items - 1) / items;
+  // One workgroup a CU; two of the few-row kernel fit and would be no faster (32 sequences of up to 8192 tokens 68.7 us
+  // with one, 72.2 with two a CU, 1 x 131072 tokens 53.7 and 56.7: more splits are more rows to join).
+  const int64_t want = (cus + items - 1) / items;
   int64_t chunk = (units + want - 1) / want;
   const int64_t unit = p.nt ? kWaves : 2;  // a block for every wave, or a pair of blocks
   chunk = (chunk + unit - 1) / unit * unit;
@@ -562,6 +772,15 @@ void launch_split(const SplitArgs& P, int nt, int64_t B, hipStream_t st) {
     hipLaunchKernelGGL((split_kernel<DT, 1>), grid, dim3(kThr), 0, st, P);
   else
     hipLaunchKernelGGL((split_kernel<DT, 2>), grid, dim3(kThr), 0, st, P);
+}
+
+template <int DT>
+void launch_combine(const CombineArgs& C, hipStream_t st) {
+  // 8 rows a workgroup where that still gives every CU work
+  if (C.rows >= 16ll * device_cu_count())
+    hipLaunchKernelGGL((combine_kernel<DT, 1>), dim3(static_cast<unsigned>((C.rows + 7) / 8)), dim3(kThr), 0, st, C);
+  else
+    hipLaunchKernelGGL((combine_kernel<DT, 8>), dim3(static_cast<unsigned>(C.rows)), dim3(kThr), 0, st, C);
 }
 
 int64_t units_of(int64_t max_len, int64_t n_index) {
@@ -644,23 +863,41 @@ extern "C" int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int
     LKV_LAUNCH_CHECK("kv8_attn split");
   }
   if (p.splits > 1) {
-    const CombineArgs C{r, part_o, part_ml, static_cast<int>(Hkv), p.splits};
-    const dim3 grid(static_cast<unsigned>(B * Hkv * cols));
+    const int64_t rows = B * Hkv * cols;
+    const CombineArgs C{r, part_o, part_ml, rows, static_cast<int>(Hkv), p.splits};
     if (dtype == LKV_DTYPE_F32)
-      hipLaunchKernelGGL(combine_kernel<LKV_DTYPE_F32>, grid, dim3(kThr), 0, st, C);
+      launch_combine<LKV_DTYPE_F32>(C, st);
     else if (dtype == LKV_DTYPE_F16)
-      hipLaunchKernelGGL(combine_kernel<LKV_DTYPE_F16>, grid, dim3(kThr), 0, st, C);
+      launch_combine<LKV_DTYPE_F16>(C, st);
     else
-      hipLaunchKernelGGL(combine_kernel<LKV_DTYPE_BF16>, grid, dim3(kThr), 0, st, C);
+      launch_combine<LKV_DTYPE_BF16>(C, st);
     LKV_LAUNCH_CHECK("kv8_attn combine");
   }
   return LKV_OK;
 }
 
 extern "C" size_t lkv_kv8_select_workspace_bytes(int64_t B, int64_t Hkv, int64_t max_len) {
-  if (B <= 0 || Hkv <= 0 || max_len < 0) return 0;
+  if (B <= 0 || Hkv <= 0 || max_len < 0 || max_len / kBlk <= kFusedBlocks) return 0;
   return static_cast<size_t>(B * Hkv * (max_len / kBlk)) * sizeof(uint32_t);
 }
+
+namespace {
+
+template <int DT>
+int launch_select(SelectArgs& P, int64_t B, hipStream_t st) {
+  const unsigned Hkv = static_cast<unsigned>(P.st.Hkv);
+  if (P.max_blocks > P.n && P.keys) {
+    const int per = 16 * kSelWaves;
+    hipLaunchKernelGGL(score_kernel<DT>, dim3(static_cast<unsigned>((P.max_blocks + per - 1) / per), Hkv,
+                                              static_cast<unsigned>(B)), dim3(kSelThr), 0, st, P);
+    LKV_LAUNCH_CHECK("kv8_select_blocks score");
+  }
+  hipLaunchKernelGGL(select_kernel<DT>, dim3(Hkv, static_cast<unsigned>(B)), dim3(kSelThr), 0, st, P);
+  LKV_LAUNCH_CHECK("kv8_select_blocks");
+  return LKV_OK;
+}
+
+}  // namespace
 
 extern "C" int lkv_kv8_select_blocks(const lkv_kv8_store* store, const void* q, const int64_t* q_strides, int dtype,
                                      int64_t Hq, const int32_t* lens, int64_t max_len, int64_t n, int64_t sink,
@@ -669,10 +906,9 @@ extern "C" int lkv_kv8_select_blocks(const lkv_kv8_store* store, const void* q, 
   if (int rc = check_attn(store, Hq, 1, max_len, "kv8_select_blocks")) return rc;
   LKV_REQUIRE(dtype == LKV_DTYPE_F32 || dtype == LKV_DTYPE_F16 || dtype == LKV_DTYPE_BF16,
               "kv8_select_blocks: dtype %d", dtype);
-  LKV_REQUIRE(n >= 1 && n < (1ll << 24) && sink >= 0 && recent >= 0 && sink + recent <= n,
+  LKV_REQUIRE(n >= 1 && n < (1ll << 24) && sink >= 0 && recent >= 0 && sink <= n && recent <= n - sink,
               "kv8_select_blocks: %lld blocks with the first %lld and the last %lld among them", (long long)n,
               (long long)sink, (long long)recent);
-  const int64_t mb = max_len / kBlk;
   const int64_t B = store->batch, Hkv = store->kv_heads;
   if (B == 0) return LKV_OK;
   LKV_REQUIRE(q && lens && index, "kv8_select_blocks: null pointer");
@@ -690,23 +926,37 @@ extern "C" int lkv_kv8_select_blocks(const lkv_kv8_store* store, const void* q, 
   P.n = static_cast<int>(n);
   P.sink = static_cast<int>(sink);
   P.recent = static_cast<int>(recent);
-  P.max_blocks = static_cast<int>(mb);
-  P.keys = static_cast<uint32_t*>(workspace);
+  P.max_len = static_cast<int>(max_len);
+  P.max_blocks = static_cast<int>(max_len / kBlk);
+  P.keys = need ? static_cast<uint32_t*>(workspace) : nullptr;
   P.index = index;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (mb > n) {  // otherwise every block is chosen
-    const int64_t tiles = (mb + 16 * kWaves - 1) / (16 * kWaves);
-    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(Hkv), static_cast<unsigned>(B));
-    if (dtype == LKV_DTYPE_F32)
-      hipLaunchKernelGGL(score_kernel<LKV_DTYPE_F32>, grid, dim3(kThr), 0, st, P);
-    else if (dtype == LKV_DTYPE_F16)
-      hipLaunchKernelGGL(score_kernel<LKV_DTYPE_F16>, grid, dim3(kThr), 0, st, P);
-    else
-      hipLaunchKernelGGL(score_kernel<LKV_DTYPE_BF16>, grid, dim3(kThr), 0, st, P);
-    LKV_LAUNCH_CHECK("kv8_select_blocks score");
-  }
-  hipLaunchKernelGGL(select_kernel, dim3(static_cast<unsigned>(Hkv), static_cast<unsigned>(B)), dim3(kSelThr), 0,
-                     st, P);
-  LKV_LAUNCH_CHECK("kv8_select_blocks");
-  return LKV_OK;
+  return dtype == LKV_DTYPE_F32   ? launch_select<LKV_DTYPE_F32>(P, B, st)
+         : dtype == LKV_DTYPE_F16 ? launch_select<LKV_DTYPE_F16>(P, B, st)
+                                  : launch_select<LKV_DTYPE_BF16>(P, B, st);
+}
+
+extern "C" size_t lkv_kv8_sparse_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_len, int64_t n) {
+  const size_t a = lkv_kv8_select_workspace_bytes(B, Hkv, max_len);
+  const size_t c = lkv_kv8_attn_workspace_bytes(B, Hq, Hkv, 1, max_len, n);
+  return a > c ? a : c;
+}
+
+extern "C" int lkv_kv8_sparse_attn(const lkv_kv8_store* store, const void* q, const int64_t* q_strides, int dtype,
+                                   int64_t Hq, const int32_t* lens, int64_t max_len, int64_t n, int64_t sink,
+                                   int64_t recent, float scale, int32_t* index, void* out, const int64_t* out_strides,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  // (the scores are done with before the attention writes its partial sums: one workspace)
+  if (int rc = check_attn(store, Hq, 1, max_len, "kv8_sparse_attn")) return rc;
+  LKV_REQUIRE(store->batch == 0 || out, "kv8_sparse_attn: null pointer");
+  if (store->batch)
+    if (int rc = check_rows(out, out_strides, dtype, "kv8_sparse_attn", "out")) return rc;
+  const size_t need = lkv_kv8_sparse_attn_workspace_bytes(store->batch, Hq, store->kv_heads, max_len, n);
+  LKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
+              "kv8_sparse_attn: workspace of %zu bytes (16-byte aligned) required, got %zu", need, workspace_bytes);
+  if (int rc = lkv_kv8_select_blocks(store, q, q_strides, dtype, Hq, lens, max_len, n, sink, recent, index, workspace,
+                                     workspace_bytes, stream))
+    return rc;
+  return lkv_kv8_attn(store, q, q_strides, dtype, Hq, 1, lens, nullptr, max_len, index, n, scale, out, out_strides,
+                      workspace, workspace_bytes, stream);
 }

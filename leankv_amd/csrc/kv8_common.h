@@ -107,20 +107,36 @@ __device__ __forceinline__ uint32_t clamp_q2(uint32_t u) {
   const u16x2 t = (x & u16x2{0x7fff, 0x7fff}) - u16x2{0x7c00, 0x7c00};
   return __builtin_bit_cast(uint32_t, static_cast<u16x2>(x + (__builtin_elementwise_min(t, one) - one)));
 }
+// Eight elements of a query row as they lie in memory, and as fp16.
 template <int DT>
-__device__ __forceinline__ f16x8 load_q8(const void* base, int64_t at) {
+struct RawQ {
+  u32x4 u[DT == LKV_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ RawQ<DT> load_raw_q8(const void* base, int64_t at) {
+  RawQ<DT> r;
+  const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const char*>(base) + at * (DT == LKV_DTYPE_F32 ? 4 : 2));
+#pragma unroll
+  for (int k = 0; k < (DT == LKV_DTYPE_F32 ? 2 : 1); ++k) r.u[k] = p[k];
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ f16x8 convert_q8(const RawQ<DT>& q) {
   u32x4 r;
-  if constexpr (DT == LKV_DTYPE_F16) {
-    r = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + at);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = clamp_q2(r[j]);
-  } else {
-    float x[8];
-    load8<DT>(base, at, x);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = pk2(clamp_q(x[2 * j]), clamp_q(x[2 * j + 1]));
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (DT == LKV_DTYPE_F16)
+      r[j] = clamp_q2(q.u[0][j]);
+    else if constexpr (DT == LKV_DTYPE_BF16)
+      r[j] = pk2(clamp_q(bf2f(q.u[0][j] & 0xffffu)), clamp_q(bf2f(q.u[0][j] >> 16)));
+    else
+      r[j] = pk2(clamp_q(__uint_as_float(q.u[j >> 1][2 * (j & 1)])), clamp_q(__uint_as_float(q.u[j >> 1][2 * (j & 1) + 1])));
   }
   return __builtin_bit_cast(f16x8, r);
+}
+template <int DT>
+__device__ __forceinline__ f16x8 load_q8(const void* base, int64_t at) {
+  return convert_q8<DT>(load_raw_q8<DT>(base, at));
 }
 
 // Four consecutive outputs of type DT at element offset `at` (a multiple of 4; the row is 16-byte aligned).

@@ -39,6 +39,16 @@ def _attn_bytes(batch: int, heads: int, kv_heads: int, S: int, max_len: int, n_i
     return _lib.load().lkv_kv8_attn_workspace_bytes(batch, heads, kv_heads, S, max_len, n_index)
 
 
+@functools.lru_cache(maxsize=256)
+def _select_bytes(batch: int, kv_heads: int, max_len: int) -> int:
+    return _lib.load().lkv_kv8_select_workspace_bytes(batch, kv_heads, max_len)
+
+
+@functools.lru_cache(maxsize=256)
+def _sparse_bytes(batch: int, heads: int, kv_heads: int, max_len: int, blocks: int) -> int:
+    return _lib.load().lkv_kv8_sparse_attn_workspace_bytes(batch, heads, kv_heads, max_len, blocks)
+
+
 def _dtype(t: torch.Tensor, what: str) -> int:
     code = _DTYPES.get(t.dtype)
     if code is None:
@@ -203,31 +213,38 @@ class KV8Store:
         return k, v
 
     # ---------------------------------------------------------------------------------------------- attention
-    def _decode(self, q, heads, dtype, p, L, index, n, scale, out):
-        """One query a sequence; out [batch, heads, 128] with dense, aligned rows."""
-        q, qs = _query_rows(q)
-        os = _strides3(out.stride(0), out.stride(1), 0)
-        nbytes = _attn_bytes(self.batch, heads, self.kv_heads, 1, L, n)
-        ws = self._empty(nbytes, torch.uint8) if nbytes else None
-        self._call("lkv_kv8_attn", q.data_ptr(), qs, dtype, heads, 1, p, None, L, index, n,
-                   _SCALE if scale is None else scale, out.data_ptr(), os, None if ws is None else ws.data_ptr(), nbytes)
-        return out
-
     def decode_attention(self, q: torch.Tensor, lens: torch.Tensor, max_len: int | None = None,
-                         scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                         scale: float | None = None, out: torch.Tensor | None = None,
+                         index: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of one query per sequence and head, q [batch, heads, 128], over everything stored (its own token
         among it): [batch, heads, 128] in q's type.  A sequence of length 0 gives zeros.  max_len: the caller's bound on
-        lens (default the capacity), which the work is split for.  scale: 1 / sqrt(128) by default."""
+        lens (default the capacity), which the work is split for.  scale: 1 / sqrt(128) by default.  index: int32
+        [batch, kv_heads, n], only these finished blocks of a kv head (as select_blocks gives them; others than finished
+        ones are skipped) and the unfinished one."""
         what = "KV8Store.decode_attention"
         heads, dtype = self._queries(q, 3, what)
         p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
+        n, list_ = 0, None
+        if index is not None:
+            if index.dtype is not torch.int32 or index.dim() != 3 or index.shape[0] != self.batch \
+                    or index.shape[1] != self.kv_heads or not index.shape[2] or index.device != self.device \
+                    or not index.is_contiguous():
+                raise LeanKVError("%s: index must be a contiguous int32 tensor [%d, %d, n] on %s"
+                                  % (what, self.batch, self.kv_heads, self.device))
+            n, list_ = index.shape[2], index.data_ptr()
         if out is None:
             out = self._empty((self.batch, heads, HEAD_DIM), q.dtype)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device \
                 or _in_place((self.batch, heads, 1), (*out.stride()[:2], 0, out.stride(2)), out) is None:
             raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
                               % (what, q.dtype, tuple(q.shape), q.device))
-        return self._decode(q, heads, dtype, p, L, None, 0, scale, out)
+        q, qs = _query_rows(q)
+        os = _strides3(out.stride(0), out.stride(1), 0)
+        nbytes = _attn_bytes(self.batch, heads, self.kv_heads, 1, L, n)
+        ws = self._empty(nbytes, torch.uint8) if nbytes else None
+        self._call("lkv_kv8_attn", q.data_ptr(), qs, dtype, heads, 1, p, None, L, list_, n,
+                   _SCALE if scale is None else scale, out.data_ptr(), os, None if ws is None else ws.data_ptr(), nbytes)
+        return out
 
     def prefill_attention(self, q: torch.Tensor, lens: torch.Tensor, q_lens: torch.Tensor | None = None,
                           max_len: int | None = None, scale: float | None = None,
@@ -254,17 +271,11 @@ class KV8Store:
         return out
 
     # ------------------------------------------------------------------------------------------------- sparse
-    def _select(self, q, heads, dtype, p, L, blocks, sink, recent, what):
+    def _choice(self, blocks, sink, recent, what):
         blocks, sink, recent = int(blocks), int(sink), int(recent)
         if blocks < 1 or sink < 0 or recent < 0 or sink + recent > blocks:
             raise LeanKVError("%s: %d blocks with the first %d and the last %d among them" % (what, blocks, sink, recent))
-        q, qs = _query_rows(q)
-        index = self._empty((self.batch, self.kv_heads, blocks), torch.int32)
-        nbytes = self.batch * self.kv_heads * (L // BLOCK) * 4
-        ws = self._empty(nbytes, torch.uint8)
-        self._call("lkv_kv8_select_blocks", q.data_ptr(), qs, dtype, heads, p, L, blocks, sink, recent,
-                   index.data_ptr(), ws.data_ptr(), nbytes)
-        return index
+        return blocks, sink, recent
 
     def select_blocks(self, q: torch.Tensor, lens: torch.Tensor, blocks: int, sink: int = 1, recent: int = 1,
                       max_len: int | None = None) -> torch.Tensor:
@@ -274,7 +285,14 @@ class KV8Store:
         what = "KV8Store.select_blocks"
         heads, dtype = self._queries(q, 3, what)
         p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
-        return self._select(q, heads, dtype, p, L, blocks, sink, recent, what)
+        blocks, sink, recent = self._choice(blocks, sink, recent, what)
+        q, qs = _query_rows(q)
+        index = self._empty((self.batch, self.kv_heads, blocks), torch.int32)
+        nbytes = _select_bytes(self.batch, self.kv_heads, L)
+        ws = self._empty(nbytes, torch.uint8) if nbytes else None
+        self._call("lkv_kv8_select_blocks", q.data_ptr(), qs, dtype, heads, p, L, blocks, sink, recent,
+                   index.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
+        return index
 
     def sparse_decode_attention(self, q: torch.Tensor, lens: torch.Tensor, blocks: int, sink: int = 1, recent: int = 1,
                                 max_len: int | None = None, scale: float | None = None):
@@ -283,6 +301,13 @@ class KV8Store:
         what = "KV8Store.sparse_decode_attention"
         heads, dtype = self._queries(q, 3, what)
         p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
-        index = self._select(q, heads, dtype, p, L, blocks, sink, recent, what)
+        blocks, sink, recent = self._choice(blocks, sink, recent, what)
+        q, qs = _query_rows(q)
+        index = self._empty((self.batch, self.kv_heads, blocks), torch.int32)
         out = self._empty((self.batch, heads, HEAD_DIM), q.dtype)
-        return self._decode(q, heads, dtype, p, L, index.data_ptr(), index.shape[2], scale, out), index
+        nbytes = _sparse_bytes(self.batch, heads, self.kv_heads, L, blocks)
+        ws = self._empty(nbytes, torch.uint8) if nbytes else None
+        self._call("lkv_kv8_sparse_attn", q.data_ptr(), qs, dtype, heads, p, L, blocks, sink, recent,
+                   _SCALE if scale is None else scale, index.data_ptr(), out.data_ptr(),
+                   _strides3(heads * HEAD_DIM, HEAD_DIM, 0), None if ws is None else ws.data_ptr(), nbytes)
+        return out, index

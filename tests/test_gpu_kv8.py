@@ -337,6 +337,35 @@ def test_all_blocks_equal_dense(cuda):
     assert (out.float() - dense.float()).abs().max() <= 2.0 ** -9 * dense.float().abs().max()
 
 
+def test_given_blocks(cuda):
+    """Attention over a list of blocks of the caller's: any order, entries that are no finished block skipped."""
+    n = 64 * 20 + 11
+    k, v = _kv(cuda, 2, 2, n, seed=12)
+    lens = [n, 64 * 6]
+    store = _store(2, 2, n, device=cuda)
+    store.update(k, v, _ints(cuda, [0, 0]), _ints(cuda, lens))
+    q = torch.randn(2, 6, D, generator=torch.Generator().manual_seed(2)).half().to(cuda)
+    lists = [[[3, -1, 19, 0, 20, 7], [5, 4, 3, 2, 1, 1 << 30]], [[-1] * 6, [5, 6, -7, 0, 19, 2]]]
+    index = torch.tensor(lists, dtype=torch.int32, device=cuda)
+    out = store.decode_attention(q, _ints(cuda, lens), index=index)
+    tokens = [[[64 * j + i for j in lists[b][h] if 0 <= j < lens[b] // 64 for i in range(64)]
+               + list(range(lens[b] // 64 * 64, lens[b])) for h in range(2)] for b in range(2)]
+    _check_attn(out.unsqueeze(2), _refs(k, v, lens), q.unsqueeze(2), lens, None, tokens=tokens)
+
+
+@pytest.mark.parametrize("sink,recent,blocks", [(3, 4, 7), (0, 0, 1), (5, 0, 5), (0, 6, 6), (2, 2, 60)])
+def test_select_forced_blocks(cuda, sink, recent, blocks):
+    """No place left for the others, no forced block, as many places as blocks."""
+    nb = 60
+    k, v = _kv(cuda, 1, 1, 64 * nb, seed=5)
+    store = _store(1, 1, 64 * nb, device=cuda)
+    store.update(k, v, _ints(cuda, [0]))
+    q = torch.randn(1, 3, D, generator=torch.Generator().manual_seed(2)).half().to(cuda)
+    index = store.select_blocks(q, _ints(cuda, [64 * nb]), blocks, sink, recent)
+    want = choose(_refs(k, v, [64 * nb])[0][0], query(q[0].cpu()), blocks, sink, recent)
+    assert index[0, 0].tolist() == want
+
+
 def test_other_stream_and_graph(cuda):
     """A decode step (update, both attentions) captured once and replayed at other lengths, with eager work between, each
     replay against the eager result; the same on a second stream."""
@@ -427,6 +456,8 @@ def test_refusals(cuda):
         lambda: store.decode_attention(q, lens, out=torch.empty(2, 4, D, device=cuda)),
         lambda: store.decode_attention(q, lens, out=torch.empty(2, 4, 2 * D, device=cuda, dtype=F16)[..., ::2]),
         lambda: store.prefill_attention(q, lens), lambda: store.prefill_attention(q.unsqueeze(2), lens, lens[:1]),
+        lambda: store.decode_attention(q, lens, index=torch.zeros(2, 2, 1, device=cuda)),
+        lambda: store.decode_attention(q, lens, index=torch.zeros(2, 2, 0, device=cuda, dtype=torch.int32)),
         lambda: store.select_blocks(q, lens, 0), lambda: store.select_blocks(q, lens, 2, 2, 1),
         lambda: store.select_blocks(q, lens, 2, -1, 1), lambda: store.sparse_decode_attention(q, lens, 1),
     ]
