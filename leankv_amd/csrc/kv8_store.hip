@@ -37,10 +37,48 @@ struct UpdateArgs {
   int S;
 };
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t umax2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ float half_lo(uint32_t u) { return static_cast<float>(__builtin_bit_cast(f16x2, u)[0]); }
+__device__ __forceinline__ float half_hi(uint32_t u) { return static_cast<float>(__builtin_bit_cast(f16x2, u)[1]); }
+
+// Eight numbers as stored, in fp16 pairs.  A row holds an infinity, a NaN or a number past fp16 now and then only: the
+// largest magnitude (as bits, two at a time) tells, and only then is every number looked at.
+template <int DT>
+__device__ __forceinline__ u32x4 load_kv8(const void* base, int64_t at) {
+  if constexpr (DT == LKV_DTYPE_F32) {
+    float x[8];
+    load8<DT>(base, at, x);
+    u32x4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = pk2(clamp_kv(x[2 * j]), clamp_kv(x[2 * j + 1]));
+    return r;
+  } else {
+    u32x4 u = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + at);
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    const uint32_t m = umax2(umax2(u[0] & kAbs, u[1] & kAbs), umax2(u[2] & kAbs, u[3] & kAbs));
+    constexpr uint32_t kFirst = DT == LKV_DTYPE_F16 ? 0x7c00u : 0x4780u;  // infinity; 65536 in bf16
+    const bool special = max(m & 0xffffu, m >> 16) >= kFirst;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a, b;
+      if constexpr (DT == LKV_DTYPE_F16)
+        a = half_lo(u[j]), b = half_hi(u[j]);
+      else
+        a = bf2f(u[j] & 0xffffu), b = __uint_as_float(u[j] & 0xffff0000u);
+      if (special) a = clamp_kv(a), b = clamp_kv(b);
+      if (DT != LKV_DTYPE_F16 || special) u[j] = pk2(a, b);
+    }
+    return u;
+  }
+}
+
 // thread: dims 8 c .. 8 c + 7 of tokens 4 a .. 4 a + 3 of the block
 template <int DT>
 __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
-  __shared__ float s_max[4];
+  __shared__ uint32_t s_max[4];
   __shared__ uint32_t s_rng[4][2][64];
   __shared__ uint32_t s_v[kD * kVRow];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -51,10 +89,8 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
   // the sequence's tokens [p0, p1); a position outside the store stores nothing, tokens past it are dropped
   const int64_t cap = static_cast<int64_t>(st.blocks) * kBlk;
   const int64_t p0 = P.pos[b];
-  if (p0 < 0 || p0 >= cap) return;
-  int64_t n = P.n_new ? P.n_new[b] : P.S;
-  n = min(n, static_cast<int64_t>(P.S));
-  if (n <= 0) return;
+  const int64_t n = min(static_cast<int64_t>(P.n_new ? P.n_new[b] : P.S), static_cast<int64_t>(P.S));
+  if (p0 < 0 || p0 >= cap || n <= 0) return;
   const int64_t p1 = min(p0 + n, cap);
   const int64_t blk = p0 / kBlk + blockIdx.x;
   const int64_t t0 = blk * kBlk;  // first token of this block
@@ -65,83 +101,88 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
 
   const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
   const void* x = P.x[which];
-  const int64_t xrow = b * P.sb[which] + h * P.sh[which];
+  const int64_t xrow = b * P.sb[which] + h * P.sh[which] + 8 * c;
   uint16_t* tail = (which ? st.v_tail : st.k_tail) + bh * kBlkBytes;
 
   if (done) {
-    float v[4][8];
+    u32x4 v[4];  // token 4 a + i: fp16 pairs of its 8 dims
     // tokens from the old tail: those before p0 (none but in the first block)
     const int old = first ? static_cast<int>(p0 - t0) : 0;
-    uint2 vt[8];
-    if (which && 4 * a < old) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) vt[j] = *reinterpret_cast<const uint2*>(tail + (8 * c + j) * kBlk + 4 * v_dword(a));
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 4 * a + i;
-      if (t >= old) {
-        load8<DT>(x, xrow + (t0 + t - p0) * P.ss[which] + 8 * c, v[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = h2f(f2h(clamp_kv(v[i][j])));
-      } else if (!which) {
-        load8<LKV_DTYPE_F16>(tail, t * kD + 8 * c, v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t w = i < 2 ? vt[j].x : vt[j].y;
-          v[i][j] = h2f(static_cast<uint16_t>((i & 1) ? w >> 16 : w & 0xffffu));
-        }
-      }
+      if (t >= old)
+        v[i] = load_kv8<DT>(x, xrow + (t0 + t - p0) * P.ss[which]);
+      else if (!which)
+        v[i] = *reinterpret_cast<const u32x4*>(tail + t * kD + 8 * c);
     }
-    float m = 0.f;
+    if (which && 4 * a < old) {
+      uint2 vt[8];  // four tokens of a dim
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vt[j] = *reinterpret_cast<const uint2*>(tail + (8 * c + j) * kBlk + 4 * v_dword(a));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * a + i < old) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = i < 2 ? vt[2 * j].x : vt[2 * j].y, hi = i < 2 ? vt[2 * j + 1].x : vt[2 * j + 1].y;
+            v[i][j] = __builtin_amdgcn_perm(hi, lo, (i & 1) ? 0x07060302u : 0x05040100u);
+          }
+        }
+    }
+    // the largest magnitude, as bits (all are finite)
+    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[i][j]));
-    m = wave_max(m);
-    if (lane == 0) s_max[wave] = m;
+      for (int j = 0; j < 4; ++j) m = umax2(m, v[i][j] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    const uint32_t wm = __float_as_uint(wave_max(h2f(static_cast<uint16_t>(m))));
+    if (lane == 0) s_max[wave] = wm;
     __syncthreads();
-    const float amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const float amax = fmaxf(fmaxf(__uint_as_float(s_max[0]), __uint_as_float(s_max[1])),
+                             fmaxf(__uint_as_float(s_max[2]), __uint_as_float(s_max[3])));
     const float inv = code_factor(amax);
-    // codes, rounded to nearest even; |x * inv| <= 127 (1 + 2^-23) rounds to 127 at most
-    int code[4][8];
+    // codes in units: the product rounded, then rounded to a whole number by adding 1.5 * 2^23 (+ 128): the sum's low
+    // byte is code + 128; |x * inv| <= 127 (1 + 2^-22) rounds to 127 at most
+    constexpr float kMagic = 12582912.f + 128.f;
+    float t[4][8];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) code[i][j] = static_cast<int>(rintf(v[i][j] * inv));
+      for (int j = 0; j < 4; ++j) {
+        t[i][2 * j] = fmaf(half_lo(v[i][j]), inv, 0.f);
+        t[i][2 * j + 1] = fmaf(half_hi(v[i][j]), inv, 0.f);
+      }
+    auto bytes = [](float a0, float a1, float a2, float a3) {
+      const uint32_t u0 = __float_as_uint(a0 + kMagic), u1 = __float_as_uint(a1 + kMagic),
+                     u2 = __float_as_uint(a2 + kMagic), u3 = __float_as_uint(a3 + kMagic);
+      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(u3, u2, 0x0c0c0400u), __builtin_amdgcn_perm(u1, u0, 0x0c0c0400u),
+                                   0x05040100u);
+    };
     const int64_t at = bh * st.blocks + blk;
     if (tid == 0) st.scales[2 * at + which] = amax * kStep;
     if (!which) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          w[k] = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[k] |= static_cast<uint32_t>(code[i][4 * k + j] + 128) << (8 * j);
-        }
-        *reinterpret_cast<uint2*>(st.k_codes + at * kBlkBytes + (4 * a + i) * kD + 8 * c) = uint2{w[0], w[1]};
-      }
-      // lowest and highest code of every dim: over the thread's 4 tokens, the wave's 16, the block's 64 (the highest as
-      // the negated lowest of the negated codes)
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint2*>(st.k_codes + at * kBlkBytes + (4 * a + i) * kD + 8 * c) =
+            uint2{bytes(t[i][0], t[i][1], t[i][2], t[i][3]), bytes(t[i][4], t[i][5], t[i][6], t[i][7])};
+      // lowest and highest code of every dim, two dims in a dword: over the thread's 4 tokens, the wave's 16, the block's
+      // 64 (the highest as the negated lowest of the negated codes)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        auto lowest = [&](int sign) {
-          int l[2];
+        uint32_t lo[2], hi[2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            l[k] = sign * code[0][2 * j + k];
-#pragma unroll
-            for (int i = 1; i < 4; ++i) l[k] = min(l[k], sign * code[i][2 * j + k]);
-          }
-          return xg_min((static_cast<uint32_t>(l[0]) & 0xffffu) | (static_cast<uint32_t>(l[1]) << 16));
-        };
-        const uint32_t lo = lowest(1), hi = lowest(-1);
+        for (int k = 0; k < 2; ++k) {
+          const int d = 2 * j + k;
+          lo[k] = __float_as_uint(fminf(fminf(t[0][d], t[1][d]), fminf(t[2][d], t[3][d])) + 12582912.f);
+          hi[k] = __float_as_uint(12582912.f - fmaxf(fmaxf(t[0][d], t[1][d]), fmaxf(t[2][d], t[3][d])));
+        }
+        const uint32_t l2 = xg_min(__builtin_amdgcn_perm(lo[1], lo[0], 0x05040100u));
+        const uint32_t h2 = xg_min(__builtin_amdgcn_perm(hi[1], hi[0], 0x05040100u));
         if (lane < 16) {
-          s_rng[wave][0][4 * c + j] = lo;
-          s_rng[wave][1][4 * c + j] = hi;
+          s_rng[wave][0][4 * c + j] = l2;
+          s_rng[wave][1][4 * c + j] = h2;
         }
       }
       __syncthreads();
@@ -161,12 +202,7 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w |= static_cast<uint32_t>(code[i][j] + 128) << (8 * i);
-        s_v[(8 * c + j) * kVRow + v_dword(a)] = w;
-      }
+      for (int j = 0; j < 8; ++j) s_v[(8 * c + j) * kVRow + v_dword(a)] = bytes(t[0][j], t[1][j], t[2][j], t[3][j]);
       __syncthreads();
       // two 16-byte pieces a thread
 #pragma unroll
@@ -186,16 +222,15 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
     const int slot = 4 * a + i;
     const int64_t t = tt + slot;
     if (t < p0 || t >= p1) continue;
-    float y[8];
-    load8<DT>(x, xrow + (t - p0) * P.ss[which] + 8 * c, y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = clamp_kv(y[j]);
+    const u32x4 y = load_kv8<DT>(x, xrow + (t - p0) * P.ss[which]);
     if (!which) {
-      *reinterpret_cast<u32x4*>(tail + slot * kD + 8 * c) =
-          u32x4{pk2(y[0], y[1]), pk2(y[2], y[3]), pk2(y[4], y[5]), pk2(y[6], y[7])};
+      *reinterpret_cast<u32x4*>(tail + slot * kD + 8 * c) = y;
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) tail[(8 * c + j) * kBlk + v_pos(slot)] = f2h(y[j]);
+      for (int j = 0; j < 4; ++j) {
+        tail[(8 * c + 2 * j) * kBlk + v_pos(slot)] = static_cast<uint16_t>(y[j] & 0xffffu);
+        tail[(8 * c + 2 * j + 1) * kBlk + v_pos(slot)] = static_cast<uint16_t>(y[j] >> 16);
+      }
     }
   }
 }
@@ -228,16 +263,16 @@ __global__ __launch_bounds__(kThr) void read_kernel(ReadArgs P) {
     for (int j = 0; j < 4; ++j) w[i][j] = 0;
   if (done) {
     const float scale = st.scales[2 * at + which];
-    auto val = [&](uint32_t byte) { return static_cast<float>(static_cast<int>(byte) - 128) * scale; };
+    // fp16(code * scale), the product in fp32
+    auto vals = [&](uint32_t codes) {
+      return pk2(fmaf(half_lo(codes), scale, 0.f), fmaf(half_hi(codes), scale, 0.f));
+    };
     if (!which) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint2 u = *reinterpret_cast<const uint2*>(st.k_codes + at * kBlkBytes + (4 * a + i) * kD + 8 * c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t x = (j < 2 ? u.x : u.y) >> (16 * (j & 1));
-          w[i][j] = pk2(val(x & 0xffu), val((x >> 8) & 0xffu));
-        }
+        for (int j = 0; j < 4; ++j) w[i][j] = vals(codes2h(j < 2 ? u.x : u.y, (j & 1) ? kSelHi : kSelLo));
       }
     } else {
 #pragma unroll
@@ -255,7 +290,7 @@ __global__ __launch_bounds__(kThr) void read_kernel(ReadArgs P) {
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          w[i][j] = pk2(val((u[2 * j] >> (8 * i)) & 0xffu), val((u[2 * j + 1] >> (8 * i)) & 0xffu));
+          w[i][j] = vals(codes2h(__builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x0c0c0400u + 0x0101u * i), kSelLo));
     }
   } else if (t0 < len) {
     const uint16_t* tail = (which ? st.v_tail : st.k_tail) + bh * kBlkBytes;
