@@ -52,8 +52,9 @@ struct PrefillArgs {
 
 template <int DT>
 __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
-  __shared__ __align__(16) uint16_t sK[2 * kKBuf];
-  __shared__ __align__(16) uint16_t sV[2 * kVBuf];
+  __shared__ __align__(16) uint16_t smem[2 * kKBuf + 2 * kVBuf];
+  uint16_t* const sK = smem;
+  uint16_t* const sV = smem + 2 * kKBuf;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, hf = lane >> 5;
@@ -302,13 +303,50 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
       for (int i = 0; i < 16; ++i) o[i & 3] = mfma32(value_op(i, 0), __builtin_bit_cast(f16x8, pf[i >> 2]), o[i & 3]);
     }
 
-    // ---- out
+    // (what follows from the lane is computed again here, from a copy: it needs no registers before)
+    int out_lane = tid & 63;
+    __asm__ volatile("" : "+v"(out_lane));
+    const int ox = out_lane & 31, oh = out_lane >> 5;
+    const int out_col = col0 + 32 * wave + ox;
+    const int out_q = out_col / G, out_h = out_col - out_q * G;
+    // ---- out: a wave's 32 rows through its part of LDS (the tiles are done with), so that a row goes out whole
     l = half_sum(l);
-    if (col < r.cols) {
-      if (P.splits == 1) {
-        const bool some = ok && l != 0.f;
-        const float inv = some ? 1.f / l : 0.f;
-        const int64_t at = b * r.o_sb + static_cast<int64_t>(h * G + qh) * r.o_sh + qs * r.o_ss + 4 * hf;
+    __syncthreads();
+    constexpr int kOutRow = 272;  // bytes of a staged row: 256 and a shift of the banks
+    static_assert(32 * kOutRow * kWaves <= 2 * (2 * kKBuf + 2 * kVBuf), "every wave's rows fit");
+    char* const rows = reinterpret_cast<char*>(smem) + 32 * kOutRow * wave;
+    char* const mine_row = rows + kOutRow * ox;
+    // the 16 bytes that a lane takes of row 4 j + lane / 16 (a row's address and whether it exists come from its lane)
+    auto out_rows = [&](int64_t at, bool exists, auto put) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = 4 * j + (out_lane >> 4);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(rows + kOutRow * row + 16 * (out_lane & 15));
+        const int64_t to = __shfl(static_cast<long long>(at), row);
+        if (__shfl(static_cast<int>(exists), row)) put(to, v);
+      }
+    };
+    if (P.splits == 1) {
+      const bool some = ok && l != 0.f;
+      const float inv = some ? 1.f / l : 0.f;
+      const int64_t at = b * r.o_sb + static_cast<int64_t>(h * G + out_h) * r.o_sh + out_q * r.o_ss;
+      if constexpr (DT == LKV_DTYPE_F32) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              f32x4 x;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = some ? o[2 * half + db][4 * k + i] * inv : 0.f;
+              *reinterpret_cast<f32x4*>(mine_row + 4 * (32 * db + 8 * k + 4 * oh)) = x;
+            }
+          out_rows(at + 64 * half, out_col < r.cols, [&](int64_t to, const u32x4& v) {
+            *reinterpret_cast<u32x4*>(static_cast<float*>(r.out) + to + 4 * (out_lane & 15)) = v;
+          });
+        }
+      } else {
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -316,20 +354,30 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = some ? o[db][4 * k + i] * inv : 0.f;
-            store4<DT>(r.out, at + 32 * db + 8 * k, x[0], x[1], x[2], x[3]);
+            store4<DT>(mine_row, 32 * db + 8 * k + 4 * oh, x[0], x[1], x[2], x[3]);
           }
-      } else {
-        const int64_t at = (bh * r.cols + col) * P.splits + split;
-        const bool some = ok && blk1 > blk0;
-        if (hf == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = some ? float2{m, l} : float2{-INFINITY, 0.f};
-        if (some) {
+        out_rows(at, out_col < r.cols, [&](int64_t to, const u32x4& v) {
+          *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(r.out) + to + 8 * (out_lane & 15)) = v;
+        });
+      }
+    } else {
+      const int64_t at = (bh * r.cols + out_col) * P.splits + split;
+      const bool some = ok && blk1 > blk0;
+      if (oh == 0 && out_col < r.cols)
+        *reinterpret_cast<float2*>(P.part_ml + 2 * at) = some ? float2{m, l} : float2{-INFINITY, 0.f};
 #pragma unroll
-          for (int db = 0; db < 4; ++db)
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<f32x4*>(P.part_o + at * kD + 32 * db + 8 * k + 4 * hf) =
-                  f32x4{o[db][4 * k], o[db][4 * k + 1], o[db][4 * k + 2], o[db][4 * k + 3]};
-        }
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const f32x16& x = o[2 * half + db];
+            *reinterpret_cast<f32x4*>(mine_row + 4 * (32 * db + 8 * k + 4 * oh)) =
+                f32x4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
+          }
+        out_rows(at * kD + 64 * half, some, [&](int64_t to, const u32x4& v) {
+          *reinterpret_cast<u32x4*>(P.part_o + to + 4 * (out_lane & 15)) = v;
+        });
       }
     }
   }
