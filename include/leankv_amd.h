@@ -705,10 +705,11 @@ int lkv_kv8_read(const lkv_kv8_store* store, const int32_t* lens, int64_t first,
  * of sequence b, which has q_lens[b] of them (null: S; at most lens[b]), sees tokens
  * 0 .. lens[b] - q_lens[b] + i; rows from q_lens[b] on, and rows that see no
  * token, are zeros.  max_len is the caller's bound on lens (the work is split
- * for it); what a longer sequence holds past it is not read.
+ * for it); of a longer sequence the finished blocks below the bound are read.
  * index (optional, S = 1): int32 [batch][kv_heads][n_index], the finished
  * blocks that a kv head's queries read (entries outside the finished blocks
- * are skipped) next to the unfinished block, which they always read.
+ * are skipped, a block listed twice counts twice) next to the unfinished
+ * block, which they always read.
  * Scores and sums are fp32 of fp16 queries and whole-number codes; the weights
  * are rounded to fp16 for the value product.
  */

@@ -84,7 +84,7 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) qraw[n][ks] = load_raw_q8<DT>(r.q, at + 64 * (ks >> 1) + 8 * (ks & 1));
   }
-  const int len = min(max(r.lens[b], 0), r.max_len);
+  const int len = held_tokens(r.lens[b], r.max_len);
   const int qlen = min(r.q_lens ? min(max(r.q_lens[b], 0), r.S) : r.S, len);
   const int nfull = len / kBlk, rest = len - nfull * kBlk;
   const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(kSelThr) void score_kernel(SelectArgs P) {
   const Store& st = P.st;
   float x[4];
   load_query4<DT>(P, b, h, 0, tid, x);
-  const int nfull = min(max(P.lens[b], 0), P.max_len) / kBlk;
+  const int nfull = held_tokens(P.lens[b], P.max_len) / kBlk;
   const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
   const int j0 = (blockIdx.x * kSelWaves + wave) * 16;
   if (static_cast<int>(blockIdx.x) * kSelWaves * 16 >= nfull) return;  // (the whole workgroup)
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
   const Store& st = P.st;
   float x[4];
   if (!P.keys) load_query4<DT>(P, b, h, 0, tid, x);  // (beside the length)
-  const int nfull = min(max(P.lens[b], 0), P.max_len) / kBlk;
+  const int nfull = held_tokens(P.lens[b], P.max_len) / kBlk;
   const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
   int* out = P.index + bh * P.n;
   if (nfull <= P.n) {  // all of them

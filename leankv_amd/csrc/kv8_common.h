@@ -168,6 +168,11 @@ __device__ __forceinline__ float groups_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// A sequence's tokens: its length, of a longer one than the caller's bound the finished blocks below the bound.
+__device__ __forceinline__ int held_tokens(int len, int max_len) {
+  return len > max_len ? max_len & ~(kBlk - 1) : max(len, 0);
+}
+
 // Query rows of one kv head as the columns of its score products: column c is query c / G, head c % G.
 struct Rows {
   const void* q;
@@ -177,7 +182,7 @@ struct Rows {
   const int* lens;    // [B] tokens held, the queries' own among them
   const int* q_lens;  // [B] queries of a sequence, or null: all S
   int G, S, cols;     // cols = S * G
-  int max_len;        // bound on lens (what a longer sequence holds past it is not read)
+  int max_len;        // bound on lens
   float scale_log2;   // scale * log2(e)
 };
 

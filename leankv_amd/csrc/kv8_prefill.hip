@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
     const int tile = P.tiles - 1 - __builtin_amdgcn_readfirstlane(piece / P.splits);
     const int split = piece - (P.tiles - 1 - tile) * P.splits;
     const int b = __builtin_amdgcn_readfirstlane(item / st.Hkv), h = item - b * st.Hkv;
-    const int len = min(max(r.lens[b], 0), r.max_len);
+    const int len = held_tokens(r.lens[b], r.max_len);
     const int qlen = min(r.q_lens ? min(max(r.q_lens[b], 0), r.S) : r.S, len);
     const int nfull = len / kBlk;
     const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;

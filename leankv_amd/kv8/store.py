@@ -139,6 +139,15 @@ class KV8Store:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.scales, self.ranges,
                                                           self.k_tail, self.v_tail))
 
+    def grown(self, capacity: int) -> "KV8Store":
+        """A store of `capacity` tokens that holds what this one does."""
+        new = KV8Store(self.batch, self.kv_heads, max(capacity, self.capacity), self.device)
+        for name in ("k_codes", "v_codes", "scales", "ranges"):
+            getattr(new, name)[:, :, :self.blocks] = getattr(self, name)
+        new.k_tail.copy_(self.k_tail)
+        new.v_tail.copy_(self.v_tail)
+        return new
+
     # ------------------------------------------------------------------------------------------------ checks
     def _call(self, name: str, *args):
         """One C entry on the store's device and that device's current stream."""
@@ -220,7 +229,7 @@ class KV8Store:
         among it): [batch, heads, 128] in q's type.  A sequence of length 0 gives zeros.  max_len: the caller's bound on
         lens (default the capacity), which the work is split for.  scale: 1 / sqrt(128) by default.  index: int32
         [batch, kv_heads, n], only these finished blocks of a kv head (as select_blocks gives them; others than finished
-        ones are skipped) and the unfinished one."""
+        ones are skipped, one listed twice counts twice) and the unfinished one."""
         what = "KV8Store.decode_attention"
         heads, dtype = self._queries(q, 3, what)
         p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)

@@ -36,6 +36,7 @@ import weakref
 import torch
 from torch.autograd import forward_ad
 
+from ..hf_cache import HFCache
 from .. import kernels as _k  # also registers torch.ops.leankv (the cache's kernels go through the dispatcher)
 from .codebook import get_codebook_tensors
 from .rotation import generate_rotation_matrices
@@ -49,11 +50,14 @@ def active_cache():
     return _ACTIVE() if _ACTIVE is not None else None
 
 
-class TurboQuantCache:
-    """Hybrid KV cache: compressed cold storage + fp16 hot window (static buffers)."""
+def set_active(cache) -> None:
+    """Called by a cache's update(): the attention function that runs next reads this cache."""
+    global _ACTIVE
+    _ACTIVE = weakref.ref(cache)
 
-    is_compileable = False
-    layer_type = None
+
+class TurboQuantCache(HFCache):
+    """Hybrid KV cache: compressed cold storage + fp16 hot window (static buffers)."""
 
     def __init__(self, bits: int = 3, head_dim: int = 128, num_layers: int = 32, hot_buffer_size: int = 64,
                  device=None, dtype: torch.dtype = torch.float16, seed: int = 42, max_seq_len: int = 4096,
@@ -156,14 +160,13 @@ class TurboQuantCache:
 
     # ----------------------------------------------------------- update
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, cache_kwargs=None):
-        global _ACTIVE
         if self._fused_pending[layer_idx] or self._prefill_pending[layer_idx]:
             raise RuntimeError(
                 "TurboQuantCache(fused_attention=True): layer %d's previous update was never attended by the "
                 "'leankv_tq' attention implementation, so the model attended to the newest tokens only; call "
                 "leankv_amd.turboquant.attention.use_on(model, cache) or build the cache with "
                 "fused_attention=False" % layer_idx)
-        _ACTIVE = weakref.ref(self)
+        set_active(self)
         B, H, S, D = key_states.shape
         if layer_idx == 0:
             self._seen_tokens += S
@@ -291,29 +294,7 @@ class TurboQuantCache:
         self._fused_pending[layer_idx] = False
         return self._get_full_cache(layer_idx)
 
-    # ----------------------------------------------------------- HF interface
-    def get_seq_length(self, layer_idx: int = 0) -> int:
-        return self._seq_lengths[layer_idx] if layer_idx < len(self._seq_lengths) else 0
-
-    def get_mask_sizes(self, query_length, layer_idx: int = 0):
-        q = query_length if isinstance(query_length, int) else int(query_length.shape[0])
-        return self.get_seq_length(layer_idx) + q, 0
-
-    def get_query_offset(self, layer_idx: int = 0) -> int:
-        """Position of the first query of the next forward (transformers' Cache contract: the cached length)."""
-        return self.get_seq_length(layer_idx)
-
-    def get_max_cache_shape(self, *args, **kwargs):
-        return None
-
-    def get_max_length(self):
-        return None
-
-    def has_previous_state(self, layer_idx=None):
-        if layer_idx is not None:
-            return layer_idx < len(self._seq_lengths) and self._seq_lengths[layer_idx] > 0
-        return any(s > 0 for s in self._seq_lengths)
-
+    # ----------------------------------------------------------- HF interface (the rest: HFCache)
     def crop(self, max_length: int):
         pass
 
@@ -338,54 +319,11 @@ class TurboQuantCache:
         self.storage_generation += 1
 
     @property
-    def seen_tokens(self):
-        return self._seen_tokens
-
-    @property
-    def key_cache(self):
-        return [torch.empty(0, device=self._device)] * len([s for s in self._seq_lengths if s > 0])
-
-    @property
-    def value_cache(self):
-        return self.key_cache
-
-    @property
-    def is_initialized(self):
-        return any(s > 0 for s in self._seq_lengths)
-
-    @property
-    def is_sliding(self):
-        return [False] * self.num_layers
-
-    @property
     def max_batch_size(self):
         for k in self._k_hot:
             if k is not None:
                 return k.shape[0]
         return 0
-
-    @property
-    def max_cache_len(self):
-        return max(self._seq_lengths) if self._seq_lengths else 0
-
-    def __len__(self) -> int:
-        return len([s for s in self._seq_lengths if s > 0])
-
-    def __getitem__(self, layer_idx: int):
-        if self._seq_lengths[layer_idx] > 0:
-            return self._get_full_cache(layer_idx)
-        raise IndexError("Layer %d not in cache" % layer_idx)
-
-    def __iter__(self):
-        for i in range(self.num_layers):
-            if self._seq_lengths[i] > 0:
-                yield self._get_full_cache(i)
-
-    def __bool__(self):
-        return True
-
-    def to_legacy_cache(self):
-        return tuple(self._get_full_cache(i) for i in range(self.num_layers) if self._seq_lengths[i] > 0)
 
     # ----------------------------------------------------------- diagnostics (cache.py:295-351)
     def get_compressed_memory_bytes(self) -> int:

@@ -207,6 +207,24 @@ def test_decode_attention_long_and_bounds(cuda):
     _check_attn(out.unsqueeze(2), refs, q.unsqueeze(2), [n], None, scale=0.3)
 
 
+def test_length_past_the_bound(cuda):
+    """Of a sequence longer than max_len (or than the store) the finished blocks below the bound count; a negative length
+    is none."""
+    n = 64 * 7 + 9
+    k, v = _kv(cuda, 3, 1, n, seed=4)
+    store = _store(3, 1, n, device=cuda)
+    store.update(k, v, _ints(cuda, [0] * 3), _ints(cuda, [n, 130, 0]))
+    q = torch.randn(3, 2, D, generator=torch.Generator().manual_seed(5)).half().to(cuda)
+    out = store.decode_attention(q, _ints(cuda, [n, 130, -3]), max_len=200)
+    _check_attn(out.unsqueeze(2), _refs(k, v, [192, 130, 0]), q.unsqueeze(2), [192, 130, 0], None)
+    out = store.prefill_attention(q.unsqueeze(2).expand(-1, -1, 80, -1), _ints(cuda, [n, 130, -3]), max_len=200)
+    _check_attn(out, _refs(k, v, [192, 130, 0]), q.unsqueeze(2).expand(-1, -1, 80, -1), [192, 130, 0], [80, 80, 0])
+    far = _ints(cuda, [2 ** 31 - 1, 130, -(2 ** 31)])
+    out = store.decode_attention(q, far)
+    _check_attn(out[1:].unsqueeze(2), _refs(k, v, [0, 130, 0])[1:], q[1:].unsqueeze(2), [130, 0], None)
+    assert torch.isfinite(out).all() and (store.select_blocks(q, far, 9)[0, 0].cpu() == torch.tensor([*range(8), -1])).all()
+
+
 def test_decode_attention_value_scales_apart(cuda):
     """Value blocks of very different scale (zero ones too) beside weights that favour the small ones."""
     n = 64 * 12 + 30
