@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kThr = 256;
 constexpr int kWaves = 4;  // of a split workgroup
+constexpr int kOneSplit = 3 * kWaves;  // so few units are one split
 constexpr int kManyCols = 256;  // columns of a workgroup of the many-row kernel
 constexpr int kManyChunk = 8;   // and the fewest blocks that a split of it gets
 
@@ -747,13 +748,16 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t cols, int64_t units) {
   const int64_t wide = p.nt ? 16 * p.nt : kManyCols;
   p.groups = static_cast<int>((cols + wide - 1) / wide);
   const int64_t items = B * Hkv * p.groups;
-  // One workgroup a CU; two of the few-row kernel fit and would be no faster (32 sequences of up to 8192 tokens 68.7 us
-  // with one, 72.2 with two a CU, 1 x 131072 tokens 53.7 and 56.7: more splits are more rows to join).
+  // One workgroup a CU; two of the few-row kernel fit and would be no faster (32 sequences of up to 8192 tokens 68.2 us
+  // with one, 70.1 with two a CU, 1 x 131072 tokens 52.5 and 53.4: more splits are more rows to join).
   const int64_t want = (cus + items - 1) / items;
   int64_t chunk = (units + want - 1) / want;
-  const int64_t unit = p.nt ? kWaves : 2;  // a block for every wave, or a pair of blocks
-  chunk = (chunk + unit - 1) / unit * unit;
-  if (!p.nt && chunk < kManyChunk) chunk = kManyChunk;
+  if (p.nt)
+    // a block for every wave; up to three for every wave are one split (512 tokens of one sequence 7.4 us, with rows to
+    // join 9.1; 1024 tokens 10.0 and 9.1)
+    chunk = units <= kOneSplit ? kOneSplit : (chunk + kWaves - 1) / kWaves * kWaves;
+  else
+    chunk = chunk < kManyChunk ? kManyChunk : chunk;
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((units + chunk - 1) / chunk);
   return p;

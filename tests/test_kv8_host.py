@@ -102,10 +102,14 @@ def test_attention_arguments():
     _refused(attn(lens=None), "null pointer")
     _refused(attn(q=P + 8), "16-byte aligned")
     _refused(attn(os_=(4096, 130, 512)), "16-byte aligned")
-    need = lib.lkv_kv8_attn_workspace_bytes(2, 8, 4, 1, 512, 0)
-    assert need > 0  # several splits for so little work
-    _refused(attn(nbytes=need - 1), "workspace")
-    _refused(attn(ws=None, nbytes=need), "workspace")
+    need = lib.lkv_kv8_attn_workspace_bytes(2, 8, 4, 1, 8192, 0)
+    assert need > 0  # several splits for so few heads
+    big = _store(blocks=128)
+    _refused(attn(big, max_len=8192, nbytes=need - 1), "workspace")
+    _refused(attn(big, max_len=8192, ws=None, nbytes=need), "workspace")
+    assert lib.lkv_kv8_attn_workspace_bytes(2, 8, 4, 1, 512, 0) == 0  # so little work is one split
+    many = lib.lkv_kv8_attn_workspace_bytes(1, 8, 4, 512, 8192, 0)
+    assert many > 0 and many % (8 * 512 * 130 * 4) == 0
     assert attn(S=0) == 0 and attn(_store(batch=0)) == 0
     assert lib.lkv_kv8_attn_workspace_bytes(2, 6, 4, 1, 512, 0) == 0
     # many sequences need no split, and no workspace
