@@ -15,13 +15,19 @@
 //                 so neither the codes nor the sums need a multiplication, and m follows the largest s + log2(vscale).
 //                 Weights are rounded to fp16 (2^-12 of each) for the product; their sum is of the unrounded ones.
 //   combine       joins the splits' (offset, sum, rows) in fp32.
-// Bound by memory: 16 KB a block and head.
+// Bound by memory where there are many blocks: 16 KB a block and head, one 4-wave workgroup a CU with all of a block's 16
+// loads of a wave in flight.  1 x 131072 tokens (32/8 heads, 269 MB): 45 us the split kernel (6.0 TB/s; a plain read loop
+// 6.0-6.3), 51-53 us a call; 32 x 8192: 92 us (5.9 TB/s); 32 sequences of 1.6-8 K tokens 68 us, the longest of them bounds
+// it.  8 waves were no faster, nontemporal loads gained 5 % there and lost as much with many sequences.
+// Bound by latency where there are few: 1 x 4133 tokens 9.8 us in a replayed graph, 5.5 the split kernel (length, then
+// loads, then one block's 440 vector instructions, then the join) and 3.5 the combine.
 //
 // Selection (lkv_kv8_select_blocks): a score per finished block, the upper bound sum_d max(q8 lo, q8 hi) of the product
 // with any of its keys, from the per-dim lowest and highest codes (256 bytes a block) and the query rows in 8 bits, on
 // v_mfma_i32_16x16x64_i8: max(q8 lo, q8 hi) = min(q8, 0) lo + max(q8, 0) hi.  The sum is a whole number below 2^24, so a
 // score has two roundings (the query's scale, the block's) whatever the order of the work, and the choice is the same
-// everywhere.  Then a radix selection per (sequence, kv head).
+// everywhere.  Then a radix selection per (sequence, kv head), by the same workgroup up to 512 blocks.  Bound by latency:
+// 128 blocks 6.8 us, 512 of 16 sequences 7.8 us; 2048 blocks 3.9 (scores) + 6.4 us.
 #include "kv8_common.h"
 
 namespace lkv {
