@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
   if (P.splits > 1 && u0 >= units) {  // nothing to do: an empty record
     const int col = col0 + tid;
     if (tid < 16 * NT && col < r.cols)
-      *reinterpret_cast<float2*>(P.part_ml + 2 * ((bh * r.cols + col) * P.splits + blockIdx.x)) = float2{-INFINITY, 0.f};
+      *reinterpret_cast<float2*>(P.part_ml + 2 * ((bh * r.cols + col) * P.splits + blockIdx.x)) = part_record(-INFINITY, 0.f);
     return;
   }
   const int u1 = min(u0 + P.chunk, units);
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
           *reinterpret_cast<f32x4*>(P.part_o + at * kD + 4 * kLanes * k + d) = acc[k];
       }
       if (P.splits > 1 && tid % kLanes == 0)
-        *reinterpret_cast<float2*>(P.part_ml + 2 * at) = row_ok ? float2{M, L} : float2{-INFINITY, 0.f};
+        *reinterpret_cast<float2*>(P.part_ml + 2 * at) = row_ok ? part_record(M, L) : part_record(-INFINITY, 0.f);
     }
   }
 }

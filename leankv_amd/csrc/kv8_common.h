@@ -2,11 +2,11 @@
 //
 // A finished block is 64 tokens of one kv head.  Its 64 x 128 keys share one scale, so do its values:
 //   scale = amax / 127, code = rint(x * (127 / amax)) in -127 .. 127, value = code * scale
-// (in fp32 with the roundings of amax * fp32(1 / 127) and x * (127 * (1 / amax))), and a code is stored as the byte code + 128.  Keys lie [token][dim].  Values lie [dim][position], so that the value
-// product reads its operand (8 tokens of one dim per lane) as it lies in memory, with no transpose in the attention
-// kernels; position 16 g + 8 ks + 4 t + i holds token 32 ks + 16 t + 4 g + i: the tokens whose weights lane group g of
-// a wave has after the 16-row score products 2 ks and 2 ks + 1.  The unfinished block of a head is fp16 in the same
-// two layouts.
+// (in fp32 with the roundings of amax * fp32(1 / 127) and x * (127 * (1 / amax))), and a code is stored as the byte
+// code + 128.  Keys lie [token][dim].  Values lie [dim][position], so that the value product reads its operand (8 tokens
+// of one dim per lane) as it lies in memory, with no transpose in the attention kernels; position 16 g + 8 ks + 4 t + i
+// holds token 32 ks + 16 t + 4 g + i: the tokens whose weights lane group g of a wave has after the 16-row score products
+// 2 ks and 2 ks + 1.  The unfinished block of a head is fp16 in the same two layouts.
 #pragma once
 
 #include "common.h"
@@ -167,6 +167,10 @@ __device__ __forceinline__ float groups_sum(float v) {
   a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
+
+// A partial sum's (offset, sum): offset -inf is an empty one, which is passed over.  A row of NaN scores has no offset
+// (max passes over NaN) but is not empty: it takes 0, so that its NaN reaches the joined row.
+__device__ __forceinline__ float2 part_record(float m, float l) { return float2{l != l ? 0.f : m, l}; }
 
 // A sequence's tokens: its length, of a longer one than the caller's bound the finished blocks below the bound.
 __device__ __forceinline__ int held_tokens(int len, int max_len) {

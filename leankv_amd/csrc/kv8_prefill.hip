@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
       const int64_t at = (bh * r.cols + out_col) * P.splits + split;
       const bool some = ok && blk1 > blk0;
       if (oh == 0 && out_col < r.cols)
-        *reinterpret_cast<float2*>(P.part_ml + 2 * at) = some ? float2{m, l} : float2{-INFINITY, 0.f};
+        *reinterpret_cast<float2*>(P.part_ml + 2 * at) = some ? part_record(m, l) : part_record(-INFINITY, 0.f);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll

@@ -252,7 +252,70 @@ def test_attention_nan_query_stays_in_its_row(cuda):
     assert torch.isnan(out[0, 1]).all() and torch.equal(out[0, ::2], want[0, ::2])
 
 
-@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_nan_query_through_partial_sums(cuda):
+    """The same where a row's sums come from several workgroups, for few rows and for many."""
+    n = 64 * 90 + 3
+    k, v = _kv(cuda, 1, 1, n, seed=8)
+    store = _store(1, 1, n, device=cuda)
+    store.update(k, v, _ints(cuda, [0]))
+    lens = _ints(cuda, [n])
+    for S in (1, 3, 130):
+        q = torch.randn(1, 2, S, D, generator=torch.Generator().manual_seed(6)).half().to(cuda)
+        want = store.prefill_attention(q, lens)
+        bad = q.clone()
+        bad[0, 1, S // 2, 5] = float("nan")
+        out = store.prefill_attention(bad, lens)
+        assert torch.isnan(out[0, 1, S // 2]).all()
+        out[0, 1, S // 2] = want[0, 1, S // 2]
+        assert torch.equal(out, want) and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("B,H,Hq,S,n", [(2, 8, 8, 4400, 4500), (1, 3, 3, 22100, 22100), (1, 8, 24, 3000, 3001)])
+def test_prefill_more_pieces_than_workgroups(cuda, B, H, Hq, S, n):
+    """Workgroups that take several pieces, one after the other: rows from everywhere."""
+    k, v = _kv(cuda, B, H, n, seed=S)
+    store = _store(B, H, n, device=cuda)
+    store.update(k, v, _ints(cuda, [0] * B))
+    q = torch.randn(B, S, Hq, D, generator=torch.Generator().manual_seed(3)).half().to(cuda).transpose(1, 2)
+    out = store.prefill_attention(q, _ints(cuda, [n] * B)).cpu()
+    assert torch.isfinite(out).all()
+    g = torch.Generator().manual_seed(S)
+    k, v = stored(k.cpu()), stored(v.cpu())
+    refs = {}
+    for _ in range(60):
+        b, h, i = (int(torch.randint(0, m, (1,), generator=g)) for m in (B, Hq, S))
+        if (b, h * H // Hq) not in refs:
+            refs[b, h * H // Hq] = Ref(k[b, h * H // Hq], v[b, h * H // Hq])
+        want, bound = refs[b, h * H // Hq].attend(query(q[b, h, i].cpu()), n - S + i + 1, SCALE, torch.finfo(F16).eps)
+        assert ((out[b, h, i].double() - want).abs() <= bound).all(), (b, h, i)
+
+
+@pytest.mark.parametrize("S", [3, 200])
+def test_out_buffers_of_other_layouts(cuda, S):
+    """Outputs written into views: by token, with rows apart, beside other data that stays."""
+    k, v = _kv(cuda, 2, 2, 300, seed=2)
+    store = _store(2, 2, 300, device=cuda)
+    store.update(k, v, _ints(cuda, [0, 0]))
+    lens = _ints(cuda, [300, 300])
+    q = torch.randn(2, 4, S, D, generator=torch.Generator().manual_seed(3)).half().to(cuda)
+    want = store.prefill_attention(q, lens)
+    for make in (lambda: torch.full((2, 4, S, D), 9.0, dtype=F16, device=cuda),
+                 lambda: torch.full((2, 4, S, 2 * D), 9.0, dtype=F16, device=cuda)[..., 8:8 + D],
+                 lambda: torch.full((S, 2, 4, D), 9.0, dtype=F16, device=cuda).permute(1, 2, 0, 3),
+                 lambda: torch.full((2, 7, S + 1, D), 9.0, dtype=F16, device=cuda)[:, 2:6, 1:]):
+        out = make()
+        assert store.prefill_attention(q, lens, out=out) is out and torch.equal(out, want)
+        base = out._base
+        if base is not None and base.numel() > out.numel():
+            assert (base == 9.0).sum() >= base.numel() - out.numel()
+    one = torch.full((2, 4, 3 * D), 9.0, dtype=F16, device=cuda)[..., D:2 * D]
+    store.decode_attention(q[:, :, 0], lens, out=one)
+    assert torch.equal(one, store.decode_attention(q[:, :, 0], lens)) and (one._base[..., :D] == 9.0).all()
+    inplace = q[:, :, 0].clone()  # over its own queries
+    assert torch.equal(store.decode_attention(inplace, lens, out=inplace), one)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("Hq,H,S,lens,q_lens", [
     (2, 1, 5, [70], None), (8, 2, 3, [3, 200, 64], None), (4, 4, 64, [64], None), (8, 8, 65, [65, 130], [65, 20]),
     (8, 2, 33, [40, 300], [1, 33]), (6, 2, 130, [130, 500, 131], [130, 77, 0]), (3, 1, 200, [263, 200], None),
