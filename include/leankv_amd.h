@@ -662,9 +662,10 @@ int lkv_decode_head(const lkv_decode_dims* dims, const void* final_norm, const v
  * held in 8 bits with one scale for its keys and one for its values:
  *   scale = amax * s, code = rint(x * (127 * (1 / amax))), value = code * scale
  * (fp32, each operation rounded; s = fp32(1 / 127), amax over the block's
- * 64 x 128 fp16 numbers; a zero block has scale 0 and codes 0); the unfinished last block of a sequence is fp16.  What is stored is
- * finite: inputs are rounded to fp16, numbers beyond +-65504 and infinities
- * become +-65504, a NaN becomes 0.  All buffers are 16-byte aligned device
+ * 64 x 128 fp16 numbers; a zero block has scale 0 and codes 0); the unfinished
+ * last block of a sequence is fp16.  What is stored is finite: inputs are
+ * rounded to fp16, numbers beyond +-65504 and infinities become +-65504, a NaN
+ * becomes 0.  All buffers are 16-byte aligned device
  * memory of the caller, cleared once before the first use.  A code is stored
  * as the byte code + 128; values lie by dim, at position 16 g + 8 k + 4 t + i
  * of a dim's 64 bytes (or fp16 numbers) token 32 k + 16 t + 4 g + i.
@@ -688,6 +689,10 @@ typedef struct lkv_kv8_store {
  * pos[b] must be what it holds.  n_new (optional) gives how many of the S
  * tokens are the sequence's (a padded batch: the rest is not read).  Tokens
  * past the store are dropped, a position outside it stores nothing.
+ * A sequence may be taken back (a smaller pos and length from then on) to any
+ * length within its unfinished block and to any multiple of 64; a finished
+ * block is not opened again: to drop some of its tokens, take the sequence
+ * back to its start and store the others anew.
  */
 int lkv_kv8_update(const lkv_kv8_store* store, const void* k, const int64_t* k_strides, const void* v,
                    const int64_t* v_strides, int dtype, int64_t S, const int32_t* pos, const int32_t* n_new,
@@ -702,8 +707,8 @@ int lkv_kv8_read(const lkv_kv8_store* store, const int32_t* lens, int64_t first,
  * Softmax attention of the S newest tokens' queries q [batch][Hq][S][128] over
  * the store (Hq a multiple of kv_heads; query head h reads kv head h /
  * (Hq / kv_heads)): out = softmax(scale * q K^T) V in the type of q.  Query i
- * of sequence b, which has q_lens[b] of them (null: S; at most lens[b]), sees tokens
- * 0 .. lens[b] - q_lens[b] + i; rows from q_lens[b] on, and rows that see no
+ * of sequence b, which has q_lens[b] of them (null: S; at most lens[b]), sees
+ * tokens 0 .. lens[b] - q_lens[b] + i; rows from q_lens[b] on, and rows that see no
  * token, are zeros.  max_len is the caller's bound on lens (the work is split
  * for it); of a longer sequence the finished blocks below the bound are read.
  * index (optional, S = 1): int32 [batch][kv_heads][n_index], the finished
@@ -711,7 +716,8 @@ int lkv_kv8_read(const lkv_kv8_store* store, const int32_t* lens, int64_t first,
  * are skipped, a block listed twice counts twice) next to the unfinished
  * block, which they always read.
  * Scores and sums are fp32 of fp16 queries and whole-number codes; the weights
- * are rounded to fp16 for the value product.
+ * are rounded to fp16 for the value product.  A query that holds a NaN gives a
+ * row of NaN, and no other one.
  */
 size_t lkv_kv8_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t S, int64_t max_len, int64_t n_index);
 int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int64_t* q_strides, int dtype, int64_t Hq, int64_t S,
@@ -721,14 +727,16 @@ int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int64_t* q_str
 
 /*
  * index [batch][kv_heads][n]: for the newest token's queries q [batch][Hq][128]
- * (strides of batch and head; a third is not used) the n finished blocks with the highest
- * score, ascending, -1 where there are fewer.  The first `sink` and the last
+ * (strides of batch and head; a third is not used) the n finished blocks with
+ * the highest score, ascending, -1 where there are fewer.  The first `sink` and the last
  * `recent` finished blocks are always among them; of equal scores the lower
  * index wins.  The score of a block is
  *   max over the kv head's queries of (float(dot) * qscale), times kscale,
  *   dot = sum_d max(q8_d lo_d, q8_d hi_d)
- * with q8 and qscale the codes and scale of the fp16 query, as a block's and lo, hi the lowest and highest key codes: an upper bound (up to the
- * query's rounding) of every product of the block, in two fp32 roundings.
+ * with q8 and qscale the codes and scale of the fp16 query, as a block's, and
+ * lo, hi the lowest and highest key codes: an upper bound (up to the query's
+ * rounding) of every product of the block, in two fp32 roundings.  (A NaN in a
+ * query counts as 0 here.)
  */
 size_t lkv_kv8_select_workspace_bytes(int64_t B, int64_t Hkv, int64_t max_len);
 int lkv_kv8_select_blocks(const lkv_kv8_store* store, const void* q, const int64_t* q_strides, int dtype, int64_t Hq,

@@ -746,11 +746,11 @@ __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
 
 }  // namespace
 
-Plan make_plan(int64_t B, int64_t Hkv, int64_t cols, int64_t units) {
+Plan make_plan(int64_t B, int64_t Hkv, int64_t cols, int64_t units, bool listed) {
   Plan p;
   if (units < 1) units = 1;
   const int64_t cus = device_cu_count();
-  p.nt = cols <= 16 ? 1 : cols <= 64 ? 2 : 0;
+  p.nt = cols <= 16 ? 1 : cols <= 64 || listed ? 2 : 0;  // (the many-row kernel takes no list)
   const int64_t wide = p.nt ? 16 * p.nt : kManyCols;
   p.groups = static_cast<int>((cols + wide - 1) / wide);
   const int64_t items = B * Hkv * p.groups;
@@ -819,7 +819,7 @@ extern "C" size_t lkv_kv8_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk
                                                int64_t n_index) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || S <= 0 || max_len < 0 || n_index < 0) return 0;
   const int64_t cols = Hq / Hkv * S;
-  return plan_bytes(make_plan(B, Hkv, cols, units_of(max_len, n_index)), B, Hkv, cols);
+  return plan_bytes(make_plan(B, Hkv, cols, units_of(max_len, n_index), n_index > 0), B, Hkv, cols);
 }
 
 extern "C" int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int64_t* q_strides, int dtype, int64_t Hq,
@@ -837,7 +837,8 @@ extern "C" int lkv_kv8_attn(const lkv_kv8_store* store, const void* q, const int
   LKV_REQUIRE(q && out && lens, "kv8_attn: null pointer");
   if (int rc = check_rows(q, q_strides, dtype, "kv8_attn", "q")) return rc;
   if (int rc = check_rows(out, out_strides, dtype, "kv8_attn", "out")) return rc;
-  Plan p = make_plan(B, Hkv, cols, units_of(max_len, n_index));
+  const Plan p = make_plan(B, Hkv, cols, units_of(max_len, n_index), n_index > 0);
+  LKV_REQUIRE(!p.nt || Hkv * p.groups < 65536, "kv8_attn: %lld query heads over a block list", (long long)Hq);
   const size_t need = plan_bytes(p, B, Hkv, cols);
   LKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
               "kv8_attn: workspace of %zu bytes (16-byte aligned) required, got %zu", need, workspace_bytes);

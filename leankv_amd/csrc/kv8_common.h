@@ -197,7 +197,7 @@ struct Plan {
   int chunk;    // key blocks per split
   int splits;
 };
-Plan make_plan(int64_t B, int64_t Hkv, int64_t cols, int64_t units);
+Plan make_plan(int64_t B, int64_t Hkv, int64_t cols, int64_t units, bool listed);
 size_t plan_bytes(const Plan& p, int64_t B, int64_t Hkv, int64_t cols);
 int launch_prefill(const Store& st, const Rows& r, const Plan& p, int dtype, int64_t B, float* part_o, float* part_ml,
                    hipStream_t stream);

@@ -193,7 +193,11 @@ class KV8Store:
     def update(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, n_new: torch.Tensor | None = None) -> None:
         """Store S new tokens of every sequence: k, v [batch, kv_heads, S, 128], sequence b's at positions pos[b] .. (what
         it holds already).  n_new: how many of the S are sequence b's (a padded batch; the rest is not read).  Tokens
-        past the capacity are dropped.  One launch; blocks that become whole are quantized."""
+        past the capacity are dropped.  One launch; blocks that become whole are quantized.
+
+        A sequence may be taken back (a smaller pos and length from then on) to any length within its unfinished block
+        and to any multiple of 64.  A finished block is not opened again: to drop some of its tokens, take the sequence
+        back to its start and store the others anew (read gives them as they are held)."""
         what = "KV8Store.update"
         nk, nv = k.shape, v.shape
         for t, n, name in ((k, nk, "k"), (v, nv, "v")):
@@ -235,7 +239,7 @@ class KV8Store:
         p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
         n, list_ = 0, None
         if index is not None:
-            if index.dtype is not torch.int32 or index.dim() != 3 or index.shape[0] != self.batch \
+            if not isinstance(index, torch.Tensor) or index.dtype is not torch.int32 or index.dim() != 3 or index.shape[0] != self.batch \
                     or index.shape[1] != self.kv_heads or not index.shape[2] or index.device != self.device \
                     or not index.is_contiguous():
                 raise LeanKVError("%s: index must be a contiguous int32 tensor [%d, %d, n] on %s"

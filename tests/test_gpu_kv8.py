@@ -367,6 +367,50 @@ def test_sparse(cuda, Hq, H, lens, blocks, sink, recent, dtype):
     _check_attn(out.unsqueeze(2), refs, q.unsqueeze(2), lens, None, tokens=tokens)
 
 
+@pytest.mark.parametrize("Hq,H", [(71, 1), (130, 2), (400, 1)])
+def test_block_list_with_many_heads(cuda, Hq, H):
+    """More query heads than the few-row kernel has columns, over a list of blocks: still only those blocks."""
+    n, blocks = 64 * 20 + 3, 4
+    k, v = _kv(cuda, 2, H, n, seed=Hq)
+    lens = [n, 64 * 9]
+    store = _store(2, H, n, device=cuda)
+    store.update(k, v, _ints(cuda, [0, 0]), _ints(cuda, lens))
+    q = torch.randn(2, Hq, D, generator=torch.Generator().manual_seed(4)).half().to(cuda)
+    out, index = store.sparse_decode_attention(q, _ints(cuda, lens), blocks)
+    refs, q16 = _refs(k, v, lens), query(q.cpu())
+    picks = [[choose(refs[b][h], q16[b, h * Hq // H:(h + 1) * Hq // H], blocks, 1, 1) for h in range(H)]
+             for b in range(2)]
+    assert index.tolist() == picks
+    tokens = [[[64 * j + i for j in p for i in range(64)] + list(range(lens[b] // 64 * 64, lens[b])) for p in picks[b]]
+              for b in range(2)]
+    _check_attn(out.unsqueeze(2), refs, q.unsqueeze(2), lens, None, tokens=tokens)
+    assert torch.equal(store.decode_attention(q, _ints(cuda, lens), index=index), out)
+
+
+def test_sequence_taken_back(cuda):
+    """Tokens dropped again: within the unfinished block, to a multiple of 64, and inside a finished block through read."""
+    n = 64 * 5 + 30
+    k, v = _kv(cuda, 3, 2, n, seed=21)
+    k2, v2 = _kv(cuda, 3, 2, 200, seed=22)
+    store = _store(3, 2, n + 300, device=cuda)
+    store.update(k, v, _ints(cuda, [0, 0, 0]))
+    back = [64 * 5 + 7, 64 * 5, 64 * 2]
+    store.update(k2, v2, _ints(cuda, back))
+    fk = torch.cat([torch.cat([k[b:b + 1, :, :m], k2[b:b + 1], k[b:b + 1, :, :back[0] - m]], 2) for b, m in enumerate(back)])
+    fv = torch.cat([torch.cat([v[b:b + 1, :, :m], v2[b:b + 1], v[b:b + 1, :, :back[0] - m]], 2) for b, m in enumerate(back)])
+    lens = [m + 200 for m in back]
+    _check_store(store, _refs(fk, fv, lens), fk, fv, lens)
+    # 10 tokens of every sequence's third block stay
+    kr, vr = store.read(_ints(cuda, lens), 64 * 2 + 10, 64 * 2)
+    store.update(kr, vr, _ints(cuda, [64 * 2] * 3))
+    gk, gv = store.read(_ints(cuda, [64 * 2 + 10] * 3), 64 * 2 + 10, 64 * 2)
+    assert torch.equal(gk, kr) and torch.equal(gv, vr)
+    q = torch.randn(3, 4, D, generator=torch.Generator().manual_seed(4)).half().to(cuda)
+    fk, fv = (torch.cat([f[:, :, :64 * 2], r], 2) for f, r in ((fk, kr), (fv, vr)))
+    out = store.decode_attention(q, _ints(cuda, [64 * 2 + 10] * 3))
+    _check_attn(out.unsqueeze(2), _refs(fk, fv, [64 * 2 + 10] * 3), q.unsqueeze(2), [64 * 2 + 10] * 3, None)
+
+
 def test_sparse_ties_take_the_lower_index(cuda):
     """Equal blocks: the lowest of them."""
     B, H, nb = 1, 2, 700
