@@ -26,8 +26,9 @@
 // with any of its keys, from the per-dim lowest and highest codes (256 bytes a block) and the query rows in 8 bits, on
 // v_mfma_i32_16x16x64_i8: max(q8 lo, q8 hi) = min(q8, 0) lo + max(q8, 0) hi.  The sum is a whole number below 2^24, so a
 // score has two roundings (the query's scale, the block's) whatever the order of the work, and the choice is the same
-// everywhere.  Then a radix selection per (sequence, kv head), by the same workgroup up to 512 blocks.  Bound by latency:
-// 128 blocks 6.8 us, 512 of 16 sequences 7.8 us; 2048 blocks 3.9 (scores) + 6.4 us.
+// everywhere.  Then a selection per (sequence, kv head), by the same workgroup up to 512 blocks: by counting up to 128, by
+// radix passes beyond.  Bound by latency: 128 blocks 6.0 us a call in a replayed graph, 300 of 16 sequences 8.7 us; 2048
+// blocks 3.9 (scores) + 6.4 us.
 #include "kv8_common.h"
 
 namespace lkv {
@@ -406,6 +407,10 @@ __global__ __launch_bounds__(kThr) void combine_kernel(CombineArgs P) {
 constexpr int kSelThr = 512;
 constexpr int kSelWaves = kSelThr / 64;
 constexpr int kLdsKeys = 8192;     // so many keys of a (sequence, kv head) stay in LDS, more are read again from memory
+// Up to so many finished blocks are chosen by counting, not by radix passes: a call over 20 blocks 4.7 us (by passes 6.8),
+// over 128 6.0 (7.6), over 256 8.7 (8.1).
+constexpr int kRankBlocks = kSelThr / 4;
+constexpr uint32_t kForcedKey = 0xfffffffeu;  // above every score's
 constexpr int kFusedBlocks = 512;  // up to so many blocks one workgroup scores and selects (2048: 36.6 us a call, apart 23.5)
 
 struct SelectArgs {
@@ -570,7 +575,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // barrier a radix pass (a histogram each, every wave finds the bin by itself).
 template <int DT>
 __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
-  __shared__ uint32_t s_key[kLdsKeys];
+  __shared__ __align__(16) uint32_t s_key[kLdsKeys];
   __shared__ __align__(16) uint32_t s_hist[4][256];
   __shared__ uint32_t s_or[kSelWaves], s_nor[kSelWaves];
   __shared__ int s_cnt[2][2][kSelWaves];
@@ -588,7 +593,14 @@ __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
     for (int j = tid; j < P.n; j += kSelThr) out[j] = j < nfull ? j : -1;
     return;
   }
-  for (int i = tid; i < 4 * 256; i += kSelThr) s_hist[0][i] = 0;
+  const bool by_rank = nfull <= kRankBlocks;
+  if (by_rank) {
+    if (tid < 3) s_key[nfull + tid] = 0;  // (below every score's)
+  } else {
+    for (int i = tid; i < 4 * 256; i += kSelThr) s_hist[0][i] = 0;
+  }
+  // the first `sink` and the last `recent` blocks are in anyway: the others compete for the remaining places
+  const int lo = min(P.sink, nfull), hi = max(nfull - P.recent, lo);  // [lo, hi) compete
   if (!P.keys) {
     const int c16 = lane & 15, g = lane >> 4;
     const int8_t* ranges = st.ranges + bh * st.blocks * 2 * kD + 16 * g;
@@ -631,25 +643,49 @@ __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
           const int j = now + 16 * kSelWaves * u + 4 * g + (c16 & 3);
           if (c16 < 4 && j < nfull) {  // (a lane writes and reads back its own)
             if (h0) best[u] = fmaxf(best[u], __uint_as_float(s_key[j]));
-            s_key[j] = end ? sort_bits(best[u] * kn[u]) : __float_as_uint(best[u]);
+            s_key[j] = !end                ? __float_as_uint(best[u])
+                       : j >= lo && j < hi ? sort_bits(best[u] * kn[u])
+                                           : kForcedKey;
           }
         }
       }
     }
   }
-  __syncthreads();  // (keys and cleared histograms)
   const uint32_t* keys = P.keys ? P.keys + bh * P.max_blocks : nullptr;
   const bool in_lds = nfull <= kLdsKeys;
   if (keys && in_lds)
-    for (int j = tid; j < nfull; j += kSelThr) s_key[j] = keys[j];  // (a thread reads back its own)
+    for (int j = tid; j < nfull; j += kSelThr) s_key[j] = j >= lo && j < hi ? keys[j] : kForcedKey;
+  __syncthreads();  // (keys and cleared histograms)
+  if (by_rank) {
+    // The number of blocks before block j in the order (key, index): four neighbouring threads a block count the keys
+    // above its own, or equal to it at a lower index (four keys at a time: key > own - 1 before j's four, key > own from
+    // there on, and j's own four once more for equal ones).
+    const int j = tid >> 2, seg = tid & 3, mine = (j & ~3) + seg;
+    const uint32_t own = s_key[min(j, nfull - 1)];
+    uint32_t rank = mine < j && mine < nfull && s_key[mine] == own ? 1u : 0u;
+    for (int c = 4 * seg; c < nfull; c += 16) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(s_key + c);
+      const uint32_t t = own - (c + 3 < j ? 1u : 0u);
+      rank += (k[0] > t ? 1u : 0u) + (k[1] > t ? 1u : 0u) + (k[2] > t ? 1u : 0u) + (k[3] > t ? 1u : 0u);
+    }
+    rank += dpp_u<0xB1>(rank);
+    rank += dpp_u<0x4E>(rank);
+    const bool in = seg == 0 && j < nfull && rank < static_cast<uint32_t>(P.n);
+    const uint64_t mask = wave_ballot(in);
+    if (lane == 0) s_cnt[0][0][wave] = __popcll(mask);
+    __syncthreads();
+    int to = lane_prefix(mask);
+#pragma unroll
+    for (int w = 0; w < kSelWaves; ++w) to += w < wave ? s_cnt[0][0][w] : 0;
+    if (in) out[to] = j;
+    return;
+  }
   auto key_at = [&](int j) { return in_lds ? s_key[j] : keys[j]; };
   constexpr int kReg = 4;  // keys of a thread in registers: j = tid + kSelThr i
   const bool in_reg = nfull <= kReg * kSelThr;
   uint32_t kr[kReg];
 #pragma unroll
   for (int i = 0; i < kReg; ++i) kr[i] = in_reg && tid + kSelThr * i < nfull ? s_key[tid + kSelThr * i] : 0u;
-  // the first `sink` and the last `recent` blocks are in anyway: the others compete for the remaining places
-  const int lo = min(P.sink, nfull), hi = max(nfull - P.recent, lo);  // [lo, hi) compete
   int need = P.n - (nfull - (hi - lo));
   // f(key) for the thread's keys that compete
   auto each_key = [&](auto f) {

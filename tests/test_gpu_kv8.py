@@ -478,6 +478,27 @@ def test_given_blocks(cuda):
     _check_attn(out.unsqueeze(2), _refs(k, v, lens), q.unsqueeze(2), lens, None, tokens=tokens)
 
 
+@pytest.mark.parametrize("bound", [None, 64 * 1000])
+@pytest.mark.parametrize("nb", [2, 3, 5, 63, 64, 65, 127, 128, 129, 130, 255, 256, 257, 300, 511, 513])
+def test_select_counts(cuda, nb, bound):
+    """Every way to choose, around the numbers of blocks where it changes; blocks that repeat, so that scores tie."""
+    B, H = 2, 2
+    store = _store(B, H, 64 * 1000, device=cuda)
+    k, _ = _kv(cuda, B, H, 64 * 7, seed=nb)
+    order = torch.randint(0, 7, (nb,), generator=torch.Generator().manual_seed(nb)).tolist()
+    k = torch.cat([k[:, :, 64 * j:64 * j + 64] for j in order], 2)
+    lens = [64 * nb, 64 * (nb - 1) + 63]
+    store.update(k, k, _ints(cuda, [0] * B), _ints(cuda, lens))
+    q = torch.randn(B, 4, D, generator=torch.Generator().manual_seed(2)).half().to(cuda)
+    refs = _refs(k, k, lens)
+    for blocks, sink, recent in ((1, 0, 0), (2, 1, 1), (nb // 2 + 1, 2 if nb > 4 else 0, 0), (nb, 0, 1), (max(nb - 1, 1), 0, 0)):
+        index = store.select_blocks(q, _ints(cuda, lens), blocks, sink, recent, max_len=bound)
+        for b in range(B):
+            for h in range(H):
+                want = choose(refs[b][h], query(q[b, 2 * h:2 * h + 2].cpu()), blocks, sink, recent)
+                assert index[b, h].tolist() == want + [-1] * (blocks - len(want)), (blocks, b, h)
+
+
 @pytest.mark.parametrize("sink,recent,blocks", [(3, 4, 7), (0, 0, 1), (5, 0, 5), (0, 6, 6), (2, 2, 60)])
 def test_select_forced_blocks(cuda, sink, recent, blocks):
     """No place left for the others, no forced block, as many places as blocks."""
