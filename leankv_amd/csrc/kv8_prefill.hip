@@ -15,13 +15,16 @@
 // the exponentials of this one, values of this one beside the next one's offsets and the staging.
 //
 // What bounds it: two waves per SIMD (240 registers each); per block and wave 1024 cycles of products and about 170 vector
-// instructions (4.4 cycles each, 8.8 an exponential, with two waves), 3300 cycles for both waves, LDS reads at a third of
-// their rate.  4096 tokens, 32/8 heads: 143-147 us (940-975 TFLOP/s; the library's fp16 product of 8192^3 1069), chunks of
-// 4 x 512 over 8192 tokens 255 us (1040 TFLOP/s).  Measured on the way: products and softmax one after the other 167 us;
-// half of the waves a phase behind, with a barrier a phase 158 us; the interleaving with the exponentials left to the
-// compiler 160 us (they move behind the staging); staging without branches, workgroups that stay and the exponentials held
-// in place 147 us; output rows through LDS 143 us.  Operands 4, 5 or 6 products ahead make no difference.  What is left
-// outside the blocks is a piece's start (10-13 k cycles: lengths, queries, first blocks) and end (4.4 k), 2 a workgroup.
+// instructions (4.5 to 6 cycles each, 12 an exponential, with two waves), 3100 cycles for both waves.  Two exponentials,
+// four other instructions and an LDS read beside a product take 47 cycles by themselves, a product alone 32.  4096 tokens,
+// 32/8 heads: 139-147 us (935-985 TFLOP/s; the library's fp16 product of 8192^3 1069; matrix units busy 54 % of the
+// cycles, vector units 59 %, LDS 36 %), chunks of 4 x 512 over 8192 tokens 245 us (1086 TFLOP/s).  Measured on the way:
+// products and softmax one after the other 167 us; half of the waves a phase behind, with a barrier a phase 158 us; the
+// interleaving with the exponentials left to the compiler 160 us (they move behind the staging); staging without branches,
+// workgroups that stay and the exponentials held in place 147 us; output rows through LDS 143 us; staging without bank
+// conflicts 139-142 us, chunks 255 to 245 us.  No faster: operands 5 or 6 products ahead, a third key buffer, no running
+// maximum (the sum of weights as the check), exponentials moved beside the value products.  What is left outside the blocks
+// is a piece's start (10-13 k cycles: lengths, queries, first blocks) and end (4.4 k), 2 a workgroup.
 #include "kv8_common.h"
 
 namespace lkv {
