@@ -148,6 +148,11 @@ class KV8Store:
         new.v_tail.copy_(self.v_tail)
         return new
 
+    def __deepcopy__(self, memo):
+        """A store of its own with the same contents (a prompt's cache that several continuations start from)."""
+        new = memo[id(self)] = self.grown(self.capacity)
+        return new
+
     # ------------------------------------------------------------------------------------------------ checks
     def _call(self, name: str, *args):
         """One C entry on the store's device and that device's current stream."""

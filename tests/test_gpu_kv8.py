@@ -555,6 +555,66 @@ def test_other_stream_and_graph(cuda):
     assert torch.equal(on_side, eager.decode_attention(q, after))
 
 
+def test_two_graphs_and_threads_at_once(cuda):
+    """Calls in flight together (two graphs on two streams, two threads on two more) share no workspace."""
+    import threading
+
+    n = 64 * 200 + 9
+    k, v = _kv(cuda, 1, 2, n, seed=31)
+    store = _store(1, 2, n, device=cuda)
+    store.update(k, v, _ints(cuda, [0]))
+    lens = _ints(cuda, [n])
+    qs = [torch.randn(1, 8, D, generator=torch.Generator().manual_seed(i)).half().to(cuda) for i in range(4)]
+
+    def step(q):
+        return (store.decode_attention(q, lens), *store.sparse_decode_attention(q, lens, 40),
+                store.prefill_attention(q.unsqueeze(2).expand(-1, -1, 70, -1), lens))
+
+    want = [step(q) for q in qs]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(4)], [], []
+    for q, s in zip(qs[:2], streams):
+        g = torch.cuda.CUDAGraph()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+            outs.append(step(q))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            got[i] = [step(qs[i]) for _ in range(30)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (2, 3)]
+    for t in threads:
+        t.start()
+    for _ in range(30):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+    for i in (2, 3):
+        assert len(got[i]) == 30 and all(torch.equal(a, b) for r in got[i] for a, b in zip(r, want[i]))
+
+
+def test_deepcopy_is_a_store_of_its_own(cuda):
+    import copy
+
+    k, v = _kv(cuda, 2, 2, 200, seed=7)
+    store = _store(2, 2, 300, device=cuda)
+    store.update(k[:, :, :100], v[:, :, :100], _ints(cuda, [0, 0]))
+    other = copy.deepcopy(store)
+    store.update(k[:, :, 100:], v[:, :, 100:], _ints(cuda, [100, 100]))
+    other.update(k[:, :, :70], v[:, :, :70], _ints(cuda, [100, 100]))
+    _check_store(store, _refs(k, v, [200, 200]), k, v, [200, 200])
+    ok, ov = torch.cat([k[:, :, :100], k[:, :, :70]], 2), torch.cat([v[:, :, :100], v[:, :, :70]], 2)
+    _check_store(other, _refs(ok, ov, [170, 170]), ok, ov, [170, 170])
+
+
 def test_offsets_past_32_bits(cuda):
     """A store whose codes pass 2^32 bytes: tokens at its end."""
     B, H, cap = 5, 8, 64 * 16400  # 5 x 8 x 16400 blocks x 8192 bytes: 5.4e9

@@ -96,6 +96,26 @@ def test_padded_batch_takes_the_masked_path(cuda):
     assert _close(got, plain) < RTOL
 
 
+def test_copies_of_a_prompt_go_their_own_ways(cuda):
+    """A prompt's cache copied for two continuations: each as from a prompt of its own."""
+    import copy
+
+    from leankv_amd.combined import optimize_model
+    from leankv_amd.kv8 import BlockInt8Cache
+
+    model, cache = optimize_model(_model(cuda, 3), kv8=True, max_seq_len=128)
+    prompt, tails = _ids(100, 1).to(cuda), [_ids(40, s).to(cuda) for s in (2, 3)]
+    with torch.no_grad():
+        model(prompt, past_key_values=cache, use_cache=True)
+        for tail in tails:
+            mine = copy.deepcopy(cache)
+            got = model(tail, past_key_values=mine, use_cache=True).logits
+            fresh = BlockInt8Cache(num_layers=mine.num_layers, max_seq_len=128, device=cuda, fused_attention=True)
+            model(prompt, past_key_values=fresh, use_cache=True)
+            assert torch.equal(got, model(tail, past_key_values=fresh, use_cache=True).logits)
+            assert mine.get_seq_length() == 140 and cache.get_seq_length() == 100
+
+
 def test_unattended_update_raises(cuda):
     from leankv_amd.kv8 import BlockInt8Cache
 
