@@ -28,7 +28,7 @@
 // score has two roundings (the query's scale, the block's) whatever the order of the work, and the choice is the same
 // everywhere.  Then a selection per (sequence, kv head), by the same workgroup up to 512 blocks: by counting up to 128, by
 // radix passes beyond.  Bound by latency: 128 blocks 6.0 us a call in a replayed graph, 300 of 16 sequences 8.7 us; 2048
-// blocks 3.9 (scores) + 6.4 us.
+// blocks 10.2 us, the scores in a launch of their own.
 #include "kv8_common.h"
 
 namespace lkv {
@@ -578,7 +578,8 @@ __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
   __shared__ __align__(16) uint32_t s_key[kLdsKeys];
   __shared__ __align__(16) uint32_t s_hist[4][256];
   __shared__ uint32_t s_or[kSelWaves], s_nor[kSelWaves];
-  __shared__ int s_cnt[2][2][kSelWaves];
+  constexpr int kReg = 4;  // keys of a thread in registers: j = tid + kSelThr i
+  __shared__ __align__(16) int s_cnt[kReg][2][kSelWaves];
   __shared__ __align__(16) QueryCodes s_q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -681,7 +682,6 @@ __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
     return;
   }
   auto key_at = [&](int j) { return in_lds ? s_key[j] : keys[j]; };
-  constexpr int kReg = 4;  // keys of a thread in registers: j = tid + kSelThr i
   const bool in_reg = nfull <= kReg * kSelThr;
   uint32_t kr[kReg];
 #pragma unroll
@@ -754,6 +754,40 @@ __global__ __launch_bounds__(kSelThr) void select_kernel(SelectArgs P) {
   }
   // the first and last blocks, the keys above `prefix` and the first `need` equal to it, in index order
   int base_gt = 0, base_eq = 0;
+  // All counts at once and one barrier, where a round for each 512 keys would be three or more (2048 blocks 11.1 -> 10.2 us a
+  // call; 1024 9.3 and 9.4, 512 9.7 and 10.2).
+  if (in_reg && nfull > 2 * kSelThr) {
+    uint64_t mg[kReg], me[kReg];
+#pragma unroll
+    for (int i = 0; i < kReg; ++i) {
+      const int j = tid + kSelThr * i;
+      const bool in = j >= lo && j < hi;
+      mg[i] = wave_ballot(j < nfull && (!in || kr[i] > prefix));
+      me[i] = wave_ballot(in && kr[i] == prefix);
+      if (lane == 0) {
+        s_cnt[i][0][wave] = __popcll(mg[i]);
+        s_cnt[i][1][wave] = __popcll(me[i]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kReg; ++i) {
+      int gt_before = base_gt + lane_prefix(mg[i]), eq_before = base_eq + lane_prefix(me[i]);
+#pragma unroll
+      for (int w = 0; w < kSelWaves; ++w) {
+        const int cg = s_cnt[i][0][w], ce = s_cnt[i][1][w];
+        if (w < wave) {
+          gt_before += cg;
+          eq_before += ce;
+        }
+        base_gt += cg;
+        base_eq += ce;
+      }
+      if ((mg[i] >> lane & 1) || ((me[i] >> lane & 1) && eq_before < need))
+        out[gt_before + min(eq_before, need)] = tid + kSelThr * i;
+    }
+    return;
+  }
   for (int j0 = 0, it = 0; j0 < nfull; j0 += kSelThr, it ^= 1) {
     const int j = j0 + tid;
     const bool in = j >= lo && j < hi;

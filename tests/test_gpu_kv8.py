@@ -427,15 +427,19 @@ def test_sparse_ties_take_the_lower_index(cuda):
     assert (index.cpu() == torch.cat([torch.arange(299), torch.arange(699, 700)])).all()
 
 
-def test_sparse_many_blocks(cuda):
-    """More blocks than the selection keeps in LDS, against a stable sort of the same scores."""
-    nb = 9001
+@pytest.mark.parametrize("nb,n", [(1024, 9), (1025, 40), (1600, 700), (2047, 3), (2048, 500), (2049, 500), (9001, 500)])
+@pytest.mark.parametrize("tied", [False, True])
+def test_sparse_many_blocks(cuda, nb, n, tied):
+    """More blocks than one round's, than the selection keeps in registers and in LDS, against a stable sort of the same
+    scores."""
     store = _store(1, 1, 64 * nb, device=cuda)
     g = torch.Generator(device=cuda).manual_seed(1)
     k = torch.randn(1, 1, 64 * nb, D, generator=g, device=cuda).half()
+    if tied:
+        k = k[:, :, :64 * 13].repeat(1, 1, nb // 13 + 1, 1)[:, :, :64 * nb].contiguous()
     store.update(k, k, _ints(cuda, [0]))
     q = torch.randn(1, 2, D, generator=g, device=cuda).half()
-    index = store.select_blocks(q, _ints(cuda, [64 * nb]), 500, 1, 1)
+    index = store.select_blocks(q, _ints(cuda, [64 * nb]), n, 1, 1)
     lo, hi = store.ranges[0, 0, :, 0].double(), store.ranges[0, 0, :, 1].double()
     best = None
     for row in q[0].float():
@@ -445,7 +449,7 @@ def test_sparse_many_blocks(cuda):
         best = sc if best is None else torch.maximum(best, sc)
     score = best * store.scales[0, 0, :, 0]
     score[0] = score[-1] = float("inf")
-    want = torch.sort(score, descending=True, stable=True).indices[:500].sort().values
+    want = torch.sort(score, descending=True, stable=True).indices[:n].sort().values
     assert torch.equal(index[0, 0].long(), want)
 
 
