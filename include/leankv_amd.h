@@ -663,7 +663,9 @@ int lkv_decode_head(const lkv_decode_dims* dims, const void* final_norm, const v
  *   scale = amax * s, code = rint(x * (127 * (1 / amax))), value = code * scale
  * (fp32, each operation rounded; s = fp32(1 / 127), amax over the block's
  * 64 x 128 fp16 numbers; a zero block has scale 0 and codes 0); the unfinished
- * last block of a sequence is fp16.  What is stored is finite: inputs are
+ * last block of a sequence is fp16 (its scales are -1), and so is, next to its
+ * codes, the last finished one: block j's fp16 tokens lie in tail j & 1.
+ * What is stored is finite: inputs are
  * rounded to fp16, numbers beyond +-65504 and infinities become +-65504, a NaN
  * becomes 0.  All buffers are 16-byte aligned device
  * memory of the caller, cleared once before the first use.  A code is stored
@@ -677,8 +679,8 @@ typedef struct lkv_kv8_store {
   void* scales;  /* fp32  [batch][kv_heads][blocks][2]: key, value        */
   void* ranges;  /* int8  [batch][kv_heads][blocks][2][128]: lowest and
                     highest key code of each dim                          */
-  void* k_tail;  /* fp16  [batch][kv_heads][64][128]                      */
-  void* v_tail;  /* fp16  [batch][kv_heads][128][64]                      */
+  void* k_tail;  /* fp16  [batch][kv_heads][2][64][128]                   */
+  void* v_tail;  /* fp16  [batch][kv_heads][2][128][64]                   */
   int64_t batch, kv_heads, blocks;
 } lkv_kv8_store;
 
@@ -689,10 +691,12 @@ typedef struct lkv_kv8_store {
  * pos[b] must be what it holds.  n_new (optional) gives how many of the S
  * tokens are the sequence's (a padded batch: the rest is not read).  Tokens
  * past the store are dropped, a position outside it stores nothing.
- * A sequence may be taken back (a smaller pos and length from then on) to any
- * length within its unfinished block and to any multiple of 64; a finished
- * block is not opened again: to drop some of its tokens, take the sequence
- * back to its start and store the others anew.
+ * A sequence may be taken back (a smaller pos and length from then on): to any
+ * multiple of 64, where it begins anew, or, no further than where it began, to
+ * any length from 64 * (n / 64 - 1) on, n the most tokens that it has held
+ * since then (drafted tokens may be dropped across the end of a block).  An
+ * older block is not opened again: to drop some of its tokens, take the
+ * sequence back to its start and store the others anew.
  */
 int lkv_kv8_update(const lkv_kv8_store* store, const void* k, const int64_t* k_strides, const void* v,
                    const int64_t* v_strides, int dtype, int64_t S, const int32_t* pos, const int32_t* n_new,

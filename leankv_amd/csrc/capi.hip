@@ -29,6 +29,6 @@ int device_cu_count() {
 
 }  // namespace lkv
 
-extern "C" int lkv_version(void) { return 100; }
+extern "C" int lkv_version(void) { return 101; }
 
 extern "C" const char* lkv_last_error(void) { return lkv::g_err; }

@@ -259,8 +259,8 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(SplitArgs P) {
   }
   // ---- the unfinished block, by the wave whose turn it is
   if (rest && u1 == units && (nlist - u0) % kWaves == wave) {
-    const uint16_t* kt = st.k_tail + bh * kBlkBytes + c16 * kD + 16 * g;
-    const uint16_t* vt = st.v_tail + bh * kBlkBytes + c16 * kBlk + 16 * g;
+    const uint16_t* kt = tail_ptr(st, false, bh, nfull) + c16 * kD + 16 * g;
+    const uint16_t* vt = tail_ptr(st, true, bh, nfull) + c16 * kBlk + 16 * g;
     step(
         [&](int T, int ks) {
           return *reinterpret_cast<const f16x8*>(kt + T * 16 * kD + 64 * (ks >> 1) + 8 * (ks & 1));

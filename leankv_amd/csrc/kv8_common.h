@@ -6,7 +6,8 @@
 // code + 128.  Keys lie [token][dim].  Values lie [dim][position], so that the value product reads its operand (8 tokens
 // of one dim per lane) as it lies in memory, with no transpose in the attention kernels; position 16 g + 8 ks + 4 t + i
 // holds token 32 ks + 16 t + 4 g + i: the tokens whose weights lane group g of a wave has after the 16-row score products
-// 2 ks and 2 ks + 1.  The unfinished block of a head is fp16 in the same two layouts.
+// 2 ks and 2 ks + 1.  The unfinished block of a head is fp16 in the same two layouts.  So is, next to its codes, the last
+// finished one, so that a sequence can be taken back into it: block j's fp16 tokens lie in tail j & 1.
 #pragma once
 
 #include "common.h"
@@ -39,10 +40,16 @@ struct Store {
   uint8_t* v_codes;   // [B][Hkv][blocks][128][64]
   float* scales;      // [B][Hkv][blocks][2]: key, value
   int8_t* ranges;     // [B][Hkv][blocks][2][128]: lowest and highest key code of a dim
-  uint16_t* k_tail;   // fp16 [B][Hkv][64][128]
-  uint16_t* v_tail;   // fp16 [B][Hkv][128][64]
+  uint16_t* k_tail;   // fp16 [B][Hkv][2][64][128]
+  uint16_t* v_tail;   // fp16 [B][Hkv][2][128][64]
   int Hkv, blocks;
 };
+
+// Block j's fp16 tokens of (sequence, kv head) bh.
+__device__ __forceinline__ uint16_t* tail_ptr(const Store& st, bool values, int64_t bh, int64_t j) {
+  return (values ? st.v_tail : st.k_tail) + (2 * bh + (j & 1)) * kBlkBytes;
+}
+constexpr float kOpenScale = -1.f;  // in the scales' place of an unfinished block
 
 // Value position of the dword of tokens 4 a .. 4 a + 3 (a = 8 ks + 4 t + g -> 4 g + 2 ks + t).
 __host__ __device__ __forceinline__ constexpr int v_dword(int a) { return 4 * (a & 3) + (a >> 2); }

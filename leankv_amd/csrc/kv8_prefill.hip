@@ -290,20 +290,11 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(PrefillArgs P) {
     }
     // ---- the unfinished block: fp16 as it is
     if (rest) {
-      if (key_thr) {
-        const uint16_t* p = st.k_tail + bh * kBlkBytes + src_off;
+      const uint16_t* p = tail_ptr(st, !key_thr, bh, blk0 + nf) + src_off;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint2 a = *reinterpret_cast<const uint2*>(p + 4 * k), c = *reinterpret_cast<const uint2*>(p + 16 + 4 * k);
-          *reinterpret_cast<u32x4*>(dst + 16 * k) = u32x4{a.x, a.y, c.x, c.y};
-        }
-      } else {
-        const uint16_t* p = st.v_tail + bh * kBlkBytes + src_off;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint2 a = *reinterpret_cast<const uint2*>(p + 4 * k), c = *reinterpret_cast<const uint2*>(p + 32 + 4 * k);
-          *reinterpret_cast<u32x4*>(dst + 16 * k) = u32x4{a.x, a.y, c.x, c.y};
-        }
+      for (int k = 0; k < 4; ++k) {
+        const uint2 a = *reinterpret_cast<const uint2*>(p + 4 * k), c = *reinterpret_cast<const uint2*>(p + src2 + 4 * k);
+        *reinterpret_cast<u32x4*>(dst + 16 * k) = u32x4{a.x, a.y, c.x, c.y};
       }
       __syncthreads();
       score_products(0);

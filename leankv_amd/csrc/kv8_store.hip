@@ -105,12 +105,17 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
   const int64_t bh = static_cast<int64_t>(b) * st.Hkv + h;
   const void* x = P.x[which];
   const int64_t xrow = b * P.sb[which] + h * P.sh[which] + 8 * c;
-  uint16_t* tail = (which ? st.v_tail : st.k_tail) + bh * kBlkBytes;
+  auto tail_of = [&](int64_t j) { return tail_ptr(st, which, bh, j); };
+  // the unfinished block behind the new tokens, and whether the last finished one shares the tail that the first
+  // workgroup reads
+  const int64_t open = p1 / kBlk, before = p0 / kBlk;
+  const bool shared = open - 1 > before && !((open - 1 - before) & 1) && p0 % kBlk;
 
   if (done) {
     u32x4 v[4];  // token 4 a + i: fp16 pairs of its 8 dims
-    // tokens from the old tail: those before p0 (none but in the first block)
+    // older tokens of the block: those before p0 (none but in the first block)
     const int old = first ? static_cast<int>(p0 - t0) : 0;
+    uint16_t* const tail = tail_of(blk);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 4 * a + i;
@@ -215,24 +220,45 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
         *reinterpret_cast<u32x4*>(st.v_codes + at * kBlkBytes + d * kBlk + 4 * q) = u32x4{s[0], s[1], s[2], s[3]};
       }
     }
+    // the last finished block's new tokens, as they are.  From the registers and behind the barriers, which wait for
+    // stores: a token that finishes a block of 64 sequences, with its read-back, 16.1 us (before them 16.6, not kept at
+    // all 15.1); read again 16.2, and 4096 tokens 18.5 instead of 15.1.
+    if (blk == open - 1 && !shared) {
+      if (!which) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * a + i >= old) *reinterpret_cast<u32x4*>(tail + (4 * a + i) * kD + 8 * c) = v[i];
+      } else if (4 * a + 3 >= old) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // the four tokens of a dim (older ones among them as they were)
+          const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+          *reinterpret_cast<uint2*>(tail + (8 * c + j) * kBlk + 4 * v_dword(a)) =
+              uint2{__builtin_amdgcn_perm(v[1][j >> 1], v[0][j >> 1], sel), __builtin_amdgcn_perm(v[3][j >> 1], v[2][j >> 1], sel)};
+        }
+      }
+    }
   }
   if (!first) return;
-  // the new tail: the tokens of the unfinished last block, in its slots
-  __syncthreads();  // (every read of the old tail is done)
-  const int64_t tt = p1 / kBlk * kBlk;
+  // the new tokens of the unfinished block, and of the last finished one where its own workgroup left them, in their slots
+  __syncthreads();  // (every read of older tokens is done)
+  if (tid == 0 && p1 > open * kBlk) st.scales[2 * (bh * st.blocks + open) + which] = kOpenScale;
+#pragma unroll 1
+  for (int64_t j = shared ? open - 1 : open; j <= open; ++j) {
+    uint16_t* const tail = tail_of(j);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int slot = 4 * a + i;
-    const int64_t t = tt + slot;
-    if (t < p0 || t >= p1) continue;
-    const u32x4 y = load_kv8<DT>(x, xrow + (t - p0) * P.ss[which]);
-    if (!which) {
-      *reinterpret_cast<u32x4*>(tail + slot * kD + 8 * c) = y;
-    } else {
+    for (int i = 0; i < 4; ++i) {
+      const int slot = 4 * a + i;
+      const int64_t t = j * kBlk + slot;
+      if (t < p0 || t >= p1) continue;
+      const u32x4 y = load_kv8<DT>(x, xrow + (t - p0) * P.ss[which]);
+      if (!which) {
+        *reinterpret_cast<u32x4*>(tail + slot * kD + 8 * c) = y;
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        tail[(8 * c + 2 * j) * kBlk + v_pos(slot)] = static_cast<uint16_t>(y[j] & 0xffffu);
-        tail[(8 * c + 2 * j + 1) * kBlk + v_pos(slot)] = static_cast<uint16_t>(y[j] >> 16);
+        for (int k = 0; k < 4; ++k) {
+          tail[(8 * c + 2 * k) * kBlk + v_pos(slot)] = static_cast<uint16_t>(y[k] & 0xffffu);
+          tail[(8 * c + 2 * k + 1) * kBlk + v_pos(slot)] = static_cast<uint16_t>(y[k] >> 16);
+        }
       }
     }
   }
@@ -296,7 +322,7 @@ __global__ __launch_bounds__(kThr) void read_kernel(ReadArgs P) {
           w[i][j] = vals(codes2h(__builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x0c0c0400u + 0x0101u * i), kSelLo));
     }
   } else if (t0 < len) {
-    const uint16_t* tail = (which ? st.v_tail : st.k_tail) + bh * kBlkBytes;
+    const uint16_t* tail = tail_ptr(st, which, bh, blk);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 4 * a + i;

@@ -4,7 +4,8 @@ Every finished block of 64 tokens of a kv head is held as one byte a number with
 for its values (amax / 127; no rotation, no codebook); the unfinished last block of a sequence is fp16.  A stored token
 costs 256 bytes a kv head instead of 512, and a number is off by at most half a code, amax / 254.  For each finished
 block the store also keeps the lowest and the highest key code of every dim, from which the sparse decode attention
-finds the blocks worth reading.
+finds the blocks worth reading; of the last finished block it keeps the fp16 tokens too, so that a sequence can be taken
+back into it (drafted tokens that were not accepted).
 
 The store does not know its sequences' lengths: they live with the caller, as int32 device tensors that every call
 takes, so that a decode step can be captured into a HIP graph and replayed with other lengths.  Nothing here
@@ -121,10 +122,11 @@ class KV8Store:
         self.v_codes = zeros(self.blocks, HEAD_DIM, BLOCK, dtype=torch.uint8)
         self.scales = zeros(self.blocks, 2, dtype=torch.float32)
         self.ranges = zeros(self.blocks, 2, HEAD_DIM, dtype=torch.int8)
-        self.k_tail = zeros(BLOCK, HEAD_DIM, dtype=torch.float16)
-        self.v_tail = zeros(HEAD_DIM, BLOCK, dtype=torch.float16)
+        # fp16 tokens of the last two blocks, block j's in [:, :, j & 1]
+        self.k_tails = zeros(2, BLOCK, HEAD_DIM, dtype=torch.float16)
+        self.v_tails = zeros(2, HEAD_DIM, BLOCK, dtype=torch.float16)
         self._struct = _lib.KV8StoreStruct(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.scales.data_ptr(),
-                                           self.ranges.data_ptr(), self.k_tail.data_ptr(), self.v_tail.data_ptr(),
+                                           self.ranges.data_ptr(), self.k_tails.data_ptr(), self.v_tails.data_ptr(),
                                            self.batch, self.kv_heads, self.blocks)
         self._ref = ctypes.byref(self._struct)
         self._index = self.device.index
@@ -137,15 +139,30 @@ class KV8Store:
     def nbytes(self) -> int:
         """Device bytes of the store."""
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.scales, self.ranges,
-                                                          self.k_tail, self.v_tail))
+                                                          self.k_tails, self.v_tails))
+
+    def _open(self, tails: torch.Tensor) -> torch.Tensor:
+        """Of every sequence and head the tail of its unfinished block, which the update left with scales of -1."""
+        block = (self.scales[..., 0] < 0).int().argmax(-1)  # (the lowest such)
+        return torch.where((block & 1).bool()[..., None, None], tails[:, :, 1], tails[:, :, 0])
+
+    @property
+    def k_tail(self) -> torch.Tensor:
+        """fp16 [batch, kv_heads, 64, 128]: a copy of the unfinished blocks' keys, as the newest update left them."""
+        return self._open(self.k_tails)
+
+    @property
+    def v_tail(self) -> torch.Tensor:
+        """fp16 [batch, kv_heads, 128, 64]: the same of their values, in the order of the codes."""
+        return self._open(self.v_tails)
 
     def grown(self, capacity: int) -> "KV8Store":
         """A store of `capacity` tokens that holds what this one does."""
         new = KV8Store(self.batch, self.kv_heads, max(capacity, self.capacity), self.device)
         for name in ("k_codes", "v_codes", "scales", "ranges"):
             getattr(new, name)[:, :, :self.blocks] = getattr(self, name)
-        new.k_tail.copy_(self.k_tail)
-        new.v_tail.copy_(self.v_tail)
+        new.k_tails.copy_(self.k_tails)
+        new.v_tails.copy_(self.v_tails)
         return new
 
     def __deepcopy__(self, memo):
@@ -203,9 +220,11 @@ class KV8Store:
         it holds already).  n_new: how many of the S are sequence b's (a padded batch; the rest is not read).  Tokens
         past the capacity are dropped.  One launch; blocks that become whole are quantized.
 
-        A sequence may be taken back (a smaller pos and length from then on) to any length within its unfinished block
-        and to any multiple of 64.  A finished block is not opened again: to drop some of its tokens, take the sequence
-        back to its start and store the others anew (read gives them as they are held)."""
+        A sequence may be taken back (a smaller pos and length from then on): to any multiple of 64, where it begins anew,
+        or, no further than where it began, to any length from 64 * (n // 64 - 1) on, n the most tokens that it has held
+        since then (so up to 64 drafted tokens may be dropped wherever blocks end).  An older block is not opened again:
+        to drop some of its tokens, take the sequence back to its start and store the others anew (read gives them as they
+        are held)."""
         what = "KV8Store.update"
         nk, nv = k.shape, v.shape
         for t, n, name in ((k, nk, "k"), (v, nv, "v")):
