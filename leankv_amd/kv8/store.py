@@ -68,6 +68,26 @@ def _in_place(shape, strides, t: torch.Tensor):
     return _strides3(b, h, s)
 
 
+@functools.lru_cache(maxsize=256)
+def _apart(sizes, strides) -> bool:
+    """Whether rows of 128 numbers at these strides lie apart from each other (outputs are written by many workgroups at
+    once)."""
+    dims = sorted((st, n) for n, st in zip(sizes, strides) if n != 1)
+    if not all(n for _, n in dims):
+        return True
+    end = HEAD_DIM  # numbers from the first to the last of the sizes so far
+    for st, n in dims:
+        if st < end:
+            break
+        end += st * (n - 1)
+    else:
+        return True
+    at = torch.zeros(1, dtype=torch.int64, device="cpu")  # rows of one size between those of another: look at every row
+    for st, n in dims:
+        at = (at.unsqueeze(1) + st * torch.arange(n, device="cpu")).flatten()
+    return bool((at.sort().values.diff() >= HEAD_DIM).all())
+
+
 def _rows(t: torch.Tensor):
     """(t or a copy of it, strides) for t [B, H, S, 128] that is read."""
     strides = _in_place(t.shape, t.stride(), t)
@@ -260,7 +280,8 @@ class KV8Store:
         among it): [batch, heads, 128] in q's type.  A sequence of length 0 gives zeros.  max_len: the caller's bound on
         lens (default the capacity), which the work is split for.  scale: 1 / sqrt(128) by default.  index: int32
         [batch, kv_heads, n], only these finished blocks of a kv head (as select_blocks gives them; others than finished
-        ones are skipped, one listed twice counts twice) and the unfinished one."""
+        ones are skipped, one listed twice counts twice) and the unfinished one.  out: a buffer like q whose rows are
+        dense, 16-byte aligned and apart from each other (q itself may be it)."""
         what = "KV8Store.decode_attention"
         heads, dtype = self._queries(q, 3, what)
         p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
@@ -278,6 +299,8 @@ class KV8Store:
                 or _in_place((self.batch, heads, 1), (*out.stride()[:2], 0, out.stride(2)), out) is None:
             raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
                               % (what, q.dtype, tuple(q.shape), q.device))
+        elif not _apart(tuple(out.shape[:2]), out.stride()[:2]):
+            raise LeanKVError("%s: rows of out overlap, strides %s" % (what, out.stride()))
         q, qs = _query_rows(q)
         os = _strides3(out.stride(0), out.stride(1), 0)
         nbytes = _attn_bytes(self.batch, heads, self.kv_heads, 1, L, n)
@@ -291,7 +314,8 @@ class KV8Store:
                           out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention of the S newest tokens' queries q [batch, heads, S, 128] (after their update): query i of a
         sequence with q_lens[b] of them (default S, at most its length) sees tokens 0 .. lens[b] - q_lens[b] + i.  Rows
-        from q_lens[b] on are zeros.  Returns [batch, heads, S, 128] in q's type, laid out [batch, S, heads, 128]."""
+        from q_lens[b] on are zeros.  Returns [batch, heads, S, 128] in q's type, laid out [batch, S, heads, 128], or out
+        (as for decode_attention)."""
         what = "KV8Store.prefill_attention"
         heads, dtype = self._queries(q, 4, what)
         p, L = self._ints(lens, what, "lens"), self._bound(max_len, what)
@@ -299,6 +323,8 @@ class KV8Store:
         S = q.shape[2]
         if out is None:  # laid out token by token, as an output projection reads it
             out = q.new_empty((self.batch, S, heads, HEAD_DIM)).transpose(1, 2)
+        elif out.dim() == 4 and not _apart(tuple(out.shape[:3]), out.stride()[:3]):
+            raise LeanKVError("%s: rows of out overlap, strides %s" % (what, out.stride()))
         os = _in_place(q.shape, out.stride(), out) if out.dim() == 4 else None
         if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or os is None:
             raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
