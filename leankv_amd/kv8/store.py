@@ -295,14 +295,15 @@ class KV8Store:
             n, list_ = index.shape[2], index.data_ptr()
         if out is None:
             out = q.new_empty((self.batch, heads, HEAD_DIM))
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device \
-                or _in_place((self.batch, heads, 1), (*out.stride()[:2], 0, out.stride(2)), out) is None:
-            raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
-                              % (what, q.dtype, tuple(q.shape), q.device))
-        elif not _apart(tuple(out.shape[:2]), out.stride()[:2]):
-            raise LeanKVError("%s: rows of out overlap, strides %s" % (what, out.stride()))
+            os = _strides3(heads * HEAD_DIM, HEAD_DIM, 0)
+        else:
+            os = None if out.dim() != 3 else _in_place((self.batch, heads, 1), (*out.stride()[:2], 0, out.stride(2)), out)
+            if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or os is None:
+                raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
+                                  % (what, q.dtype, tuple(q.shape), q.device))
+            if not _apart(tuple(out.shape[:2]), out.stride()[:2]):
+                raise LeanKVError("%s: rows of out overlap, strides %s" % (what, out.stride()))
         q, qs = _query_rows(q)
-        os = _strides3(out.stride(0), out.stride(1), 0)
         nbytes = _attn_bytes(self.batch, heads, self.kv_heads, 1, L, n)
         ws = self._workspace(nbytes)
         self._call("lkv_kv8_attn", q.data_ptr(), qs, dtype, heads, 1, p, None, L, list_, n,

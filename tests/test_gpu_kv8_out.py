@@ -1,4 +1,5 @@
-"""Output buffers of KV8Store's attention: over the queries, and no rows over each other."""
+"""Output buffers of KV8Store's attention: over the queries, any strides that single sizes may have, and no
+rows over each other."""
 import pytest
 import torch
 from kv8_ref import D
@@ -36,3 +37,15 @@ def test_over_its_own_queries(cuda, S, n):
     q = torch.randn(2, 10, S, D, generator=torch.Generator().manual_seed(4)).half().to(cuda)
     want = store.prefill_attention(q, lens)
     assert store.prefill_attention(q, lens, out=q) is q and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("B,H,Hq", [(1, 1, 1), (1, 2, 4), (3, 1, 1)])
+def test_strides_of_single_sizes_are_free(cuda, B, H, Hq):
+    store, lens = _store(cuda, B, H, 100, seed=1)
+    q = torch.randn(B, Hq, D, generator=torch.Generator().manual_seed(2)).half().to(cuda)
+    want = store.decode_attention(q, lens)
+    strides = (1 if B == 1 else Hq * D, 3 if Hq == 1 else D, 1)
+    out = torch.zeros(B * Hq * D, dtype=q.dtype, device=cuda).as_strided((B, Hq, D), strides)
+    assert store.decode_attention(q, lens, out=out) is out and torch.equal(out, want)
+    out4 = torch.zeros(B * Hq * D, dtype=q.dtype, device=cuda).as_strided((B, Hq, 1, D), (*strides[:2], 5, 1))
+    assert torch.equal(store.prefill_attention(q.unsqueeze(2), lens, out=out4).squeeze(2), want)

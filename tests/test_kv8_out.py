@@ -62,3 +62,12 @@ def test_rows_over_each_other_are_refused(shape, strides):
 def test_rows_apart_are_taken(shape, strides):
     with pytest.raises(Reached):
         (_decode if len(shape) == 3 else _prefill)(_strided(shape, strides))
+
+
+@pytest.mark.parametrize("shape,strides,passed", [
+    ((1, 4, D), (1, D, 1), (0, D, 0)), ((3, 1, D), (2 * D, 3, 1), (2 * D, 0, 0)), ((1, 1, D), (7, 5, 1), (0, 0, 0)),
+    ((1, 2, 1, D), (3, D, 5, 1), (0, D, 0))])
+def test_strides_of_single_sizes_are_free(shape, strides, passed):
+    with pytest.raises(Reached) as e:
+        (_decode if len(shape) == 3 else _prefill)(_strided(shape, strides))
+    assert e.value.args[0][-1] == passed
