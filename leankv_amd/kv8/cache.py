@@ -8,7 +8,7 @@ attention implementation; a deferred update that none of its calls consumed make
 lets a single-token step read, of every head's finished blocks, only the n with the highest score (KV8Store.select_blocks)
 once there are more.
 
-No gradient flows through the stored tokens.
+No gradient flows through the stored tokens: with gradients enabled a forward pass runs, its backward pass raises.
 """
 
 from __future__ import annotations

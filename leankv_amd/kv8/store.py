@@ -19,6 +19,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import LeanKVError, check
@@ -107,6 +108,27 @@ def _query_rows(q: torch.Tensor):
     return q, strides
 
 
+def _follow(what: str, *tensors) -> bool:
+    """Whether autograd follows one of the tensors.  A forward-mode tangent would be lost at once and is refused."""
+    if getattr(forward_ad, "_current_level", -1) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise LeanKVError("%s: the 8-bit store has no forward-mode derivative" % what)
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+class _NoBackward(torch.autograd.Function):
+    """Ties an output to what autograd follows, so that a backward pass through it raises instead of leaving it out."""
+
+    @staticmethod
+    def forward(ctx, out, what, anchor):
+        ctx.what = what
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise LeanKVError("%s: the 8-bit store has no backward pass" % ctx.what)
+
+
 class KV8Store:
     """Keys and values of `batch` sequences x `kv_heads` heads of 128 dims, up to `capacity` tokens each (rounded up to
     whole blocks of 64), in 8 bits with a scale for each block and head.
@@ -120,7 +142,10 @@ class KV8Store:
 
     pos, lens, n_new and q_lens are int32 device tensors [batch]; lens counts every stored token, the queries' own among
     them, and may not pass the capacity.  Inputs are float16, bfloat16 or float32 of any strides; they are rounded to
-    float16 first (infinities and larger numbers to +-65504; a NaN key or value is stored as 0).  There is no gradient."""
+    float16 first (infinities and larger numbers to +-65504; a NaN key or value is stored as 0).  There is no gradient: a
+    backward pass through the outputs of queries, keys or values that autograd follows raises."""
+
+    _followed = False  # autograd followed keys or values that were stored
 
     def __init__(self, batch: int, kv_heads: int, capacity: int, device="cuda"):
         if batch < 1 or kv_heads < 1 or capacity < 1:
@@ -183,6 +208,7 @@ class KV8Store:
             getattr(new, name)[:, :, :self.blocks] = getattr(self, name)
         new.k_tails.copy_(self.k_tails)
         new.v_tails.copy_(self.v_tails)
+        new._followed = self._followed
         return new
 
     def __deepcopy__(self, memo):
@@ -234,6 +260,17 @@ class KV8Store:
     def _workspace(self, nbytes: int):
         return self.k_codes.new_empty(nbytes) if nbytes else None
 
+    def _output(self, out: torch.Tensor, what: str, q: torch.Tensor | None = None) -> torch.Tensor:
+        """out as the caller gets it: with autograd following q or what is stored, tied to it."""
+        follows = q is not None and _follow(what, q)
+        if not follows and not (self._followed and torch.is_grad_enabled()):
+            return out
+        return _NoBackward.apply(out, what, q if follows else torch.zeros((), device="cpu", requires_grad=True))
+
+    def _no_grad_out(self, q: torch.Tensor, what: str) -> None:
+        if _follow(what, q) or (self._followed and torch.is_grad_enabled()):
+            raise LeanKVError("%s: out= does not support autograd, which follows q or what is stored" % what)
+
     # ------------------------------------------------------------------------------------------------ storing
     def update(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, n_new: torch.Tensor | None = None) -> None:
         """Store S new tokens of every sequence: k, v [batch, kv_heads, S, 128], sequence b's at positions pos[b] .. (what
@@ -256,6 +293,8 @@ class KV8Store:
             raise LeanKVError("%s: k and v must be alike, got %s %s and %s %s"
                               % (what, k.dtype, tuple(nk), v.dtype, tuple(nv)))
         dtype = _dtype(k, what)
+        if _follow(what, k, v):
+            self._followed = True
         p = self._ints(pos, what, "pos")
         m = None if n_new is None else self._ints(n_new, what, "n_new")
         (k, ks), (v, vs) = _rows(k), _rows(v)
@@ -268,7 +307,8 @@ class KV8Store:
         if not 0 <= first <= n <= self.blocks * BLOCK:
             raise LeanKVError("%s: tokens %d .. %d outside a store of %d" % (what, first, n, self.blocks * BLOCK))
         p = self._ints(lens, what, "lens")
-        k, v = self._empty((2, self.batch, self.kv_heads, n - first, HEAD_DIM), torch.float16).unbind(0)
+        kv = self._output(self._empty((2, self.batch, self.kv_heads, n - first, HEAD_DIM), torch.float16), what)
+        k, v = kv[0], kv[1]
         self._call("lkv_kv8_read", p, first, n - first, k.data_ptr(), v.data_ptr())
         return k, v
 
@@ -294,9 +334,10 @@ class KV8Store:
                                   % (what, self.batch, self.kv_heads, self.device))
             n, list_ = index.shape[2], index.data_ptr()
         if out is None:
-            out = q.new_empty((self.batch, heads, HEAD_DIM))
+            out = self._output(q.new_empty((self.batch, heads, HEAD_DIM)), what, q)
             os = _strides3(heads * HEAD_DIM, HEAD_DIM, 0)
         else:
+            self._no_grad_out(q, what)
             os = None if out.dim() != 3 else _in_place((self.batch, heads, 1), (*out.stride()[:2], 0, out.stride(2)), out)
             if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or os is None:
                 raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
@@ -323,9 +364,11 @@ class KV8Store:
         m = None if q_lens is None else self._ints(q_lens, what, "q_lens")
         S = q.shape[2]
         if out is None:  # laid out token by token, as an output projection reads it
-            out = q.new_empty((self.batch, S, heads, HEAD_DIM)).transpose(1, 2)
-        elif out.dim() == 4 and not _apart(tuple(out.shape[:3]), out.stride()[:3]):
-            raise LeanKVError("%s: rows of out overlap, strides %s" % (what, out.stride()))
+            out = self._output(q.new_empty((self.batch, S, heads, HEAD_DIM)), what, q).transpose(1, 2)
+        else:
+            self._no_grad_out(q, what)
+            if out.dim() == 4 and not _apart(tuple(out.shape[:3]), out.stride()[:3]):
+                raise LeanKVError("%s: rows of out overlap, strides %s" % (what, out.stride()))
         os = _in_place(q.shape, out.stride(), out) if out.dim() == 4 else None
         if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or os is None:
             raise LeanKVError("%s: out must be like q, %s %s on %s, with dense 16-byte aligned rows"
@@ -371,7 +414,7 @@ class KV8Store:
         blocks, sink, recent = self._choice(blocks, sink, recent, what)
         q, qs = _query_rows(q)
         index = self._empty((self.batch, self.kv_heads, blocks), torch.int32)
-        out = q.new_empty((self.batch, heads, HEAD_DIM))
+        out = self._output(q.new_empty((self.batch, heads, HEAD_DIM)), what, q)
         nbytes = _sparse_bytes(self.batch, heads, self.kv_heads, L, blocks)
         ws = self._workspace(nbytes)
         self._call("lkv_kv8_sparse_attn", q.data_ptr(), qs, dtype, heads, p, L, blocks, sink, recent,
