@@ -39,7 +39,8 @@ class BlockInt8Cache(HFCache):
                              % (sparse_blocks, sink_blocks, recent_blocks))
         self.head_dim, self.num_layers = head_dim, num_layers
         self._device = torch.device(device) if device is not None else torch.device("cuda")
-        self._dtype = dtype  # of the K / V that update returns and that are read back (None: the keys')
+        self._asked_dtype = dtype  # of the K / V that update returns and that are read back (None: the keys')
+        self._dtype = dtype
         self._init_cap = max(int(max_seq_len), 1)
         self.fused_attention = bool(fused_attention)
         self.sparse_blocks, self.sink_blocks, self.recent_blocks = sparse_blocks, sink_blocks, recent_blocks
@@ -163,6 +164,7 @@ class BlockInt8Cache(HFCache):
         self._seq_lengths = [0] * n
         self._fused_pending, self._prefill_pending = [False] * n, [False] * n
         self._seen_tokens = 0
+        self._dtype = self._asked_dtype
 
     def get_total_cache_bytes(self) -> int:
         """Bytes that the held tokens take: codes and scales and ranges of finished blocks, fp16 of the others."""
