@@ -108,11 +108,11 @@ def _query_rows(q: torch.Tensor):
     return q, strides
 
 
-def _follow(what: str, *tensors) -> bool:
-    """Whether autograd follows one of the tensors.  A forward-mode tangent would be lost at once and is refused."""
-    if getattr(forward_ad, "_current_level", -1) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+def _follow(what: str, a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether autograd follows a or b.  A forward-mode tangent would be lost at once and is refused."""
+    if getattr(forward_ad, "_current_level", -1) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (a, b)):
         raise LeanKVError("%s: the 8-bit store has no forward-mode derivative" % what)
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    return (a.requires_grad or b.requires_grad) and torch.is_grad_enabled()
 
 
 class _NoBackward(torch.autograd.Function):
@@ -262,13 +262,13 @@ class KV8Store:
 
     def _output(self, out: torch.Tensor, what: str, q: torch.Tensor | None = None) -> torch.Tensor:
         """out as the caller gets it: with autograd following q or what is stored, tied to it."""
-        follows = q is not None and _follow(what, q)
+        follows = q is not None and _follow(what, q, q)
         if not follows and not (self._followed and torch.is_grad_enabled()):
             return out
         return _NoBackward.apply(out, what, q if follows else torch.zeros((), device="cpu", requires_grad=True))
 
     def _no_grad_out(self, q: torch.Tensor, what: str) -> None:
-        if _follow(what, q) or (self._followed and torch.is_grad_enabled()):
+        if _follow(what, q, q) or (self._followed and torch.is_grad_enabled()):
             raise LeanKVError("%s: out= does not support autograd, which follows q or what is stored" % what)
 
     # ------------------------------------------------------------------------------------------------ storing
@@ -307,8 +307,10 @@ class KV8Store:
         if not 0 <= first <= n <= self.blocks * BLOCK:
             raise LeanKVError("%s: tokens %d .. %d outside a store of %d" % (what, first, n, self.blocks * BLOCK))
         p = self._ints(lens, what, "lens")
-        kv = self._output(self._empty((2, self.batch, self.kv_heads, n - first, HEAD_DIM), torch.float16), what)
-        k, v = kv[0], kv[1]
+        kv = self._empty((2, self.batch, self.kv_heads, n - first, HEAD_DIM), torch.float16)
+        if self._followed:
+            kv = self._output(kv, what)
+        k, v = kv.unbind(0)
         self._call("lkv_kv8_read", p, first, n - first, k.data_ptr(), v.data_ptr())
         return k, v
 
