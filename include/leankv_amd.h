@@ -714,7 +714,9 @@ int lkv_kv8_read(const lkv_kv8_store* store, const int32_t* lens, int64_t first,
  * of sequence b, which has q_lens[b] of them (null: S; at most lens[b]), sees
  * tokens 0 .. lens[b] - q_lens[b] + i; rows from q_lens[b] on, and rows that see no
  * token, are zeros.  max_len is the caller's bound on lens (the work is split
- * for it); of a longer sequence the finished blocks below the bound are read.
+ * for it).  A longer sequence counts as one that ends with the last finished
+ * block below the bound: lens[b] above is then that shorter length, and the
+ * queries' positions move down with it.
  * index (optional, S = 1): int32 [batch][kv_heads][n_index], the finished
  * blocks that a kv head's queries read (entries outside the finished blocks
  * are skipped, a block listed twice counts twice) next to the unfinished

@@ -61,7 +61,7 @@ def optimize_model(model, teal_sparsity: Optional[float] = None, teal_thresholds
 
     kv8 (not in the reference): an 8-bit cache with a scale for each block of 64 tokens and head (kv8.BlockInt8Cache)
     instead of a TurboQuant one; with kv8_sparse_blocks a single-token step reads only that many of every head's
-    finished blocks, those with the highest score.
+    finished blocks, those with the highest score.  fast_decode does not apply to it: generate runs the patched HF forward.
 
     fast_decode (not in the reference): with both TEAL and TurboQuant on the HIP kernels, single-token
     decode calls of generate run the fused, graph-replayed decode step (engine.GenerateFastPath) when the

@@ -17,10 +17,14 @@
 //   combine       joins the splits' (offset, sum, rows) in fp32.
 // Bound by memory where there are many blocks: 16 KB a block and head, one 4-wave workgroup a CU with all of a block's 16
 // loads of a wave in flight.  1 x 131072 tokens (32/8 heads, 269 MB): 45 us the split kernel (6.0 TB/s; a plain read loop
-// 6.0-6.3), 51-53 us a call; 32 x 8192: 92 us (5.9 TB/s); 32 sequences of 1.6-8 K tokens 68 us, the longest of them bounds
+// 6.0-6.3), 51-53 us a call; 32 x 8192: 90-92 us (5.9 TB/s); 32 sequences of 1.6-8 K tokens 68 us, the longest of them bounds
 // it.  8 waves were no faster, nontemporal loads gained 5 % there and lost as much with many sequences.
-// Bound by latency where there are few: 1 x 4133 tokens 9.8 us in a replayed graph, 5.5 the split kernel (length, then
-// loads, then one block's 440 vector instructions, then the join) and 3.5 the combine.
+// The work is split for max_len, not for the lengths: 1 x 4133 tokens take 12 us a call with max_len (or a store) of up to
+// 8192, 13 with 32768 and 31 with 131072, where two splits hold all of them.  From one (sequence, kv head) pair a CU on a pair
+// is one workgroup's: 32 sequences of which one has 131072 tokens and the others 2048 take 770 us.
+// Bound by latency where there are few: 1 x 4133 tokens 9.2-9.8 us in a replayed graph, 5.5 the split kernel (length, then
+// loads, then one block's 440 vector instructions, then the join) and 3.5 the combine.  5 queries of 8 x 4096 tokens: four
+// blocks a wave, 16.3 us traced, of which vector work is 38 % and products 13 %; what starts and ends a split is not covered.
 //
 // Selection (lkv_kv8_select_blocks): a score per finished block, the upper bound sum_d max(q8 lo, q8 hi) of the product
 // with any of its keys, from the per-dim lowest and highest codes (256 bytes a block) and the query rows in 8 bits, on
@@ -411,7 +415,11 @@ constexpr int kLdsKeys = 8192;     // so many keys of a (sequence, kv head) stay
 // over 128 6.0 (7.6), over 256 8.7 (8.1).
 constexpr int kRankBlocks = kSelThr / 4;
 constexpr uint32_t kForcedKey = 0xfffffffeu;  // above every score's
-constexpr int kFusedBlocks = 512;  // up to so many blocks one workgroup scores and selects (2048: 36.6 us a call, apart 23.5)
+// Up to so many blocks (of max_len) one workgroup scores and selects, beyond that the scores are a launch of their own.  A
+// selection in a replayed graph, one launch against two: 300 blocks 8.6 and 8.6 us (16 sequences 8.9 and 9.9), 400 9.1 and
+// 8.4 (9.4, 9.9), 512 9.8 and 8.5 (10.4, 10.0), 640 11.8 and 9.3 (12.2, 11.8), 2048 23.0 and 10.3 (24.6, 20.8); a call outside a
+// graph pays 2.5 us for the second launch.
+constexpr int kFusedBlocks = 512;
 
 struct SelectArgs {
   Store st;

@@ -179,7 +179,8 @@ __device__ __forceinline__ float groups_sum(float v) {
 // (max passes over NaN) but is not empty: it takes 0, so that its NaN reaches the joined row.
 __device__ __forceinline__ float2 part_record(float m, float l) { return float2{l != l ? 0.f : m, l}; }
 
-// A sequence's tokens: its length, of a longer one than the caller's bound the finished blocks below the bound.
+// A sequence's tokens: its length; one that is longer than the caller's bound ends with the last finished block below it (its
+// queries' positions count from that end too).
 __device__ __forceinline__ int held_tokens(int len, int max_len) {
   return len > max_len ? max_len & ~(kBlk - 1) : max(len, 0);
 }

@@ -8,7 +8,9 @@
 // finish no block go to the fp16 tail.  The workgroup of the first touched block also writes the new tail, after its
 // own reads of the old one, so no other workgroup touches the tail.
 // Bound by memory for prompts: a value is read once (2 bytes) and written once (1 byte); 8 x 4096 tokens of 8 heads, 201 MB,
-// 36 us in a replayed graph (5.6 TB/s; a device copy 5.0).  4096 tokens of one sequence 7.0 us, one token 2.5 us, or 4.1
+// 49 us in a replayed graph that goes round six stores (4.1 TB/s; a device copy 5.0), 37 over one store, which stays in the
+// last-level cache.  Sixteen ragged prompts of up to 1201 tokens 31 us traced (2.3 TB/s): the grid is for the longest, over
+// 40 % of the workgroups find no block.  4096 tokens of one sequence 10.3 us (40 stores in turn), one token 2.8 us, or 4.5
 // where it finishes a block (an empty launch 2.1).  What a value costs in instructions matters as much: magnitudes are
 // compared as bits, two at a time, and a code is one product and one addition (10.1 -> 9.1 us for 4096 tokens, profiled).
 #include "kv8_common.h"
@@ -233,7 +235,8 @@ __global__ __launch_bounds__(kThr) void update_kernel(UpdateArgs P) {
         for (int j = 0; j < 8; ++j) {  // the four tokens of a dim (older ones among them as they were)
           const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
           *reinterpret_cast<uint2*>(tail + (8 * c + j) * kBlk + 4 * v_dword(a)) =
-              uint2{__builtin_amdgcn_perm(v[1][j >> 1], v[0][j >> 1], sel), __builtin_amdgcn_perm(v[3][j >> 1], v[2][j >> 1], sel)};
+              uint2{__builtin_amdgcn_perm(v[1][j >> 1], v[0][j >> 1], sel),
+                    __builtin_amdgcn_perm(v[3][j >> 1], v[2][j >> 1], sel)};
         }
       }
     }
@@ -272,7 +275,8 @@ struct ReadArgs {
 };
 
 // One workgroup per (key or value, sequence, kv head, block of 64 tokens): codes in 16-byte pieces, values through LDS
-// back to rows, fp16 rows out in 16-byte pieces.  Bound by memory: 8 x 4096 tokens of 8 heads, 201 MB, 31 us.
+// back to rows, fp16 rows out in 16-byte pieces.  Bound by memory: 8 x 4096 tokens of 8 heads, 201 MB, 34 us
+// (5.9 TB/s, six stores in turn).
 __global__ __launch_bounds__(kThr) void read_kernel(ReadArgs P) {
   __shared__ uint32_t s_v[kD * kVRow];
   const int tid = threadIdx.x;

@@ -120,7 +120,8 @@ class BlockInt8Cache(HFCache):
         st, lens = self._stores[layer_idx], self._len_dev[layer_idx]
         q = query.squeeze(2)
         scale = 1.0 / math.sqrt(self.head_dim) if scaling is None else float(scaling)
-        # (sized for the store's capacity: the same split of the work at every step)
+        # (sized for the store's capacity: the same split of the work at every step, which a short sequence pays for in a
+        # store with much more room: 4133 tokens 12 us a layer in one of 8192, 31 in one of 131072)
         if self.sparse_blocks is not None and self._seq_lengths[layer_idx] // BLOCK > self.sparse_blocks:
             out, _ = st.sparse_decode_attention(q, lens, self.sparse_blocks, self.sink_blocks, self.recent_blocks,
                                                 scale=scale)

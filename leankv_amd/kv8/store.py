@@ -141,7 +141,9 @@ class KV8Store:
         k, v = store.read(lens, n)                     # the K / V that attention sees, fp16
 
     pos, lens, n_new and q_lens are int32 device tensors [batch]; lens counts every stored token, the queries' own among
-    them, and may not pass the capacity.  Inputs are float16, bfloat16 or float32 of any strides; they are rounded to
+    them, and may not pass the capacity or max_len (a longer sequence counts as one that ends with the last finished block
+    below, its queries the last tokens of that).  The work is split for max_len: give it where the capacity is many times
+    the lengths.  Inputs are float16, bfloat16 or float32 of any strides; they are rounded to
     float16 first (infinities and larger numbers to +-65504; a NaN key or value is stored as 0).  There is no gradient: a
     backward pass through the outputs of queries, keys or values that autograd follows raises."""
 
