@@ -8,7 +8,7 @@
 // finish no block go to the fp16 tail.  The workgroup of the first touched block also writes the new tail, after its
 // own reads of the old one, so no other workgroup touches the tail.
 // Bound by memory for prompts: a value is read once (2 bytes) and written once (1 byte); 8 x 4096 tokens of 8 heads, 201 MB,
-// 49 us in a replayed graph that goes round six stores (4.1 TB/s; a device copy 5.0), 37 over one store, which stays in the
+// 49 us in a replayed graph over six stores in turn (4.1 TB/s; a device copy 5.0), 37 over one store, which stays in the
 // last-level cache.  Sixteen ragged prompts of up to 1201 tokens 31 us traced (2.3 TB/s): the grid is for the longest, over
 // 40 % of the workgroups find no block.  4096 tokens of one sequence 10.3 us (40 stores in turn), one token 2.8 us, or 4.5
 // where it finishes a block (an empty launch 2.1).  What a value costs in instructions matters as much: magnitudes are
