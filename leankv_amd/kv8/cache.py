@@ -9,6 +9,8 @@ lets a single-token step read, of every head's finished blocks, only the n with 
 once there are more.
 
 No gradient flows through the stored tokens: with gradients enabled a forward pass runs, its backward pass raises.
+Lengths live on the host here: a step that is to be captured into a HIP graph and replayed at other lengths is built from
+KV8Store, whose lengths are device tensors.
 """
 
 from __future__ import annotations
