@@ -33,7 +33,7 @@ extern "C" {
 
 #define LKV_DTYPE_F32 0
 #define LKV_DTYPE_F16 1
-#define LKV_DTYPE_BF16 2 /* the lkv_kv8_* entry points only */
+#define LKV_DTYPE_BF16 2 /* the lkv_kv8_*, lkv_pages_* and lkv_packed_* entry points only */
 
 /* Library version (major*10000 + minor*100 + patch) and last error text. */
 int lkv_version(void);
@@ -756,6 +756,121 @@ int lkv_kv8_sparse_attn(const lkv_kv8_store* store, const void* q, const int64_t
                         const int32_t* lens, int64_t max_len, int64_t n, int64_t sink, int64_t recent, float scale,
                         int32_t* index, void* out, const int64_t* out_strides, void* workspace,
                         size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* 16-bit paged KV cache and the attention of packed prompts                 */
+/* (no reference counterpart)                                                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Keys and values of up to `seqs` sequences in pages of page_size tokens (a
+ * power of two, 16 .. 256), `pages` of them in each of `layers` layers, heads of
+ * 128 dims, dtype LKV_DTYPE_F16 or LKV_DTYPE_BF16.  Sequence s holds lens[s]
+ * tokens; token t lies in page table[s][t / page_size], slot t % page_size, in
+ * every layer.  Entries behind a sequence's last page are -1.  refs[p] is the
+ * number of entries that name page p (0: free).  Sequences that were forked
+ * name the same pages.  All buffers are device memory of the caller, the pool
+ * 16-byte aligned, table -1 and the others 0 before the first use (what lies in
+ * free pages does not matter).
+ */
+typedef struct lkv_pages {
+  void* pool;     /* [layers][pages][2 (K, V)][kv_heads][page_size][128]     */
+  int32_t* table; /* [seqs][width]                                          */
+  int32_t* lens;  /* [seqs]                                                 */
+  int32_t* refs;  /* [pages]                                                */
+  int32_t* taken; /* [seqs]: new tokens that the last lkv_pages_extend took  */
+  int64_t layers, pages, kv_heads, page_size, seqs, width;
+  int dtype;
+} lkv_pages;
+
+/*
+ * Room for new tokens: sequence s takes cu[s + 1] - cu[s] of them (cu null: one
+ * token for every sequence that holds some), lens grows by that.  New pages are
+ * the lowest free ones, in the order of the sequences.  A last page that is not
+ * full and that other sequences name too is replaced by a copy of its tokens in
+ * a new page (before the sequence's other new pages), unless all of the
+ * sequences that name it take new tokens and this is the first of them.  A
+ * sequence gets its pages if they and those of all sequences before it fit:
+ * otherwise, and where it would pass width * page_size tokens, it takes nothing.
+ * taken[s] says what it took.
+ */
+size_t lkv_pages_extend_workspace_bytes(int64_t pages, int64_t seqs);
+int lkv_pages_extend(const lkv_pages* st, const int32_t* cu, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * k and v [rows][kv_heads][128] of the pool's type, each with its strides of row
+ * and head in elements (rows dense and 16-byte aligned), to the places that the
+ * last lkv_pages_extend made for them in one layer: row cu[s] + i is token
+ * lens[s] - taken[s] + i of sequence s, for i < taken[s]; other rows are not
+ * read.  cu null: row s is sequence s's.
+ */
+int lkv_pages_store(const lkv_pages* st, int64_t layer, const void* k, const int64_t* k_strides, const void* v,
+                    const int64_t* v_strides, int64_t rows, const int32_t* cu, void* stream);
+
+/* k, v = [seqs][kv_heads][n][128]: tokens 0 .. n - 1 of every sequence in one
+ * layer, zeros past its length. */
+int lkv_pages_read(const lkv_pages* st, int64_t layer, int64_t n, void* k, void* v, void* stream);
+
+/*
+ * Sequence s becomes the first min(lens[parent[s]], cut[s]) tokens of sequence
+ * parent[s], all at once: pages are shared, not copied.  parent null: s itself;
+ * cut null: all tokens; a parent outside 0 .. seqs - 1 or a cut below 1: an
+ * empty sequence.  Pages that no sequence names any more are free.  taken
+ * becomes 0.
+ */
+size_t lkv_pages_fork_workspace_bytes(int64_t seqs, int64_t width);
+int lkv_pages_fork(const lkv_pages* st, const int32_t* parent, const int32_t* cut, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/*
+ * The n pages in use become pages 0 .. n - 1: of those from n on, the r-th goes
+ * to the r-th free page below n, in every layer; table and refs follow.
+ * in_use[0] = n (device memory).
+ */
+size_t lkv_pages_compact_workspace_bytes(int64_t pages);
+int lkv_pages_compact(const lkv_pages* st, int32_t* in_use, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Softmax attention of one query per sequence, q [seqs][Hq][128] (strides of
+ * sequence and head, rows dense and 16-byte aligned; Hq a multiple of kv_heads,
+ * query head h reads kv head h / (Hq / kv_heads)), over the lens[s] tokens that
+ * it holds in one layer: out = softmax(scale * q K^T) V in the pool's type,
+ * zeros for an empty sequence.  The work is split for max_len, a bound on lens
+ * (longer sequences count as max_len).  Neighbouring sequences on the same pages
+ * are read once for several of them.  Scores and sums are fp32; the weights are
+ * rounded to the pool's type for the value product.
+ */
+size_t lkv_pages_decode_attn_workspace_bytes(int64_t seqs, int64_t Hq, int64_t kv_heads, int64_t max_len);
+int lkv_pages_decode_attn(const lkv_pages* st, int64_t layer, const void* q, const int64_t* q_strides, int64_t Hq,
+                          int64_t max_len, float scale, void* out, const int64_t* out_strides, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * Causal attention of packed sequences: rows cu[b] .. cu[b + 1] - 1 of
+ * q [rows][Hq][128] and k, v [rows][Hkv][128] (float16 or bfloat16, strides of
+ * row and head) are sequence b; query i of it sees its tokens 0 .. i.  cu int32
+ * [B + 1] on the device, ascending.  max_len is a bound on the lengths (the work
+ * is split for it; longer ones are right too).  Rows that belong to no sequence
+ * are zeros with fill = 1 and left as they are with fill = 0.
+ */
+size_t lkv_packed_attn_workspace_bytes(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_len);
+int lkv_packed_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                    const int64_t* v_strides, int dtype, int64_t rows, int64_t Hq, int64_t Hkv, const int32_t* cu,
+                    int64_t B, int64_t max_len, float scale, void* out, const int64_t* out_strides, int fill,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same over pages: rows cu[s] .. cu[s + 1] - 1 of q are the queries of the
+ * newest tokens of sequence s (at most lens[s]: further rows are zeros); query i
+ * of m sees tokens 0 .. lens[s] - m + i.  max_new and max_len are bounds on the
+ * rows of a sequence and on lens, for which the work is split.
+ */
+size_t lkv_pages_prefill_attn_workspace_bytes(int64_t rows, int64_t seqs, int64_t Hq, int64_t kv_heads,
+                                              int64_t max_new, int64_t max_len);
+int lkv_pages_prefill_attn(const lkv_pages* st, int64_t layer, const void* q, const int64_t* q_strides, int64_t rows,
+                           int64_t Hq, const int32_t* cu, int64_t max_new, int64_t max_len, float scale, void* out,
+                           const int64_t* out_strides, int fill, void* workspace, size_t workspace_bytes,
+                           void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,6 +10,7 @@ Module map (mirrors the reference's public API):
   leankv_amd.turboquant.cache         TurboQuantCache (static packed storage)
   leankv_amd.turboquant.attention     fused decode attention for HF models
   leankv_amd.kv8                      8-bit block-scaled KV cache (no reference counterpart)
+  leankv_amd.paged                    16-bit paged KV cache, attention of packed prompts (no reference counterpart)
   leankv_amd.combined                 optimize_model / load_model
   leankv_amd.engine                   graph-captured static decode engine
   leankv_amd.kernels                  torch wrappers of the C ABI (include/leankv_amd.h)

@@ -21,7 +21,7 @@ from .build import LIB_PATH
 LKV_OK = 0
 LKV_DTYPE_F32 = 0
 LKV_DTYPE_F16 = 1
-LKV_DTYPE_BF16 = 2  # lkv_kv8_* only
+LKV_DTYPE_BF16 = 2  # lkv_kv8_*, lkv_pages_* and lkv_packed_* only
 
 _c_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -100,6 +100,22 @@ SIGNATURES = {
     "lkv_kv8_sparse_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "lkv_kv8_sparse_attn": (_int, [_c_p, _c_p, _c_p, _int, _i64, _c_p, _i64, _i64, _i64, _i64, _f32, _c_p, _c_p, _c_p,
                                    _c_p, _sz, _c_p]),
+    "lkv_pages_extend_workspace_bytes": (_sz, [_i64, _i64]),
+    "lkv_pages_extend": (_int, [_c_p, _c_p, _c_p, _sz, _c_p]),
+    "lkv_pages_store": (_int, [_c_p, _i64, _c_p, _c_p, _c_p, _c_p, _i64, _c_p, _c_p]),
+    "lkv_pages_read": (_int, [_c_p, _i64, _i64, _c_p, _c_p, _c_p]),
+    "lkv_pages_fork_workspace_bytes": (_sz, [_i64, _i64]),
+    "lkv_pages_fork": (_int, [_c_p, _c_p, _c_p, _c_p, _sz, _c_p]),
+    "lkv_pages_compact_workspace_bytes": (_sz, [_i64]),
+    "lkv_pages_compact": (_int, [_c_p, _c_p, _c_p, _sz, _c_p]),
+    "lkv_pages_decode_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "lkv_pages_decode_attn": (_int, [_c_p, _i64, _c_p, _c_p, _i64, _i64, _f32, _c_p, _c_p, _c_p, _sz, _c_p]),
+    "lkv_packed_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "lkv_packed_attn": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _int, _i64, _i64, _i64, _c_p, _i64, _i64, _f32, _c_p,
+                               _c_p, _int, _c_p, _sz, _c_p]),
+    "lkv_pages_prefill_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "lkv_pages_prefill_attn": (_int, [_c_p, _i64, _c_p, _c_p, _i64, _i64, _c_p, _i64, _i64, _f32, _c_p, _c_p, _int, _c_p,
+                                      _sz, _c_p]),
     "lkv_decode_head": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p, _sz, _c_p]),
 }
 
@@ -142,6 +158,14 @@ class KV8StoreStruct(ctypes.Structure):
 
     _fields_ = [("k_codes", _c_p), ("v_codes", _c_p), ("scales", _c_p), ("ranges", _c_p), ("k_tail", _c_p),
                 ("v_tail", _c_p), ("batch", _i64), ("kv_heads", _i64), ("blocks", _i64)]
+
+
+class PagesStruct(ctypes.Structure):
+    """lkv_pages (include/leankv_amd.h)."""
+
+    _fields_ = [("pool", _c_p), ("table", _c_p), ("lens", _c_p), ("refs", _c_p), ("taken", _c_p), ("layers", _i64),
+                ("pages", _i64), ("kv_heads", _i64), ("page_size", _i64), ("seqs", _i64), ("width", _i64),
+                ("dtype", _int)]
 
 
 _lib = None

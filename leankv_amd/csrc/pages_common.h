@@ -1,0 +1,92 @@
+// Layout and device helpers of the 16-bit paged KV cache and of the attention of prompts (pages_table.hip,
+// pages_decode.hip, packed_attn.hip).
+//
+// A page holds the keys and values of page_size tokens of one sequence in one layer, [2][kv heads][page_size][128]: the
+// rows of a head lie one behind the other, so that a workgroup that reads one kv head reads whole runs of memory.  A
+// sequence is a row of page ids and a length; the same page id may stand in several rows (refs counts them).
+#pragma once
+
+#include "common.h"
+
+namespace lkv {
+namespace pages {
+
+constexpr int kD = 128;
+constexpr int kMaxSeqs = 4096;  // rows of a page table, sequences of a packed batch (lengths are staged in LDS)
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+struct Pages {
+  uint16_t* pool;  // [layers][pages][2][H][1 << lg][128]
+  int* table;      // [seqs][width]
+  int* lens;       // [seqs]
+  int* refs;       // [pages]
+  int* taken;      // [seqs]
+  int layers, pages, H, lg, seqs, width;
+};
+
+__host__ __device__ __forceinline__ int page_size(const Pages& st) { return 1 << st.lg; }
+// Numbers of a head's rows in one page, and of a page.
+__device__ __forceinline__ int64_t run_numbers(const Pages& st) { return static_cast<int64_t>(kD) << st.lg; }
+__device__ __forceinline__ int64_t page_numbers(const Pages& st) { return 2 * st.H * run_numbers(st); }
+// A sequence's tokens, and the page that an entry of its row names: inside the table and the pool whatever they hold.
+__device__ __forceinline__ int held(const Pages& st, int len) { return min(max(len, 0), st.width << st.lg); }
+__device__ __forceinline__ int page_id(const Pages& st, int entry) { return min(max(entry, 0), st.pages - 1); }
+
+__device__ __forceinline__ uint32_t pk2(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
+}
+__device__ __forceinline__ uint32_t pk2bf(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  if constexpr (DT == LKV_DTYPE_F16)
+    return pk2(lo, hi);
+  else
+    return pk2bf(lo, hi);
+}
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (DT == LKV_DTYPE_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (DT == LKV_DTYPE_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// log2 of the softmax weights as 16 bits hold them: a new offset puts the largest at 2^6, and there is none until a weight
+// passes 2^15, so that most tiles need no rescaled sums.  A weight keeps fp16's 11 bits down to 2^-20 of the largest.
+constexpr float kTopWeight = 6.f, kMaxWeight = 15.f;
+
+// A partial sum's (offset, sum): offset -inf is an empty one, which is passed over.  A row of NaN scores has no offset
+// (max passes over NaN) but is not empty: it takes 0, so that its NaN reaches the joined row.
+__device__ __forceinline__ float2 part_record(float m, float l) { return float2{l != l ? 0.f : m, l}; }
+
+// Joins the partial sums of rows of 128 numbers (pages_decode.hip): part_ml [rows][splits][2], part_o [rows][splits][128],
+// row r's result to out + (r / heads) * o_st + (r % heads) * o_sh.  cu (optional): rows of tokens before cu[0] or from
+// cu[n] on are skipped.
+int launch_join(const float* part_o, const float* part_ml, int64_t rows, int64_t splits, int64_t heads, void* out,
+                int64_t o_st, int64_t o_sh, int dtype, const int* cu, int n, hipStream_t stream, const char* what);
+
+// Checks of what the C entries take (pages_table.hip).
+int check_pages(const lkv_pages* p, const char* what);
+Pages device_pages(const lkv_pages* p);
+int check_rows(const void* x, const int64_t* strides, const char* what, const char* name);
+
+}  // namespace pages
+}  // namespace lkv
