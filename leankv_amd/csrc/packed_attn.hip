@@ -31,6 +31,7 @@ constexpr int kVRow = kD + 32;    // and of a value row: the transposing read's 
 constexpr int kKBuf = kTile * kKRow, kVBuf = kTile * kVRow;
 constexpr int kXcds = 8;
 constexpr int kManyChunk = 8;     // fewest tiles of a split
+constexpr int kPlan = 64;         // pieces of a workgroup that are found at once
 constexpr int kAgain = 128;       // words of marks (rounds past 4096 share them: gone through again without need)
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -51,9 +52,9 @@ struct Args {
   int64_t k_sh, v_sh;  // strides of head and row
   int k_st, v_st;
   const uint16_t* q;
-  int64_t q_st, q_sh;
+  uint32_t q_st, q_sh;
   uint16_t* out;
-  int64_t o_st, o_sh;
+  uint32_t o_st, o_sh;
   const int* cu;
   int B, rows;         // sequences, packed rows
   Pages st;            // PAGED: the store, and the layer's pages
@@ -61,6 +62,8 @@ struct Args {
   int H, G, Hq;
   int chunk, splits;   // tiles of a split
   int fill;
+  uint32_t g_mul;      // x / G = x * g_mul >> g_shift for x below 2^31
+  int g_shift, g_small;  // and x * g_small >> 16 for x below G + 32, where G is below 32
   float scale_log2;
   float* part_o;       // [rows * Hq][splits][128]
   float* part_ml;      // [rows * Hq][splits][2]
@@ -74,6 +77,10 @@ __device__ __forceinline__ ArgsPtr args_again() {
   return p;
 }
 
+__device__ __forceinline__ int by_heads(const Args& P, int x) {
+  return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * P.g_mul >> P.g_shift);
+}
+
 // Column tiles of sequence b with more than x tokens to read, of tiles with m rows in all and q of them queries of the last
 // of len tokens.
 __device__ __forceinline__ int tiles_over(int x, int len, int m, int G) {
@@ -82,17 +89,27 @@ __device__ __forceinline__ int tiles_over(int x, int len, int m, int G) {
   const int under = y <= 0 ? 0 : y >= q ? all : min(all, y * G / kCols);
   return x < 0 ? all : all - under;
 }
-__device__ __forceinline__ int wave_total(int v) {
-#pragma unroll
-  for (int x = 32; x; x >>= 1) v += __shfl_xor(v, x);
-  return __builtin_amdgcn_readfirstlane(v);
+// Sums over a wave by lane permutes of the vector unit (no LDS round trips: a piece is found with several of them).
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ int moved(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
 }
+__device__ __forceinline__ int wave_prefix(int v) {  // inclusive
+  v += moved<0x111>(v);       // row_shr 1, 2, 4, 8
+  v += moved<0x112>(v);
+  v += moved<0x114>(v);
+  v += moved<0x118>(v);
+  v += moved<0x142, 0xA>(v);  // row_bcast 15, 31
+  v += moved<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
 
 // Goes through the workgroup's pieces.  CARE: those that the first time marked in s_again, with care for values that are no
 // numbers.  Returns whether any is to be gone through again.
 template <int DT, bool PAGED, bool CARE>
 __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const int* s_len, const int* s_rows,
-                                           uint32_t* s_again, int wave, int longest, int pieces) {
+                                           const int* s_first, int4* s_plan, uint32_t* s_again, int wave, int longest, int pieces) {
   uint16_t* const sK = smem;
   uint16_t* const sV = smem + 2 * kKBuf;
   const int lane = lane_prefix(~0ull);
@@ -104,7 +121,8 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
   const int srow = lane >> 4, spiece = 8 * (lane & 15);
   const int64_t run = PAGED ? run_numbers(P.st) : 0;
   const int k_st = PAGED ? kD : P.k_st, v_st = PAGED ? kD : P.v_st;
-  const int koff = 2 * (srow * k_st + spiece), voff = PAGED ? koff : 2 * (srow * v_st + spiece);
+  const int koff[2] = {2 * (srow * k_st + spiece), 2 * ((srow + 4) * k_st + spiece)};
+  const int voff[2] = {2 * (srow * v_st + spiece), 2 * ((srow + 4) * v_st + spiece)};
   uint16_t* const kdst = sK + (8 * wave + srow) * kKRow + spiece;
   uint16_t* const vdst = sV + (8 * wave + srow) * kVRow + spiece;
   const uint16_t* const krow = sK + c32 * kKRow + 8 * hf;
@@ -119,22 +137,26 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
   const int width = static_cast<int>(gridDim.x) / lanes;
   const int own = static_cast<int>(blockIdx.x) / lanes, xcd = static_cast<int>(blockIdx.x) % lanes;
   const int per_lane = pieces * P.splits * heads_lane;
-#pragma unroll 1
-  for (int round = 0; round * width < per_lane; ++round) {
-    const int pos = round * width + ((round & 1) ? width - 1 - own : own);
-    if (pos >= per_lane) continue;  // uniform
-    if (CARE && !((s_again[(round >> 5) & (kAgain - 1)] >> (round & 31)) & 1)) continue;  // uniform
-    const int ps = __builtin_amdgcn_readfirstlane(pos / heads_lane);
-    const int h = (pos - ps * heads_lane) * lanes + xcd;
-    const int piece = __builtin_amdgcn_readfirstlane(ps / P.splits), split = ps - piece * P.splits;
-    // ---- the piece-th column tile by falling length: its length in tiles of tokens, then its place among those
-    int b = 0, tile;
-    {
+  const int every = (per_lane + width - 1) / width;  // rounds, of which the last may have nothing for this workgroup
+  auto place_of = [&](int round) { return round * width + ((round & 1) ? width - 1 - own : own); };
+  const int rounds = every && place_of(every - 1) >= per_lane ? every - 1 : every;
+  // Each begins with another of its pieces, so that not all fetch queries and put rows away at the same time.
+  const int shift = rounds ? own % rounds : 0;
+  auto turn_of = [&](int round) { return round + shift < rounds ? round + shift : round + shift - rounds; };
+
+  // ---- what the pieces of rounds r .. r + 63 are, found by the waves side by side: the n-th column tile by falling length
+  // (its length in tiles of tokens, then its place among those)
+  auto find_pieces = [&](int r) {
+    for (int i = wave; i < min(kPlan, rounds - r); i += kWaves) {
+      const int pos = place_of(turn_of(r + i));
+      const int ps = __builtin_amdgcn_readfirstlane(pos / heads_lane);
+      const int h = (pos - ps * heads_lane) * lanes + xcd;
+      const int piece = __builtin_amdgcn_readfirstlane(ps / P.splits), split = ps - piece * P.splits;
       int lo = -1, hi = (longest + kTile - 1) / kTile, over = 0;  // more than `piece` tiles over 64 lo, none over 64 hi
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         int n = 0;
-        for (int i = lane; i < P.B; i += 64) n += tiles_over(mid * kTile, s_len[i], s_rows[i], G);
+        for (int j = lane; j < P.B; j += 64) n += tiles_over(mid * kTile, s_len[j], s_rows[j], G);
         n = wave_total(n);
         if (n > piece) {
           lo = mid;
@@ -144,18 +166,12 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
         }
       }
       const int x = lo < 0 ? -1 : lo * kTile, x2 = hi * kTile;
-      int rank = piece - over;
-      tile = 0;
+      int rank = piece - over, b = 0, tile = 0;
       for (int base = 0; base < P.B; base += 64) {
-        const int i = base + lane;
-        const int high = i < P.B ? tiles_over(x2, s_len[i], s_rows[i], G) : 0;
-        const int n = i < P.B ? tiles_over(x, s_len[i], s_rows[i], G) - high : 0;
-        int sum = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const int y = __shfl_up(sum, d);
-          if (lane >= d) sum += y;
-        }
+        const int j = base + lane;
+        const int high = j < P.B ? tiles_over(x2, s_len[j], s_rows[j], G) : 0;
+        const int n = j < P.B ? tiles_over(x, s_len[j], s_rows[j], G) - high : 0;
+        const int sum = wave_prefix(n);
         const uint64_t past = wave_ballot(sum > rank);
         if (past) {
           const int at = __builtin_ctzll(past);
@@ -168,86 +184,153 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
         }
         rank -= __builtin_amdgcn_readlane(sum, 63);
       }
-      b = __builtin_amdgcn_readfirstlane(b);
-      tile = __builtin_amdgcn_readfirstlane(tile);
-    }
-    const int len = __builtin_amdgcn_readfirstlane(s_len[b]), m_rows = __builtin_amdgcn_readfirstlane(s_rows[b]);
-    const int row0 = __builtin_amdgcn_readfirstlane(min(max(P.cu[b], 0), P.rows));
-    const int qlen = min(m_rows, len), cols = m_rows * G;
-    const int col0 = tile * kCols;
-    const int q_first = __builtin_amdgcn_readfirstlane(col0 / G);
-    const int last = min(__builtin_amdgcn_readfirstlane((col0 + kCols - 1) / G), qlen - 1);  // its last query
-    const int kend = last >= q_first ? len - qlen + last + 1 : 0;
-    // tiles [blk0, blk0 + nt) of 64 tokens: what the piece's last column sees, of the split's
-    const int blk0 = split * P.chunk;
-    const int all_t = (kend + kTile - 1) / kTile;
-    const int nt = max((split == P.splits - 1 ? all_t : min(blk0 + P.chunk, all_t)) - blk0, 0);
-
-    // ---- a tile's rows: descriptors of the wave's 8 rows of keys and values
-    u32x4 kw[2], vw[2];
-    auto first_of = [&](int t) { return (blk0 + t) * kTile + 8 * wave; };
-    auto page_of = [&](int t) {  // (past the last tile: the last page, of which nothing is read)
-      const int e = min(first_of(t), len - 1) >> P.st.lg;
-      return page_id(P.st, P.st.table[static_cast<int64_t>(b) * P.st.width + e]);
-    };
-    auto rows_of = [&](int t) { return t < nt ? min(max(len - first_of(t), 0), 8) : 0; };
-    auto load_rows = [&](u32x4 (&w)[2], const uint16_t* p, int n, int stride, int off) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int rows = min(max(n - 4 * j, 0), 4);
-        const int bytes = rows ? 2 * ((rows - 1) * stride + kD) : 0;
-        const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p + (rows ? 4 * j * stride : 0)), 0, bytes,
-                                                         0x00020000);
-        w[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+      // tiles [blk0, blk0 + nt) of 64 tokens: what its last column sees, of the split's
+      const int len = s_len[b], rows = s_rows[b], qlen = min(rows, len), col0 = tile * kCols;
+      const int last = min(by_heads(P, col0 + kCols - 1), qlen - 1);  // its last query
+      const int kend = last >= by_heads(P, col0) ? len - qlen + last + 1 : 0;
+      const int blk0 = split * P.chunk, all_t = (kend + kTile - 1) / kTile;
+      const int nt = max((split == P.splits - 1 ? all_t : min(blk0 + P.chunk, all_t)) - blk0, 0);
+      if (lane == 0) {
+        s_plan[3 * i] = int4{b, h, split, len};
+        s_plan[3 * i + 1] = int4{s_first[b], qlen, rows * G, col0};
+        s_plan[3 * i + 2] = int4{blk0, nt, 0, 0};
       }
-    };
-    auto load_k = [&](int t, int page) {
-      const int n = rows_of(t), at = first_of(t);
-      load_rows(kw, PAGED ? P.kv + (static_cast<int64_t>(page) * 2 * P.H + h) * run + (at & (page_size(P.st) - 1)) * kD
-                          : P.k + (n ? static_cast<int64_t>(row0 + at) * k_st : 0) + h * P.k_sh, n, k_st, koff);
-    };
-    auto load_v = [&](int t, int page) {
-      const int n = rows_of(t), at = first_of(t);
-      load_rows(vw, PAGED ? P.kv + ((static_cast<int64_t>(page) * 2 + 1) * P.H + h) * run + (at & (page_size(P.st) - 1)) * kD
-                          : P.v + (n ? static_cast<int64_t>(row0 + at) * v_st : 0) + h * P.v_sh, n, v_st, voff);
-    };
-    auto stage_k = [&](int t, int j) {
-      *reinterpret_cast<u32x4*>(kdst + (t & 1) * kKBuf + 4 * j * kKRow) = kw[j];
-    };
-    auto stage_v = [&](int t, int j) {
-      *reinterpret_cast<u32x4*>(vdst + (t & 1) * kVBuf + 4 * j * kVRow) = vw[j];
-    };
-    u32x4 k1[2];
-    int page1 = 0, page2 = 0;  // pages of the wave's rows in the next tiles
-    auto first_loads = [&]() {
-      if (!nt) return;
+    }
+  };
+
+  struct Piece {
+    int b, h, split, len, row0, qlen, cols, col0, blk0, nt;
+  };
+  auto open = [&](int round) {
+    if ((round & (kPlan - 1)) == 0) {
+      __syncthreads();  // (what it held is read)
+      find_pieces(round);
+      __syncthreads();
+    }
+    const int4* f = s_plan + 3 * (round & (kPlan - 1));
+    const int4 x = f[0], y = f[1], z = f[2];
+    Piece c;
+    c.b = __builtin_amdgcn_readfirstlane(x.x);
+    c.h = __builtin_amdgcn_readfirstlane(x.y);
+    c.split = __builtin_amdgcn_readfirstlane(x.z);
+    c.len = __builtin_amdgcn_readfirstlane(x.w);
+    c.row0 = __builtin_amdgcn_readfirstlane(y.x);
+    c.qlen = __builtin_amdgcn_readfirstlane(y.y);
+    c.cols = __builtin_amdgcn_readfirstlane(y.z);
+    c.col0 = __builtin_amdgcn_readfirstlane(y.w);
+    c.blk0 = __builtin_amdgcn_readfirstlane(z.x);
+    c.nt = __builtin_amdgcn_readfirstlane(z.y);
+    return c;
+  };
+
+  // ---- a tile's rows: descriptors of the wave's 8 rows of keys and values
+  u32x4 kw[2], vw[2], k1[2];
+  // lane i: the page of the wave's rows in tile 64 k + i (past the last tile: the last page, of which nothing is read).
+  // (Scalar loads would share their counter with the LDS reads, which then could not be waited for one by one.)
+  int pages64 = 0;
+  int page1 = 0, page2 = 0;  // pages of the wave's rows in the next tiles
+  auto first_of = [&](const Piece& c, int t) { return (c.blk0 + t) * kTile + 8 * wave; };
+  auto page_of = [&](const Piece& c, int t) {
+    if ((t & 63) == 0) {
+      const int e = min(first_of(c, t + lane), c.len - 1) >> P.st.lg;
+      pages64 = page_id(P.st, P.st.table[static_cast<int64_t>(c.b) * P.st.width + e]);
+    }
+    return __builtin_amdgcn_readlane(pages64, t & 63);
+  };
+  auto load_rows = [&](const Piece& c, int t, u32x4 (&w)[2], const uint16_t* base, int page, int stride, int64_t head,
+                       const int (&off)[2]) {
+    const int at = first_of(c, t);
+    const uint16_t* p = PAGED ? base + (static_cast<int64_t>(page) * 2 * P.H + c.h) * run + (at & (page_size(P.st) - 1)) * kD
+                              : base + static_cast<int64_t>(c.row0 + at) * stride + c.h * head;
+    // (a row ends within its stride: what lies behind the last one is never asked for)
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, 2 * stride * min(max(c.len - at, 0), 8),
+                                                     0x00020000);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) w[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off[j], 0, 0));
+  };
+  auto load_k = [&](const Piece& c, int t, u32x4 (&w)[2], int page) {
+    load_rows(c, t, w, PAGED ? P.kv : P.k, page, k_st, P.k_sh, koff);
+  };
+  auto load_v = [&](const Piece& c, int t, int page) {
+    load_rows(c, t, vw, PAGED ? P.kv + P.H * run : P.v, page, v_st, P.v_sh, voff);
+  };
+  auto stage_k = [&](int t, int j) { *reinterpret_cast<u32x4*>(kdst + (t & 1) * kKBuf + 4 * j * kKRow) = kw[j]; };
+  auto stage_v = [&](int t, int j) { *reinterpret_cast<u32x4*>(vdst + (t & 1) * kVBuf + 4 * j * kVRow) = vw[j]; };
+  // the wave's column r of a piece: query q0 + the first, head the second (r below 32)
+  struct Cols {
+    int q0, h0;
+  };
+  auto first_column = [&](const Piece& c) {
+    const int x = c.col0 + 32 * wave, q0 = by_heads(P, x);
+    return Cols{q0, x - q0 * G};
+  };
+  auto column = [&](const Cols& w, int r) {
+    const int x = w.h0 + r, dq = G < 32 ? x * P.g_small >> 16 : (x >= G ? 1 : 0);
+    return int2{dq, x - dq * G};
+  };
+  // the wave's own part of LDS, where its query rows and its output rows turn between rows and operands
+  constexpr int kOutRow = 272;  // bytes of a row there: 256 and a shift of the banks
+  static_assert(32 * kOutRow * kWaves <= 2 * (2 * kKBuf + 2 * kVBuf), "every wave's rows fit");
+  char* const turn = reinterpret_cast<char*>(smem) + 32 * kOutRow * wave;
+  u32x4 qf[8];  // the wave's query rows, 16 bytes of row 4 j + lane / 16; then B: of the lane's column dims 16 kb + 8 hf ..
+  // (A column behind the last row is the last row once more, computed and not put away.)
+  auto load_queries = [&](const Piece& c) {
+    const Cols w = first_column(c);
+    const int end = max(c.qlen * G - 1 - c.col0 - 32 * wave, 0);
+    const ArgsPtr Z = args_again();
+    const uint32_t q_st = Z->q_st, q_sh = Z->q_sh;
+    const uint16_t* p = Z->q + static_cast<uint64_t>(c.row0 + min(w.q0, max(c.qlen - 1, 0))) * q_st +
+                        static_cast<uint64_t>(c.h * G) * q_sh + spiece;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int2 x = column(w, min(4 * j + srow, end));
+      qf[j] = *reinterpret_cast<const u32x4*>(p + (static_cast<uint64_t>(static_cast<uint32_t>(x.x)) * q_st +
+                                                   static_cast<uint64_t>(static_cast<uint32_t>(x.y)) * q_sh));
+    }
+  };
+  auto turn_queries = [&]() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) *reinterpret_cast<u32x4*>(turn + kOutRow * (4 * j + srow) + 2 * spiece) = qf[j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int kb = 0; kb < 8; ++kb) qf[kb] = *reinterpret_cast<const u32x4*>(turn + kOutRow * c32 + 32 * kb + 16 * hf);
+  };
+  // the first rows of a piece on their way (the keys of its second tile too), while the one before is put away
+  auto first_loads = [&](const Piece& c) {
+    if (c.nt) {
       int page0 = 0;
       if constexpr (PAGED) {
-        page0 = page_of(0);
-        page1 = page_of(1);
-        page2 = page_of(2);
+        page0 = page_of(c, 0);
+        page1 = page_of(c, 1);
+        page2 = page_of(c, 2);
       }
-      load_k(1, page1);
-      k1[0] = kw[0];
-      k1[1] = kw[1];
-      load_k(0, page0);
-      load_v(0, page0);
-    };
-    if constexpr (!CARE) first_loads();
-    // ---- the lane's column: query qs, head qh
-    const int col = col0 + 32 * wave + c32, qs = col / G, qh = col - qs * G;
-    const bool ok = col < cols && qs < qlen;
-    const int lim = ok ? len - qlen + qs + 1 : 0x7fffffff;  // tokens it sees
-    u32x4 qf[8];  // B: dims 16 kb + 8 hf ..
-    {
-      const ArgsPtr Z = args_again();
-      const uint16_t* p = Z->q + (row0 + qs) * Z->q_st + (static_cast<int64_t>(h) * G + qh) * Z->q_sh + 8 * hf;
-#pragma unroll
-      for (int kb = 0; kb < 8; ++kb) qf[kb] = ok ? *reinterpret_cast<const u32x4*>(p + 16 * kb) : u32x4{};
+      load_k(c, 0, kw, page0);
+      load_k(c, 1, k1, page1);
+      load_v(c, 0, page0);
     }
-    // tokens that every column of the wave sees
-    const int wq = __builtin_amdgcn_readfirstlane((col0 + 32 * wave) / G);
-    const int lim_min = wq < qlen ? len - qlen + wq + 1 : 0x7fffffff;
+    load_queries(c);
+  };
+  if (!rounds) return false;
+  Piece c = open(0);
+  if constexpr (!CARE) first_loads(c);
+#pragma unroll 1
+  for (int round = 0;;) {
+    if (CARE) {
+      if (round) c = open(round);
+      if (!((s_again[(round >> 5) & (kAgain - 1)] >> (round & 31)) & 1)) {  // uniform
+        if (++round == rounds) break;
+        continue;
+      }
+      load_queries(c);
+    }
+    const int len = c.len, qlen = c.qlen, blk0 = c.blk0, nt = c.nt;
+    // ---- the lane's column: tokens that it sees; those that every column of the wave sees
+    turn_queries();
+    const Cols w = first_column(c);
+    const int wave_cols = min(qlen * G - c.col0 - 32 * wave, 32);  // columns of the wave that are rows
+    const bool works = wave_cols > 0, ok = c32 < wave_cols;
+    const int lim = len - qlen + w.q0 + column(w, max(min(c32, wave_cols - 1), 0)).x + 1;
+    const int lim_min = len - qlen + w.q0 + 1;
 
     float m, l;
     f32x16 o[4];   // dims 32 db + 8 (i / 4) + 4 hf + i % 4
@@ -293,6 +376,25 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
 #pragma unroll
       for (int e = 0; e < 32; ++e) s[e] -= mu;
     };
+    // the same for the first tile, where there are no sums yet
+    auto general0 = [&]() {
+      float mx = -INFINITY;
+      if ((blk0 + 1) * kTile > lim_min) {  // uniform
+        const int left = lim - blk0 * kTile - 4 * hf;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] = 8 * (e >> 2) + (e & 3) < left ? sc[e >> 4][e & 15] * kc : -INFINITY;
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) sc[kt] = sc[kt] * kc;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
+      mx = half_max(mx);
+      m = mx == -INFINITY ? mx : mx - kTopWeight;
+      const float mu = mx == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) s[e] = sc[e >> 4][e & 15] - mu;
+    };
     // weights 2 i, 2 i + 1 of the present tile, into the value operand
     auto weights = [&](int i) {
       const float a = exp2_(s[2 * i]), c = exp2_(s[2 * i + 1]);
@@ -302,7 +404,7 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
       __asm__ volatile("" : "+v"(u));  // (no instruction: keeps the work beside the product that it stands next to)
       pf[i >> 2][i & 3] = u;
     };
-    m = ok ? -INFINITY : 0.f;  // a column that is no row keeps offset 0 over zero scores
+    m = -INFINITY;
     l = 0.f;
 #pragma unroll
     for (int db = 0; db < 4; ++db) o[db] = f32x16{};
@@ -310,9 +412,9 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
 #pragma unroll 1
       for (int t = 0; t < nt; ++t) {
         int page0 = 0;
-        if constexpr (PAGED) page0 = page_of(t);
-        load_k(t, page0);
-        load_v(t, page0);
+        if constexpr (PAGED) page0 = page_of(c, t);
+        load_k(c, t, kw, page0);
+        load_v(c, t, page0);
         __syncthreads();  // the buffers are free
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -376,99 +478,127 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
           stage_k(0, j);
           stage_v(0, j);
         }
-        kw[0] = k1[0];
-        kw[1] = k1[1];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) stage_k(1, j);
-        load_v(1, page1);
-        load_k(2, page2);
+        for (int j = 0; j < 2; ++j) *reinterpret_cast<u32x4*>(kdst + kKBuf + 4 * j * kKRow) = k1[j];
+        load_v(c, 1, page1);
+        load_k(c, 2, kw, page2);
         if constexpr (PAGED) {
           page1 = page2;
-          page2 = page_of(3);
+          page2 = page_of(c, 3);
         }
       }
       __syncthreads();
-      if (nt) {
+      if (works && nt) {
         score_products(0);
-        general(0);
+        general0();
       }
       __syncthreads();  // (the keys of tile 0 are overwritten next)
       // ---- A tile is two stretches of 16 products, each with vector work between them: the scores of tile t + 1 beside
       // the weights of tile t, then the values of tile t beside the offsets of tile t + 1 and the staging of the next
-      // tiles.  Keys and values have two buffers: what a tile overwrites was last read in the tile before.  (Past the last
-      // tile the scores are of zeros, unused.)
-#pragma unroll 1
-      for (int t = 0; t < nt; ++t) {
-        ws[0] = ws[1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) fr[i] = key_op(i, t + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          sc[i & 1] = mfma32<DT>(fr[i % kAhead], qf[i >> 1], i < 2 ? f32x16{} : sc[i & 1]);
-          fr[i % kAhead] = i + kAhead < 16 ? key_op(i + kAhead, t + 1) : value_op(i + kAhead - 16, t);
-          weights(i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        l += ws[0] + ws[1];
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          o[i & 3] = mfma32<DT>(fr[i % kAhead], pf[i >> 2], o[i & 3]);
-          if (i + kAhead < 16) fr[i % kAhead] = value_op(i + kAhead, t);
-          if ((i & 3) == 0) {
-            if (i < 8)
-              stage_k(t + 2, i >> 2);
-            else
-              stage_v(t + 1, (i >> 2) - 2);
-          }
-          s[2 * i] = fmaf(sc[i >> 3][2 * i & 15], kc, -m);
-          s[2 * i + 1] = fmaf(sc[i >> 3][(2 * i + 1) & 15], kc, -m);
-          mx = fmaxf(fmaxf(mx, s[2 * i]), s[2 * i + 1]);
-        }
-        load_v(t + 2, page1);
-        load_k(t + 3, page2);
+      // tiles.  Keys and values have two buffers: what a tile overwrites was last read in the tile before.
+      auto load_next = [&](int t) {
+        load_v(c, t + 2, page1);
+        load_k(c, t + 3, kw, page2);
         if constexpr (PAGED) {
           page1 = page2;
-          page2 = page_of(t + 4);
+          page2 = page_of(c, t + 4);
         }
-        if (t + 1 < nt && ((blk0 + t + 2) * kTile > lim_min || wave_ballot(mx > kMaxWeight) != 0)) general(t + 1);  // uniform
-        __syncthreads();
+      };
+      if (works) {
+#pragma unroll 1
+        for (int t = 0; t + 1 < nt; ++t) {
+          ws[0] = ws[1] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) fr[i] = key_op(i, t + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sc[i & 1] = mfma32<DT>(fr[i % kAhead], qf[i >> 1], i < 2 ? f32x16{} : sc[i & 1]);
+            fr[i % kAhead] = i + kAhead < 16 ? key_op(i + kAhead, t + 1) : value_op(i + kAhead - 16, t);
+            weights(i);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          l += ws[0] + ws[1];
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            o[i & 3] = mfma32<DT>(fr[i % kAhead], pf[i >> 2], o[i & 3]);
+            if (i + kAhead < 16) fr[i % kAhead] = value_op(i + kAhead, t);
+            if ((i & 3) == 0) {
+              if (i < 8)
+                stage_k(t + 2, i >> 2);
+              else
+                stage_v(t + 1, (i >> 2) - 2);
+            }
+            s[2 * i] = fmaf(sc[i >> 3][2 * i & 15], kc, -m);
+            s[2 * i + 1] = fmaf(sc[i >> 3][(2 * i + 1) & 15], kc, -m);
+            mx = fmaxf(fmaxf(mx, s[2 * i]), s[2 * i + 1]);
+          }
+          load_next(t);
+          if ((blk0 + t + 2) * kTile > lim_min || wave_ballot(mx > kMaxWeight) != 0) general(t + 1);  // uniform
+          __syncthreads();
+        }
+        if (nt) {  // the last tile
+          ws[0] = ws[1] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) weights(i);
+          l += ws[0] + ws[1];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i & 3] = mfma32<DT>(value_op(i, nt - 1), pf[i >> 2], o[i & 3]);
+        }
+      } else {  // no columns: the wave's part of the staging
+#pragma unroll 1
+        for (int t = 0; t + 1 < nt; ++t) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            stage_k(t + 2, j);
+            stage_v(t + 1, j);
+          }
+          load_next(t);
+          __syncthreads();
+        }
       }
-      float odd = 0.f;
+      __syncthreads();  // the tiles are done with
+    }
+
+    if constexpr (!CARE) {  // an infinity or NaN times 0 is NaN, and NaN != 0
+      f32x4 odd = f32x4{};
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) odd = fmaf(o[db][i], 0.f, odd);  // (an infinity or NaN times 0 is NaN, and NaN != 0)
-      if (__syncthreads_or(ok && odd != 0.f)) {
-        if (wave == 0 && lane == 0) s_again[(round >> 5) & (kAgain - 1)] |= 1u << (round & 31);
+        for (int i = 0; i < 16; ++i) odd[i & 3] = fmaf(o[db][i], 0.f, odd[i & 3]);
+      if (wave_ballot(ok && (odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.f)) {
+        if (lane == 0) atomicOr(&s_again[(round >> 5) & (kAgain - 1)], 1u << (round & 31));
         again = true;
       }
     }
-
+    Piece next = c;
+    const bool more = round + 1 < rounds;
+    if constexpr (!CARE) {
+      if (more) {
+        next = open(round + 1);
+        first_loads(next);
+      }
+    }
     const ArgsPtr Z = args_again();
     // (what follows from the lane is computed again here, from a copy: it needs no registers before)
     int out_lane = lane_prefix(~0ull);
     __asm__ volatile("" : "+v"(out_lane));
     const int ox = out_lane & 31, oh = out_lane >> 5;
-    const int out_col = col0 + 32 * wave + ox;
-    const int out_q = out_col / G, out_h = out_col - out_q * G;
-    const int64_t out_row = row0 + out_q, out_head = static_cast<int64_t>(h) * G + out_h;
     // ---- out: a wave's 32 rows through its part of LDS (the tiles are done with), so that a row goes out whole
     l = half_sum(l);
-    __syncthreads();
-    constexpr int kOutRow = 272;  // bytes of a staged row: 256 and a shift of the banks
-    static_assert(32 * kOutRow * kWaves <= 2 * (2 * kKBuf + 2 * kVBuf), "every wave's rows fit");
-    char* const rows = reinterpret_cast<char*>(smem) + 32 * kOutRow * wave;
-    char* const mine_row = rows + kOutRow * ox;
-    // the 16 bytes that a lane takes of row 4 j + lane / 16 (a row's address and whether it exists come from its lane)
-    auto out_rows = [&](int64_t at, bool exists, auto put) {
+    if constexpr (CARE) __syncthreads();  // (the tiles' last barrier, otherwise)
+    char* const mine_row = turn + kOutRow * ox;
+    // row 4 j + lane / 16 as a lane puts it away: 16 bytes of it to put(query, head, bytes)
+    const Cols first = first_column(c);
+    const int ends = c.cols - c.col0 - 32 * wave;
+    auto out_rows = [&](int end, auto put) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int row = 4 * j + (out_lane >> 4);
-        const u32x4 v = *reinterpret_cast<const u32x4*>(rows + kOutRow * row + 16 * (out_lane & 15));
-        const int64_t to = __shfl(static_cast<long long>(at), row);
-        if (__shfl(static_cast<int>(exists), row)) put(to, v);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(turn + kOutRow * row + 16 * (out_lane & 15));
+        const int2 x = column(first, row);
+        if (row < end) put(static_cast<uint32_t>(x.x), static_cast<uint32_t>(x.y), v);
       }
     };
     if (Z->splits == 1) {
@@ -484,14 +614,20 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
           *reinterpret_cast<uint2*>(mine_row + 2 * (32 * db + 8 * k + 4 * oh)) =
               uint2{pack<DT>(x[0], x[1]), pack<DT>(x[2], x[3])};
         }
-      out_rows(out_row * Z->o_st + out_head * Z->o_sh, out_col < cols, [&](int64_t to, const u32x4& v) {
-        *reinterpret_cast<u32x4*>(Z->out + to + 8 * (out_lane & 15)) = v;
+      uint16_t* const base = Z->out + static_cast<uint64_t>(c.row0 + first.q0) * Z->o_st + static_cast<uint64_t>(c.h * G) * Z->o_sh;
+      const uint32_t o_st = Z->o_st, o_sh = Z->o_sh;
+      out_rows(ends, [&](uint32_t q, uint32_t x, const u32x4& v) {
+        *reinterpret_cast<u32x4*>(base + (static_cast<uint64_t>(q) * o_st + static_cast<uint64_t>(x) * o_sh + 8 * (out_lane & 15))) = v;
       });
     } else {
-      const int64_t at = (out_row * Z->Hq + out_head) * Z->splits + split;
-      const bool some = ok && nt > 0;
-      if (oh == 0 && out_col < cols)
-        *reinterpret_cast<float2*>(Z->part_ml + 2 * at) = some ? part_record(m, l) : part_record(-INFINITY, 0.f);
+      // (a split without tokens leaves its rows unwritten: its record is empty)
+      const int64_t base = (static_cast<int64_t>(c.row0 + first.q0) * Z->Hq + c.h * G) * Z->splits + c.split;
+      const uint32_t by_q = Z->Hq * Z->splits, by_h = Z->splits;
+      if (oh == 0 && ox < ends) {
+        const int2 x = column(first, ox);
+        const int64_t at = base + static_cast<int64_t>(x.x) * by_q + static_cast<int64_t>(x.y) * by_h;
+        *reinterpret_cast<float2*>(Z->part_ml + 2 * at) = ok && nt > 0 ? part_record(m, l) : part_record(-INFINITY, 0.f);
+      }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -502,11 +638,15 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
             *reinterpret_cast<f32x4*>(mine_row + 4 * (32 * db + 8 * k + 4 * oh)) =
                 f32x4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
           }
-        out_rows(at * kD + 64 * half, some, [&](int64_t to, const u32x4& v) {
-          *reinterpret_cast<u32x4*>(Z->part_o + to + 4 * (out_lane & 15)) = v;
+        out_rows(nt ? wave_cols : 0, [&](uint32_t q, uint32_t x, const u32x4& v) {
+          const int64_t at = base + static_cast<int64_t>(q) * by_q + static_cast<int64_t>(x) * by_h;
+          *reinterpret_cast<u32x4*>(Z->part_o + at * kD + 64 * half + 4 * (out_lane & 15)) = v;
         });
       }
     }
+    if (!more) break;
+    c = next;
+    ++round;
   }
   return again;
 }
@@ -514,7 +654,8 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
 template <int DT, bool PAGED>
 __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
   __shared__ __align__(16) uint16_t smem[2 * kKBuf + 2 * kVBuf];
-  __shared__ int s_len[kMaxSeqs], s_rows[kMaxSeqs];
+  __shared__ int s_len[kMaxSeqs], s_rows[kMaxSeqs], s_first[kMaxSeqs];
+  __shared__ int4 s_plan[3 * kPlan];
   __shared__ uint32_t s_again[kAgain];  // pieces to go through again, by round
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tid = threadIdx.x, lane = tid & 63;
@@ -524,6 +665,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
   int longest = 0;
   for (int b = tid; b < P.B; b += kThr) {
     const int a = min(max(P.cu[b], 0), P.rows), e = min(max(P.cu[b + 1], a), P.rows);
+    s_first[b] = a;
     s_rows[b] = e - a;
     s_len[b] = PAGED ? held(P.st, P.st.lens[b]) : e - a;
   }
@@ -539,9 +681,9 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
   longest = __builtin_amdgcn_readfirstlane(longest);
   pieces = wave_total(pieces);
 
-  if (go_through<DT, PAGED, false>(P, smem, s_len, s_rows, s_again, wave, longest, pieces)) {
-    __syncthreads();
-    go_through<DT, PAGED, true>(P, smem, s_len, s_rows, s_again, wave, longest, pieces);
+  const bool again = go_through<DT, PAGED, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces);
+  if (__syncthreads_or(again)) {
+    go_through<DT, PAGED, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces);
   }
 
   // ---- rows of no sequence
@@ -588,6 +730,10 @@ int launch(Args A, const Plan& p, int dtype, void* workspace, size_t workspace_b
   const size_t need = plan_bytes(p, A.rows, A.Hq);
   LKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
               "%s: a 16-byte aligned workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
+  A.g_shift = 31;
+  while ((1ll << (A.g_shift - 31)) < A.G) ++A.g_shift;
+  A.g_mul = static_cast<uint32_t>((1ull << A.g_shift) / A.G + 1);
+  A.g_small = A.G < 32 ? 65536 / A.G + 1 : 0;
   A.chunk = p.chunk;
   A.splits = p.splits;
   A.part_o = static_cast<float*>(workspace);
@@ -644,19 +790,20 @@ extern "C" int lkv_packed_attn(const void* q, const int64_t* q_strides, const vo
   if (int rc = check_rows(v, v_strides, what, "v")) return rc;
   if (int rc = check_rows(out, out_strides, what, "out")) return rc;
   LKV_REQUIRE(k_strides[0] < (1ll << 26) && v_strides[0] < (1ll << 26), "%s: strides of rows of k or v past 2^26", what);
+  LKV_REQUIRE(rows == 1 || (k_strides[0] >= kD && v_strides[0] >= kD), "%s: rows of k or v overlap", what);
   Args A{};
   A.q = static_cast<const uint16_t*>(q);
-  A.q_st = q_strides[0];
-  A.q_sh = q_strides[1];
+  A.q_st = static_cast<uint32_t>(q_strides[0]);
+  A.q_sh = static_cast<uint32_t>(q_strides[1]);
   A.k = static_cast<const uint16_t*>(k);
-  A.k_st = static_cast<int>(k_strides[0]);
+  A.k_st = rows == 1 ? kD : static_cast<int>(k_strides[0]);
   A.k_sh = k_strides[1];
   A.v = static_cast<const uint16_t*>(v);
-  A.v_st = static_cast<int>(v_strides[0]);
+  A.v_st = rows == 1 ? kD : static_cast<int>(v_strides[0]);
   A.v_sh = v_strides[1];
   A.out = static_cast<uint16_t*>(out);
-  A.o_st = out_strides[0];
-  A.o_sh = out_strides[1];
+  A.o_st = static_cast<uint32_t>(out_strides[0]);
+  A.o_sh = static_cast<uint32_t>(out_strides[1]);
   A.cu = cu;
   A.B = static_cast<int>(B);
   A.rows = static_cast<int>(rows);
@@ -692,11 +839,11 @@ extern "C" int lkv_pages_prefill_attn(const lkv_pages* p, int64_t layer, const v
   if (int rc = check_rows(out, out_strides, what, "out")) return rc;
   Args A{};
   A.q = static_cast<const uint16_t*>(q);
-  A.q_st = q_strides[0];
-  A.q_sh = q_strides[1];
+  A.q_st = static_cast<uint32_t>(q_strides[0]);
+  A.q_sh = static_cast<uint32_t>(q_strides[1]);
   A.out = static_cast<uint16_t*>(out);
-  A.o_st = out_strides[0];
-  A.o_sh = out_strides[1];
+  A.o_st = static_cast<uint32_t>(out_strides[0]);
+  A.o_sh = static_cast<uint32_t>(out_strides[1]);
   A.cu = cu;
   A.B = static_cast<int>(p->seqs);
   A.rows = static_cast<int>(rows);

@@ -67,6 +67,17 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f3
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
                                                    0);
 }
+// acc + the two numbers of u (exact products with 1, subnormal ones too): sums of softmax weights as they are multiplied, so
+// that what rounding does to a weight that outweighs the others cancels in the quotient.
+template <int DT>
+__device__ __forceinline__ float add_pair(uint32_t u, float acc) {
+  if constexpr (DT == LKV_DTYPE_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, u), f16x2{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)},
+                                  acc, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u),
+                                           bf16x2{static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)}, acc, false);
+}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // log2 of the softmax weights as 16 bits hold them: a new offset puts the largest at 2^6, and there is none until a weight

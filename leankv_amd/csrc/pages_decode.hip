@@ -185,11 +185,10 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(DecodeArgs P) {
     const float mu = m == -INFINITY ? 0.f : m;
     float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[e] = exp2_(x[e] - mu);
-      l += w[e];
-    }
+    for (int e = 0; e < 8; ++e) w[e] = exp2_(x[e] - mu);
     const u32x4 pb = u32x4{pack<DT>(w[0], w[1]), pack<DT>(w[2], w[3]), pack<DT>(w[4], w[5]), pack<DT>(w[6], w[7])};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) l = add_pair<DT>(pb[e], l);
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       u32x4 a;

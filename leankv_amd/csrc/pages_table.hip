@@ -441,7 +441,8 @@ Pages device_pages(const lkv_pages* p) {
 
 int check_rows(const void* x, const int64_t* strides, const char* what, const char* name) {
   LKV_REQUIRE(x && strides, "%s: null pointer", what);
-  LKV_REQUIRE(aligned16(x) && strides[0] >= 0 && strides[1] >= 0 && (strides[0] | strides[1]) % 8 == 0,
+  LKV_REQUIRE(aligned16(x) && strides[0] >= 0 && strides[1] >= 0 && (strides[0] | strides[1]) % 8 == 0 &&
+                  (strides[0] | strides[1]) < (1ll << 31),
               "%s: rows of %s must be 16-byte aligned, strides %lld, %lld", what, name, (long long)strides[0],
               (long long)strides[1]);
   return LKV_OK;

@@ -32,15 +32,15 @@ def in_place(t: torch.Tensor):
         r = 0
     if n[1] <= 1:
         h = 0
-    if d != 1 or (r | h) % 8 or t.data_ptr() % 16 or r >= 1 << 26:
+    if d != 1 or (r | h) % 8 or t.data_ptr() % 16 or r >= 1 << 26 or h >= 1 << 31:
         return None
     return strides2(r, h)
 
 
-def rows(t: torch.Tensor):
-    """(t or a copy of it, strides) for t [rows, heads, 128] that is read."""
+def rows(t: torch.Tensor, apart: bool = False):
+    """(t or a copy of it, strides) for t [rows, heads, 128] that is read; with rows apart, if they have to be."""
     st = in_place(t)
-    if st is None:
+    if st is None or (apart and st[0] < HEAD_DIM and t.shape[0] > 1):
         t = t.detach().clone(memory_format=torch.contiguous_format)
         st = in_place(t)
     return t, st
@@ -146,7 +146,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if follows:
             raise LeanKVError("%s: out= does not support autograd, which follows q, k or v" % what)
         os = out_rows(out, q, what)
-    (q, qs), (k, ks), (v, vs) = rows(q), rows(k), rows(v)
+    (q, qs), (k, ks), (v, vs) = rows(q), rows(k, apart=True), rows(v, apart=True)
     batch = cu_seqlens.shape[0] - 1
     nbytes = _bytes(n, batch, heads, kv_heads, bound)
     ws = q.new_empty(nbytes // 2) if nbytes else None

@@ -11,8 +11,9 @@ D = 128
 def attention(q, k, v, seen, scale=None):
     """(out, bound) of q [m, D] over k, v [n, D] in float64: row i sees tokens 0 .. seen[i] - 1; zeros where it sees none.
 
-    bound: with u half a step of the type and p the softmax weights, A = sum p |v|: the weights' rounding gives u A, the
-    output's rounding u |out| <= u A (and 2^-25 where fp16 is subnormal); fp32 scores of 128 products are off by at most
+    bound: with u half a step of the type and p the softmax weights, A = sum p |v|: the weights are rounded in the numerator and
+    in their sum, sum p (1 + e) v / sum p (1 + e) with |e| <= u, which is off by u sum p |v - out| <= u (A + |out|) <= 2 u A;
+    the output's rounding gives u |out| <= u A (and 2^-25 where fp16 is subnormal); fp32 scores of 128 products are off by at most
     129 * 2^-24 * scale * sum |q||k|, the weights by that relative error (numerator and denominator) and 2^-22 of the
     exponential; fp32 sums over n tokens by n 2^-24 A; an fp16 weight below 2^-14 is off by 2^-25, the largest is at least 2^6
     (a quarter of that where partial sums move their offsets): n 2^-29 max|v|."""
@@ -32,7 +33,7 @@ def attention(q, k, v, seen, scale=None):
     w = w / torch.where(total > 0, total, 1.0)
     out, A = w @ v, w @ v.abs()
     relative = 2 * (129 * 2.0 ** -24 * size + 2.0 ** -22)
-    bound = (2 * u + relative + n * 2.0 ** -24) * A + tiny + n * 2.0 ** -29 * v.abs().amax()
+    bound = (3 * u + relative + n * 2.0 ** -24) * A + tiny + n * 2.0 ** -29 * v.abs().amax()
     return out, bound
 
 
