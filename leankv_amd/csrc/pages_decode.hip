@@ -7,10 +7,12 @@
 //                   out^T   (16 dims x 16 columns) += A = 16 dims of 32 rows of values (paired by v_perm), B = the weights.
 //   join          combines the splits' (offset, sum, row) in fp32.
 //
-// A product has 16 columns and a sequence fills Hq / Hkv of them.  The others are given to its neighbours: of the
-// 16 / (Hq / Hkv) sequences of an aligned group, those whose pages in this split are the same (forked from one prompt) and
-// end at the same token are the columns of one workgroup, that of the first of them; the workgroups of the others end at
-// once.  Pages are compared where they are staged, so sharing needs no plan and no call of its own.
+// A product has 16 columns and a sequence fills Hq / Hkv of them.  The others, and those of a second product over the same
+// rows, are given to its neighbours: of the 32 / (Hq / Hkv) sequences of an aligned group, those that begin the split on the
+// same page (forked from one prompt) are read once as far as all of them name the same pages.  Their workgroups divide that
+// part among themselves, each for the columns of all; what follows each reads for its own.  A split has a record for its own
+// part and one for every sequence of the group.  Pages are compared where they are staged, so sharing needs no plan and no
+// call of its own.
 #include "pages_common.h"
 
 namespace lkv {
@@ -45,94 +47,49 @@ struct DecodeArgs {
   uint16_t* out;
   int64_t o_ss, o_sh;
   int Hq, G;
+  int g_small;  // c / G = c * g_small >> 16 for columns c of a group
   int tiles;    // column tiles of a kv head: 1, or ceil(G / 16)
-  int group;    // sequences of a group: 16 / G, at least 1
+  int group;    // sequences of a group: 32 / G, or 1 where none are shared
   int max_len, chunk, splits;  // tokens of a split
+  int slots;    // records of a row: splits, or splits (group + 1): a split's own part, and the shared ones
   float scale_log2;
-  float* part_o;   // [seqs * Hq][splits][128]
-  float* part_ml;  // [seqs * Hq][splits][2]
+  float* part_o;   // [seqs * Hq][slots][128]
+  float* part_ml;  // [seqs * Hq][slots][2]
 };
 
-template <int DT>
-__global__ __launch_bounds__(kThr, 2) void split_kernel(DecodeArgs P) {
-  constexpr int kRow = kD + 4;  // floats of a staged row
-  __shared__ __align__(16) float s_o[kWaves][16][kRow];
-  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
-  __shared__ int s_page[kMaxPages];
-  __shared__ int s_other;  // sequences of the group that read other pages
+constexpr int kRow = kD + 4;  // floats of a staged row
+struct Staged {
+  float o[kWaves][16][kRow];
+  float m[kWaves][32], l[kWaves][32];
+  int page[kMaxPages];
+  int end[32], same[32], member[32];
+};
+
+// Attention over tokens [lo, hi) of the workgroup's split for `cols` columns, 16 NT at most; where(c, seq, head) says what
+// column c is and slot where its record goes (no slots: the result itself).
+template <int DT, int NT, class Where>
+__device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, int page0, int lo, int hi, int cols, int slot,
+                                       Where where) {
   const Pages& st = P.st;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, h = blockIdx.y / P.tiles, tile = blockIdx.y - h * P.tiles, s = blockIdx.z;
-  const int G = P.G;
-
-  const int len = min(held(st, st.lens[s]), P.max_len);
-  const int t0 = split * P.chunk, t1 = min(t0 + P.chunk, len);
-  // columns of the workgroup's own sequence: heads 16 tile .. of its kv head
-  const int own_heads = min(G - 16 * tile, 16);
-  if (t0 >= t1) {  // uniform: nothing here
-    if (P.splits == 1) {
-      for (int e = tid; e < own_heads * (kD / 8); e += kThr)
-        *reinterpret_cast<u32x4*>(P.out + s * P.o_ss + (static_cast<int64_t>(h) * G + 16 * tile + e / (kD / 8)) * P.o_sh +
-                                  8 * (e % (kD / 8))) = u32x4{};
-    } else if (tid < own_heads) {
-      const int64_t row = static_cast<int64_t>(s) * P.Hq + h * G + 16 * tile + tid;
-      *reinterpret_cast<float2*>(P.part_ml + 2 * (row * P.splits + split)) = part_record(-INFINITY, 0.f);
-    }
-    return;
-  }
-
-  // ---- the split's pages, and who else reads them
-  const int base = s - s % P.group;
-  const int members = min(P.group, st.seqs - base);
-  const int page0 = t0 >> st.lg, pages = ((t1 - 1) >> st.lg) - page0 + 1;
-  int mine = 1 << (s - base);  // members in this workgroup, as bits
-  if (P.group > 1) {
-    if (tid == 0) s_other = 0;
-    __syncthreads();
-  }
-  {
-    const int* row = st.table + static_cast<int64_t>(s) * st.width + page0;
-    int other = 0;
-    for (int i = tid; i < pages; i += kThr) {
-      const int p = page_id(st, row[i]);
-      s_page[i] = p;
-      for (int j = 0; j < members; ++j) {
-        const int q = page_id(st, st.table[static_cast<int64_t>(base + j) * st.width + page0 + i]);
-        other |= q != p ? 1 << j : 0;
-      }
-    }
-    if (P.group > 1) {
-      if (tid < members && min(t0 + P.chunk, min(held(st, st.lens[base + tid]), P.max_len)) != t1) other |= 1 << tid;
-      if (other) atomicOr(&s_other, other);
-    }
-  }
-  __syncthreads();
-  if (P.group > 1) {
-    mine = ~__builtin_amdgcn_readfirstlane(s_other) & ((1 << members) - 1);
-    if (mine & ((1 << (s - base)) - 1)) return;  // uniform: an earlier sequence's workgroup does it
-  }
-
-  // ---- the lane's column: head `head` of sequence `seq`
-  const int slot = P.group > 1 ? c16 / G : 0;
-  const bool ok = P.group > 1 ? slot < members && ((mine >> slot) & 1) : c16 < own_heads;
-  const int seq = P.group > 1 ? base + min(slot, members - 1) : s;
-  const int head = h * G + (P.group > 1 ? c16 - slot * G : 16 * tile + min(c16, own_heads - 1));
-  u32x4 qf[4];  // dims 32 kb + 8 g ..
-  {
+  u32x4 qf[NT][4];  // dims 32 kb + 8 g ..
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {  // (a column past the last is the last once more)
+    int seq, head;
+    where(min(16 * n + c16, cols - 1), seq, head);
     const uint16_t* p = P.q + seq * P.q_ss + head * P.q_sh + 8 * g;
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb) qf[kb] = ok ? *reinterpret_cast<const u32x4*>(p + 32 * kb) : u32x4{};
+    for (int kb = 0; kb < 4; ++kb) qf[n][kb] = *reinterpret_cast<const u32x4*>(p + 32 * kb);
   }
-
-  // ---- chunks c = t0 + 32 (wave + 4 i): keys of tokens c + 16 tt + lane % 16, values j of tokens
+  // ---- chunks c = lo + 32 (wave + 4 i): keys of tokens c + 16 tt + lane % 16, values j of tokens
   // c + 16 (j / 4) + 4 (lane / 16) + j % 4; tokens past the end read the last one, masked below
   const int64_t run = run_numbers(st);
   const int mask = page_size(st) - 1;
   auto at = [&](int t) {  // a token's row of keys in the layer
-    t = min(t, t1 - 1);
-    return s_page[(t >> st.lg) - page0] * (2 * st.H * run) + h * run + (t & mask) * kD;
+    t = min(t, hi - 1);
+    return sh.page[(t >> st.lg) - page0] * (2 * st.H * run) + h * run + (t & mask) * kD;
   };
   u32x4 kr[2][4], vr[8];
   auto load_chunk = [&](int c) {
@@ -146,105 +103,217 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(DecodeArgs P) {
     for (int j = 0; j < 8; ++j)
       vr[j] = *reinterpret_cast<const u32x4*>(P.kv + at(c + 16 * (j >> 2) + 4 * g + (j & 3)) + st.H * run + 8 * c16);
   };
-  float m = -INFINITY, l = 0.f;
-  f32x4 o[8];  // o[t] row 4 g + i: dim 8 (4 g + i) + t of the lane's column
+  float m[NT], l[NT];
+  f32x4 o[NT][8];  // o[n][t] row 4 g + i: dim 8 (4 g + i) + t of the lane's column of tile n
 #pragma unroll
-  for (int t = 0; t < 8; ++t) o[t] = f32x4{};
-  int c = t0 + kChunk * wave;
-  if (c < t1) load_chunk(c);
-  for (; c < t1; c += kStep) {
-    f32x4 sc[2];
+  for (int n = 0; n < NT; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      sc[tt] = f32x4{};
+    for (int t = 0; t < 8; ++t) o[n][t] = f32x4{};
+  }
+  int c = lo + kChunk * wave;
+  if (c < hi) load_chunk(c);
+#pragma unroll 1
+  for (; c < hi; c += kStep) {
+    const bool last = c + kChunk > hi;  // uniform: rows past the end are no numbers of this sequence
+    if (last) {
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb) sc[tt] = mfma16<DT>(kr[tt][kb], qf[kb], sc[tt]);
+      for (int e = 0; e < 8; ++e)
+        if (c + 16 * (e >> 2) + 4 * g + (e & 3) >= hi) vr[e] = u32x4{};
     }
-    float x[8], mx = -INFINITY;
+    u32x4 pb[NT];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = sc[e >> 2][e & 3] * P.scale_log2;
-    if (c + kChunk > t1) {  // uniform: the last tokens.  Rows past them are no numbers of this sequence
+    for (int n = 0; n < NT; ++n) {
+      f32x4 sc[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool past = c + 16 * (e >> 2) + 4 * g + (e & 3) >= t1;
-        x[e] = past ? -INFINITY : x[e];
-        if (past) vr[e] = u32x4{};
+      for (int tt = 0; tt < 2; ++tt) {
+        sc[tt] = f32x4{};
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) sc[tt] = mfma16<DT>(kr[tt][kb], qf[n][kb], sc[tt]);
       }
+      float x[8], mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = sc[e >> 2][e & 3] * P.scale_log2;
+      if (last) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = c + 16 * (e >> 2) + 4 * g + (e & 3) >= hi ? -INFINITY : x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
+      if (wave_ballot(mx - m[n] > kMaxWeight || m[n] == -INFINITY)) {  // uniform: a new offset somewhere
+        mx = groups_max(mx);
+        const float mn = mx - m[n] > kMaxWeight ? mx - kTopWeight : m[n];
+        const float alpha = exp2_(m[n] - (mn == -INFINITY ? 0.f : mn));
+        m[n] = mn;
+        l[n] *= alpha;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) o[n][t] = o[n][t] * alpha;
+      }
+      const float mu = m[n] == -INFINITY ? 0.f : m[n];
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = exp2_(x[e] - mu);
+      pb[n] = u32x4{pack<DT>(w[0], w[1]), pack<DT>(w[2], w[3]), pack<DT>(w[4], w[5]), pack<DT>(w[6], w[7])};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) l[n] = add_pair<DT>(pb[n][e], l[n]);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
-    if (wave_ballot(mx - m > kMaxWeight || m == -INFINITY)) {  // uniform: a new offset somewhere
-      mx = groups_max(mx);
-      const float mn = mx - m > kMaxWeight ? mx - kTopWeight : m;
-      const float alpha = exp2_(m - (mn == -INFINITY ? 0.f : mn));
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) o[t] = o[t] * alpha;
-    }
-    const float mu = m == -INFINITY ? 0.f : m;
-    float w[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = exp2_(x[e] - mu);
-    const u32x4 pb = u32x4{pack<DT>(w[0], w[1]), pack<DT>(w[2], w[3]), pack<DT>(w[4], w[5]), pack<DT>(w[6], w[7])};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) l = add_pair<DT>(pb[e], l);
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       u32x4 a;
 #pragma unroll
       for (int pp = 0; pp < 4; ++pp)
         a[pp] = __builtin_amdgcn_perm(vr[2 * pp + 1][t >> 1], vr[2 * pp][t >> 1], (t & 1) ? 0x07060302u : 0x05040100u);
-      o[t] = mfma16<DT>(a, pb, o[t]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[n][t] = mfma16<DT>(a, pb[n], o[n][t]);
     }
-    if (c + kStep < t1) load_chunk(c + kStep);
+    if (c + kStep < hi) load_chunk(c + kStep);
   }
 
-  // ---- the four waves' sums
-  l = groups_sum(l);
-  if (g == 0) {
-    s_m[wave][c16] = l != l ? 0.f : m;
-    s_l[wave][c16] = l;
+  // ---- the four waves' sums, a column tile after the other
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float ln = groups_sum(l[n]);
+    __syncthreads();  // (what lies there is read)
+    if (g == 0) {
+      sh.m[wave][c16] = ln != ln ? 0.f : m[n];
+      sh.l[wave][c16] = ln;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float* dst = &sh.o[wave][c16][8 * (4 * g + i)];
+      *reinterpret_cast<f32x4*>(dst) = f32x4{o[n][0][i], o[n][1][i], o[n][2][i], o[n][3][i]};
+      *reinterpret_cast<f32x4*>(dst + 4) = f32x4{o[n][4][i], o[n][5][i], o[n][6][i], o[n][7][i]};
+    }
+    __syncthreads();
+    const int col = tid >> 4, d = 8 * (tid & 15);
+    if (16 * n + col >= cols) continue;
+    int seq, head;
+    where(16 * n + col, seq, head);
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sh.m[w][col]);
+    float L = 0.f, r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = sh.m[w][col];
+      if (mw == -INFINITY) continue;  // no weight yet: its sums are zeros
+      const float wt = exp2_(mw - M);
+      L = fmaf(wt, sh.l[w][col], L);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = fmaf(wt, sh.o[w][col][d + i], r[i]);
+    }
+    if (P.slots == 1) {
+      const float inv = L != 0.f ? 1.f / L : 0.f;
+      *reinterpret_cast<u32x4*>(P.out + seq * P.o_ss + head * P.o_sh + d) =
+          u32x4{pack<DT>(r[0] * inv, r[1] * inv), pack<DT>(r[2] * inv, r[3] * inv), pack<DT>(r[4] * inv, r[5] * inv),
+                pack<DT>(r[6] * inv, r[7] * inv)};
+      continue;
+    }
+    const int64_t rec = (static_cast<int64_t>(seq) * P.Hq + head) * P.slots + slot;
+    if ((tid & 15) == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * rec) = part_record(M, L);
+    *reinterpret_cast<f32x4*>(P.part_o + rec * kD + d) = f32x4{r[0], r[1], r[2], r[3]};
+    *reinterpret_cast<f32x4*>(P.part_o + rec * kD + d + 4) = f32x4{r[4], r[5], r[6], r[7]};
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float* dst = &s_o[wave][c16][8 * (4 * g + i)];
-    *reinterpret_cast<f32x4*>(dst) = f32x4{o[0][i], o[1][i], o[2][i], o[3][i]};
-    *reinterpret_cast<f32x4*>(dst + 4) = f32x4{o[4][i], o[5][i], o[6][i], o[7][i]};
-  }
-  __syncthreads();
-  const int col = tid >> 4, d = 8 * (tid & 15);
-  const int cslot = P.group > 1 ? col / G : 0;
-  const bool cok = P.group > 1 ? cslot < members && ((mine >> cslot) & 1) : col < own_heads;
-  if (!cok) return;
-  const int cseq = P.group > 1 ? base + cslot : s;
-  const int64_t chead = h * G + (P.group > 1 ? col - cslot * G : 16 * tile + col);
-  float M = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][col]);
-  float L = 0.f, r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float mw = s_m[w][col];
-    if (mw == -INFINITY) continue;  // no weight yet: its sums are zeros
-    const float wt = exp2_(mw - M);
-    L = fmaf(wt, s_l[w][col], L);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = fmaf(wt, s_o[w][col][d + i], r[i]);
-  }
-  if (P.splits == 1) {
-    const float inv = L != 0.f ? 1.f / L : 0.f;
-    *reinterpret_cast<u32x4*>(P.out + cseq * P.o_ss + chead * P.o_sh + d) =
-        u32x4{pack<DT>(r[0] * inv, r[1] * inv), pack<DT>(r[2] * inv, r[3] * inv), pack<DT>(r[4] * inv, r[5] * inv),
-              pack<DT>(r[6] * inv, r[7] * inv)};
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThr, 2) void split_kernel(DecodeArgs P) {
+  __shared__ __align__(16) Staged sh;
+  const Pages& st = P.st;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = blockIdx.x, h = blockIdx.y / P.tiles, tile = blockIdx.y - h * P.tiles, s = blockIdx.z;
+  const int G = P.G;
+
+  const int len = min(held(st, st.lens[s]), P.max_len);
+  const int t0 = split * P.chunk, t1 = min(t0 + P.chunk, len);
+  // columns of the workgroup's own sequence: heads 16 tile .. of its kv head
+  const int own_heads = min(G - 16 * tile, 16), own_head = h * G + 16 * tile;
+  const int slot = P.group > 1 ? split * (P.group + 1) : split;  // of its own record
+  auto empty = [&](int from, int n) {  // records without tokens
+    for (int e = tid; e < n * own_heads; e += kThr) {
+      const int x = e / n, at = from + e - x * n;
+      *reinterpret_cast<float2*>(P.part_ml + 2 * ((static_cast<int64_t>(s) * P.Hq + own_head + x) * P.slots + at)) =
+          part_record(-INFINITY, 0.f);
+    }
+  };
+  if (t0 >= t1) {  // uniform: nothing here
+    if (P.slots == 1) {
+      for (int e = tid; e < own_heads * (kD / 8); e += kThr)
+        *reinterpret_cast<u32x4*>(P.out + s * P.o_ss + (own_head + e / (kD / 8)) * P.o_sh + 8 * (e % (kD / 8))) = u32x4{};
+    } else {
+      empty(slot, P.group > 1 ? P.group + 1 : 1);
+    }
     return;
   }
-  const int64_t rec = (static_cast<int64_t>(cseq) * P.Hq + chead) * P.splits + split;
-  if ((tid & 15) == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * rec) = part_record(M, L);
-  *reinterpret_cast<f32x4*>(P.part_o + rec * kD + d) = f32x4{r[0], r[1], r[2], r[3]};
-  *reinterpret_cast<f32x4*>(P.part_o + rec * kD + d + 4) = f32x4{r[4], r[5], r[6], r[7]};
+
+  // ---- the split's pages; of the group's sequences where they end and how many pages they begin alike
+  const int page0 = t0 >> st.lg, pages = ((t1 - 1) >> st.lg) - page0 + 1;
+  const int* row = st.table + static_cast<int64_t>(s) * st.width + page0;
+  for (int i = tid; i < pages; i += kThr) sh.page[i] = page_id(st, row[i]);
+  const int base = s - s % P.group, members = min(P.group, st.seqs - base);
+  if (P.group > 1) {
+    for (int j = wave; j < members; j += kWaves) {
+      const int end = min(t0 + P.chunk, min(held(st, st.lens[base + j]), P.max_len));
+      const int n = end > t0 ? min(((end - 1) >> st.lg) - page0 + 1, pages) : 0;
+      const int* other = st.table + static_cast<int64_t>(base + j) * st.width + page0;
+      int same = n;
+      for (int i = 0; i < n; i += 64) {
+        const int k = min(i + lane, n - 1);
+        const uint64_t differs = wave_ballot(page_id(st, row[k]) != page_id(st, other[k]));
+        if (differs) {
+          same = min(n, i + static_cast<int>(__builtin_ctzll(differs)));
+          break;
+        }
+      }
+      if (lane == 0) {
+        sh.end[j] = end;
+        sh.same[j] = same;
+      }
+    }
+  }
+  __syncthreads();
+  int shared = t0, rank = 0, count = 0;  // shared tokens [t0, shared) of `count` sequences, this one the rank-th of them
+  if (P.group > 1) {
+    const int same = lane < members ? sh.same[lane] : 0;
+    const uint32_t alike = static_cast<uint32_t>(wave_ballot(same > 0));
+    int end = same > 0 ? min(sh.end[lane], (page0 + same) << st.lg) : 0x7fffffff;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) end = min(end, __shfl_xor(end, x));
+    end = __builtin_amdgcn_readfirstlane(end);
+    if (__popc(alike) > 1 && end - t0 >= kStep) {  // (less is not worth a second part)
+      shared = end;
+      count = __popc(alike);
+      rank = __popc(alike & ((1u << (s - base)) - 1));
+      if (wave == 0 && same > 0) sh.member[__popc(alike & ((1u << lane) - 1))] = lane;
+    }
+    __syncthreads();
+    empty(slot + 1 + count, P.group - count);
+  }
+  if (count) {
+    const int cols = count * G;
+    auto where = [&](int c, int& seq, int& head) {
+      const int i = c * P.g_small >> 16;
+      seq = base + sh.member[i];
+      head = h * G + c - i * G;
+    };
+    const int part = ((shared - t0 + count - 1) / count + kChunk - 1) & ~(kChunk - 1);
+    const int lo = min(t0 + rank * part, shared), hi = min(lo + part, shared);
+    if (cols <= 16)
+      attend<DT, 1>(P, sh, h, page0, lo, hi, cols, slot + 1 + rank, where);
+    else
+      attend<DT, 2>(P, sh, h, page0, lo, hi, cols, slot + 1 + rank, where);
+  }
+  if (shared < t1)
+    attend<DT, 1>(P, sh, h, page0, shared, t1, own_heads, slot, [&](int c, int& seq, int& head) {
+      seq = s;
+      head = own_head + c;
+    });
+  else
+    empty(slot, 1);
 }
 
 struct JoinArgs {
@@ -304,17 +373,19 @@ __global__ __launch_bounds__(kThr) void join_kernel(JoinArgs A) {
 }
 
 struct DecodePlan {
-  int chunk, splits;
+  int chunk, splits, group, slots;
 };
 
 DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len) {
-  const int64_t tiles = (Hq / Hkv + 15) / 16, pairs = S * Hkv * tiles;
+  const int64_t G = Hq / Hkv, tiles = (G + 15) / 16, pairs = S * Hkv * tiles;
   const int64_t steps = (max_len + kStep - 1) / kStep;
+  // Two workgroups a CU, the most that its registers hold at a time (32 x 8192 tokens, 32/8 heads: 186 us, with four 191, 131072
+  // tokens 100 and 108 us).  One split, which needs no join and shares nothing, where a workgroup a CU walks at most 8 steps
+  // (32 x 1024: 24.2 us, in two splits 27.6), and up to 3 steps anyway.
+  const int64_t cus = device_cu_count();
   int64_t splits = 1;
-  if (steps > 3) {
-    const int64_t target = 4ll * device_cu_count();
-    splits = (target + pairs - 1) / pairs;
-    splits = splits < 1 ? 1 : splits;
+  if (steps > (pairs >= cus ? 8 : 3)) {
+    splits = (2 * cus + pairs - 1) / pairs;
     splits = splits > steps ? steps : splits;
     splits = splits > kMaxSplits ? kMaxSplits : splits;
   }
@@ -325,6 +396,8 @@ DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len) {
   DecodePlan p;
   p.splits = static_cast<int>(steps <= chunk ? 1 : (steps + chunk - 1) / chunk);
   p.chunk = static_cast<int>(chunk * kStep);
+  p.group = p.splits > 1 && S > 1 && G <= 16 ? static_cast<int>(32 / G) : 1;
+  p.slots = p.group > 1 ? p.splits * (p.group + 1) : p.splits;
   return p;
 }
 
@@ -360,7 +433,7 @@ using namespace lkv::pages;
 extern "C" size_t lkv_pages_decode_attn_workspace_bytes(int64_t seqs, int64_t Hq, int64_t Hkv, int64_t max_len) {
   if (seqs < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || max_len < 0) return 0;
   const DecodePlan p = decode_plan(seqs, Hq, Hkv, max_len);
-  return p.splits == 1 ? 0 : static_cast<size_t>(seqs * Hq) * p.splits * (kD + 2) * 4;
+  return p.slots == 1 ? 0 : static_cast<size_t>(seqs * Hq) * p.slots * (kD + 2) * 4;
 }
 
 extern "C" int lkv_pages_decode_attn(const lkv_pages* p, int64_t layer, const void* q, const int64_t* q_strides,
@@ -393,13 +466,15 @@ extern "C" int lkv_pages_decode_attn(const lkv_pages* p, int64_t layer, const vo
   A.Hq = static_cast<int>(Hq);
   A.G = static_cast<int>(G);
   A.tiles = static_cast<int>(tiles);
-  A.group = G <= 8 ? static_cast<int>(16 / G) : 1;
+  A.group = plan.group;
+  A.g_small = static_cast<int>(65536 / G + 1);
+  A.slots = plan.slots;
   A.max_len = static_cast<int>(max_len);
   A.chunk = plan.chunk;
   A.splits = plan.splits;
   A.scale_log2 = scale * kLog2e;
   A.part_o = static_cast<float*>(workspace);
-  A.part_ml = A.part_o + static_cast<size_t>(p->seqs * Hq) * plan.splits * kD;
+  A.part_ml = A.part_o + static_cast<size_t>(p->seqs * Hq) * plan.slots * kD;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(plan.splits), static_cast<unsigned>(p->kv_heads * tiles),
                   static_cast<unsigned>(p->seqs));
@@ -408,7 +483,7 @@ extern "C" int lkv_pages_decode_attn(const lkv_pages* p, int64_t layer, const vo
   else
     hipLaunchKernelGGL(split_kernel<LKV_DTYPE_BF16>, grid, dim3(kThr), 0, s, A);
   LKV_LAUNCH_CHECK(what);
-  if (plan.splits == 1) return LKV_OK;
-  return launch_join(A.part_o, A.part_ml, p->seqs * Hq, plan.splits, Hq, out, A.o_ss, A.o_sh, p->dtype, nullptr, 0, s,
+  if (plan.slots == 1) return LKV_OK;
+  return launch_join(A.part_o, A.part_ml, p->seqs * Hq, plan.slots, Hq, out, A.o_ss, A.o_sh, p->dtype, nullptr, 0, s,
                      "pages_decode_attn join");
 }
