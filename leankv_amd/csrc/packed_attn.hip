@@ -30,7 +30,8 @@ constexpr int kKRow = kD + 8;     // 16-bit numbers of a staged key row: 16 rows
 constexpr int kVRow = kD + 32;    // and of a value row: the transposing read's 4 rows of 64 bytes do
 constexpr int kKBuf = kTile * kKRow, kVBuf = kTile * kVRow;
 constexpr int kXcds = 8;
-constexpr int kManyChunk = 8;     // fewest tiles of a split
+constexpr int kLeast = 4;         // fewest tiles of a part of the longest piece
+constexpr int kMostCuts = 32;
 constexpr int kPlan = 64;         // pieces of a workgroup that are found at once
 constexpr int kAgain = 128;       // words of marks (rounds past 4096 share them: gone through again without need)
 
@@ -60,10 +61,11 @@ struct Args {
   Pages st;            // PAGED: the store, and the layer's pages
   const uint16_t* kv;
   int H, G, Hq;
-  int chunk, splits;   // tiles of a split
+  int splits;          // most parts of a piece, 1: none is cut
   int fill;
   uint32_t g_mul;      // x / G = x * g_mul >> g_shift for x below 2^31
-  int g_shift, g_small;  // and x * g_small >> 16 for x below G + 32, where G is below 32
+  int g_shift;
+  int g_small, g_big;  // for x below G + 32: (x * g_small >> 16) + (x >= g_big), g_small 0 from G = 32 on, g_big G then
   float scale_log2;
   float* part_o;       // [rows * Hq][splits][128]
   float* part_ml;      // [rows * Hq][splits][2]
@@ -105,17 +107,31 @@ __device__ __forceinline__ int wave_prefix(int v) {  // inclusive
 }
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
 
+// Parts of the column tiles with more than x tokens to read, where a tile of T tiles of tokens is ceil(T / chunk) parts (at
+// most cuts): one for every j with T > j chunk.  By the lanes of a wave, a (sequence, j) each.
+__device__ __forceinline__ int parts_over(int x, const int* s_len, const int* s_rows, int B, int G, int cuts, int chunk) {
+  int n = 0;
+  const float by = 1.f / cuts;
+  for (int i = lane_prefix(~0ull); i < B * cuts; i += 64) {
+    const int b = static_cast<int>((i + 0.5f) * by), j = i - b * cuts;  // (exact: i is below 2^18)
+    n += tiles_over(j ? max(x, j * chunk * kTile) : x, s_len[b], s_rows[b], G);
+  }
+  return wave_total(n);
+}
+
 // Goes through the workgroup's pieces.  CARE: those that the first time marked in s_again, with care for values that are no
 // numbers.  Returns whether any is to be gone through again.
 template <int DT, bool PAGED, bool CARE>
-__device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const int* s_len, const int* s_rows,
-                                           const int* s_first, int4* s_plan, uint32_t* s_again, int wave, int longest, int pieces) {
+__device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const int* s_len, const int* s_rows,
+                                           const int* s_first, int4* s_plan, uint32_t* s_again, int wave, int longest,
+                                           int pieces, int cuts, int chunk) {
   uint16_t* const sK = smem;
   uint16_t* const sV = smem + 2 * kKBuf;
-  const int lane = lane_prefix(~0ull);
+  int lane = lane_prefix(~0ull);
+  if (CARE) __asm__ volatile("" : "+v"(lane));  // (what follows from it is not kept from the first time)
   const int c32 = lane & 31, hf = lane >> 5;
   const int G = P.G;
-  bool again = false;
+  int again = 0;
 
   // ---- staging: thread's rows 8 wave + lane / 16 and 4 further, piece lane % 16 of 16 bytes
   const int srow = lane >> 4, spiece = 8 * (lane & 15);
@@ -136,7 +152,7 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
   const int heads_lane = P.H / lanes;
   const int width = static_cast<int>(gridDim.x) / lanes;
   const int own = static_cast<int>(blockIdx.x) / lanes, xcd = static_cast<int>(blockIdx.x) % lanes;
-  const int per_lane = pieces * P.splits * heads_lane;
+  const int per_lane = pieces * heads_lane;
   const int every = (per_lane + width - 1) / width;  // rounds, of which the last may have nothing for this workgroup
   auto place_of = [&](int round) { return round * width + ((round & 1) ? width - 1 - own : own); };
   const int rounds = every && place_of(every - 1) >= per_lane ? every - 1 : every;
@@ -144,20 +160,19 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
   const int shift = rounds ? own % rounds : 0;
   auto turn_of = [&](int round) { return round + shift < rounds ? round + shift : round + shift - rounds; };
 
-  // ---- what the pieces of rounds r .. r + 63 are, found by the waves side by side: the n-th column tile by falling length
-  // (its length in tiles of tokens, then its place among those)
+  // ---- what the pieces of rounds r .. r + 63 are, found by the waves side by side: the n-th part of a column tile by the
+  // tile's falling length (its length in tiles of tokens, then its place among those)
   auto find_pieces = [&](int r) {
+    const ArgsPtr Z = args_again();
+    const int n_seqs = Z->B;
     for (int i = wave; i < min(kPlan, rounds - r); i += kWaves) {
       const int pos = place_of(turn_of(r + i));
-      const int ps = __builtin_amdgcn_readfirstlane(pos / heads_lane);
-      const int h = (pos - ps * heads_lane) * lanes + xcd;
-      const int piece = __builtin_amdgcn_readfirstlane(ps / P.splits), split = ps - piece * P.splits;
-      int lo = -1, hi = (longest + kTile - 1) / kTile, over = 0;  // more than `piece` tiles over 64 lo, none over 64 hi
+      const int piece = __builtin_amdgcn_readfirstlane(pos / heads_lane);
+      const int h = (pos - piece * heads_lane) * lanes + xcd;
+      int lo = -1, hi = (longest + kTile - 1) / kTile, over = 0;  // more than `piece` parts over 64 lo, none over 64 hi
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        int n = 0;
-        for (int j = lane; j < P.B; j += 64) n += tiles_over(mid * kTile, s_len[j], s_rows[j], G);
-        n = wave_total(n);
+        const int n = parts_over(mid * kTile, s_len, s_rows, n_seqs, G, cuts, chunk);
         if (n > piece) {
           lo = mid;
         } else {
@@ -165,12 +180,15 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
           over = n;
         }
       }
+      // its tile has hi tiles of tokens (none with hi = 0): ns parts, as all between
+      const int ns = max((hi + chunk - 1) / chunk, 1);
       const int x = lo < 0 ? -1 : lo * kTile, x2 = hi * kTile;
-      int rank = piece - over, b = 0, tile = 0;
-      for (int base = 0; base < P.B; base += 64) {
+      int rank = (piece - over) / ns, b = 0, tile = 0;
+      const int split = piece - over - rank * ns;
+      for (int base = 0; base < n_seqs; base += 64) {
         const int j = base + lane;
-        const int high = j < P.B ? tiles_over(x2, s_len[j], s_rows[j], G) : 0;
-        const int n = j < P.B ? tiles_over(x, s_len[j], s_rows[j], G) - high : 0;
+        const int high = j < n_seqs ? tiles_over(x2, s_len[j], s_rows[j], G) : 0;
+        const int n = j < n_seqs ? tiles_over(x, s_len[j], s_rows[j], G) - high : 0;
         const int sum = wave_prefix(n);
         const uint64_t past = wave_ballot(sum > rank);
         if (past) {
@@ -188,18 +206,19 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
       const int len = s_len[b], rows = s_rows[b], qlen = min(rows, len), col0 = tile * kCols;
       const int last = min(by_heads(P, col0 + kCols - 1), qlen - 1);  // its last query
       const int kend = last >= by_heads(P, col0) ? len - qlen + last + 1 : 0;
-      const int blk0 = split * P.chunk, all_t = (kend + kTile - 1) / kTile;
-      const int nt = max((split == P.splits - 1 ? all_t : min(blk0 + P.chunk, all_t)) - blk0, 0);
+      const int all_t = (kend + kTile - 1) / kTile;
+      const int part = (all_t + ns - 1) / ns, blk0 = split * part;
+      const int nt = max(min(part, all_t - blk0), 0);
       if (lane == 0) {
         s_plan[3 * i] = int4{b, h, split, len};
         s_plan[3 * i + 1] = int4{s_first[b], qlen, rows * G, col0};
-        s_plan[3 * i + 2] = int4{blk0, nt, 0, 0};
+        s_plan[3 * i + 2] = int4{blk0, nt, ns, 0};
       }
     }
   };
 
   struct Piece {
-    int b, h, split, len, row0, qlen, cols, col0, blk0, nt;
+    int b, h, split, len, row0, qlen, cols, col0, blk0, nt, ns;
   };
   auto open = [&](int round) {
     if ((round & (kPlan - 1)) == 0) {
@@ -220,6 +239,7 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
     c.col0 = __builtin_amdgcn_readfirstlane(y.w);
     c.blk0 = __builtin_amdgcn_readfirstlane(z.x);
     c.nt = __builtin_amdgcn_readfirstlane(z.y);
+    c.ns = __builtin_amdgcn_readfirstlane(z.z);
     return c;
   };
 
@@ -265,7 +285,7 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
     return Cols{q0, x - q0 * G};
   };
   auto column = [&](const Cols& w, int r) {
-    const int x = w.h0 + r, dq = G < 32 ? x * P.g_small >> 16 : (x >= G ? 1 : 0);
+    const int x = w.h0 + r, dq = (x * P.g_small >> 16) + (x >= P.g_big ? 1 : 0);
     return int2{dq, x - dq * G};
   };
   // the wave's own part of LDS, where its query rows and its output rows turn between rows and operands
@@ -279,11 +299,13 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
     const int end = max(c.qlen * G - 1 - c.col0 - 32 * wave, 0);
     const ArgsPtr Z = args_again();
     const uint32_t q_st = Z->q_st, q_sh = Z->q_sh;
+    int r0 = srow;
+    __asm__ volatile("" : "+v"(r0));  // (its sums are made where they are used)
     const uint16_t* p = Z->q + static_cast<uint64_t>(c.row0 + min(w.q0, max(c.qlen - 1, 0))) * q_st +
                         static_cast<uint64_t>(c.h * G) * q_sh + spiece;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int2 x = column(w, min(4 * j + srow, end));
+      const int2 x = column(w, min(4 * j + r0, end));
       qf[j] = *reinterpret_cast<const u32x4*>(p + (static_cast<uint64_t>(static_cast<uint32_t>(x.x)) * q_st +
                                                    static_cast<uint64_t>(static_cast<uint32_t>(x.y)) * q_sh));
     }
@@ -310,7 +332,7 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
     }
     load_queries(c);
   };
-  if (!rounds) return false;
+  if (!rounds) return 0;
   Piece c = open(0);
   if constexpr (!CARE) first_loads(c);
 #pragma unroll 1
@@ -569,7 +591,7 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
         for (int i = 0; i < 16; ++i) odd[i & 3] = fmaf(o[db][i], 0.f, odd[i & 3]);
       if (wave_ballot(ok && (odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.f)) {
         if (lane == 0) atomicOr(&s_again[(round >> 5) & (kAgain - 1)], 1u << (round & 31));
-        again = true;
+        again = 1;
       }
     }
     Piece next = c;
@@ -601,7 +623,13 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
         if (row < end) put(static_cast<uint32_t>(x.x), static_cast<uint32_t>(x.y), v);
       }
     };
-    if (Z->splits == 1) {
+    const int slots = Z->splits;
+    if (c.ns == 1) {
+      if (slots > 1 && oh == 0 && ox < ends) {  // (a mark for the join: this row is done)
+        const int2 x = column(first, ox);
+        const int64_t at = static_cast<int64_t>(c.row0 + first.q0 + x.x) * Z->Hq + c.h * G + x.y;
+        *reinterpret_cast<float2*>(Z->part_ml + 2 * at * slots) = float2{-INFINITY, -1.f};
+      }
       const bool some = ok && l != 0.f;
       const float inv = some ? 1.f / l : 0.f;
 #pragma unroll
@@ -621,12 +649,15 @@ __device__ __forceinline__ bool go_through(const Args& P, uint16_t* smem, const 
       });
     } else {
       // (a split without tokens leaves its rows unwritten: its record is empty)
-      const int64_t base = (static_cast<int64_t>(c.row0 + first.q0) * Z->Hq + c.h * G) * Z->splits + c.split;
-      const uint32_t by_q = Z->Hq * Z->splits, by_h = Z->splits;
+      const int64_t base = (static_cast<int64_t>(c.row0 + first.q0) * Z->Hq + c.h * G) * slots + c.split;
+      const uint32_t by_q = Z->Hq * slots, by_h = slots;
       if (oh == 0 && ox < ends) {
         const int2 x = column(first, ox);
         const int64_t at = base + static_cast<int64_t>(x.x) * by_q + static_cast<int64_t>(x.y) * by_h;
-        *reinterpret_cast<float2*>(Z->part_ml + 2 * at) = ok && nt > 0 ? part_record(m, l) : part_record(-INFINITY, 0.f);
+        float2* const ml = reinterpret_cast<float2*>(Z->part_ml) + at;
+        *ml = ok && nt > 0 ? part_record(m, l) : part_record(-INFINITY, 0.f);
+        if (c.split == 0)
+          for (int i = c.ns; i < slots; ++i) ml[i] = part_record(-INFINITY, 0.f);
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -657,6 +688,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
   __shared__ int s_len[kMaxSeqs], s_rows[kMaxSeqs], s_first[kMaxSeqs];
   __shared__ int4 s_plan[3 * kPlan];
   __shared__ uint32_t s_again[kAgain];  // pieces to go through again, by round
+  __shared__ int s_any;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tid = threadIdx.x, lane = tid & 63;
   const int G = P.G;
@@ -670,6 +702,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
     s_len[b] = PAGED ? held(P.st, P.st.lens[b]) : e - a;
   }
   if (tid < kAgain) s_again[tid] = 0;
+  if (tid == 0) s_any = 0;
   __syncthreads();
   int pieces = 0;  // column tiles of all sequences
   for (int b = lane; b < P.B; b += 64) {
@@ -681,9 +714,66 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
   longest = __builtin_amdgcn_readfirstlane(longest);
   pieces = wave_total(pieces);
 
-  const bool again = go_through<DT, PAGED, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces);
-  if (__syncthreads_or(again)) {
-    go_through<DT, PAGED, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces);
+  // ---- into how many parts the longest pieces are cut.  What that takes, in tiles: the longest part, or the workgroups' mean
+  // and some of a part, about 4 a round for beginning and ending pieces, and writing and joining the parts' rows.  The waves
+  // look at every eighth number each.
+  int cuts = 1, chunk = 1 << 24;
+  if (P.splits > 1) {
+    float work = 0.f;
+    int cols = 0;
+    for (int b = lane; b < P.B; b += 64) {
+      const int len = s_len[b], rows = s_rows[b], q = min(rows, len);
+      work += tiles_over(-1, len, rows, G) * (len - 0.5f * q + 0.5f * min(kCols / G, q) + 0.5f * kTile) * (1.f / kTile);
+      cols += rows * G;
+    }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) work += __shfl_xor(work, x);
+    cols = wave_total(cols);
+    const float grid = gridDim.x, mean = work * P.H / grid;
+    const int most = (longest + kTile - 1) / kTile;
+    float best = INFINITY;
+    int best_k = 1, best_n = pieces;
+    for (int k = wave + 1; k <= P.splits; k += kWaves) {
+      const int part = (most + k - 1) / k;
+      int n = pieces, cut = 0;  // parts in all, column tiles that are cut
+      if (k > 1) {
+        if (part < kLeast) break;
+        n = parts_over(-1, s_len, s_rows, P.B, G, k, part);
+        for (int b = lane; b < P.B; b += 64) cut += tiles_over(part * kTile, s_len[b], s_rows[b], G);
+        cut = wave_total(cut);
+      }
+      const float items = static_cast<float>(n) * P.H;
+      const float load = items <= grid ? part : fmaxf(mean + 0.3f * part, part);
+      const float join = k > 1 ? 1.f + static_cast<float>(min(cut * kCols, cols)) * (P.H * k) * (1040 / 7.6e6f) : 0.f;
+      const float takes = (load + 4.f * ceilf(items / grid) + join) * (k > 1 ? 1.05f : 1.f);
+      if (takes < best) {
+        best = takes;
+        best_k = k;
+        best_n = n;
+      }
+    }
+    if (lane == 0) s_plan[wave] = int4{__float_as_int(best), best_k, best_n, 0};
+    __syncthreads();
+    best = INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const int4 x = s_plan[w];
+      if (__int_as_float(x.x) < best || w == 0) {
+        best = __int_as_float(x.x);
+        cuts = x.y;
+        pieces = x.z;
+      }
+    }
+    cuts = __builtin_amdgcn_readfirstlane(cuts);
+    pieces = __builtin_amdgcn_readfirstlane(pieces);
+    if (cuts > 1) chunk = (most + cuts - 1) / cuts;
+  }
+
+  const int again = go_through<DT, PAGED, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk);
+  if (again && lane == 0) s_any = 1;
+  __syncthreads();
+  if (s_any) {
+    go_through<DT, PAGED, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk);
   }
 
   // ---- rows of no sequence
@@ -691,7 +781,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
   if (Z->fill) {
     const int a = min(max(Z->cu[0], 0), Z->rows), e = min(max(Z->cu[Z->B], a), Z->rows);
     const int64_t per = static_cast<int64_t>(Z->Hq) * (kD / 8), n = (a + Z->rows - e) * per;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThr + tid; i < n; i += static_cast<int64_t>(gridDim.x) * kThr) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThr + 64 * wave + lane_prefix(~0ull); i < n; i += static_cast<int64_t>(gridDim.x) * kThr) {
       const int64_t r = i / per, x = i - r * per;
       const int64_t row = r < a ? r : r - a + e;
       *reinterpret_cast<u32x4*>(Z->out + row * Z->o_st + x / (kD / 8) * Z->o_sh + 8 * (x % (kD / 8))) = u32x4{};
@@ -701,24 +791,33 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
 
 struct Plan {
   int64_t pieces;  // most column tiles of a kv head, over all sequences
-  int chunk, splits;
+  int splits;      // parts that a piece may be cut into (the kernel decides, by the lengths)
 };
 
-Plan make_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_len) {
+// enough: so many pieces are shared out evenly enough as they are.
+Plan make_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_len, int64_t enough) {
   const int64_t G = Hq / Hkv;
   const int64_t each = B * ((max_new * G + kCols - 1) / kCols), packed = rows * G / kCols + B;
   Plan p;
   p.pieces = each < packed ? each : packed;
   p.pieces = p.pieces < 1 ? 1 : p.pieces;
-  const int64_t cus = device_cu_count(), tiles = (max_len + kTile - 1) / kTile;
-  int64_t splits = cus / (p.pieces * Hkv);
-  const int64_t most = tiles / kManyChunk;
-  splits = splits > most ? most : splits;
-  splits = splits < 1 ? 1 : splits;
-  const int64_t chunk = (tiles + splits - 1) / splits;
-  p.chunk = static_cast<int>(chunk < 1 ? 1 : chunk);
-  p.splits = static_cast<int>(tiles <= p.chunk ? 1 : (tiles + p.chunk - 1) / p.chunk);
+  const int64_t cus = device_cu_count(), tiles = (max_len + kTile - 1) / kTile, work = p.pieces * Hkv;
+  int64_t splits = work >= enough ? 1 : (2 * cus + work - 1) / work;
+  splits = splits > tiles / kLeast ? tiles / kLeast : splits;
+  p.splits = static_cast<int>(splits < 1 ? 1 : splits > kMostCuts ? kMostCuts : splits);
   return p;
+}
+
+// Whole prompts: a piece for three CUs in four.  (1 x 2048 tokens, 32/8 heads, a piece a CU: cutting the longer ones would cost
+// as much in rows to join as it gains.)
+Plan packed_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_len) {
+  const int64_t most = max_len < rows ? max_len : rows;
+  return make_plan(rows, B, Hq, Hkv, most, most, device_cu_count() * 3ll / 4);
+}
+// Over pages: three pieces a CU.  (Chunks to 512 over 1.6-8 K tokens of 4 sequences, 0.8 pieces a CU: 254 us as they are, 210
+// with the longest cut in two; the launch that joins costs 5 us where none is cut.)
+Plan pages_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_len) {
+  return make_plan(rows, B, Hq, Hkv, max_new < rows ? max_new : rows, max_len, 3ll * device_cu_count());
 }
 
 size_t plan_bytes(const Plan& p, int64_t rows, int64_t Hq) {
@@ -734,7 +833,7 @@ int launch(Args A, const Plan& p, int dtype, void* workspace, size_t workspace_b
   while ((1ll << (A.g_shift - 31)) < A.G) ++A.g_shift;
   A.g_mul = static_cast<uint32_t>((1ull << A.g_shift) / A.G + 1);
   A.g_small = A.G < 32 ? 65536 / A.G + 1 : 0;
-  A.chunk = p.chunk;
+  A.g_big = A.G < 32 ? 0x7fffffff : A.G;
   A.splits = p.splits;
   A.part_o = static_cast<float*>(workspace);
   A.part_ml = A.part_o + static_cast<size_t>(A.rows) * A.Hq * p.splits * kD;
@@ -770,8 +869,7 @@ using namespace lkv::pages;
 
 extern "C" size_t lkv_packed_attn_workspace_bytes(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_len) {
   if (rows < 1 || B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || max_len < 0) return 0;
-  const int64_t most = max_len < rows ? max_len : rows;
-  return plan_bytes(make_plan(rows, B, Hq, Hkv, most, most), rows, Hq);
+  return plan_bytes(packed_plan(rows, B, Hq, Hkv, max_len), rows, Hq);
 }
 
 extern "C" int lkv_packed_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -812,15 +910,14 @@ extern "C" int lkv_packed_attn(const void* q, const int64_t* q_strides, const vo
   A.Hq = static_cast<int>(Hq);
   A.fill = fill;
   A.scale_log2 = scale * kLog2e;
-  const int64_t most = max_len < rows ? max_len : rows;
-  return launch<false>(A, make_plan(rows, B, Hq, Hkv, most, most), dtype, workspace, workspace_bytes,
+  return launch<false>(A, packed_plan(rows, B, Hq, Hkv, max_len), dtype, workspace, workspace_bytes,
                        static_cast<hipStream_t>(stream), what);
 }
 
 extern "C" size_t lkv_pages_prefill_attn_workspace_bytes(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv,
                                                          int64_t max_new, int64_t max_len) {
   if (rows < 1 || seqs < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || max_new < 0 || max_len < 0) return 0;
-  return plan_bytes(make_plan(rows, seqs, Hq, Hkv, max_new < rows ? max_new : rows, max_len), rows, Hq);
+  return plan_bytes(pages_plan(rows, seqs, Hq, Hkv, max_new, max_len), rows, Hq);
 }
 
 extern "C" int lkv_pages_prefill_attn(const lkv_pages* p, int64_t layer, const void* q, const int64_t* q_strides,
@@ -854,6 +951,6 @@ extern "C" int lkv_pages_prefill_attn(const lkv_pages* p, int64_t layer, const v
   A.Hq = static_cast<int>(Hq);
   A.fill = fill;
   A.scale_log2 = scale * kLog2e;
-  return launch<true>(A, make_plan(rows, p->seqs, Hq, p->kv_heads, max_new < rows ? max_new : rows, max_len), p->dtype,
+  return launch<true>(A, pages_plan(rows, p->seqs, Hq, p->kv_heads, max_new, max_len), p->dtype,
                       workspace, workspace_bytes, static_cast<hipStream_t>(stream), what);
 }

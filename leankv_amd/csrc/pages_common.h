@@ -90,7 +90,7 @@ __device__ __forceinline__ float2 part_record(float m, float l) { return float2{
 
 // Joins the partial sums of rows of 128 numbers (pages_decode.hip): part_ml [rows][splits][2], part_o [rows][splits][128],
 // row r's result to out + (r / heads) * o_st + (r % heads) * o_sh.  cu (optional): rows of tokens before cu[0] or from
-// cu[n] on are skipped.
+// cu[n] on are skipped.  So is a row whose first sum is negative.
 int launch_join(const float* part_o, const float* part_ml, int64_t rows, int64_t splits, int64_t heads, void* out,
                 int64_t o_st, int64_t o_sh, int dtype, const int* cu, int n, hipStream_t stream, const char* what);
 

@@ -338,6 +338,7 @@ __global__ __launch_bounds__(kThr) void join_kernel(JoinArgs A) {
   const int t = row / A.heads, head = row - t * A.heads;
   if (A.cu && (t < A.cu[0] || t >= A.cu[A.n])) return;
   const float2* ml = reinterpret_cast<const float2*>(A.part_ml) + static_cast<int64_t>(row) * A.splits;
+  if (ml[0].y < 0.f) return;  // the row is done (no sum of weights is negative)
   const float* po = A.part_o + static_cast<int64_t>(row) * A.splits * kD + d;
   float M = -INFINITY;
   for (int i = tid & 31; i < A.splits; i += 32) M = fmaxf(M, ml[i].x);
