@@ -27,6 +27,8 @@ def strides2(row: int, head: int):
 def in_place(t: torch.Tensor):
     """The strides of row and head of t [rows, heads, 128] as the kernels take them, None where its rows are not dense or not
     16-byte aligned.  Strides of single sizes count as 0 (torch leaves them free)."""
+    if t.is_contiguous() and not t.data_ptr() % 16:
+        return strides2(t.shape[1] * HEAD_DIM, HEAD_DIM)
     n, (r, h, d) = t.shape, t.stride()
     if n[0] <= 1:
         r = 0
@@ -64,7 +66,10 @@ def follow(what: str, *tensors: torch.Tensor) -> bool:
     """Whether autograd follows one of them.  A forward-mode tangent would be lost at once and is refused."""
     if getattr(forward_ad, "_current_level", -1) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise LeanKVError("%s: there is no forward-mode derivative" % what)
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    for t in tensors:
+        if t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 class _NoBackward(torch.autograd.Function):
@@ -85,16 +90,15 @@ def tied(out: torch.Tensor, what: str, *anchors: torch.Tensor) -> torch.Tensor:
     return _NoBackward.apply(out, what, *anchors)
 
 
-def call(index: int, name: str, *args) -> None:
-    """One C entry on a device and that device's current stream."""
-    fn = getattr(_lib.load(), name)
+def call(index: int, fn, *args) -> None:
+    """One C entry (of the loaded library) on a device and that device's current stream."""
     if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
-        check(rc, name)
+        check(rc, fn.__name__)
 
 
 @functools.lru_cache(maxsize=256)
@@ -150,7 +154,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     batch = cu_seqlens.shape[0] - 1
     nbytes = _bytes(n, batch, heads, kv_heads, bound)
     ws = q.new_empty(nbytes // 2) if nbytes else None
-    call(index, "lkv_packed_attn", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, DTYPES[q.dtype], n, heads, kv_heads,
+    call(index, _lib.load().lkv_packed_attn, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, DTYPES[q.dtype], n, heads, kv_heads,
          cu_seqlens.data_ptr(), batch, bound, SCALE if scale is None else scale, out.data_ptr(), os, int(fill),
          None if ws is None else ws.data_ptr(), nbytes)
     return out

@@ -90,7 +90,7 @@ class PagedKV:
                                         self.kv_heads, self.page_size, self.max_seqs, self.width, DTYPES[dtype])
         self._ref = ctypes.byref(self._struct)
         self._index = self.device.index
-        lib = _lib.load()
+        self._lib = lib = _lib.load()
         self._extend_bytes = lib.lkv_pages_extend_workspace_bytes(self.num_pages, self.max_seqs)
         self._fork_bytes = lib.lkv_pages_fork_workspace_bytes(self.max_seqs, self.width)
         self._compact_bytes = lib.lkv_pages_compact_workspace_bytes(self.num_pages)
@@ -162,7 +162,7 @@ class PagedKV:
         takes nothing: taken says what each took.  Two launches."""
         p = self._cu(cu, "PagedKV.extend")
         ws = self._workspace(self._extend_bytes)
-        call(self._index, "lkv_pages_extend", self._ref, p, ws.data_ptr(), self._extend_bytes)
+        call(self._index, self._lib.lkv_pages_extend, self._ref, p, ws.data_ptr(), self._extend_bytes)
 
     def store(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor | None = None) -> None:
         """Keys and values [rows, kv_heads, 128] of what the last extend made room for, in one layer: rows cu[s] .. of
@@ -179,7 +179,7 @@ class PagedKV:
         if follow(what, k, v):
             self._followed = True
         (k, ks), (v, vs) = rows(k), rows(v)
-        call(self._index, "lkv_pages_store", self._ref, layer, k.data_ptr(), ks, v.data_ptr(), vs, k.shape[0], p)
+        call(self._index, self._lib.lkv_pages_store, self._ref, layer, k.data_ptr(), ks, v.data_ptr(), vs, k.shape[0], p)
 
     def read(self, layer: int, n: int):
         """(K, V) [max_seqs, kv_heads, n, 128]: tokens 0 .. n - 1 of every sequence in one layer, zeros past its length."""
@@ -191,7 +191,7 @@ class PagedKV:
         if self._followed and torch.is_grad_enabled():
             kv = tied(kv, what, torch.zeros((), device="cpu", requires_grad=True))
         k, v = kv.unbind(0)
-        call(self._index, "lkv_pages_read", self._ref, layer, n, k.data_ptr(), v.data_ptr())
+        call(self._index, self._lib.lkv_pages_read, self._ref, layer, n, k.data_ptr(), v.data_ptr())
         return k, v
 
     # -------------------------------------------------------------------------------------------------- pages
@@ -203,7 +203,7 @@ class PagedKV:
         p = None if parent is None else self._ints(parent, self.max_seqs, what, "parent")
         c = None if lens is None else self._ints(lens, self.max_seqs, what, "lens")
         ws = self._workspace(self._fork_bytes)
-        call(self._index, "lkv_pages_fork", self._ref, p, c, ws.data_ptr(), self._fork_bytes)
+        call(self._index, self._lib.lkv_pages_fork, self._ref, p, c, ws.data_ptr(), self._fork_bytes)
 
     def truncate(self, lens: torch.Tensor) -> None:
         """Every sequence keeps at most its first lens[s] tokens (int32 [max_seqs]; drafted tokens that were not accepted)."""
@@ -230,7 +230,7 @@ class PagedKV:
         their number, int32 [1] on the device.  Two launches."""
         ws = self._workspace(self._compact_bytes)
         in_use = self._books.new_empty(1)
-        call(self._index, "lkv_pages_compact", self._ref, in_use.data_ptr(), ws.data_ptr(), self._compact_bytes)
+        call(self._index, self._lib.lkv_pages_compact, self._ref, in_use.data_ptr(), ws.data_ptr(), self._compact_bytes)
         return in_use
 
     def resized(self, num_pages: int) -> "PagedKV":
@@ -279,7 +279,7 @@ class PagedKV:
         q, qs = rows(q)
         nbytes = _decode_bytes(self.max_seqs, heads, self.kv_heads, bound)
         ws = self._workspace(nbytes) if nbytes else None
-        call(self._index, "lkv_pages_decode_attn", self._ref, layer, q.data_ptr(), qs, heads, bound,
+        call(self._index, self._lib.lkv_pages_decode_attn, self._ref, layer, q.data_ptr(), qs, heads, bound,
              SCALE if scale is None else scale, out.data_ptr(), os, None if ws is None else ws.data_ptr(), nbytes)
         return out
 
@@ -305,6 +305,6 @@ class PagedKV:
         q, qs = rows(q)
         nbytes = _prefill_bytes(n, self.max_seqs, heads, self.kv_heads, new, bound)
         ws = self._workspace(nbytes) if nbytes else None
-        call(self._index, "lkv_pages_prefill_attn", self._ref, layer, q.data_ptr(), qs, n, heads, p, new, bound,
+        call(self._index, self._lib.lkv_pages_prefill_attn, self._ref, layer, q.data_ptr(), qs, n, heads, p, new, bound,
              SCALE if scale is None else scale, out.data_ptr(), os, int(fill), None if ws is None else ws.data_ptr(), nbytes)
         return out
