@@ -22,15 +22,22 @@ namespace lkv {
 namespace pages {
 namespace {
 
-constexpr int kWaves = 8;
-constexpr int kThr = 64 * kWaves;
-constexpr int kCols = 32 * kWaves;
-constexpr int kTile = 64;         // tokens of a tile
-constexpr int kKRow = kD + 8;     // 16-bit numbers of a staged key row: 16 rows' 16-byte reads fall in distinct banks
-constexpr int kVRow = kD + 32;    // and of a value row: the transposing read's 4 rows of 64 bytes do
-constexpr int kKBuf = kTile * kKRow, kVBuf = kTile * kVRow;
+constexpr int kKRow = kD + 8;   // 16-bit numbers of a staged key row: 16 rows' 16-byte reads fall in distinct banks
+constexpr int kVRow = kD + 32;  // and of a value row: the transposing read's 4 rows of 64 bytes do
+// A workgroup of W waves: 8 (one a CU), or 4 (two a CU).
+template <int W>
+struct Shape {
+  static constexpr int kPerCu = 8 / W;
+  static constexpr int kThr = 64 * W;
+  static constexpr int kCols = 32 * W;     // columns
+  static constexpr int kTile = 8 * W;      // tokens of a tile: a wave stages 8 rows
+  static constexpr int kSub = kTile / 32;  // products along its tokens
+  static constexpr int kProducts = 8 * kSub;             // of its scores, and of its values
+  static constexpr int kFirst = kProducts * 3 / 4;       // pairs of weights beside the score products, the others beside the values
+  static constexpr int kKBuf = kTile * kKRow, kVBuf = kTile * kVRow;
+  static constexpr int kLeast = 6 * kPerCu;  // fewest tiles of a part of the longest piece
+};
 constexpr int kXcds = 8;
-constexpr int kLeast = 4;         // fewest tiles of a part of the longest piece
 constexpr int kMostCuts = 32;
 constexpr int kPlan = 64;         // pieces of a workgroup that are found at once
 constexpr int kAgain = 128;       // words of marks (rounds past 4096 share them: gone through again without need)
@@ -85,7 +92,9 @@ __device__ __forceinline__ int by_heads(const Args& P, int x) {
 
 // Column tiles of sequence b with more than x tokens to read, of tiles with m rows in all and q of them queries of the last
 // of len tokens.
+template <int W>
 __device__ __forceinline__ int tiles_over(int x, int len, int m, int G) {
+  constexpr int kCols = Shape<W>::kCols;
   const int q = min(m, len), all = (m * G + kCols - 1) / kCols;
   const int y = x - (len - q);
   const int under = y <= 0 ? 0 : y >= q ? all : min(all, y * G / kCols);
@@ -109,22 +118,27 @@ __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readl
 
 // Parts of the column tiles with more than x tokens to read, where a tile of T tiles of tokens is ceil(T / chunk) parts (at
 // most cuts): one for every j with T > j chunk.  By the lanes of a wave, a (sequence, j) each.
+template <int W>
 __device__ __forceinline__ int parts_over(int x, const int* s_len, const int* s_rows, int B, int G, int cuts, int chunk) {
+  constexpr int kTile = Shape<W>::kTile;
   int n = 0;
   const float by = 1.f / cuts;
   for (int i = lane_prefix(~0ull); i < B * cuts; i += 64) {
     const int b = static_cast<int>((i + 0.5f) * by), j = i - b * cuts;  // (exact: i is below 2^18)
-    n += tiles_over(j ? max(x, j * chunk * kTile) : x, s_len[b], s_rows[b], G);
+    n += tiles_over<W>(j ? max(x, j * chunk * kTile) : x, s_len[b], s_rows[b], G);
   }
   return wave_total(n);
 }
 
 // Goes through the workgroup's pieces.  CARE: those that the first time marked in s_again, with care for values that are no
 // numbers.  Returns whether any is to be gone through again.
-template <int DT, bool PAGED, bool CARE>
+template <int DT, bool PAGED, int W, bool CARE>
 __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const int* s_len, const int* s_rows,
                                            const int* s_first, int4* s_plan, uint32_t* s_again, int wave, int longest,
                                            int pieces, int cuts, int chunk) {
+  using S = Shape<W>;
+  constexpr int kWaves = W, kCols = S::kCols, kTile = S::kTile, kSub = S::kSub, kProducts = S::kProducts, kFirst = S::kFirst;
+  constexpr int kKBuf = S::kKBuf, kVBuf = S::kVBuf;
   uint16_t* const sK = smem;
   uint16_t* const sV = smem + 2 * kKBuf;
   int lane = lane_prefix(~0ull);
@@ -172,7 +186,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
       int lo = -1, hi = (longest + kTile - 1) / kTile, over = 0;  // more than `piece` parts over 64 lo, none over 64 hi
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        const int n = parts_over(mid * kTile, s_len, s_rows, n_seqs, G, cuts, chunk);
+        const int n = parts_over<W>(mid * kTile, s_len, s_rows, n_seqs, G, cuts, chunk);
         if (n > piece) {
           lo = mid;
         } else {
@@ -187,8 +201,8 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
       const int split = piece - over - rank * ns;
       for (int base = 0; base < n_seqs; base += 64) {
         const int j = base + lane;
-        const int high = j < n_seqs ? tiles_over(x2, s_len[j], s_rows[j], G) : 0;
-        const int n = j < n_seqs ? tiles_over(x, s_len[j], s_rows[j], G) - high : 0;
+        const int high = j < n_seqs ? tiles_over<W>(x2, s_len[j], s_rows[j], G) : 0;
+        const int n = j < n_seqs ? tiles_over<W>(x, s_len[j], s_rows[j], G) - high : 0;
         const int sum = wave_prefix(n);
         const uint64_t past = wave_ballot(sum > rank);
         if (past) {
@@ -356,15 +370,15 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
 
     float m, l;
     f32x16 o[4];   // dims 32 db + 8 (i / 4) + 4 hf + i % 4
-    f32x16 sc[2];  // scores of tokens 32 kt + 8 (i / 4) + 4 hf + i % 4
-    float s[32];   // log2 weights of the present tile, relative to m
+    f32x16 sc[kSub];  // scores of tokens 32 kt + 8 (i / 4) + 4 hf + i % 4
+    float s[16 * kSub];  // log2 weights of the present tile, relative to m
     float ws[2];
-    u32x4 pf[4];   // its weights
+    u32x4 pf[2 * kSub];  // its weights
     constexpr int kAhead = 4;  // operands on their way from LDS
     u32x4 fr[kAhead];
-    // operand i of the 16 score products (tile t's keys) and of the 16 value products
+    // operand i of the score products (tile t's keys) and of the value products
     auto key_op = [&](int i, int t) {
-      return *reinterpret_cast<const u32x4*>(krow + (t & 1) * kKBuf + 32 * (i & 1) * kKRow + 16 * (i >> 1));
+      return *reinterpret_cast<const u32x4*>(krow + (t & 1) * kKBuf + 32 * (i % kSub) * kKRow + 16 * (i / kSub));
     };
     auto value_op = [&](int i, int t) {
       const uint16_t* p = vrow + (t & 1) * kVBuf + 16 * (i >> 2) * kVRow + 32 * (i & 3);
@@ -375,14 +389,15 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
     const float kc = P.scale_log2;
     auto score_products = [&](int t) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i & 1] = mfma32<DT>(key_op(i, t), qf[i >> 1], i < 2 ? f32x16{} : sc[i & 1]);
+      for (int i = 0; i < kProducts; ++i)
+        sc[i % kSub] = mfma32<DT>(key_op(i, t), qf[i / kSub], i < kSub ? f32x16{} : sc[i % kSub]);
     };
     // masks and a new offset, where a column of the wave needs one
     auto general = [&](int t) {
       const int left = lim - (blk0 + t) * kTile - 4 * hf;
       float mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
+      for (int e = 0; e < 16 * kSub; ++e) {
         const float x = sc[e >> 4][e & 15] * kc;
         s[e] = 8 * (e >> 2) + (e & 3) < left ? x : -INFINITY;
         mx = fmaxf(mx, s[e]);
@@ -396,7 +411,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
 #pragma unroll
       for (int db = 0; db < 4; ++db) o[db] = o[db] * alpha;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) s[e] -= mu;
+      for (int e = 0; e < 16 * kSub; ++e) s[e] -= mu;
     };
     // the same for the first tile, where there are no sums yet
     auto general0 = [&]() {
@@ -404,18 +419,18 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
       if ((blk0 + 1) * kTile > lim_min) {  // uniform
         const int left = lim - blk0 * kTile - 4 * hf;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] = 8 * (e >> 2) + (e & 3) < left ? sc[e >> 4][e & 15] * kc : -INFINITY;
+        for (int e = 0; e < 16 * kSub; ++e) sc[e >> 4][e & 15] = 8 * (e >> 2) + (e & 3) < left ? sc[e >> 4][e & 15] * kc : -INFINITY;
       } else {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) sc[kt] = sc[kt] * kc;
+        for (int kt = 0; kt < kSub; ++kt) sc[kt] = sc[kt] * kc;
       }
 #pragma unroll
-      for (int e = 0; e < 32; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
+      for (int e = 0; e < 16 * kSub; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
       mx = half_max(mx);
       m = mx == -INFINITY ? mx : mx - kTopWeight;
       const float mu = mx == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) s[e] = sc[e >> 4][e & 15] - mu;
+      for (int e = 0; e < 16 * kSub; ++e) s[e] = sc[e >> 4][e & 15] - mu;
     };
     // weights 2 i, 2 i + 1 of the present tile, into the value operand
     auto weights = [&](int i) {
@@ -448,7 +463,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
         general(t);
         ws[0] = ws[1] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) weights(i);
+        for (int i = 0; i < kProducts; ++i) weights(i);
         l += ws[0] + ws[1];
         __builtin_amdgcn_sched_barrier(0);
         constexpr uint32_t kInf = DT == LKV_DTYPE_F16 ? 0x7c00u : 0x7f80u;
@@ -459,7 +474,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
         for (int db = 0; db < 4; ++db) {
           f32x16 count = f32x16{};  // +inf counts 1, -inf 128, NaN both
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
+          for (int ks = 0; ks < 2 * kSub; ++ks) {
             const u32x4 raw = value_op(4 * ks + db, 0);
             u32x4 fine, kind, seen;
             int left = lim - (blk0 + t) * kTile - 4 * hf;
@@ -534,28 +549,33 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
           for (int i = 0; i < kAhead; ++i) fr[i] = key_op(i, t + 1);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            sc[i & 1] = mfma32<DT>(fr[i % kAhead], qf[i >> 1], i < 2 ? f32x16{} : sc[i & 1]);
-            fr[i % kAhead] = i + kAhead < 16 ? key_op(i + kAhead, t + 1) : value_op(i + kAhead - 16, t);
-            weights(i);
+          for (int i = 0; i < kProducts; ++i) {
+            sc[i % kSub] = mfma32<DT>(fr[i % kAhead], qf[i / kSub], i < kSub ? f32x16{} : sc[i % kSub]);
+            fr[i % kAhead] = i + kAhead < kProducts ? key_op(i + kAhead, t + 1) : value_op(i + kAhead - kProducts, t);
+            if ((i + 1) * kFirst / kProducts > i * kFirst / kProducts) weights(i * kFirst / kProducts);
             __builtin_amdgcn_sched_barrier(0);
           }
-          l += ws[0] + ws[1];
           float mx = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < kProducts; ++i) {
             o[i & 3] = mfma32<DT>(fr[i % kAhead], pf[i >> 2], o[i & 3]);
-            if (i + kAhead < 16) fr[i % kAhead] = value_op(i + kAhead, t);
-            if ((i & 3) == 0) {
-              if (i < 8)
-                stage_k(t + 2, i >> 2);
+            if (i + kAhead < kProducts) fr[i % kAhead] = value_op(i + kAhead, t);
+            if (i % (kProducts / 4) == 0) {
+              const int j = i / (kProducts / 4);
+              if (j < 2)
+                stage_k(t + 2, j);
               else
-                stage_v(t + 1, (i >> 2) - 2);
+                stage_v(t + 1, j - 2);
             }
+            // (the last weights: before the products that take them, and before their scores are written over)
+            constexpr int kLast = kProducts - kFirst, kBy = 2 * kLast;
+            if (i < kBy && (i + 1) * kLast / kBy > i * kLast / kBy) weights(kFirst + i * kLast / kBy);
             s[2 * i] = fmaf(sc[i >> 3][2 * i & 15], kc, -m);
             s[2 * i + 1] = fmaf(sc[i >> 3][(2 * i + 1) & 15], kc, -m);
             mx = fmaxf(fmaxf(mx, s[2 * i]), s[2 * i + 1]);
+            __builtin_amdgcn_sched_barrier(0);
           }
+          l += ws[0] + ws[1];
           load_next(t);
           if ((blk0 + t + 2) * kTile > lim_min || wave_ballot(mx > kMaxWeight) != 0) general(t + 1);  // uniform
           __syncthreads();
@@ -563,10 +583,10 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
         if (nt) {  // the last tile
           ws[0] = ws[1] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) weights(i);
+          for (int i = 0; i < kProducts; ++i) weights(i);
           l += ws[0] + ws[1];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i & 3] = mfma32<DT>(value_op(i, nt - 1), pf[i >> 2], o[i & 3]);
+          for (int i = 0; i < kProducts; ++i) o[i & 3] = mfma32<DT>(value_op(i, nt - 1), pf[i >> 2], o[i & 3]);
         }
       } else {  // no columns: the wave's part of the staging
 #pragma unroll 1
@@ -682,9 +702,11 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
   return again;
 }
 
-template <int DT, bool PAGED>
-__global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
-  __shared__ __align__(16) uint16_t smem[2 * kKBuf + 2 * kVBuf];
+template <int DT, bool PAGED, int W>
+__global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
+  using S = Shape<W>;
+  constexpr int kWaves = W, kPerCu = S::kPerCu, kThr = S::kThr, kCols = S::kCols, kTile = S::kTile, kLeast = S::kLeast;
+  __shared__ __align__(16) uint16_t smem[2 * S::kKBuf + 2 * S::kVBuf];
   __shared__ int s_len[kMaxSeqs], s_rows[kMaxSeqs], s_first[kMaxSeqs];
   __shared__ int4 s_plan[3 * kPlan];
   __shared__ uint32_t s_again[kAgain];  // pieces to go through again, by round
@@ -707,7 +729,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
   int pieces = 0;  // column tiles of all sequences
   for (int b = lane; b < P.B; b += 64) {
     longest = max(longest, s_len[b]);
-    pieces += tiles_over(-1, s_len[b], s_rows[b], G);
+    pieces += tiles_over<W>(-1, s_len[b], s_rows[b], G);
   }
 #pragma unroll
   for (int x = 32; x; x >>= 1) longest = max(longest, __shfl_xor(longest, x));
@@ -723,7 +745,7 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
     int cols = 0;
     for (int b = lane; b < P.B; b += 64) {
       const int len = s_len[b], rows = s_rows[b], q = min(rows, len);
-      work += tiles_over(-1, len, rows, G) * (len - 0.5f * q + 0.5f * min(kCols / G, q) + 0.5f * kTile) * (1.f / kTile);
+      work += tiles_over<W>(-1, len, rows, G) * (len - 0.5f * q + 0.5f * min(kCols / G, q) + 0.5f * kTile) * (1.f / kTile);
       cols += rows * G;
     }
 #pragma unroll
@@ -738,14 +760,14 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
       int n = pieces, cut = 0;  // parts in all, column tiles that are cut
       if (k > 1) {
         if (part < kLeast) break;
-        n = parts_over(-1, s_len, s_rows, P.B, G, k, part);
-        for (int b = lane; b < P.B; b += 64) cut += tiles_over(part * kTile, s_len[b], s_rows[b], G);
+        n = parts_over<W>(-1, s_len, s_rows, P.B, G, k, part);
+        for (int b = lane; b < P.B; b += 64) cut += tiles_over<W>(part * kTile, s_len[b], s_rows[b], G);
         cut = wave_total(cut);
       }
       const float items = static_cast<float>(n) * P.H;
       const float load = items <= grid ? part : fmaxf(mean + 0.3f * part, part);
-      const float join = k > 1 ? 1.f + static_cast<float>(min(cut * kCols, cols)) * (P.H * k) * (1040 / 7.6e6f) : 0.f;
-      const float takes = (load + 4.f * ceilf(items / grid) + join) * (k > 1 ? 1.05f : 1.f);
+      const float join = k > 1 ? 2.5f * kPerCu + static_cast<float>(min(cut * kCols, cols)) * (P.H * k) * (1040 * kPerCu / 7.6e6f) : 0.f;
+      const float takes = (load + 4.f * kPerCu * ceilf(items / grid) + join) * (k > 1 ? 1.05f : 1.f);
       if (takes < best) {
         best = takes;
         best_k = k;
@@ -769,11 +791,11 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
     if (cuts > 1) chunk = (most + cuts - 1) / cuts;
   }
 
-  const int again = go_through<DT, PAGED, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk);
+  const int again = go_through<DT, PAGED, W, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk);
   if (again && lane == 0) s_any = 1;
   __syncthreads();
   if (s_any) {
-    go_through<DT, PAGED, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk);
+    go_through<DT, PAGED, W, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk);
   }
 
   // ---- rows of no sequence
@@ -790,38 +812,58 @@ __global__ __launch_bounds__(kThr, 1) void prefill_kernel(Args P) {
 }
 
 struct Plan {
+  int waves;       // of a workgroup
   int64_t pieces;  // most column tiles of a kv head, over all sequences
   int splits;      // parts that a piece may be cut into (the kernel decides, by the lengths)
 };
 
-// enough: so many pieces are shared out evenly enough as they are.
-Plan make_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_len, int64_t enough) {
+// enough: so many pieces a CU are shared out evenly enough as they are.
+template <int W>
+Plan plan_for(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_len, float enough) {
+  using S = Shape<W>;
   const int64_t G = Hq / Hkv;
-  const int64_t each = B * ((max_new * G + kCols - 1) / kCols), packed = rows * G / kCols + B;
+  const int64_t each = B * ((max_new * G + S::kCols - 1) / S::kCols), packed = rows * G / S::kCols + B;
   Plan p;
+  p.waves = W;
   p.pieces = each < packed ? each : packed;
   p.pieces = p.pieces < 1 ? 1 : p.pieces;
-  const int64_t cus = device_cu_count(), tiles = (max_len + kTile - 1) / kTile, work = p.pieces * Hkv;
-  int64_t splits = work >= enough ? 1 : (2 * cus + work - 1) / work;
-  splits = splits > tiles / kLeast ? tiles / kLeast : splits;
+  const int64_t cus = device_cu_count() * S::kPerCu, tiles = (max_len + S::kTile - 1) / S::kTile, work = p.pieces * Hkv;
+  int64_t splits = work >= enough * cus ? 1 : (2 * cus + work - 1) / work;
+  splits = splits > tiles / S::kLeast ? tiles / S::kLeast : splits;
   p.splits = static_cast<int>(splits < 1 ? 1 : splits > kMostCuts ? kMostCuts : splits);
   return p;
 }
-
-// Whole prompts: a piece for three CUs in four.  (1 x 2048 tokens, 32/8 heads, a piece a CU: cutting the longer ones would cost
-// as much in rows to join as it gains.)
+// Whole prompts.  Up to 256 tokens two workgroups of 4 waves a CU, where beginning and ending pieces is most of the work and one
+// fills the other's waits (64 prompts to 150 tokens, 32/8 heads: 30.2 us with 8 waves, 24.5 with 4; 64 x 64 24.9 and 22.2; 16 x
+// 512 63 and 65; 1 x 8192 525 and 605: every row of keys and values is staged twice as often).  From three pieces for four CUs
+// on none is cut (1 x 2048 tokens, a piece a CU: cutting the longer ones costs as much in rows to join as it gains).
 Plan packed_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_len) {
   const int64_t most = max_len < rows ? max_len : rows;
-  return make_plan(rows, B, Hq, Hkv, most, most, device_cu_count() * 3ll / 4);
+  return most <= 256 ? plan_for<4>(rows, B, Hq, Hkv, most, most, 0.75f) : plan_for<8>(rows, B, Hq, Hkv, most, most, 0.75f);
 }
-// Over pages: three pieces a CU.  (Chunks to 512 over 1.6-8 K tokens of 4 sequences, 0.8 pieces a CU: 254 us as they are, 210
-// with the longest cut in two; the launch that joins costs 5 us where none is cut.)
+// Over pages, from three pieces a CU on none is cut.  (Chunks to 512 over 1.6-8 K tokens of 4 sequences, 0.8 pieces a CU: 268 us as
+// they are, 239 with the longest cut in two; the launch that joins costs 5 us where none is cut.)
 Plan pages_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_len) {
-  return make_plan(rows, B, Hq, Hkv, max_new < rows ? max_new : rows, max_len, 3ll * device_cu_count());
+  return plan_for<8>(rows, B, Hq, Hkv, max_new < rows ? max_new : rows, max_len, 3.f);
 }
 
 size_t plan_bytes(const Plan& p, int64_t rows, int64_t Hq) {
   return p.splits == 1 ? 0 : static_cast<size_t>(rows * Hq) * p.splits * (kD + 2) * 4;
+}
+
+template <bool PAGED, int W>
+int launch_shape(const Args& A, const Plan& p, int dtype, hipStream_t s, const char* what) {
+  using S = Shape<W>;
+  const int64_t work = p.pieces * p.splits * A.H, cus = device_cu_count() * S::kPerCu;
+  const int64_t most = (static_cast<int64_t>(A.rows) * A.G / S::kCols + A.B) * p.splits * A.H;  // whatever cu holds
+  LKV_REQUIRE(most < (1ll << 30), "%s: %lld pieces of work", what, (long long)most);
+  const dim3 grid(static_cast<unsigned>(work < cus ? work : cus));
+  if (dtype == LKV_DTYPE_F16)
+    hipLaunchKernelGGL((prefill_kernel<LKV_DTYPE_F16, PAGED, W>), grid, dim3(S::kThr), 0, s, A);
+  else
+    hipLaunchKernelGGL((prefill_kernel<LKV_DTYPE_BF16, PAGED, W>), grid, dim3(S::kThr), 0, s, A);
+  LKV_LAUNCH_CHECK(what);
+  return LKV_OK;
 }
 
 template <bool PAGED>
@@ -837,16 +879,12 @@ int launch(Args A, const Plan& p, int dtype, void* workspace, size_t workspace_b
   A.splits = p.splits;
   A.part_o = static_cast<float*>(workspace);
   A.part_ml = A.part_o + static_cast<size_t>(A.rows) * A.Hq * p.splits * kD;
-  const int64_t work = p.pieces * p.splits * A.H, cus = device_cu_count();
-  const int64_t most = (static_cast<int64_t>(A.rows) * A.G / kCols + A.B) * p.splits * A.H;  // whatever cu holds
-  LKV_REQUIRE(most < (1ll << 30), "%s: %lld pieces of work", what, (long long)most);
-  const dim3 grid(static_cast<unsigned>(work < cus ? work : cus));
-  if (dtype == LKV_DTYPE_F16)
-    hipLaunchKernelGGL((prefill_kernel<LKV_DTYPE_F16, PAGED>), grid, dim3(kThr), 0, s, A);
+  int rc;
+  if constexpr (PAGED)
+    rc = launch_shape<true, 8>(A, p, dtype, s, what);
   else
-    hipLaunchKernelGGL((prefill_kernel<LKV_DTYPE_BF16, PAGED>), grid, dim3(kThr), 0, s, A);
-  LKV_LAUNCH_CHECK(what);
-  if (p.splits == 1) return LKV_OK;
+    rc = p.waves == 4 ? launch_shape<false, 4>(A, p, dtype, s, what) : launch_shape<false, 8>(A, p, dtype, s, what);
+  if (rc || p.splits == 1) return rc;
   return launch_join(A.part_o, A.part_ml, static_cast<int64_t>(A.rows) * A.Hq, p.splits, A.Hq, A.out, A.o_st, A.o_sh,
                      dtype, A.cu, A.B, s, what);
 }

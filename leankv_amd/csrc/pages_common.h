@@ -12,7 +12,7 @@ namespace lkv {
 namespace pages {
 
 constexpr int kD = 128;
-constexpr int kMaxSeqs = 4096;  // rows of a page table, sequences of a packed batch (lengths are staged in LDS)
+constexpr int kMaxSeqs = 2048;  // rows of a page table, sequences of a packed batch (lengths are staged in LDS)
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -15,7 +15,7 @@ from .._lib import LeanKVError, check
 HEAD_DIM = 128
 DTYPES = {torch.float16: _lib.LKV_DTYPE_F16, torch.bfloat16: _lib.LKV_DTYPE_BF16}
 SCALE = 1.0 / math.sqrt(HEAD_DIM)
-MAX_SEQS = 4096
+MAX_SEQS = 2048
 _I64x2 = ctypes.c_int64 * 2
 
 
@@ -111,7 +111,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of sequences that lie one behind the other: q [tokens, heads, 128], k and v [tokens, kv_heads, 128]
     (heads a multiple of kv_heads; query head h reads kv head h * kv_heads // heads), float16 or bfloat16.  cu_seqlens: int32
-    [n + 1] on the device, ascending; rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 are sequence i, up to 4096 of them.  Returns
+    [n + 1] on the device, ascending; rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 are sequence i, up to 2048 of them.  Returns
     [tokens, heads, 128] in q's type; rows of no sequence are zeros, or, in a buffer given as `out` (dense 16-byte aligned
     rows apart from each other; q itself may be it), left as they are.  max_len: the caller's bound on the lengths (default:
     all tokens), which the work is split for.  scale: 1 / sqrt(128) by default.
