@@ -763,7 +763,7 @@ int lkv_kv8_sparse_attn(const lkv_kv8_store* store, const void* q, const int64_t
 /* ------------------------------------------------------------------------ */
 
 /*
- * Keys and values of up to `seqs` sequences in pages of page_size tokens (a
+ * Keys and values of up to `seqs` (at most 2048) sequences in pages of page_size tokens (a
  * power of two, 16 .. 256), `pages` of them in each of `layers` layers, heads of
  * 128 dims, dtype LKV_DTYPE_F16 or LKV_DTYPE_BF16.  Sequence s holds lens[s]
  * tokens; token t lies in page table[s][t / page_size], slot t % page_size, in

@@ -56,18 +56,24 @@ def load_model(model_name: str, dtype=torch.float16, device_map="cuda"):
 def optimize_model(model, teal_sparsity: Optional[float] = None, teal_thresholds_path: Optional[str] = None,
                    turboquant_bits: Optional[int] = None, use_paged_cache: bool = False, page_size: int = 16,
                    max_pages: int = 2048, use_kernels: bool = True, max_seq_len: int = 4096,
-                   fast_decode: bool = True, kv8: bool = False, kv8_sparse_blocks: Optional[int] = None):
+                   fast_decode: bool = True, kv8: bool = False, kv8_sparse_blocks: Optional[int] = None,
+                   paged_kv: bool = False):
     """Apply TEAL and/or a quantized KV cache; returns (model, cache or None).
 
     kv8 (not in the reference): an 8-bit cache with a scale for each block of 64 tokens and head (kv8.BlockInt8Cache)
     instead of a TurboQuant one; with kv8_sparse_blocks a single-token step reads only that many of every head's
     finished blocks, those with the highest score.  fast_decode does not apply to it: generate runs the patched HF forward.
 
+    paged_kv (not in the reference): a cache in 16-bit pages of page_size tokens (paged.PagedCache), which beam search forks
+    and assisted generation cuts; the patched HF forward here too.
+
     fast_decode (not in the reference): with both TEAL and TurboQuant on the HIP kernels, single-token
     decode calls of generate run the fused, graph-replayed decode step (engine.GenerateFastPath) when the
     call is one it serves; every other call runs the patched HF forward."""
     if kv8 and (turboquant_bits is not None or use_paged_cache):
         raise ValueError("kv8 is a cache of its own: not with turboquant_bits or use_paged_cache")
+    if paged_kv and (kv8 or turboquant_bits is not None or use_paged_cache):
+        raise ValueError("paged_kv is a cache of its own: not with kv8, turboquant_bits or use_paged_cache")
     if kv8_sparse_blocks is not None and not kv8:
         raise ValueError("kv8_sparse_blocks needs kv8=True")
     if teal_sparsity is not None or teal_thresholds_path is not None:
@@ -86,6 +92,12 @@ def optimize_model(model, teal_sparsity: Optional[float] = None, teal_thresholds
         cache = BlockInt8Cache(head_dim=head_dim, num_layers=cfg.num_hidden_layers, device=model.device,
                                max_seq_len=max_seq_len, fused_attention=use_kernels, sparse_blocks=kv8_sparse_blocks)
         print("[LeanKV] 8-bit KV cache enabled (head_dim=%d, sparse_blocks=%s)" % (head_dim, kv8_sparse_blocks))
+    elif paged_kv:
+        from .paged.cache import PagedCache
+
+        cache = PagedCache(head_dim=head_dim, num_layers=cfg.num_hidden_layers, device=model.device,
+                           max_seq_len=max_seq_len, page_size=page_size, fused_attention=use_kernels)
+        print("[LeanKV] paged 16-bit KV cache enabled (head_dim=%d, page_size=%d)" % (head_dim, page_size))
     elif turboquant_bits is not None:
         cache = TurboQuantCache(bits=turboquant_bits, head_dim=head_dim, num_layers=cfg.num_hidden_layers,
                                 device=model.device, dtype=torch.float16, max_seq_len=max_seq_len,

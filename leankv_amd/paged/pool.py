@@ -233,20 +233,48 @@ class PagedKV:
         call(self._index, self._lib.lkv_pages_compact, self._ref, in_use.data_ptr(), ws.data_ptr(), self._compact_bytes)
         return in_use
 
-    def resized(self, num_pages: int) -> "PagedKV":
-        """A pool of num_pages pages that holds what this one does.  A smaller one is for the pages that compact has moved to
-        the front; pages in use behind them raise (this looks at the device and waits for it)."""
+    def _like(self, num_pages: int, max_seqs: int, max_len: int) -> "PagedKV":
+        """A pool of other sizes whose first pages are this one's."""
+        new = PagedKV(self.num_layers, self.kv_heads, num_pages, max_seqs, max_len, self.page_size, self.dtype, self.device)
+        n = min(num_pages, self.num_pages)
+        new.pool[:, :n] = self.pool[:, :n]
+        new._followed = self._followed
+        return new
+
+    def resized(self, num_pages: int, max_len: int | None = None) -> "PagedKV":
+        """A pool of num_pages pages (and sequences of up to max_len tokens, at least as many as now) that holds what this one
+        does.  A smaller one is for the pages that compact has moved to the front; pages in use behind them raise (this looks
+        at the device and waits for it)."""
         n = min(int(num_pages), self.num_pages)
         if num_pages < 1 or (n < self.num_pages and bool((self.refs[n:] > 0).any())):
             raise LeanKVError("PagedKV.resized: pages from %d on are in use (compact moves them)" % num_pages)
-        new = PagedKV(self.num_layers, self.kv_heads, num_pages, self.max_seqs, self.max_len, self.page_size, self.dtype,
-                      self.device)
-        new.pool[:, :n] = self.pool[:, :n]
-        new.table.copy_(self.table)
+        new = self._like(int(num_pages), self.max_seqs, max(self.max_len, max_len or 0))
+        new.table[:, :self.width] = self.table
         new.lens.copy_(self.lens)
         new.taken.copy_(self.taken)
         new.refs[:n] = self.refs[:n]
-        new._followed = self._followed
+        return new
+
+    def chosen(self, index: torch.Tensor) -> "PagedKV":
+        """A pool of index.numel() sequences, the i-th of which holds what sequence index[i] of this one does (a batch made
+        larger or smaller).  Pages are shared as fork shares them; there are as many pages a sequence as here, and at least
+        as many in all."""
+        if index.dim() != 1 or not 1 <= index.shape[0] <= MAX_SEQS or index.dtype not in (torch.int32, torch.int64) \
+                or index.device != self.device:
+            raise LeanKVError("PagedKV.chosen: 1 to %d sequence numbers on %s expected" % (MAX_SEQS, self.device))
+        if bool(((index < 0) | (index >= self.max_seqs)).any()):  # (this waits for the device)
+            raise LeanKVError("PagedKV.chosen: sequence numbers outside 0 .. %d" % (self.max_seqs - 1))
+        n, each = index.shape[0], -(-self.num_pages // self.max_seqs)
+        new = self._like(max(self.num_pages, n * each), n, self.max_len)
+        new.table.copy_(self.table[index])
+        new.lens.copy_(self.lens[index])
+        named = new.table[new.table >= 0].long()
+        new.refs.index_add_(0, named, torch.ones_like(named, dtype=torch.int32))
+        return new
+
+    def __deepcopy__(self, memo):
+        """A pool of its own with the same contents."""
+        new = memo[id(self)] = self.resized(self.num_pages)
         return new
 
     def snapshot(self) -> torch.Tensor:

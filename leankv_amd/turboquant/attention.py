@@ -4,8 +4,8 @@ The reference returns dequantized fp16 K/V from TurboQuantCache.update and lets
 HF run SDPA on them (leankv/turboquant/cache.py:124-127;
 transformers/integrations/sdpa_attention.py:79-105).  With this function
 registered (transformers AttentionInterface) and selected as the model's
-attention implementation, attention over a TurboQuantCache or a
-kv8.BlockInt8Cache built with ``fused_attention=True`` reads the packed store:
+attention implementation, attention over a TurboQuantCache, a
+kv8.BlockInt8Cache or a paged.PagedCache built with ``fused_attention=True`` reads the store:
 a single-token decode step runs the split-K decode kernel, a several-token update (prefill or chunk) the
 causal prefill kernel.  Causality there is positional: query i of S sees keys
 up to position kv_len - S + i, HF's causal mask with the cache offset.

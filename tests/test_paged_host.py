@@ -160,3 +160,27 @@ def test_the_model_of_the_tables():
     assert t.compact() == 2 and t.rows == [[], [0, 1], []] and t.moves == {3: 1}
     t.extend([0, 100, 0])
     assert t.taken == [0, 0, 0] and t.lens == [0, 21, 0]
+
+
+def test_hf_cache_refuses():
+    from leankv_amd.paged import PagedCache
+
+    for kw in (dict(head_dim=64), dict(num_layers=0), dict(page_size=24)):
+        with pytest.raises(ValueError, match="PagedCache"):
+            PagedCache(**kw)
+    cache = PagedCache(num_layers=2, device="cuda")
+    assert cache.get_seq_length() == 0 and not len(cache) and cache.max_batch_size == 0 and not cache.is_initialized
+    assert cache.get_total_cache_bytes() == 0 and cache.get_compression_ratio() == 0.0
+    cache.crop(5)
+    cache.reorder_cache(torch.tensor([0]))
+    cache.batch_repeat_interleave(2)
+    with pytest.raises(IndexError):
+        cache[0]
+
+
+def test_optimize_model_takes_one_cache():
+    from leankv_amd.combined import optimize_model
+
+    for kw in (dict(kv8=True), dict(turboquant_bits=3), dict(use_paged_cache=True)):
+        with pytest.raises(ValueError, match="paged_kv"):
+            optimize_model(None, paged_kv=True, **kw)
