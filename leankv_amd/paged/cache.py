@@ -74,7 +74,7 @@ class PagedCache(HFCache):
             cap = kv.max_len
             while cap < tokens:
                 cap *= 2
-            self.kv = kv = kv.resized(B * (cap // self.page_size), cap)
+            self.kv = kv = kv.resized(max(kv.num_pages, B * (cap // self.page_size)), cap)
         return kv
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, cache_kwargs=None):

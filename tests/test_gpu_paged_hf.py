@@ -156,6 +156,12 @@ def test_chosen_batches_and_bf16(cuda):
         assert torch.equal(a, want) and torch.equal(b, torch.cat([k[2 * layer + 1].repeat_interleave(2, 0), -more], 2))
     cache.batch_select_indices(torch.tensor([3, 0, 3], device=cuda))
     assert torch.equal(cache[1][0], want[[3, 0, 3]]) and cache.max_batch_size == 3
+    grown = copy.deepcopy(cache)  # fewer sequences than before, past the length that there was room for
+    grown.batch_select_indices(torch.tensor([0], device=cuda))
+    tail = torch.randn(1, 2, 50, 128, generator=gen).bfloat16().cuda()
+    for layer in range(2):
+        a, _ = grown.update(tail, tail, layer)
+    assert torch.equal(a, torch.cat([want[3:], tail], 2)) and grown.kv.max_len >= 72
     cache.crop(-3)
     assert cache.get_seq_length(0) == 19 and torch.equal(cache[1][0], want[[3, 0, 3], :, :19])
     cache.crop(0)
