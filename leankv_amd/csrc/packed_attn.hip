@@ -466,10 +466,6 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
         for (int i = 0; i < kProducts; ++i) weights(i);
         l += ws[0] + ws[1];
         __builtin_amdgcn_sched_barrier(0);
-        constexpr uint32_t kInf = DT == LKV_DTYPE_F16 ? 0x7c00u : 0x7f80u;
-        constexpr uint32_t kOne = DT == LKV_DTYPE_F16 ? 0x3c00u : 0x3f80u;  // 1
-        constexpr uint32_t k128 = DT == LKV_DTYPE_F16 ? 0x5800u : 0x4300u;  // 128
-        constexpr uint32_t k129 = DT == LKV_DTYPE_F16 ? 0x5808u : 0x4301u;  // 129
 #pragma unroll
         for (int db = 0; db < 4; ++db) {
           f32x16 count = f32x16{};  // +inf counts 1, -inf 128, NaN both
@@ -479,20 +475,12 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
             u32x4 fine, kind, seen;
             int left = lim - (blk0 + t) * kTile - 4 * hf;
             __asm__ volatile("" : "+v"(left));  // (its comparisons are made where they are used)
+            no_numbers<DT>(raw, fine, kind);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              uint32_t f = 0, n = 0, z = 0;
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const uint32_t y = (raw[j] >> (16 * x)) & 0xffffu, a = y & 0x7fffu;
-                f |= (a >= kInf ? 0u : y) << (16 * x);
-                n |= (a < kInf ? 0u : a > kInf ? k129 : (y >> 15) ? k128 : kOne) << (16 * x);
-                const int e = 2 * j + x;  // token 16 ks + 4 hf + e % 4 + 8 (e / 4)
-                z |= (16 * ks + (e & 3) + 8 * (e >> 2) < left ? kOne : 0u) << (16 * x);
-              }
-              fine[j] = f;
-              kind[j] = n;
-              seen[j] = z;
+              // token 16 ks + 4 hf + e % 4 + 8 (e / 4), e = 2 j and 2 j + 1
+              const int at = 16 * ks + (2 * j & 3) + 8 * (j >> 1);
+              seen[j] = (at < left ? one_bits<DT>() : 0u) | (at + 1 < left ? one_bits<DT>() << 16 : 0u);
             }
             o[db] = mfma32<DT>(fine, pf[ks], o[db]);
             count = mfma32<DT>(kind, seen, count);
@@ -500,9 +488,9 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float minus = floorf(count[i] * (1.f / 128.f)), plus = count[i] - 128.f * minus;
-            if (plus > 0.f) o[db][i] += INFINITY;
-            if (minus > 0.f) o[db][i] -= INFINITY;
+            float sum = o[db][i];
+            add_counted(count[i], sum);
+            o[db][i] = sum;
           }
         }
       }
@@ -889,6 +877,11 @@ int launch(Args A, const Plan& p, int dtype, void* workspace, size_t workspace_b
                      dtype, A.cu, A.B, s, what);
 }
 
+// So few columns of a kv head that the few-row kernel, whose waves read their rows by themselves, takes them.
+bool few(int64_t rows, int64_t Hq, int64_t Hkv, int64_t max_new) {
+  return (max_new < rows ? max_new : rows) * (Hq / Hkv) <= 32;
+}
+
 int check_queries(int64_t rows, int64_t Hq, int64_t Hkv, const int32_t* cu, const char* what) {
   LKV_REQUIRE(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq < (1 << 20), "%s: %lld query heads over %lld kv heads", what,
               (long long)Hq, (long long)Hkv);
@@ -955,6 +948,7 @@ extern "C" int lkv_packed_attn(const void* q, const int64_t* q_strides, const vo
 extern "C" size_t lkv_pages_prefill_attn_workspace_bytes(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv,
                                                          int64_t max_new, int64_t max_len) {
   if (rows < 1 || seqs < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || max_new < 0 || max_len < 0) return 0;
+  if (few(rows, Hq, Hkv, max_new)) return few_rows_bytes(rows, seqs, Hq, Hkv, max_len);
   return plan_bytes(pages_plan(rows, seqs, Hq, Hkv, max_new, max_len), rows, Hq);
 }
 
@@ -972,6 +966,9 @@ extern "C" int lkv_pages_prefill_attn(const lkv_pages* p, int64_t layer, const v
   if (rows == 0) return LKV_OK;
   if (int rc = check_rows(q, q_strides, what, "q")) return rc;
   if (int rc = check_rows(out, out_strides, what, "out")) return rc;
+  if (few(rows, Hq, p->kv_heads, max_new))
+    return launch_few_rows(p, layer, q, q_strides, rows, Hq, cu, max_len, scale, out, out_strides, fill, workspace,
+                           workspace_bytes, static_cast<hipStream_t>(stream), what);
   Args A{};
   A.q = static_cast<const uint16_t*>(q);
   A.q_st = static_cast<uint32_t>(q_strides[0]);

@@ -80,6 +80,35 @@ __device__ __forceinline__ float add_pair(uint32_t u, float acc) {
 }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Values that are no numbers, where a product multiplies one that a column does not see by 0: `fine` has 0 in their place and
+// `kind` 1 for +inf, 128 for -inf, 129 (both) for NaN, 0 for numbers.  A product of kinds with ones for what a column sees
+// counts both, up to 127 of each, and add_counted() adds them to its sum.
+template <int DT>
+__host__ __device__ __forceinline__ constexpr uint32_t inf_bits() { return DT == LKV_DTYPE_F16 ? 0x7c00u : 0x7f80u; }
+template <int DT>
+__host__ __device__ __forceinline__ constexpr uint32_t one_bits() { return DT == LKV_DTYPE_F16 ? 0x3c00u : 0x3f80u; }
+template <int DT>
+__device__ __forceinline__ void no_numbers(const u32x4& raw, u32x4& fine, u32x4& kind) {
+  constexpr uint32_t k128 = DT == LKV_DTYPE_F16 ? 0x5800u : 0x4300u, k129 = DT == LKV_DTYPE_F16 ? 0x5808u : 0x4301u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t f = 0, n = 0;
+#pragma unroll
+    for (int x = 0; x < 32; x += 16) {
+      const uint32_t y = raw[j] >> x & 0xffffu, a = y & 0x7fffu;
+      f |= (a >= inf_bits<DT>() ? 0u : y) << x;
+      n |= (a < inf_bits<DT>() ? 0u : a > inf_bits<DT>() ? k129 : y >> 15 ? k128 : one_bits<DT>()) << x;
+    }
+    fine[j] = f;
+    kind[j] = n;
+  }
+}
+__device__ __forceinline__ void add_counted(float count, float& sum) {
+  const float minus = floorf(count * (1.f / 128.f)), plus = count - 128.f * minus;
+  if (plus > 0.f) sum += INFINITY;
+  if (minus > 0.f) sum -= INFINITY;
+}
+
 // log2 of the softmax weights as 16 bits hold them: a new offset puts the largest at 2^6, and there is none until a weight
 // passes 2^15, so that most tiles need no rescaled sums.  A weight keeps fp16's 11 bits down to 2^-20 of the largest.
 constexpr float kTopWeight = 6.f, kMaxWeight = 15.f;
@@ -93,6 +122,12 @@ __device__ __forceinline__ float2 part_record(float m, float l) { return float2{
 // cu[n] on are skipped.  So is a row whose first sum is negative.
 int launch_join(const float* part_o, const float* part_ml, int64_t rows, int64_t splits, int64_t heads, void* out,
                 int64_t o_st, int64_t o_sh, int dtype, const int* cu, int n, hipStream_t stream, const char* what);
+
+// lkv_pages_prefill_attn of a few rows a sequence (pages_decode.hip): up to 32 columns of a kv head, and right for more.
+size_t few_rows_bytes(int64_t rows, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len);
+int launch_few_rows(const lkv_pages* p, int64_t layer, const void* q, const int64_t* q_strides, int64_t rows, int64_t Hq,
+                    const int32_t* cu, int64_t max_len, float scale, void* out, const int64_t* out_strides, int fill,
+                    void* workspace, size_t workspace_bytes, hipStream_t s, const char* what);
 
 // Checks of what the C entries take (pages_table.hip).
 int check_pages(const lkv_pages* p, const char* what);

@@ -1,4 +1,5 @@
-// Attention of one query per sequence over the 16-bit paged KV cache (lkv_pages_decode_attn), and the join of partial sums.
+// Attention of one query per sequence over the 16-bit paged KV cache (lkv_pages_decode_attn), of a few (lkv_pages_prefill_attn with
+// up to 32 columns = queries x heads of a kv head), and the join of partial sums.
 //
 //   split kernel  grid (splits, kv heads x column tiles, sequences), 4 waves.  A wave takes every 4th chunk of 32 tokens of
 //                 its split, each row read once and straight into registers, and runs on v_mfma_f32_16x16x32
@@ -13,6 +14,10 @@
 // part among themselves, each for the columns of all; what follows each reads for its own.  A split has a record for its own
 // part and one for every sequence of the group.  Pages are compared where they are staged, so sharing needs no plan and no
 // call of its own.
+//
+// A few newest queries of a sequence (drafted tokens, checked in one pass) are the columns of its workgroups in the same way;
+// those that do not see the last tokens have weight 0 there.  Where such a token's value is no number, 0 times it is none
+// either: it counts as 0 then, and a second product counts, of each kind, those that a column sees.
 #include "pages_common.h"
 
 namespace lkv {
@@ -52,6 +57,8 @@ struct DecodeArgs {
   int group;    // sequences of a group: 32 / G, or 1 where none are shared
   int max_len, chunk, splits;  // tokens of a split
   int slots;    // records of a row: splits, or splits (group + 1): a split's own part, and the shared ones
+  const int* cu;  // rows of several queries a sequence: where they begin
+  int rows, fill;
   float scale_log2;
   float* part_o;   // [seqs * Hq][slots][128]
   float* part_ml;  // [seqs * Hq][slots][2]
@@ -65,23 +72,26 @@ struct Staged {
   int end[32], same[32], member[32];
 };
 
-// Attention over tokens [lo, hi) of the workgroup's split for `cols` columns, 16 NT at most; where(c, seq, head) says what
-// column c is and slot where its record goes (no slots: the result itself).
-template <int DT, int NT, class Where>
-__device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, int page0, int lo, int hi, int cols, int slot,
-                                       Where where) {
+// Attention over tokens [lo, hi) of the workgroup's split for `cols` columns, 16 NT at most; where(c, row, head) says which query
+// column c is and slot where its record goes (no slots: the result itself).  Column c sees tokens below sees(c) (MASKED), all
+// of them those below `free`.  pages(i): the i-th page id of the sequence's row from page0 on.
+template <int DT, int NT, bool MASKED, class Where, class Sees, class PageOf>
+__device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, int page0, int lo, int hi, int free, int cols,
+                                       int slot, Where where, Sees sees, PageOf pages) {
   const Pages& st = P.st;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   u32x4 qf[NT][4];  // dims 32 kb + 8 g ..
+  int lim[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {  // (a column past the last is the last once more)
-    int seq, head;
-    where(min(16 * n + c16, cols - 1), seq, head);
-    const uint16_t* p = P.q + seq * P.q_ss + head * P.q_sh + 8 * g;
+    int row, head;
+    where(min(16 * n + c16, cols - 1), row, head);
+    const uint16_t* p = P.q + row * P.q_ss + head * P.q_sh + 8 * g;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) qf[n][kb] = *reinterpret_cast<const u32x4*>(p + 32 * kb);
+    lim[n] = MASKED ? min(sees(min(16 * n + c16, cols - 1)), hi) : hi;
   }
   // ---- chunks c = lo + 32 (wave + 4 i): keys of tokens c + 16 tt + lane % 16, values j of tokens
   // c + 16 (j / 4) + 4 (lane / 16) + j % 4; tokens past the end read the last one, masked below
@@ -89,7 +99,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, i
   const int mask = page_size(st) - 1;
   auto at = [&](int t) {  // a token's row of keys in the layer
     t = min(t, hi - 1);
-    return sh.page[(t >> st.lg) - page0] * (2 * st.H * run) + h * run + (t & mask) * kD;
+    return pages((t >> st.lg) - page0) * (2 * st.H * run) + h * run + (t & mask) * kD;
   };
   u32x4 kr[2][4], vr[8];
   auto load_chunk = [&](int c) {
@@ -116,11 +126,20 @@ __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, i
   if (c < hi) load_chunk(c);
 #pragma unroll 1
   for (; c < hi; c += kStep) {
-    const bool last = c + kChunk > hi;  // uniform: rows past the end are no numbers of this sequence
+    const bool last = c + kChunk > free;  // uniform: rows past the end are no numbers of this sequence
+    bool odd = false;                     // uniform: a value that not all columns see is no number
     if (last) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (c + 16 * (e >> 2) + 4 * g + (e & 3) >= hi) vr[e] = u32x4{};
+      if constexpr (MASKED) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) any |= (vr[e][k] & 0x7fffu) >= inf_bits<DT>() || (vr[e][k] >> 16 & 0x7fffu) >= inf_bits<DT>();
+        odd = wave_ballot(any) != 0;
+      }
     }
     u32x4 pb[NT];
 #pragma unroll
@@ -137,7 +156,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, i
       for (int e = 0; e < 8; ++e) x[e] = sc[e >> 2][e & 3] * P.scale_log2;
       if (last) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = c + 16 * (e >> 2) + 4 * g + (e & 3) >= hi ? -INFINITY : x[e];
+        for (int e = 0; e < 8; ++e) x[e] = c + 16 * (e >> 2) + 4 * g + (e & 3) >= lim[n] ? -INFINITY : x[e];
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
@@ -164,6 +183,31 @@ __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, i
 #pragma unroll
       for (int pp = 0; pp < 4; ++pp)
         a[pp] = __builtin_amdgcn_perm(vr[2 * pp + 1][t >> 1], vr[2 * pp][t >> 1], (t & 1) ? 0x07060302u : 0x05040100u);
+      if constexpr (MASKED) {
+        if (odd) {
+          u32x4 fine, kind;
+          no_numbers<DT>(a, fine, kind);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            u32x4 seen;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int t0 = c + 16 * (k >> 1) + 4 * g + 2 * (k & 1);  // its two tokens
+              seen[k] = (t0 < lim[n] ? one_bits<DT>() : 0u) | (t0 + 1 < lim[n] ? one_bits<DT>() << 16 : 0u);
+            }
+            o[n][t] = mfma16<DT>(fine, pb[n], o[n][t]);
+            const f32x4 count = mfma16<DT>(kind, seen, f32x4{});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float sum = o[n][t][i];
+              add_counted(count[i], sum);
+              o[n][t][i] = sum;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          continue;
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) o[n][t] = mfma16<DT>(a, pb[n], o[n][t]);
     }
@@ -186,10 +230,12 @@ __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, i
       *reinterpret_cast<f32x4*>(dst + 4) = f32x4{o[n][4][i], o[n][5][i], o[n][6][i], o[n][7][i]};
     }
     __syncthreads();
-    const int col = tid >> 4, d = 8 * (tid & 15);
+    int thread = tid;
+    __asm__ volatile("" : "+v"(thread));  // (what follows from it is not kept through the chunks)
+    const int col = thread >> 4, d = 8 * (thread & 15);
     if (16 * n + col >= cols) continue;
-    int seq, head;
-    where(16 * n + col, seq, head);
+    int row, head;
+    where(16 * n + col, row, head);
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sh.m[w][col]);
@@ -207,13 +253,13 @@ __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, i
     }
     if (P.slots == 1) {
       const float inv = L != 0.f ? 1.f / L : 0.f;
-      *reinterpret_cast<u32x4*>(P.out + seq * P.o_ss + head * P.o_sh + d) =
+      *reinterpret_cast<u32x4*>(P.out + row * P.o_ss + head * P.o_sh + d) =
           u32x4{pack<DT>(r[0] * inv, r[1] * inv), pack<DT>(r[2] * inv, r[3] * inv), pack<DT>(r[4] * inv, r[5] * inv),
                 pack<DT>(r[6] * inv, r[7] * inv)};
       continue;
     }
-    const int64_t rec = (static_cast<int64_t>(seq) * P.Hq + head) * P.slots + slot;
-    if ((tid & 15) == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * rec) = part_record(M, L);
+    const int64_t rec = (static_cast<int64_t>(row) * P.Hq + head) * P.slots + slot;
+    if (d == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * rec) = part_record(M, L);
     *reinterpret_cast<f32x4*>(P.part_o + rec * kD + d) = f32x4{r[0], r[1], r[2], r[3]};
     *reinterpret_cast<f32x4*>(P.part_o + rec * kD + d + 4) = f32x4{r[4], r[5], r[6], r[7]};
   }
@@ -276,6 +322,8 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(DecodeArgs P) {
     }
   }
   __syncthreads();
+  auto page_at = [&](int i) { return sh.page[i]; };
+  auto all = [](int) { return 0; };
   int shared = t0, rank = 0, count = 0;  // shared tokens [t0, shared) of `count` sequences, this one the rank-th of them
   if (P.group > 1) {
     const int same = lane < members ? sh.same[lane] : 0;
@@ -303,17 +351,70 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(DecodeArgs P) {
     const int part = ((shared - t0 + count - 1) / count + kChunk - 1) & ~(kChunk - 1);
     const int lo = min(t0 + rank * part, shared), hi = min(lo + part, shared);
     if (cols <= 16)
-      attend<DT, 1>(P, sh, h, page0, lo, hi, cols, slot + 1 + rank, where);
+      attend<DT, 1, false>(P, sh, h, page0, lo, hi, hi, cols, slot + 1 + rank, where, all, page_at);
     else
-      attend<DT, 2>(P, sh, h, page0, lo, hi, cols, slot + 1 + rank, where);
+      attend<DT, 2, false>(P, sh, h, page0, lo, hi, hi, cols, slot + 1 + rank, where, all, page_at);
   }
   if (shared < t1)
-    attend<DT, 1>(P, sh, h, page0, shared, t1, own_heads, slot, [&](int c, int& seq, int& head) {
+    attend<DT, 1, false>(P, sh, h, page0, shared, t1, t1, own_heads, slot, [&](int c, int& seq, int& head) {
       seq = s;
       head = own_head + c;
-    });
+    }, all, page_at);
   else
     empty(slot, 1);
+}
+
+// The newest queries of every sequence, rows cu[s] .. of q: grid (splits, kv heads, sequences).
+template <int DT>
+__global__ __launch_bounds__(kThr, 2) void rows_kernel(DecodeArgs P) {
+  __shared__ __align__(16) Staged sh;
+  const Pages& st = P.st;
+  const int tid = threadIdx.x;
+  const int split = blockIdx.x, h = blockIdx.y, s = blockIdx.z, G = P.G;
+  const int row0 = min(max(P.cu[s], 0), P.rows), m = min(max(P.cu[s + 1], row0), P.rows) - row0;
+  const int len = held(st, st.lens[s]), qlen = min(m, len);
+  if (P.fill) {  // rows of no sequence
+    const int a = min(max(P.cu[0], 0), P.rows), e = min(max(P.cu[st.seqs], a), P.rows);
+    const int64_t per = static_cast<int64_t>(P.Hq) * (kD / 8), n = (a + P.rows - e) * per;
+    const int64_t block = blockIdx.x + static_cast<int64_t>(gridDim.x) * (blockIdx.y + gridDim.y * blockIdx.z);
+    for (int64_t i = block * kThr + tid; i < n; i += static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z * kThr) {
+      const int64_t r = i / per, x = i - r * per, row = r < a ? r : r - a + e;
+      *reinterpret_cast<u32x4*>(P.out + row * P.o_ss + x / (kD / 8) * P.o_sh + 8 * (x % (kD / 8))) = u32x4{};
+    }
+  }
+  const int t0 = split * P.chunk, t1 = split == P.splits - 1 ? len : min(t0 + P.chunk, len);
+  // queries that there are no tokens for, or none in this split
+  const int from = t0 < t1 ? qlen : 0;
+  for (int e = tid; e < (m - from) * G * (kD / 8); e += kThr) {
+    const int x = e / (kD / 8), i = from + x / G;
+    const int64_t row = row0 + i, head = h * G + x % G;
+    if (P.slots == 1)
+      *reinterpret_cast<u32x4*>(P.out + row * P.o_ss + head * P.o_sh + 8 * (e % (kD / 8))) = u32x4{};
+    else if (e % (kD / 8) == 0)
+      *reinterpret_cast<float2*>(P.part_ml + 2 * ((row * P.Hq + head) * P.slots + split)) = part_record(-INFINITY, 0.f);
+  }
+  if (t0 >= t1 || !qlen) return;  // uniform
+
+  const int page0 = t0 >> st.lg, pages = ((t1 - 1) >> st.lg) - page0 + 1;
+  const int* table = st.table + static_cast<int64_t>(s) * st.width + page0;
+  for (int i = tid; i < min(pages, kMaxPages); i += kThr) sh.page[i] = page_id(st, table[i]);
+  __syncthreads();
+  auto page_at = [&](int i) { return i < kMaxPages ? sh.page[i] : page_id(st, table[i]); };
+#pragma unroll 1
+  for (int col0 = 0; col0 < qlen * G; col0 += 32) {
+    const int cols = min(qlen * G - col0, 32);
+    auto where = [&](int c, int& row, int& head) {
+      const int i = (col0 + c) / G;
+      row = row0 + i;
+      head = h * G + col0 + c - i * G;
+    };
+    auto sees = [&](int c) { return len - qlen + (col0 + c) / G + 1; };
+    const int free = min(sees(0), t1);
+    if (cols <= 16)
+      attend<DT, 1, true>(P, sh, h, page0, t0, t1, free, cols, split, where, sees, page_at);
+    else
+      attend<DT, 2, true>(P, sh, h, page0, t0, t1, free, cols, split, where, sees, page_at);
+  }
 }
 
 struct JoinArgs {
@@ -377,8 +478,8 @@ struct DecodePlan {
   int chunk, splits, group, slots;
 };
 
-DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len) {
-  const int64_t G = Hq / Hkv, tiles = (G + 15) / 16, pairs = S * Hkv * tiles;
+DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len, bool rows = false) {
+  const int64_t G = Hq / Hkv, tiles = rows ? 1 : (G + 15) / 16, pairs = S * Hkv * tiles;
   const int64_t steps = (max_len + kStep - 1) / kStep;
   // Two workgroups a CU, the most that its registers hold at a time (32 x 8192 tokens, 32/8 heads: 186 us, with four 191, 131072
   // tokens 100 and 108 us).  One split, which needs no join and shares nothing, where a workgroup a CU walks at most 8 steps
@@ -397,7 +498,7 @@ DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len) {
   DecodePlan p;
   p.splits = static_cast<int>(steps <= chunk ? 1 : (steps + chunk - 1) / chunk);
   p.chunk = static_cast<int>(chunk * kStep);
-  p.group = p.splits > 1 && S > 1 && G <= 16 ? static_cast<int>(32 / G) : 1;
+  p.group = !rows && p.splits > 1 && S > 1 && G <= 16 ? static_cast<int>(32 / G) : 1;
   p.slots = p.group > 1 ? p.splits * (p.group + 1) : p.splits;
   return p;
 }
@@ -423,6 +524,49 @@ int launch_join(const float* part_o, const float* part_ml, int64_t rows, int64_t
   }
   LKV_LAUNCH_CHECK(what);
   return LKV_OK;
+}
+
+size_t few_rows_bytes(int64_t rows, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len) {
+  const DecodePlan p = decode_plan(S, Hq, Hkv, max_len, true);
+  return p.slots == 1 ? 0 : static_cast<size_t>(rows * Hq) * p.slots * (kD + 2) * 4;
+}
+
+int launch_few_rows(const lkv_pages* p, int64_t layer, const void* q, const int64_t* q_strides, int64_t rows, int64_t Hq,
+                    const int32_t* cu, int64_t max_len, float scale, void* out, const int64_t* out_strides, int fill,
+                    void* workspace, size_t workspace_bytes, hipStream_t s, const char* what) {
+  const size_t need = few_rows_bytes(rows, p->seqs, Hq, p->kv_heads, max_len);
+  LKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
+              "%s: a 16-byte aligned workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
+  const DecodePlan plan = decode_plan(p->seqs, Hq, p->kv_heads, max_len, true);
+  DecodeArgs A{};
+  A.st = device_pages(p);
+  A.kv = A.st.pool + layer * p->pages * 2 * p->kv_heads * p->page_size * kD;
+  A.q = static_cast<const uint16_t*>(q);
+  A.q_ss = q_strides[0];
+  A.q_sh = q_strides[1];
+  A.out = static_cast<uint16_t*>(out);
+  A.o_ss = out_strides[0];
+  A.o_sh = out_strides[1];
+  A.Hq = static_cast<int>(Hq);
+  A.G = static_cast<int>(Hq / p->kv_heads);
+  A.max_len = static_cast<int>(max_len);
+  A.chunk = plan.chunk;
+  A.splits = A.slots = plan.splits;
+  A.cu = cu;
+  A.rows = static_cast<int>(rows);
+  A.fill = fill;
+  A.scale_log2 = scale * kLog2e;
+  A.part_o = static_cast<float*>(workspace);
+  A.part_ml = A.part_o + static_cast<size_t>(rows * Hq) * plan.slots * kD;
+  const dim3 grid(static_cast<unsigned>(plan.splits), static_cast<unsigned>(p->kv_heads), static_cast<unsigned>(p->seqs));
+  if (p->dtype == LKV_DTYPE_F16)
+    hipLaunchKernelGGL(rows_kernel<LKV_DTYPE_F16>, grid, dim3(kThr), 0, s, A);
+  else
+    hipLaunchKernelGGL(rows_kernel<LKV_DTYPE_BF16>, grid, dim3(kThr), 0, s, A);
+  LKV_LAUNCH_CHECK(what);
+  if (plan.slots == 1) return LKV_OK;
+  return launch_join(A.part_o, A.part_ml, rows * Hq, plan.slots, Hq, out, A.o_ss, A.o_sh, p->dtype, cu,
+                     static_cast<int>(p->seqs), s, what);
 }
 
 }  // namespace pages

@@ -178,6 +178,50 @@ def test_packed_large_scores(cuda):
         check(packed_attention(q.cuda(), k.cuda(), v.cuda(), _ints([0, n])), want, bound)
 
 
+@pytest.mark.parametrize("max_len", [100, 300])
+def test_packed_many_sequences(cuda, max_len):
+    """More pieces a workgroup than are found at once: 2000 sequences alike give 2000 results alike."""
+    from leankv_amd.paged import packed_attention
+
+    gen = torch.Generator().manual_seed(31)
+    n, B, heads = 100, 2000, 32
+    q, k, v = _rows(gen, n, heads, F16), _rows(gen, n, 1, F16), _rows(gen, n, 1, F16)
+    want, bound = packed(q, k, v, [0, n])
+    at = torch.arange(0, n * B + 1, n, dtype=torch.int32, device="cuda")
+    got = packed_attention(*(t.cuda().repeat(B, 1, 1) for t in (q, k, v)), at, max_len=max_len).view(B, n, heads, D)
+    check(got[0], want, bound)
+    assert bool((got == got[0]).all())
+
+
+def test_packed_most_sequences(cuda):
+    """Sequences of none to three tokens, as many as there may be; their stored rows in pages."""
+    from leankv_amd.paged import PagedKV, packed_attention
+
+    rng = random.Random(5)
+    lens = [rng.randint(0, 3) for _ in range(2048)]
+    gen = torch.Generator().manual_seed(32)
+    at = _starts(lens)
+    q, k, v = (_rows(gen, at[-1], h, BF16) for h in (2, 1, 1))
+    want, bound = packed(q, k, v, at)
+    check(packed_attention(q.cuda(), k.cuda(), v.cuda(), _ints(at), max_len=3), want, bound)
+    cache = PagedKV(1, 1, 2100, 2048, 16, page_size=16, dtype=BF16)
+    cache.extend(_ints(at))
+    cache.store(0, k.cuda(), v.cuda(), _ints(at))
+    kk, vv = cache.read(0, 3)
+    for s in range(0, 2048, 7):
+        assert torch.equal(kk[s, 0, :lens[s]].cpu(), k[at[s]:at[s + 1], 0]) and not kk[s, 0, lens[s]:].any()
+        assert torch.equal(vv[s, 0, :lens[s]].cpu(), v[at[s]:at[s + 1], 0])
+    check(cache.prefill_attention(0, q.cuda(), _ints(at), max_new=3), want, bound)
+    q1 = _rows(gen, 2048, 2, BF16)
+    some = [s for s in range(2048) if lens[s]][:300]
+    got = cache.decode_attention(0, q1.cuda()).cpu()
+    for s in some:
+        for h in range(2):
+            w, b = attention(q1[s, h:h + 1], k[at[s]:at[s + 1], 0], v[at[s]:at[s + 1], 0], torch.tensor([lens[s]]))
+            check(got[s, h:h + 1], w, b)
+    assert not got[[s for s in range(2048) if not lens[s]]].any()
+
+
 # -------------------------------------------------------------------------------------------------- over pages
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("heads,kv,dtype", [(8, 2, F16), (7, 1, BF16)])
@@ -206,6 +250,48 @@ def test_prefill_few_rows_of_long_sequences(cuda, heads, kv, new, dtype):
     q = _rows(gen, at[-1], heads, dtype)
     want, bound = packed(q, None, None, at, paged=lambda b: held[0][b])
     check(cache.prefill_attention(0, q.cuda(), _ints(at), max_new=max(new)), want, bound)
+
+
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("heads,kv,new,dtype", [(8, 2, 5, F16), (8, 2, 8, BF16), (4, 4, 32, F16), (14, 2, 3, BF16), (32, 2, 2, F16),
+                                                (12, 1, 2, BF16), (20, 1, 1, F16)])
+def test_prefill_few_rows(cuda, page, heads, kv, new, dtype):
+    """Up to 32 columns of a kv head; more rows than max_new says, and longer sequences than max_len, are right too."""
+    gen = torch.Generator().manual_seed(page + heads + new)
+    lens = [1, 2, 0, 31, 33, 64, 130, 300, 700]
+    news = [1, 3, 2, new, new, 0, 1, new, new]
+    cache, _, held = _cache(gen, lens, kv, page, dtype, layers=2)
+    at = _starts(news, first=2)
+    q = _rows(gen, at[-1] + 1, heads, dtype)
+    want, bound = packed(q, None, None, at, paged=lambda b: held[1][b])
+    for kw in (dict(max_new=new), dict(max_new=1, max_len=40), dict(max_new=new, max_len=700), {}):
+        got = cache.prefill_attention(1, q.cuda(), _ints(at), **kw)
+        check(got, want, bound, str(kw))
+        assert not got[:2].any() and not got[at[-1]:].any()
+    out = torch.full_like(got, 5.0)
+    cache.prefill_attention(1, q.cuda(), _ints(at), max_new=new, out=out)
+    assert torch.equal(out[2:at[-1]], cache.prefill_attention(1, q.cuda(), _ints(at), max_new=new)[2:at[-1]])
+    assert (out[:2] == 5).all() and (out[at[-1]:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("max_new", [6, 40])
+def test_prefill_values_that_are_no_numbers(cuda, dtype, max_new):
+    """A drafted token's value has no part in the rows of the tokens before it, whatever it is."""
+    gen = torch.Generator().manual_seed(41)
+    n, m, page = 100, 6, 16
+    cache, rows, held = _cache(gen, [n], 1, page, dtype)
+    q = _rows(gen, m, 4, dtype)
+    want, bound = packed(q, None, None, [0, m], paged=lambda b: held[0][b])
+    mask = torch.zeros(want.shape, dtype=torch.bool)
+    for i, d, x in ((2, 7, math.inf), (4, 7, -math.inf), (3, 9, -math.inf), (5, 3, math.nan), (1, 100, math.nan)):
+        t = n - m + i
+        cache.pool[0, rows[0][t // page], 1, 0, t % page, d] = x
+        mask[i:, :, d] = True
+    got = cache.prefill_attention(0, q.cuda(), _ints([0, m]), max_new=max_new).cpu().double()
+    check(torch.where(mask, want, got), want, bound)
+    assert (got[2:4, :, 7] == math.inf).all() and got[4:, :, 7].isnan().all() and (got[3:, :, 9] == -math.inf).all()
+    assert got[5, :, 3].isnan().all() and got[1:, :, 100].isnan().all()
 
 
 @pytest.mark.parametrize("page", [16, 64, 256])
