@@ -116,18 +116,49 @@ __device__ __forceinline__ int wave_prefix(int v) {  // inclusive
 }
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
 
-// Parts of the column tiles with more than x tokens to read, where a tile of T tiles of tokens is ceil(T / chunk) parts (at
-// most cuts): one for every j with T > j chunk.  By the lanes of a wave, a (sequence, j) each.
+// A column tile of T tiles of tokens is j + 1 = ceil(T / chunk) parts (at most `cuts`) of ceil(T / (j + 1)) tiles at most, which
+// are more than x < chunk where T > x (j + 1).  Parts of more than x tiles, of all column tiles (x = -1: all parts), are then
+// the sum over j of (j + 1) times the tiles with max(j chunk, x (j + 1)) < T <= (j + 1) chunk: with N(y) the tiles with T > y,
+//   sum over j of (j + 1) N(max(j chunk, x (j + 1))) - sum over j of j N(j chunk),
+// the second the same for all x (`less`).  By the lanes of a wave, a (sequence, j) each.
 template <int W>
-__device__ __forceinline__ int parts_over(int x, const int* s_len, const int* s_rows, int B, int G, int cuts, int chunk) {
+__device__ __forceinline__ int parts_over(int x, const int* s_len, const int* s_rows, int B, int G, int cuts, int chunk, int less) {
   constexpr int kTile = Shape<W>::kTile;
   int n = 0;
   const float by = 1.f / cuts;
   for (int i = lane_prefix(~0ull); i < B * cuts; i += 64) {
     const int b = static_cast<int>((i + 0.5f) * by), j = i - b * cuts;  // (exact: i is below 2^18)
-    n += tiles_over<W>(j ? max(x, j * chunk * kTile) : x, s_len[b], s_rows[b], G);
+    n += (j + 1) * tiles_over<W>(max(j ? j * chunk : -1, x * (j + 1)) * kTile, s_len[b], s_rows[b], G);
+  }
+  return wave_total(n) - less;
+}
+template <int W>
+__device__ __forceinline__ int parts_less(const int* s_len, const int* s_rows, int B, int G, int cuts, int chunk) {
+  int n = 0;
+  const float by = 1.f / cuts;
+  for (int i = lane_prefix(~0ull); i < B * cuts; i += 64) {
+    const int b = static_cast<int>((i + 0.5f) * by), j = i - b * cuts;
+    if (j) n += j * tiles_over<W>(j * chunk * Shape<W>::kTile, s_len[b], s_rows[b], G);
   }
   return wave_total(n);
+}
+// The tiles of the piece-th longest part (from 0), and how many are longer.
+template <int W>
+__device__ __forceinline__ int part_at(int piece, const int* s_len, const int* s_rows, int B, int G, int longest, int cuts,
+                                       int chunk, int less, int& over) {
+  int lo = -1, hi = min((longest + Shape<W>::kTile - 1) / Shape<W>::kTile, chunk);
+  over = 0;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    const int n = parts_over<W>(mid, s_len, s_rows, B, G, cuts, chunk, less);
+    if (n > piece) {
+      lo = mid;
+    } else {
+      hi = mid;
+      over = n;
+    }
+  }
+  return hi;
 }
 
 // Goes through the workgroup's pieces.  CARE: those that the first time marked in s_again, with care for values that are no
@@ -135,7 +166,7 @@ __device__ __forceinline__ int parts_over(int x, const int* s_len, const int* s_
 template <int DT, bool PAGED, int W, bool CARE>
 __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const int* s_len, const int* s_rows,
                                            const int* s_first, int4* s_plan, uint32_t* s_again, int wave, int longest,
-                                           int pieces, int cuts, int chunk) {
+                                           int pieces, int cuts, int chunk, int less) {
   using S = Shape<W>;
   constexpr int kWaves = W, kCols = S::kCols, kTile = S::kTile, kSub = S::kSub, kProducts = S::kProducts, kFirst = S::kFirst;
   constexpr int kKBuf = S::kKBuf, kVBuf = S::kVBuf;
@@ -174,8 +205,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
   const int shift = rounds ? own % rounds : 0;
   auto turn_of = [&](int round) { return round + shift < rounds ? round + shift : round + shift - rounds; };
 
-  // ---- what the pieces of rounds r .. r + 63 are, found by the waves side by side: the n-th part of a column tile by the
-  // tile's falling length (its length in tiles of tokens, then its place among those)
+  // ---- what the pieces of rounds r .. r + 63 are, found by the waves side by side: the n-th part by the parts' falling length
   auto find_pieces = [&](int r) {
     const ArgsPtr Z = args_again();
     const int n_seqs = Z->B;
@@ -183,35 +213,28 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
       const int pos = place_of(turn_of(r + i));
       const int piece = __builtin_amdgcn_readfirstlane(pos / heads_lane);
       const int h = (pos - piece * heads_lane) * lanes + xcd;
-      int lo = -1, hi = (longest + kTile - 1) / kTile, over = 0;  // more than `piece` parts over 64 lo, none over 64 hi
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        const int n = parts_over<W>(mid * kTile, s_len, s_rows, n_seqs, G, cuts, chunk);
-        if (n > piece) {
-          lo = mid;
-        } else {
-          hi = mid;
-          over = n;
+      int over;
+      const int size = part_at<W>(piece, s_len, s_rows, n_seqs, G, longest, cuts, chunk, less, over);
+      // which of those of its length: by sequence, parts of a tile, and the tile's falling length
+      int rank = piece - over, b = 0, tile = 0, split = 0, ns = 1;
+      const float by = 1.f / cuts;
+      for (int base = 0; base < n_seqs * cuts; base += 64) {
+        const int e = base + lane, at_b = static_cast<int>((e + 0.5f) * by), j = e - at_b * cuts;
+        int n = 0, high = 0;  // its parts, and its column tiles that are longer
+        if (e < n_seqs * cuts) {
+          const int len = s_len[at_b], rows = s_rows[at_b], least = j ? j * chunk : -1;
+          high = tiles_over<W>(max(least, size * (j + 1)) * kTile, len, rows, G);
+          n = (j + 1) * (tiles_over<W>(max(least, (size - 1) * (j + 1)) * kTile, len, rows, G) - high);
         }
-      }
-      // its tile has hi tiles of tokens (none with hi = 0): ns parts, as all between
-      const int ns = max((hi + chunk - 1) / chunk, 1);
-      const int x = lo < 0 ? -1 : lo * kTile, x2 = hi * kTile;
-      int rank = (piece - over) / ns, b = 0, tile = 0;
-      const int split = piece - over - rank * ns;
-      for (int base = 0; base < n_seqs; base += 64) {
-        const int j = base + lane;
-        const int high = j < n_seqs ? tiles_over<W>(x2, s_len[j], s_rows[j], G) : 0;
-        const int n = j < n_seqs ? tiles_over<W>(x, s_len[j], s_rows[j], G) - high : 0;
         const int sum = wave_prefix(n);
         const uint64_t past = wave_ballot(sum > rank);
         if (past) {
           const int at = __builtin_ctzll(past);
-          b = base + at;
-          const int before = __builtin_amdgcn_readlane(sum - n, at);
-          // its tiles from the longest: `high` are longer than these
-          const int all = (s_rows[b] * G + kCols - 1) / kCols;
-          tile = all - 1 - __builtin_amdgcn_readlane(high, at) - (rank - before);
+          b = __builtin_amdgcn_readlane(at_b, at);
+          ns = __builtin_amdgcn_readlane(j, at) + 1;
+          const int mine = rank - __builtin_amdgcn_readlane(sum - n, at), of_tile = mine / ns;
+          split = mine - of_tile * ns;
+          tile = (s_rows[b] * G + kCols - 1) / kCols - 1 - __builtin_amdgcn_readlane(high, at) - of_tile;
           break;
         }
         rank -= __builtin_amdgcn_readlane(sum, 63);
@@ -725,9 +748,9 @@ __global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
   pieces = wave_total(pieces);
 
   // ---- into how many parts the longest pieces are cut.  What that takes, in tiles: the longest part, or the workgroups' mean
-  // and some of a part, about 4 a round for beginning and ending pieces, and writing and joining the parts' rows.  The waves
-  // look at every eighth number each.
-  int cuts = 1, chunk = 1 << 24;
+  // and some of a part (in two rounds what the last of the first and the first of the second take, if that is more), about 4 a
+  // round for beginning and ending pieces, and writing and joining the parts' rows.  The waves look at every eighth number each.
+  int cuts = 1, chunk = 1 << 24, less = 0;
   if (P.splits > 1) {
     float work = 0.f;
     int cols = 0;
@@ -741,49 +764,62 @@ __global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
     cols = wave_total(cols);
     const float grid = gridDim.x, mean = work * P.H / grid;
     const int most = (longest + kTile - 1) / kTile;
-    float best = INFINITY;
-    int best_k = 1, best_n = pieces;
     for (int k = wave + 1; k <= P.splits; k += kWaves) {
       const int part = (most + k - 1) / k;
-      int n = pieces, cut = 0;  // parts in all, column tiles that are cut
+      int n = pieces, cut = 0, lost = 0;  // parts in all, column tiles that are cut
       if (k > 1) {
-        if (part < kLeast) break;
-        n = parts_over<W>(-1, s_len, s_rows, P.B, G, k, part);
+        lost = parts_less<W>(s_len, s_rows, P.B, G, k, part);
+        n = parts_over<W>(-1, s_len, s_rows, P.B, G, k, part, lost);
         for (int b = lane; b < P.B; b += 64) cut += tiles_over<W>(part * kTile, s_len[b], s_rows[b], G);
         cut = wave_total(cut);
       }
       const float items = static_cast<float>(n) * P.H;
-      const float load = items <= grid ? part : fmaxf(mean + 0.3f * part, part);
+      const float load = items <= grid ? part : fmaxf(mean + (items <= 2.f * grid ? 0.15f : 0.3f) * part, part);
       const float join = k > 1 ? 2.5f * kPerCu + static_cast<float>(min(cut * kCols, cols)) * (P.H * k) * (1040 * kPerCu / 7.6e6f) : 0.f;
-      const float takes = (load + 4.f * kPerCu * ceilf(items / grid) + join) * (k > 1 ? 1.05f : 1.f);
-      if (takes < best) {
-        best = takes;
-        best_k = k;
-        best_n = n;
-      }
+      const float around = 4.f * kPerCu * ceilf(items / grid) + join;
+      const bool two = items > grid && items <= 2.f * grid;
+      if (lane == 0)
+        s_plan[k - 1] = int4{__float_as_int(k > 1 && part < kLeast ? INFINITY : (load + around) * (k > 1 ? 1.05f : 1.f)), n, lost,
+                             __float_as_int(two ? around : -1.f)};
     }
-    if (lane == 0) s_plan[wave] = int4{__float_as_int(best), best_k, best_n, 0};
     __syncthreads();
-    best = INFINITY;
+    // (what those two parts take is only looked for where it could matter)
+    int4 mine = int4{__float_as_int(INFINITY), 0, 0, 0};
+    if (lane < P.splits) mine = s_plan[lane];
+    float best = __int_as_float(mine.w) < 0.f ? __int_as_float(mine.x) : INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const int4 x = s_plan[w];
-      if (__int_as_float(x.x) < best || w == 0) {
-        best = __int_as_float(x.x);
-        cuts = x.y;
-        pieces = x.z;
-      }
+    for (int x = 32; x; x >>= 1) best = fminf(best, __shfl_xor(best, x));
+    __syncthreads();
+    for (int k = wave + 1; k <= P.splits; k += kWaves) {
+      const float takes = __int_as_float(__builtin_amdgcn_readlane(mine.x, k - 1));
+      const float around = __int_as_float(__builtin_amdgcn_readlane(mine.w, k - 1));
+      if (around < 0.f || takes >= best) continue;
+      const int n = __builtin_amdgcn_readlane(mine.y, k - 1), lost = __builtin_amdgcn_readlane(mine.z, k - 1);
+      const int nth = min(static_cast<int>(gridDim.x) / P.H, n - 1), part = k > 1 ? (most + k - 1) / k : 1 << 24;
+      int over, two = 0;
+#pragma unroll 1
+      for (int i = max(nth - 1, 0); i <= nth; ++i)
+        two += part_at<W>(i, s_len, s_rows, P.B, G, longest, k, part, lost, over);
+      if (lane == 0) s_plan[k - 1].x = __float_as_int(fmaxf(takes, (two + around) * (k > 1 ? 1.05f : 1.f)));
     }
+    __syncthreads();
+    best = lane < P.splits ? __int_as_float(s_plan[lane].x) : INFINITY;
+    float least = best;
+#pragma unroll
+    for (int x = 32; x; x >>= 1) least = fminf(least, __shfl_xor(least, x));
+    const int at = __builtin_ctzll(wave_ballot(best == least));
+    cuts = at + 1;
+    pieces = __builtin_amdgcn_readlane(mine.y, at);
+    less = __builtin_amdgcn_readlane(mine.z, at);
     cuts = __builtin_amdgcn_readfirstlane(cuts);
-    pieces = __builtin_amdgcn_readfirstlane(pieces);
     if (cuts > 1) chunk = (most + cuts - 1) / cuts;
   }
 
-  const int again = go_through<DT, PAGED, W, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk);
+  const int again = go_through<DT, PAGED, W, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk, less);
   if (again && lane == 0) s_any = 1;
   __syncthreads();
   if (s_any) {
-    go_through<DT, PAGED, W, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk);
+    go_through<DT, PAGED, W, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk, less);
   }
 
   // ---- rows of no sequence
@@ -816,7 +852,7 @@ Plan plan_for(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new,
   p.pieces = each < packed ? each : packed;
   p.pieces = p.pieces < 1 ? 1 : p.pieces;
   const int64_t cus = device_cu_count() * S::kPerCu, tiles = (max_len + S::kTile - 1) / S::kTile, work = p.pieces * Hkv;
-  int64_t splits = work >= enough * cus ? 1 : (2 * cus + work - 1) / work;
+  int64_t splits = work >= enough * cus ? 1 : (3 * cus + work - 1) / work;
   splits = splits > tiles / S::kLeast ? tiles / S::kLeast : splits;
   p.splits = static_cast<int>(splits < 1 ? 1 : splits > kMostCuts ? kMostCuts : splits);
   return p;
@@ -829,10 +865,11 @@ Plan packed_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_l
   const int64_t most = max_len < rows ? max_len : rows;
   return most <= 256 ? plan_for<4>(rows, B, Hq, Hkv, most, most, 0.75f) : plan_for<8>(rows, B, Hq, Hkv, most, most, 0.75f);
 }
-// Over pages, from three pieces a CU on none is cut.  (Chunks to 512 over 1.6-8 K tokens of 4 sequences, 0.8 pieces a CU: 268 us as
-// they are, 239 with the longest cut in two; the launch that joins costs 5 us where none is cut.)
+// Over pages, from two pieces a CU on none is cut (the launch that joins costs 5 us where none is).  Chunks to 512 over 1.6-8 K
+// tokens of 4 sequences, 0.8 pieces a CU: 268 us as they are, 230 in two parts taken by the length of their tiles, 168 in three
+// by their own length; 12 sequences of 0.4-17 K, 1.5 pieces a CU: 458 and 301 us.
 Plan pages_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_len) {
-  return plan_for<8>(rows, B, Hq, Hkv, max_new < rows ? max_new : rows, max_len, 3.f);
+  return plan_for<8>(rows, B, Hq, Hkv, max_new < rows ? max_new : rows, max_len, 2.f);
 }
 
 size_t plan_bytes(const Plan& p, int64_t rows, int64_t Hq) {
