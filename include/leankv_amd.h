@@ -837,7 +837,7 @@ int lkv_pages_compact(const lkv_pages* st, int32_t* in_use, void* workspace, siz
  * it holds in one layer: out = softmax(scale * q K^T) V in the pool's type,
  * zeros for an empty sequence.  The work is split for max_len, a bound on lens
  * (longer sequences count as max_len).  Neighbouring sequences on the same pages
- * are read once for several of them.  Scores and sums are fp32; the weights are
+ * are read once for several of them.  out may be q.  Scores and sums are fp32; the weights are
  * rounded to the pool's type for the value product.
  */
 size_t lkv_pages_decode_attn_workspace_bytes(int64_t seqs, int64_t Hq, int64_t kv_heads, int64_t max_len);
@@ -851,7 +851,8 @@ int lkv_pages_decode_attn(const lkv_pages* st, int64_t layer, const void* q, con
  * row and head) are sequence b; query i of it sees its tokens 0 .. i.  cu int32
  * [B + 1] on the device, ascending.  max_len is a bound on the lengths (the work
  * is split for it; longer ones are right too).  Rows that belong to no sequence
- * are zeros with fill = 1 and left as they are with fill = 0.
+ * are zeros with fill = 1 and left as they are with fill = 0.  out does not
+ * overlap q, k or v.
  */
 size_t lkv_packed_attn_workspace_bytes(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_len);
 int lkv_packed_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -863,7 +864,8 @@ int lkv_packed_attn(const void* q, const int64_t* q_strides, const void* k, cons
  * The same over pages: rows cu[s] .. cu[s + 1] - 1 of q are the queries of the
  * newest tokens of sequence s (at most lens[s]: further rows are zeros); query i
  * of m sees tokens 0 .. lens[s] - m + i.  max_new and max_len are bounds on the
- * rows of a sequence and on lens, for which the work is split.
+ * rows of a sequence and on lens, for which the work is split.  out does not
+ * overlap q.
  */
 size_t lkv_pages_prefill_attn_workspace_bytes(int64_t rows, int64_t seqs, int64_t Hq, int64_t kv_heads,
                                               int64_t max_new, int64_t max_len);

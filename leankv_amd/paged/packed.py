@@ -62,6 +62,11 @@ def out_rows(out: torch.Tensor, like: torch.Tensor, what: str):
     return st
 
 
+def apart(q: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """q, or a copy where out is written over it (its rows are read again where a value is no number)."""
+    return q.clone(memory_format=torch.contiguous_format) if out.data_ptr() == q.data_ptr() and q.numel() else q
+
+
 def follow(what: str, *tensors: torch.Tensor) -> bool:
     """Whether autograd follows one of them.  A forward-mode tangent would be lost at once and is refused."""
     if getattr(forward_ad, "_current_level", -1) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
@@ -113,7 +118,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     (heads a multiple of kv_heads; query head h reads kv head h * kv_heads // heads), float16 or bfloat16.  cu_seqlens: int32
     [n + 1] on the device, ascending; rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 are sequence i, up to 2048 of them.  Returns
     [tokens, heads, 128] in q's type; rows of no sequence are zeros, or, in a buffer given as `out` (dense 16-byte aligned
-    rows apart from each other; q itself may be it), left as they are.  max_len: the caller's bound on the lengths (default:
+    rows apart from each other; q itself may be it, and is copied then), left as they are.  max_len: the caller's bound on the lengths (default:
     all tokens), which the work is split for.  scale: 1 / sqrt(128) by default.
 
     Inputs may have any strides (rows that are not dense or not 16-byte aligned are copied).  A token that a query does not
@@ -150,6 +155,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if follows:
             raise LeanKVError("%s: out= does not support autograd, which follows q, k or v" % what)
         os = out_rows(out, q, what)
+        q = apart(q, out)
     (q, qs), (k, ks), (v, vs) = rows(q), rows(k, apart=True), rows(v, apart=True)
     batch = cu_seqlens.shape[0] - 1
     nbytes = _bytes(n, batch, heads, kv_heads, bound)

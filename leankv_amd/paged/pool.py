@@ -15,7 +15,7 @@ import torch
 
 from .. import _lib
 from .._lib import LeanKVError
-from .packed import DTYPES, HEAD_DIM, MAX_SEQS, SCALE, call, follow, out_rows, rows, strides2, tied
+from .packed import DTYPES, HEAD_DIM, MAX_SEQS, SCALE, apart, call, follow, out_rows, rows, strides2, tied
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
@@ -316,7 +316,8 @@ class PagedKV:
                           out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention of the newest tokens' queries (after their store), q [rows, heads, 128]: rows cu[s] .. cu[s + 1] - 1
         are those of sequence s (further ones than it holds tokens are zeros), and query i of m sees tokens 0 .. lens[s] - m +
-        i.  Returns [rows, heads, 128]; rows of no sequence are zeros, or, in a buffer given as `out`, left as they are.
+        i.  Returns [rows, heads, 128]; rows of no sequence are zeros, or, in a buffer given as `out` (q itself may be it, and is
+        copied then), left as they are.
         max_new, max_len: the caller's bounds on the rows of a sequence and on lens, which the work is split for.  (A sequence
         that extend refused, taken[s] = 0, has its rows computed as those of the tokens that it holds.)"""
         what = "PagedKV.prefill_attention"
@@ -330,7 +331,7 @@ class PagedKV:
         new = n if max_new is None else min(int(max_new), n)
         fill = out is None
         out, os = self._output(q, out, what)
-        q, qs = rows(q)
+        q, qs = rows(q if fill else apart(q, out))
         nbytes = _prefill_bytes(n, self.max_seqs, heads, self.kv_heads, new, bound)
         ws = self._workspace(nbytes) if nbytes else None
         call(self._index, self._lib.lkv_pages_prefill_attn, self._ref, layer, q.data_ptr(), qs, n, heads, p, new, bound,

@@ -294,6 +294,46 @@ def test_prefill_values_that_are_no_numbers(cuda, dtype, max_new):
     assert got[5, :, 3].isnan().all() and got[1:, :, 100].isnan().all()
 
 
+@pytest.mark.parametrize("new", [4, 100])
+def test_results_over_their_queries(cuda, new):
+    """q as out, also where rows are gone through again for a value that is no number."""
+    from leankv_amd.paged import packed_attention
+
+    gen = torch.Generator().manual_seed(57)
+    n, page = 700, 64
+    cache, rows, _ = _cache(gen, [n, n], 2, page, F16)
+    t = n - new + new // 2
+    cache.pool[0, rows[0][t // page], 1, 0, t % page, 5] = math.nan
+    at = _ints([0, new, 2 * new])
+    q = _rows(gen, 2 * new, 8, F16).cuda()
+    want = cache.prefill_attention(0, q, at, max_new=new)
+    assert want[new // 2:new, :4, 5].isnan().all() and not want[:new // 2].isnan().any() and not want[new:].isnan().any()
+    over = q.clone()
+    assert cache.prefill_attention(0, over, at, max_new=new, out=over) is over
+    assert torch.equal(over.nan_to_num(9.0), want.nan_to_num(9.0))
+    k, v = _rows(gen, 2 * new, 2, F16).cuda(), _rows(gen, 2 * new, 2, F16).cuda()
+    v[new // 2, 1, 7] = math.inf
+    want, over = packed_attention(q, k, v, at), q.clone()
+    packed_attention(over, k, v, at, out=over)
+    assert torch.equal(over.nan_to_num(9.0), want.nan_to_num(9.0))
+    q1 = _rows(gen, 2, 8, F16).cuda()
+    want, over = cache.decode_attention(0, q1), q1.clone()
+    cache.decode_attention(0, over, out=over)
+    assert torch.equal(over.nan_to_num(9.0), want.nan_to_num(9.0))
+
+
+def test_bounds_of_nothing(cuda):
+    """max_len = 0 says that every sequence is empty (decode); for prefill bounds only divide the work."""
+    gen = torch.Generator().manual_seed(58)
+    cache, _, _ = _cache(gen, [100, 3], 2, 16, F16)
+    assert not cache.decode_attention(0, _rows(gen, 2, 8, F16).cuda(), max_len=0).any()
+    q, at = _rows(gen, 43, 8, F16).cuda(), _ints([0, 40, 43])
+    want = cache.prefill_attention(0, q, at)
+    for kw in (dict(max_new=0), dict(max_len=0), dict(max_new=0, max_len=0), dict(max_new=1, max_len=1)):
+        err = (cache.prefill_attention(0, q, at, **kw).double() - want.double()).norm() / want.double().norm()
+        assert err < 2 * 2.0 ** -11 + 2 * 2.0 ** -11, kw  # both round the weights and the result to float16
+
+
 @pytest.mark.parametrize("page", [16, 64, 256])
 @pytest.mark.parametrize("heads,kv,dtype", [(8, 2, F16), (3, 3, BF16), (7, 1, F16), (12, 1, BF16), (40, 2, F16), (16, 1, BF16)])
 def test_decode(cuda, page, heads, kv, dtype):
