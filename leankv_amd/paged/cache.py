@@ -155,14 +155,18 @@ class PagedCache(HFCache):
             raise RuntimeError("PagedCache.%s: an update awaits its attention" % what)
 
     def crop(self, max_length: int):
-        """Keeps the first max_length tokens (negative: drops that many)."""
+        """Keeps the first max_length tokens (0 or negative: drops that many from the end, as HF's caches do).  An integer, or
+        a tensor of one (assisted generation gives it; one on the device is waited for)."""
         self._idle("crop")
-        n = self._seq_lengths[0]
-        keep = max(0, n + max_length) if max_length < 0 else min(n, max_length)
+        n, max_length = self._seq_lengths[0], int(max_length)
+        keep = max(0, n + max_length) if max_length <= 0 else min(n, max_length)
         if self.kv is not None and keep < n:
             self.kv.truncate(torch.full((self.kv.max_seqs,), keep, dtype=torch.int32, device=self.kv.device))
         self._seq_lengths = [min(keep, x) for x in self._seq_lengths]
         self._seen_tokens = self._seq_lengths[0]
+
+    def activate_past_recording(self):
+        """Called before tokens that may be cut again (assisted generation); pages need no record of them."""
 
     def reorder_cache(self, beam_idx: torch.LongTensor):
         """Sequence b goes on from sequence beam_idx[b] (beam search): pages are shared, not copied."""

@@ -118,6 +118,31 @@ def test_beam_search(cuda):
     assert int((cache.kv.refs > 0).sum()) < 24
 
 
+def test_assisted_generation(cuda):
+    """Tokens looked up in the prompt are checked several at a time, and those not taken cut off again."""
+    from leankv_amd.combined import optimize_model
+    from leankv_amd.paged import PagedCache
+    from transformers import DynamicCache
+
+    ids = _ids(12, 21).repeat(1, 4).to(cuda)
+
+    def go(model, cache):
+        with torch.no_grad():
+            return model.generate(ids, attention_mask=torch.ones_like(ids), max_new_tokens=40, past_key_values=cache,
+                                  prompt_lookup_num_tokens=5, do_sample=False, pad_token_id=0)
+
+    want = go(_model(cuda, 8), DynamicCache())
+    assert torch.equal(go(_model(cuda, 8), PagedCache(num_layers=2, device=cuda, max_seq_len=32, page_size=16)), want)
+    model, cache = optimize_model(_model(cuda, 8), paged_kv=True, max_seq_len=64)
+    got = go(model, cache)
+    assert got.shape == want.shape and cache.get_seq_length(0) < got.shape[1]
+    # a step's choice is the largest logit within the bound of its row's logits, twice (its own and the largest one's)
+    with torch.no_grad():
+        logits = _model(cuda, 8)(got).logits.float()[:, 47:-1]
+    lost = logits.amax(-1) - logits.gather(-1, got[:, 48:].unsqueeze(-1)).squeeze(-1)
+    assert float(lost.max()) < 2 * RTOL * float(logits.abs().max())
+
+
 def test_padding_and_generate(cuda):
     from leankv_amd.combined import optimize_model
     from transformers import DynamicCache
@@ -164,7 +189,9 @@ def test_chosen_batches_and_bf16(cuda):
     assert torch.equal(a, torch.cat([want[3:], tail], 2)) and grown.kv.max_len >= 72
     cache.crop(-3)
     assert cache.get_seq_length(0) == 19 and torch.equal(cache[1][0], want[[3, 0, 3], :, :19])
-    cache.crop(0)
+    cache.crop(0)  # (HF's caches drop as many tokens as a number below 1 says)
+    assert cache.get_seq_length(1) == 19
+    cache.crop(torch.tensor(-19))
     assert cache.get_seq_length(1) == 0 and not (cache.kv.refs > 0).any()
     a, _ = cache.update(more[:3], more[:3], 0)
     assert torch.equal(a, more[:3])
