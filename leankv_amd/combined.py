@@ -15,7 +15,8 @@ Differences, all in the direction of the fast path:
     (leankv/turboquant/paged_cache.py), which HF generate never calls and
     which is not built here; it raises RuntimeError, as the reference does
     where FlashInfer is not installed (combined.py:98-102).  The paged
-    TurboQuant layout is leankv_amd.turboquant.paged_tq_cache.
+    TurboQuant layout is leankv_amd.turboquant.paged_tq_cache, the 16-bit
+    pages of this package leankv_amd.paged (paged_kv=True).
 """
 
 from __future__ import annotations

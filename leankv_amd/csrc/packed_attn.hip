@@ -16,6 +16,12 @@
 // A masked token has weight 0, but 0 times an infinite or NaN value is not 0.  Where a row ends up with such a number its
 // workgroup goes through the piece again with care: values that are no numbers count as 0 in the masked tiles' products, and
 // a second product counts, of each kind, those that a column sees.
+//
+// 8 waves, a CU's whole LDS: a row is staged once for 256 columns, and 212 registers hold a wave's queries, its sums and both
+// operands on their way.  Bound by the products (54 % of the SIMDs' cycles over a prompt of 8192) and the vector work beside them
+// (52 %): 3480 cycles a tile for the two waves of a SIMD, 2048 of them products, and 12 thousand to begin and end a piece.
+// 32/8 heads: a prompt of 8192 tokens 496-530 us, 1037-1109 TFLOP/s (1.96 GHz under that load; the library's product of 8192^3
+// reaches 1241); 4 x 512 queries over 8192 tokens 264-272 us, up to 1017 TFLOP/s; 16 prompts to 1201 tokens 109-118 us.
 #include "pages_common.h"
 
 namespace lkv {
@@ -33,7 +39,8 @@ struct Shape {
   static constexpr int kTile = 8 * W;      // tokens of a tile: a wave stages 8 rows
   static constexpr int kSub = kTile / 32;  // products along its tokens
   static constexpr int kProducts = 8 * kSub;             // of its scores, and of its values
-  static constexpr int kFirst = kProducts * 3 / 4;       // pairs of weights beside the score products, the others beside the values
+  static constexpr int kFirst = kProducts * 3 / 4;       // pairs of weights beside the score products, the others beside the
+                                                         // values (all beside the scores: 525 us over 8192 tokens, so 517)
   static constexpr int kKBuf = kTile * kKRow, kVBuf = kTile * kVRow;
   static constexpr int kLeast = 6 * kPerCu;  // fewest tiles of a part of the longest piece
 };
@@ -116,13 +123,14 @@ __device__ __forceinline__ int wave_prefix(int v) {  // inclusive
 }
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
 
-// A column tile of T tiles of tokens is j + 1 = ceil(T / chunk) parts (at most `cuts`) of ceil(T / (j + 1)) tiles at most, which
-// are more than x < chunk where T > x (j + 1).  Parts of more than x tiles, of all column tiles (x = -1: all parts), are then
-// the sum over j of (j + 1) times the tiles with max(j chunk, x (j + 1)) < T <= (j + 1) chunk: with N(y) the tiles with T > y,
+// A column tile of T tiles of tokens is j + 1 = ceil(T / chunk) parts (at most `cuts`) of ceil(T / (j + 1)) tiles at most,
+// which are more than x < chunk where T > x (j + 1).  Parts of more than x tiles, of all column tiles (x = -1: all parts), are
+// then the sum over j of (j + 1) times the tiles with max(j chunk, x (j + 1)) < T <= (j + 1) chunk: with N(y) the tiles with T > y,
 //   sum over j of (j + 1) N(max(j chunk, x (j + 1))) - sum over j of j N(j chunk),
 // the second the same for all x (`less`).  By the lanes of a wave, a (sequence, j) each.
 template <int W>
-__device__ __forceinline__ int parts_over(int x, const int* s_len, const int* s_rows, int B, int G, int cuts, int chunk, int less) {
+__device__ __forceinline__ int parts_over(int x, const int* s_len, const int* s_rows, int B, int G, int cuts, int chunk,
+                                          int less) {
   constexpr int kTile = Shape<W>::kTile;
   int n = 0;
   const float by = 1.f / cuts;
@@ -673,7 +681,8 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
           *reinterpret_cast<uint2*>(mine_row + 2 * (32 * db + 8 * k + 4 * oh)) =
               uint2{pack<DT>(x[0], x[1]), pack<DT>(x[2], x[3])};
         }
-      uint16_t* const base = Z->out + static_cast<uint64_t>(c.row0 + first.q0) * Z->o_st + static_cast<uint64_t>(c.h * G) * Z->o_sh;
+      uint16_t* const base =
+          Z->out + static_cast<uint64_t>(c.row0 + first.q0) * Z->o_st + static_cast<uint64_t>(c.h * G) * Z->o_sh;
       const uint32_t o_st = Z->o_st, o_sh = Z->o_sh;
       out_rows(ends, [&](uint32_t q, uint32_t x, const u32x4& v) {
         *reinterpret_cast<u32x4*>(base + (static_cast<uint64_t>(q) * o_st + static_cast<uint64_t>(x) * o_sh + 8 * (out_lane & 15))) = v;
@@ -748,8 +757,9 @@ __global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
   pieces = wave_total(pieces);
 
   // ---- into how many parts the longest pieces are cut.  What that takes, in tiles: the longest part, or the workgroups' mean
-  // and some of a part (in two rounds what the last of the first and the first of the second take, if that is more), about 4 a
-  // round for beginning and ending pieces, and writing and joining the parts' rows.  The waves look at every eighth number each.
+  // and some of a part (in two rounds what the last of the first and the first of the second take, if that is more), about 4
+  // a round for beginning and ending pieces, and writing and joining the parts' rows.  The waves look at every eighth number
+  // each.
   int cuts = 1, chunk = 1 << 24, less = 0;
   if (P.splits > 1) {
     float work = 0.f;
@@ -775,12 +785,13 @@ __global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
       }
       const float items = static_cast<float>(n) * P.H;
       const float load = items <= grid ? part : fmaxf(mean + (items <= 2.f * grid ? 0.15f : 0.3f) * part, part);
-      const float join = k > 1 ? 2.5f * kPerCu + static_cast<float>(min(cut * kCols, cols)) * (P.H * k) * (1040 * kPerCu / 7.6e6f) : 0.f;
+      const float part_rows = static_cast<float>(min(cut * kCols, cols)) * (P.H * k);
+      const float join = k > 1 ? 2.5f * kPerCu + part_rows * (1040 * kPerCu / 7.6e6f) : 0.f;
       const float around = 4.f * kPerCu * ceilf(items / grid) + join;
       const bool two = items > grid && items <= 2.f * grid;
       if (lane == 0)
-        s_plan[k - 1] = int4{__float_as_int(k > 1 && part < kLeast ? INFINITY : (load + around) * (k > 1 ? 1.05f : 1.f)), n, lost,
-                             __float_as_int(two ? around : -1.f)};
+        s_plan[k - 1] = int4{__float_as_int(k > 1 && part < kLeast ? INFINITY : (load + around) * (k > 1 ? 1.05f : 1.f)), n,
+                             lost, __float_as_int(two ? around : -1.f)};
     }
     __syncthreads();
     // (what those two parts take is only looked for where it could matter)
@@ -815,11 +826,13 @@ __global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
     if (cuts > 1) chunk = (most + cuts - 1) / cuts;
   }
 
-  const int again = go_through<DT, PAGED, W, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk, less);
+  const int again = go_through<DT, PAGED, W, false>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces,
+                                                    cuts, chunk, less);
   if (again && lane == 0) s_any = 1;
   __syncthreads();
   if (s_any) {
-    go_through<DT, PAGED, W, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk, less);
+    go_through<DT, PAGED, W, true>(P, smem, s_len, s_rows, s_first, s_plan, s_again, wave, longest, pieces, cuts, chunk,
+                                   less);
   }
 
   // ---- rows of no sequence
@@ -827,7 +840,8 @@ __global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
   if (Z->fill) {
     const int a = min(max(Z->cu[0], 0), Z->rows), e = min(max(Z->cu[Z->B], a), Z->rows);
     const int64_t per = static_cast<int64_t>(Z->Hq) * (kD / 8), n = (a + Z->rows - e) * per;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThr + 64 * wave + lane_prefix(~0ull); i < n; i += static_cast<int64_t>(gridDim.x) * kThr) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThr;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThr + 64 * wave + lane_prefix(~0ull); i < n; i += step) {
       const int64_t r = i / per, x = i - r * per;
       const int64_t row = r < a ? r : r - a + e;
       *reinterpret_cast<u32x4*>(Z->out + row * Z->o_st + x / (kD / 8) * Z->o_sh + 8 * (x % (kD / 8))) = u32x4{};

@@ -1,5 +1,5 @@
-// Attention of one query per sequence over the 16-bit paged KV cache (lkv_pages_decode_attn), of a few (lkv_pages_prefill_attn with
-// up to 32 columns = queries x heads of a kv head), and the join of partial sums.
+// Attention of one query per sequence over the 16-bit paged KV cache (lkv_pages_decode_attn), of a few (lkv_pages_prefill_attn
+// with up to 32 columns = queries x heads of a kv head), and the join of partial sums.
 //
 //   split kernel  grid (splits, kv heads x column tiles, sequences), 4 waves.  A wave takes every 4th chunk of 32 tokens of
 //                 its split, each row read once and straight into registers, and runs on v_mfma_f32_16x16x32
@@ -18,6 +18,12 @@
 // A few newest queries of a sequence (drafted tokens, checked in one pass) are the columns of its workgroups in the same way;
 // those that do not see the last tokens have weight 0 there.  Where such a token's value is no number, 0 times it is none
 // either: it counts as 0 then, and a second product counts, of each kind, those that a column sees.
+//
+// Bound by memory: a wave's next chunk (16 KB) is on its way while it computes this one, 8 waves a CU (230 registers), so that
+// 128 KB a CU are.  32/8 heads: 32 sequences of 8192 tokens 187 us, 5.7 TB/s; 32 of 1.6-8 K 135 us, 4.8 TB/s (the longest end
+// last); 131072 tokens of one sequence 101 us, of them 95 (5.7 TB/s) reading and 7 joining 64 splits; 32 beams over 4 prompts of
+// 8192 tokens, 152 MB read once, 35 us.  5 drafted tokens of 8 sequences of 4096 32 us, of them 26 (5.1 TB/s) reading; in the
+// prefill kernel, whose waves wait for each other's rows, 37.
 #include "pages_common.h"
 
 namespace lkv {
@@ -72,9 +78,9 @@ struct Staged {
   int end[32], same[32], member[32];
 };
 
-// Attention over tokens [lo, hi) of the workgroup's split for `cols` columns, 16 NT at most; where(c, row, head) says which query
-// column c is and slot where its record goes (no slots: the result itself).  Column c sees tokens below sees(c) (MASKED), all
-// of them those below `free`.  pages(i): the i-th page id of the sequence's row from page0 on.
+// Attention over tokens [lo, hi) of the workgroup's split for `cols` columns, 16 NT at most; where(c, row, head) says which
+// query column c is and slot where its record goes (no slots: the result itself).  Column c sees tokens below sees(c) (MASKED),
+// all of them those below `free`.  pages(i): the i-th page id of the sequence's row from page0 on.
 template <int DT, int NT, bool MASKED, class Where, class Sees, class PageOf>
 __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, int page0, int lo, int hi, int free, int cols,
                                        int slot, Where where, Sees sees, PageOf pages) {
@@ -137,7 +143,8 @@ __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, i
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) any |= (vr[e][k] & 0x7fffu) >= inf_bits<DT>() || (vr[e][k] >> 16 & 0x7fffu) >= inf_bits<DT>();
+          for (int k = 0; k < 4; ++k)
+            any |= (vr[e][k] & 0x7fffu) >= inf_bits<DT>() || (vr[e][k] >> 16 & 0x7fffu) >= inf_bits<DT>();
         odd = wave_ballot(any) != 0;
       }
     }
@@ -481,8 +488,8 @@ struct DecodePlan {
 DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len, bool rows = false) {
   const int64_t G = Hq / Hkv, tiles = rows ? 1 : (G + 15) / 16, pairs = S * Hkv * tiles;
   const int64_t steps = (max_len + kStep - 1) / kStep;
-  // Two workgroups a CU, the most that its registers hold at a time (32 x 8192 tokens, 32/8 heads: 186 us, with four 191, 131072
-  // tokens 100 and 108 us).  One split, which needs no join and shares nothing, where a workgroup a CU walks at most 8 steps
+  // Two workgroups a CU, the most that its registers hold at a time (32 x 8192 tokens, 32/8 heads: 186 us, with four 191,
+  // 131072 tokens 100 and 108 us).  One split, which needs no join and shares nothing, where a workgroup a CU walks at most 8 steps
   // (32 x 1024: 24.2 us, in two splits 27.6), and up to 3 steps anyway.
   const int64_t cus = device_cu_count();
   int64_t splits = 1;

@@ -9,6 +9,8 @@
 //   compact   one workgroup ranks free pages below and used pages from n on; a second launch moves pages and renames
 //             table entries.  Pages that move and the places they move to are apart, so that nothing is overwritten early.
 //   store     a wave per token.
+// Each is a launch or two of 2 to 8 us (latency: a few dependent reads of the tables) but for what is moved: store 90.6 MB read
+// and written in 16-17 us (5.4 TB/s), compact 359 MB in 73 us (4.9 TB/s; a device copy reaches 5.13).
 #include "pages_common.h"
 
 namespace lkv {

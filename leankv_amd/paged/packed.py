@@ -118,8 +118,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     (heads a multiple of kv_heads; query head h reads kv head h * kv_heads // heads), float16 or bfloat16.  cu_seqlens: int32
     [n + 1] on the device, ascending; rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 are sequence i, up to 2048 of them.  Returns
     [tokens, heads, 128] in q's type; rows of no sequence are zeros, or, in a buffer given as `out` (dense 16-byte aligned
-    rows apart from each other; q itself may be it, and is copied then), left as they are.  max_len: the caller's bound on the lengths (default:
-    all tokens), which the work is split for.  scale: 1 / sqrt(128) by default.
+    rows apart from each other; q itself may be it, and is copied then), left as they are.  max_len: the caller's bound on the
+    lengths (default: all tokens), which the work is split for.  scale: 1 / sqrt(128) by default.
 
     Inputs may have any strides (rows that are not dense or not 16-byte aligned are copied).  A token that a query does not
     see has no part in its row, whatever it holds; a NaN in a query gives a row of NaN.  There is no gradient: a backward pass
@@ -134,7 +134,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                               % (what, name, t.dtype, t.device))
     n, heads, kv_heads = q.shape[0], q.shape[1], k.shape[1]
     if k.shape != v.shape or k.shape[0] != n or not kv_heads or not heads or heads % kv_heads:
-        raise LeanKVError("%s: q %s, k %s and v %s do not belong together" % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+        raise LeanKVError("%s: q %s, k %s and v %s do not belong together"
+                          % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     index = q.get_device()
     if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 \
             or not 2 <= cu_seqlens.shape[0] <= MAX_SEQS + 1 or not cu_seqlens.is_cuda \
@@ -160,7 +161,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     batch = cu_seqlens.shape[0] - 1
     nbytes = _bytes(n, batch, heads, kv_heads, bound)
     ws = q.new_empty(nbytes // 2) if nbytes else None
-    call(index, _lib.load().lkv_packed_attn, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, DTYPES[q.dtype], n, heads, kv_heads,
-         cu_seqlens.data_ptr(), batch, bound, SCALE if scale is None else scale, out.data_ptr(), os, int(fill),
+    call(index, _lib.load().lkv_packed_attn, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, DTYPES[q.dtype], n, heads,
+         kv_heads, cu_seqlens.data_ptr(), batch, bound, SCALE if scale is None else scale, out.data_ptr(), os, int(fill),
          None if ws is None else ws.data_ptr(), nbytes)
     return out
