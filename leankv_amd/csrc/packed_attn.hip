@@ -263,7 +263,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
   };
 
   struct Piece {
-    int b, h, split, len, row0, qlen, cols, col0, blk0, nt, ns;
+    int b, h, split, len, row0, qlen, cols, col0, blk0, nt, ns, end;  // end: of the tokens that are read
   };
   auto open = [&](int round) {
     if ((round & (kPlan - 1)) == 0) {
@@ -285,6 +285,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
     c.blk0 = __builtin_amdgcn_readfirstlane(z.x);
     c.nt = __builtin_amdgcn_readfirstlane(z.y);
     c.ns = __builtin_amdgcn_readfirstlane(z.z);
+    c.end = min(c.len, (c.blk0 + c.nt) * kTile);
     return c;
   };
 
@@ -308,7 +309,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
     const uint16_t* p = PAGED ? base + (static_cast<int64_t>(page) * 2 * P.H + c.h) * run + (at & (page_size(P.st) - 1)) * kD
                               : base + static_cast<int64_t>(c.row0 + at) * stride + c.h * head;
     // (a row ends within its stride: what lies behind the last one is never asked for)
-    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, 2 * stride * min(max(c.len - at, 0), 8),
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, 2 * stride * min(max(c.end - at, 0), 8),
                                                      0x00020000);
 #pragma unroll
     for (int j = 0; j < 2; ++j) w[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off[j], 0, 0));
@@ -362,7 +363,8 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
 #pragma unroll
     for (int kb = 0; kb < 8; ++kb) qf[kb] = *reinterpret_cast<const u32x4*>(turn + kOutRow * c32 + 32 * kb + 16 * hf);
   };
-  // the first rows of a piece on their way (the keys of its second tile too), while the one before is put away
+  // the first rows of a piece on their way (the keys of its second tile too), while the last tile of the one before is computed
+  // and its rows are put away (asked for after that tile: chunks 1 to 3 % slower)
   auto first_loads = [&](const Piece& c) {
     if (c.nt) {
       int page0 = 0;
@@ -399,6 +401,8 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
     const int lim = len - qlen + w.q0 + column(w, max(min(c32, wave_cols - 1), 0)).x + 1;
     const int lim_min = len - qlen + w.q0 + 1;
 
+    Piece next = c;
+    const bool more = round + 1 < rounds;
     float m, l;
     f32x16 o[4];   // dims 32 db + 8 (i / 4) + 4 hf + i % 4
     f32x16 sc[kSub];  // scores of tokens 32 kt + 8 (i / 4) + 4 hf + i % 4
@@ -599,14 +603,6 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
           if ((blk0 + t + 2) * kTile > lim_min || wave_ballot(mx > kMaxWeight) != 0) general(t + 1);  // uniform
           __syncthreads();
         }
-        if (nt) {  // the last tile
-          ws[0] = ws[1] = 0.f;
-#pragma unroll
-          for (int i = 0; i < kProducts; ++i) weights(i);
-          l += ws[0] + ws[1];
-#pragma unroll
-          for (int i = 0; i < kProducts; ++i) o[i & 3] = mfma32<DT>(value_op(i, nt - 1), pf[i >> 2], o[i & 3]);
-        }
       } else {  // no columns: the wave's part of the staging
 #pragma unroll 1
         for (int t = 0; t + 1 < nt; ++t) {
@@ -618,6 +614,18 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
           load_next(t);
           __syncthreads();
         }
+      }
+      if (more) {
+        next = open(round + 1);
+        first_loads(next);
+      }
+      if (works && nt) {  // the last tile
+        ws[0] = ws[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) weights(i);
+        l += ws[0] + ws[1];
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) o[i & 3] = mfma32<DT>(value_op(i, nt - 1), pf[i >> 2], o[i & 3]);
       }
       __syncthreads();  // the tiles are done with
     }
@@ -631,14 +639,6 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
       if (wave_ballot(ok && (odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.f)) {
         if (lane == 0) atomicOr(&s_again[(round >> 5) & (kAgain - 1)], 1u << (round & 31));
         again = 1;
-      }
-    }
-    Piece next = c;
-    const bool more = round + 1 < rounds;
-    if constexpr (!CARE) {
-      if (more) {
-        next = open(round + 1);
-        first_loads(next);
       }
     }
     const ArgsPtr Z = args_again();
