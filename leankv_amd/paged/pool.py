@@ -94,6 +94,9 @@ class PagedKV:
         self._extend_bytes = lib.lkv_pages_extend_workspace_bytes(self.num_pages, self.max_seqs)
         self._fork_bytes = lib.lkv_pages_fork_workspace_bytes(self.max_seqs, self.width)
         self._compact_bytes = lib.lkv_pages_compact_workspace_bytes(self.num_pages)
+        # of the calls that change the tables, which are ordered as the tables are
+        self._scratch = self._books.new_empty(max(self._extend_bytes, self._fork_bytes, self._compact_bytes) // 4)
+        self._scratch_ptr = self._scratch.data_ptr()
 
     @property
     def max_len(self) -> int:
@@ -137,7 +140,8 @@ class PagedKV:
             raise LeanKVError("%s: max_len=%d outside sequences of up to %d tokens" % (what, max_len, self.max_len))
         return int(max_len)
 
-    # Workspaces are allocated for their call, on the current stream: calls on several streams and captured graphs share none.
+    # Workspaces of attention are allocated for their call, on the current stream: calls on several streams and captured graphs
+    # share none.
     def _workspace(self, nbytes: int):
         return self._books.new_empty(nbytes // 4)
 
@@ -161,8 +165,7 @@ class PagedKV:
         sequence that would pass max_len, and one whose pages with those of all sequences before it are more than are free,
         takes nothing: taken says what each took.  Two launches."""
         p = self._cu(cu, "PagedKV.extend")
-        ws = self._workspace(self._extend_bytes)
-        call(self._index, self._lib.lkv_pages_extend, self._ref, p, ws.data_ptr(), self._extend_bytes)
+        call(self._index, self._lib.lkv_pages_extend, self._ref, p, self._scratch_ptr, self._extend_bytes)
 
     def store(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor | None = None) -> None:
         """Keys and values [rows, kv_heads, 128] of what the last extend made room for, in one layer: rows cu[s] .. of
@@ -202,8 +205,7 @@ class PagedKV:
         what = "PagedKV.fork"
         p = None if parent is None else self._ints(parent, self.max_seqs, what, "parent")
         c = None if lens is None else self._ints(lens, self.max_seqs, what, "lens")
-        ws = self._workspace(self._fork_bytes)
-        call(self._index, self._lib.lkv_pages_fork, self._ref, p, c, ws.data_ptr(), self._fork_bytes)
+        call(self._index, self._lib.lkv_pages_fork, self._ref, p, c, self._scratch_ptr, self._fork_bytes)
 
     def truncate(self, lens: torch.Tensor) -> None:
         """Every sequence keeps at most its first lens[s] tokens (int32 [max_seqs]; drafted tokens that were not accepted)."""
@@ -228,9 +230,8 @@ class PagedKV:
     def compact(self) -> torch.Tensor:
         """The pages in use become the first ones of the pool, in every layer: those behind fill the gaps, in order.  Returns
         their number, int32 [1] on the device.  Two launches."""
-        ws = self._workspace(self._compact_bytes)
         in_use = self._books.new_empty(1)
-        call(self._index, self._lib.lkv_pages_compact, self._ref, in_use.data_ptr(), ws.data_ptr(), self._compact_bytes)
+        call(self._index, self._lib.lkv_pages_compact, self._ref, in_use.data_ptr(), self._scratch_ptr, self._compact_bytes)
         return in_use
 
     def _like(self, num_pages: int, max_seqs: int, max_len: int) -> "PagedKV":
