@@ -104,7 +104,7 @@ __device__ __forceinline__ int tiles_over(int x, int len, int m, int G) {
   constexpr int kCols = Shape<W>::kCols;
   const int q = min(m, len), all = (m * G + kCols - 1) / kCols;
   const int y = x - (len - q);
-  const int under = y <= 0 ? 0 : y >= q ? all : min(all, y * G / kCols);
+  const int under = y >= q ? all : y <= 0 ? 0 : min(all, y * G / kCols);
   return x < 0 ? all : all - under;
 }
 // Sums over a wave by lane permutes of the vector unit (no LDS round trips: a piece is found with several of them).

@@ -322,6 +322,20 @@ def test_results_over_their_queries(cuda, new):
     assert torch.equal(over.nan_to_num(9.0), want.nan_to_num(9.0))
 
 
+@pytest.mark.parametrize("new,kv,heads", [([0, 2], 4, 132), ([300], 1, 4), ([70, 0, 64], 2, 8)])
+def test_rows_of_sequences_that_hold_nothing(cuda, new, kv, heads):
+    """Rows are zeros where no sequence holds a token, whichever kernel takes them."""
+    gen = torch.Generator().manual_seed(59)
+    cache, _, _ = _cache(gen, [0] * len(new), kv, 16, F16, room=700)
+    at = _starts(new, first=1)
+    q = _rows(gen, at[-1] + 1, heads, F16).cuda()
+    for kw in ({}, dict(max_new=max(new)), dict(max_new=1), dict(max_new=max(new), max_len=1)):
+        out = torch.full_like(q, 5.0)
+        cache.prefill_attention(0, q, _ints(at), out=out, **kw)
+        assert not out[1:at[-1]].any() and (out[0] == 5).all() and (out[at[-1]:] == 5).all()
+        assert not cache.prefill_attention(0, q, _ints(at), **kw).any()
+
+
 def test_bounds_of_nothing(cuda):
     """max_len = 0 says that every sequence is empty (decode); for prefill bounds only divide the work."""
     gen = torch.Generator().manual_seed(58)
