@@ -454,14 +454,31 @@ __global__ __launch_bounds__(kThr) void join_kernel(JoinArgs A) {
   for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
   float L = 0.f;
   f32x4 o = f32x4{};
-  for (int i = ONE ? 0 : grp; i < A.splits; i += ONE ? 1 : 8) {
-    const float2 r = ml[i];
-    if (r.x == -INFINITY) continue;  // an empty part: its row was not written
-    const float w = exp2_(r.x - M);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * kD);
-    L = fmaf(w, r.y, L);
+  for (int base = 0; base < A.splits; base += 32) {
+    const int i = base + (tid & 31);
+    const float2 r = i < A.splits ? ml[i] : part_record(-INFINITY, 0.f);
+    const float w = exp2_(r.x - M), wl = w * r.y;
+    // the group's parts that are not empty (the rows of those were not written), four at a time on their way
+    const uint64_t full = wave_ballot(r.x != -INFINITY && (ONE || (i & 7) == grp));
+    for (uint32_t left = static_cast<uint32_t>(tid & 32 ? full >> 32 : full); left;) {
+      f32x4 x[4];
+      int at[4];
+      bool is[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = fmaf(w, x[k], o[k]);
+      for (int k = 0; k < 4; ++k) {
+        is[k] = left != 0;
+        at[k] = is[k] ? __builtin_ctz(left) : at[0];
+        left &= left - 1;
+        x[k] = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(base + at[k]) * kD);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = __shfl(w, at[k], 32), fl = __shfl(wl, at[k], 32);
+        L += is[k] ? fl : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = is[k] ? fmaf(f, x[k][j], o[j]) : o[j];
+      }
+    }
   }
   if constexpr (!ONE) {
     *reinterpret_cast<f32x4*>(&s_o[grp][d]) = o;
