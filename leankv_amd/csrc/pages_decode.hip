@@ -444,19 +444,20 @@ __global__ __launch_bounds__(kThr) void join_kernel(JoinArgs A) {
   const int row = ONE ? blockIdx.x * 8 + grp : blockIdx.x;
   if (row >= A.rows) return;  // (whole groups; with ONE no barrier follows)
   const int t = row / A.heads, head = row - t * A.heads;
-  if (A.cu && (t < A.cu[0] || t >= A.cu[A.n])) return;
   const float2* ml = reinterpret_cast<const float2*>(A.part_ml) + static_cast<int64_t>(row) * A.splits;
-  if (ml[0].y < 0.f) return;  // the row is done (no sum of weights is negative)
+  const float2 first = (tid & 31) < A.splits ? ml[tid & 31] : part_record(-INFINITY, 0.f);
+  if (A.cu && (t < A.cu[0] || t >= A.cu[A.n])) return;
+  if (__shfl(first.y, 0, 32) < 0.f) return;  // the row is done (no sum of weights is negative)
   const float* po = A.part_o + static_cast<int64_t>(row) * A.splits * kD + d;
-  float M = -INFINITY;
-  for (int i = tid & 31; i < A.splits; i += 32) M = fmaxf(M, ml[i].x);
+  float M = first.x;
+  for (int i = (tid & 31) + 32; i < A.splits; i += 32) M = fmaxf(M, ml[i].x);
 #pragma unroll
   for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
   float L = 0.f;
   f32x4 o = f32x4{};
   for (int base = 0; base < A.splits; base += 32) {
     const int i = base + (tid & 31);
-    const float2 r = i < A.splits ? ml[i] : part_record(-INFINITY, 0.f);
+    const float2 r = base == 0 ? first : i < A.splits ? ml[i] : part_record(-INFINITY, 0.f);
     const float w = exp2_(r.x - M), wl = w * r.y;
     // the group's parts that are not empty (the rows of those were not written), four at a time on their way
     const uint64_t full = wave_ballot(r.x != -INFINITY && (ONE || (i & 7) == grp));
