@@ -20,8 +20,9 @@
 // 8 waves, a CU's whole LDS: a row is staged once for 256 columns, and 212 registers hold a wave's queries, its sums and both
 // operands on their way.  Bound by the products (54 % of the SIMDs' cycles over a prompt of 8192) and the vector work beside them
 // (52 %): 3480 cycles a tile for the two waves of a SIMD, 2048 of them products, and 12 thousand to begin and end a piece.
-// 32/8 heads: a prompt of 8192 tokens 496-530 us, 1037-1109 TFLOP/s (1.96 GHz under that load; the library's product of 8192^3
-// reaches 1241); 4 x 512 queries over 8192 tokens 264-272 us, up to 1017 TFLOP/s; 16 prompts to 1201 tokens 109-118 us.
+// 32/8 heads: a prompt of 8192 tokens 496-606 us by card, 907-1109 TFLOP/s (1.96 GHz under that load where it takes 530; the
+// library's product of 8192^3 reached 1241); 4 x 512 queries over 8192 tokens 260-312 us, up to 1030 TFLOP/s; 16 prompts to 1201
+// tokens 109-130 us.  Two workgroups a CU of 4 waves and 64-token tiles: 580 where it took 523.
 #include "pages_common.h"
 
 namespace lkv {
