@@ -872,13 +872,17 @@ Plan plan_for(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new,
   p.splits = static_cast<int>(splits < 1 ? 1 : splits > kMostCuts ? kMostCuts : splits);
   return p;
 }
-// Whole prompts.  Up to 256 tokens two workgroups of 4 waves a CU, where beginning and ending pieces is most of the work and one
-// fills the other's waits (64 prompts to 150 tokens, 32/8 heads: 30.2 us with 8 waves, 24.5 with 4; 64 x 64 24.9 and 22.2; 16 x
-// 512 63 and 65; 1 x 8192 525 and 605: every row of keys and values is staged twice as often).  From three pieces for four CUs
-// on none is cut (1 x 2048 tokens, a piece a CU: cutting the longer ones costs as much in rows to join as it gains).
+// Whole prompts.  Two workgroups of 4 waves a CU up to 256 tokens, where beginning and ending pieces is most of the work and one
+// fills the other's waits, and up to 2048 tokens where 8 waves would have no more than a piece for each CU (half as large, twice
+// as many are shared out more evenly).  With 8 waves, and with 4, 32/8 heads: 64 prompts to 150 tokens 30.2 and 24.5 us, 64 x 64
+// 24.9 and 22.2, 1 x 512 22.8 and 20.8, 900, 300 and 200 tokens 32.7 and 30.3, 1 x 2048 65.3 and 65; but 16 x 512 63 and 65, 1 x
+// 8192 525 and 605: every row of keys and values is staged twice as often.  From 0.75 pieces a workgroup on (4 waves: 0.6) none
+// is cut (1 x 2048 tokens, a piece a CU: cutting the longer ones costs as much in rows to join as it gains).
 Plan packed_plan(int64_t rows, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_len) {
   const int64_t most = max_len < rows ? max_len : rows;
-  return most <= 256 ? plan_for<4>(rows, B, Hq, Hkv, most, most, 0.75f) : plan_for<8>(rows, B, Hq, Hkv, most, most, 0.75f);
+  const Plan p = plan_for<8>(rows, B, Hq, Hkv, most, most, 0.75f);
+  const bool four = most <= 256 || (most <= 2048 && p.pieces * Hkv <= device_cu_count());
+  return four ? plan_for<4>(rows, B, Hq, Hkv, most, most, 0.6f) : p;
 }
 // Over pages, from two pieces a CU on none is cut (the launch that joins costs 5 us where none is).  Chunks to 512 over 1.6-8 K
 // tokens of 4 sequences, 0.8 pieces a CU: 268 us as they are, 230 in two parts taken by the length of their tiles, 168 in three
