@@ -789,10 +789,13 @@ typedef struct lkv_pages {
  * the lowest free ones, in the order of the sequences.  A last page that is not
  * full and that other sequences name too is replaced by a copy of its tokens in
  * a new page (before the sequence's other new pages), unless all of the
- * sequences that name it take new tokens and this is the first of them.  A
- * sequence gets its pages if they and those of all sequences before it fit:
- * otherwise, and where it would pass width * page_size tokens, it takes nothing.
- * taken[s] says what it took.
+ * sequences that name it are to take new tokens and this is the first of them,
+ * which goes on in the page itself.  A sequence gets its pages if they and those
+ * of all sequences before it fit: otherwise, and where it would pass
+ * width * page_size tokens, it takes nothing.  If one that takes nothing for want
+ * of pages holds more tokens of a shared last page than the first on that page
+ * does, that first one takes nothing either: no sequence's tokens are written
+ * over.  taken[s] says what it took.
  */
 size_t lkv_pages_extend_workspace_bytes(int64_t pages, int64_t seqs);
 int lkv_pages_extend(const lkv_pages* st, const int32_t* cu, void* workspace, size_t workspace_bytes, void* stream);

@@ -2,8 +2,8 @@
 //
 // All bookkeeping lives on the device, so that a step that grows or forks sequences is captured once and replayed.
 //   extend    one workgroup: what every sequence needs (new pages, and a copy of a shared last page that is not full),
-//             prefix sums over the sequences, the lowest free pages by a scan of refs, table and lens.  Then one launch
-//             that copies the shared tokens in every layer (nothing to do in most steps).
+//             prefix sums over the sequences, the lowest free pages by a scan of refs, who waits where those run out, table
+//             and lens.  Then one launch that copies the shared tokens in every layer (nothing to do in most steps).
 //   fork      a workgroup per sequence writes its new row to the workspace and counts refs by integer atomics (their order
 //             does not matter); a second launch puts the rows in place, since sequences take each other's rows.
 //   compact   one workgroup ranks free pages below and used pages from n on; a second launch moves pages and renames
@@ -63,7 +63,7 @@ __device__ __forceinline__ int new_tokens(const ExtendArgs& A, int s, int len) {
 
 __global__ __launch_bounds__(kPlanThr) void extend_kernel(ExtendArgs A) {
   __shared__ int s_last[kMaxSeqs];       // a shared last page that is not full, or -1
-  __shared__ int s_meta[kMaxSeqs];       // 2 * pages held + whether the last one is to be copied
+  __shared__ int s_meta[kMaxSeqs];       // 4 * pages held + 2 * whether it waits for another + whether the last one is to be copied
   __shared__ int s_begin[kMaxSeqs + 1];  // pages needed by the sequences before
   __shared__ int s_wave[kPlanThr / 64];
   __shared__ int s_copies;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(kPlanThr) void extend_kernel(ExtendArgs A) {
   const int tid = threadIdx.x, S = st.seqs, mask = page_size(st) - 1;
   if (tid == 0) s_copies = 0;
 
-  bool shared = false;
+  int shared = 0;
   for (int s = tid; s < S; s += kPlanThr) {
     const int len = held(st, st.lens[s]), n = new_tokens(A, s, len);
     const int old = (len + mask) >> st.lg;
@@ -81,11 +81,12 @@ __global__ __launch_bounds__(kPlanThr) void extend_kernel(ExtendArgs A) {
       if (st.refs[last] <= 1) last = -1;
     }
     s_last[s] = last;
-    s_meta[s] = 2 * old;
+    s_meta[s] = 4 * old;
     s_begin[s] = ((len + n + mask) >> st.lg) - old;
-    shared |= last >= 0;
+    shared |= last >= 0 ? 1 : 0;
   }
-  if (__syncthreads_or(shared)) {
+  shared = __syncthreads_or(shared);
+  if (shared) {
     for (int s = tid; s < S; s += kPlanThr) {
       const int last = s_last[s];
       if (last < 0) continue;
@@ -134,6 +135,21 @@ __global__ __launch_bounds__(kPlanThr) void extend_kernel(ExtendArgs A) {
   const int got = min(found, total);
   __threadfence_block();
   __syncthreads();
+  // Pages ran out.  A copy that is not there leaves its sequence on the shared page, so the first of the page, which would go on
+  // in it, waits too where that sequence holds more tokens of it than the first does.
+  if (got < total && shared) {
+    for (int s = tid; s < S; s += kPlanThr) {
+      const int last = s_last[s];
+      if (last < 0 || (s_meta[s] & 1)) continue;
+      const int len = held(st, st.lens[s]);
+      for (int t = s + 1; t < S; ++t)
+        if (s_last[t] == last && s_begin[t + 1] > got && held(st, st.lens[t]) > len) {
+          s_meta[s] += 2;
+          break;
+        }
+    }
+    __syncthreads();
+  }
   for (int r = tid; r < got; r += kPlanThr) {
     int lo = 0, hi = S;  // the sequence with s_begin[s] <= r < s_begin[s + 1]
     while (hi - lo > 1) {
@@ -143,8 +159,8 @@ __global__ __launch_bounds__(kPlanThr) void extend_kernel(ExtendArgs A) {
       else
         hi = mid;
     }
-    if (s_begin[lo + 1] > got) continue;  // its pages are not all there
-    const int j = r - s_begin[lo], old = s_meta[lo] >> 1, copy = s_meta[lo] & 1;
+    if (s_begin[lo + 1] > got || (s_meta[lo] & 2)) continue;  // its pages are not all there, or it waits
+    const int j = r - s_begin[lo], old = s_meta[lo] >> 2, copy = s_meta[lo] & 1;
     const int page = A.free_list[r];
     st.refs[page] = 1;
     st.table[static_cast<int64_t>(lo) * st.width + old + j - copy] = page;
@@ -160,7 +176,7 @@ __global__ __launch_bounds__(kPlanThr) void extend_kernel(ExtendArgs A) {
   if (tid == 0) A.copies[0] = s_copies;
   for (int s = tid; s < S; s += kPlanThr) {
     const int len = held(st, st.lens[s]);
-    const bool fits = s_begin[s + 1] == s_begin[s] || s_begin[s + 1] <= got;
+    const bool fits = (s_begin[s + 1] == s_begin[s] || s_begin[s + 1] <= got) && !(s_meta[s] & 2);
     const int n = fits ? new_tokens(A, s, len) : 0;
     st.lens[s] = len + n;
     st.taken[s] = n;

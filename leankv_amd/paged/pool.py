@@ -161,9 +161,10 @@ class PagedKV:
     def extend(self, cu: torch.Tensor | None = None) -> None:
         """Room for the rows of every sequence (without cu: one token for every sequence that holds some): lens grows, new
         pages are the lowest free ones in the order of the sequences.  A last page that is not full and that others name too
-        is replaced by a copy of its tokens, unless all that name it grow and this sequence is the first of them.  A
-        sequence that would pass max_len, and one whose pages with those of all sequences before it are more than are free,
-        takes nothing: taken says what each took.  Two launches."""
+        is replaced by a copy of its tokens, unless all that name it are to grow and this sequence is the first of them,
+        which goes on in it.  A sequence that would pass max_len, and one whose pages with those of all sequences before it
+        are more than are free, takes nothing, and neither does the first on a page of which another, refused for want of
+        pages, holds more tokens (what a sequence holds is never written over): taken says what each took.  Two launches."""
         p = self._cu(cu, "PagedKV.extend")
         call(self._index, self._lib.lkv_pages_extend, self._ref, p, self._scratch_ptr, self._extend_bytes)
 
