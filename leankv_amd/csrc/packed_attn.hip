@@ -11,7 +11,7 @@
 //   from the lane's own registers (the values' token order is the order in which a lane holds its scores).
 // A wave's 32 products a tile are in two stretches of 16 with vector work between them: scores of the next tile beside the
 // exponentials of this one, values of this one beside the next one's offsets and the staging.  The running offset moves
-// only when a weight passes 2^15, so that most tiles need no max over lanes and no rescale.
+// only when a weight passes 2^15 (bf16: 2^-20), so that most tiles need no max over lanes and no rescale.
 //
 // A masked token has weight 0, but 0 times an infinite or NaN value is not 0.  Where a row ends up with such a number its
 // workgroup goes through the piece again with care: values that are no numbers count as 0 in the masked tiles' products, and
@@ -439,7 +439,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
         mx = fmaxf(mx, s[e]);
       }
       mx = half_max(mx);
-      const float mn = mx - m > kMaxWeight ? mx - kTopWeight : m;
+      const float mn = mx - m > max_weight<DT>() ? mx - top_weight<DT>() : m;
       const float mu = mn == -INFINITY ? 0.f : mn;
       const float alpha = exp2_(m - mu);
       m = mn;
@@ -463,7 +463,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
 #pragma unroll
       for (int e = 0; e < 16 * kSub; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
       mx = half_max(mx);
-      m = mx == -INFINITY ? mx : mx - kTopWeight;
+      m = mx == -INFINITY ? mx : mx - top_weight<DT>();
       const float mu = mx == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int e = 0; e < 16 * kSub; ++e) s[e] = sc[e >> 4][e & 15] - mu;
@@ -601,7 +601,7 @@ __device__ __forceinline__ int go_through(const Args& P, uint16_t* smem, const i
           }
           l += ws[0] + ws[1];
           load_next(t);
-          if ((blk0 + t + 2) * kTile > lim_min || wave_ballot(mx > kMaxWeight) != 0) general(t + 1);  // uniform
+          if ((blk0 + t + 2) * kTile > lim_min || wave_ballot(mx > max_weight<DT>()) != 0) general(t + 1);  // uniform
           __syncthreads();
         }
       } else {  // no columns: the wave's part of the staging

@@ -109,9 +109,15 @@ __device__ __forceinline__ void add_counted(float count, float& sum) {
   if (minus > 0.f) sum -= INFINITY;
 }
 
-// log2 of the softmax weights as 16 bits hold them: a new offset puts the largest at 2^6, and there is none until a weight
-// passes 2^15, so that most tiles need no rescaled sums.  A weight keeps fp16's 11 bits down to 2^-20 of the largest.
-constexpr float kTopWeight = 6.f, kMaxWeight = 15.f;
+// log2 of the softmax weights as 16 bits hold them: a new offset puts the largest at 2^top, and there is none until a weight
+// passes 2^most, so that most tiles need no rescaled sums.  fp16 keeps a weight's 11 bits down to 2^-20 of the largest.  bf16
+// has fp32's exponents, and so do its values: with weights of at most 2^-20 the weighted values of a million tokens add up to
+// no more than the largest of them, so that finite ones give finite rows, and values down to 2^-97 are multiplied without
+// loss (with fp16's offsets values from 5e36 on gave infinities).
+template <int DT>
+__host__ __device__ __forceinline__ constexpr float top_weight() { return DT == LKV_DTYPE_F16 ? 6.f : -29.f; }
+template <int DT>
+__host__ __device__ __forceinline__ constexpr float max_weight() { return DT == LKV_DTYPE_F16 ? 15.f : -20.f; }
 
 // A partial sum's (offset, sum): offset -inf is an empty one, which is passed over.  A row of NaN scores has no offset
 // (max passes over NaN) but is not empty: it takes 0, so that its NaN reaches the joined row.

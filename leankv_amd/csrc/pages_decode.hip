@@ -167,9 +167,9 @@ __device__ __forceinline__ void attend(const DecodeArgs& P, Staged& sh, int h, i
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
-      if (wave_ballot(mx - m[n] > kMaxWeight || m[n] == -INFINITY)) {  // uniform: a new offset somewhere
+      if (wave_ballot(mx - m[n] > max_weight<DT>() || m[n] == -INFINITY)) {  // uniform: a new offset somewhere
         mx = groups_max(mx);
-        const float mn = mx - m[n] > kMaxWeight ? mx - kTopWeight : m[n];
+        const float mn = mx - m[n] > max_weight<DT>() ? mx - top_weight<DT>() : m[n];
         const float alpha = exp2_(m[n] - (mn == -INFINITY ? 0.f : mn));
         m[n] = mn;
         l[n] *= alpha;
