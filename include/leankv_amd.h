@@ -840,8 +840,9 @@ int lkv_pages_compact(const lkv_pages* st, int32_t* in_use, void* workspace, siz
  * it holds in one layer: out = softmax(scale * q K^T) V in the pool's type,
  * zeros for an empty sequence.  The work is split for max_len, a bound on lens
  * (longer sequences count as max_len).  Neighbouring sequences on the same pages
- * are read once for several of them.  out may be q.  Scores and sums are fp32; the weights are
- * rounded to the pool's type for the value product.
+ * are read once for several of them.  out may be q with q's strides, and does not
+ * overlap it otherwise.  Scores and sums are fp32; the weights are rounded to the
+ * pool's type for the value product.
  */
 size_t lkv_pages_decode_attn_workspace_bytes(int64_t seqs, int64_t Hq, int64_t kv_heads, int64_t max_len);
 int lkv_pages_decode_attn(const lkv_pages* st, int64_t layer, const void* q, const int64_t* q_strides, int64_t Hq,

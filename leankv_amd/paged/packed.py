@@ -62,9 +62,30 @@ def out_rows(out: torch.Tensor, like: torch.Tensor, what: str):
     return st
 
 
-def apart(q: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
-    """q, or a copy where out is written over it (its rows are read again where a value is no number)."""
-    return q.clone(memory_format=torch.contiguous_format) if out.data_ptr() == q.data_ptr() and q.numel() else q
+def _size(t: torch.Tensor, first: int) -> int:
+    """Bytes from the first to the last number of t's dims from `first` on."""
+    return 2 * (1 + sum(st * (n - 1) for st, n in zip(t.stride()[first:], t.shape[first:])))
+
+
+def meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a and b [rows, heads, 128] may have numbers in common: not if they lie behind each other, or are parts of the
+    rows of one buffer that do (q, k and v of a projection)."""
+    if not a.numel() or not b.numel():
+        return False
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa + _size(a, 0) <= pb or pb + _size(b, 0) <= pa:
+        return False
+    row = 2 * a.stride(0)
+    if row and a.stride(0) == b.stride(0):
+        off = (pb - pa) % row
+        return off < _size(a, 1) or off + _size(b, 1) > row
+    return True
+
+
+def apart(t: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """t, or a copy where out is written over it: the call reads t until it ends (queries too, whose rows are read again where a
+    value is no number)."""
+    return t.clone(memory_format=torch.contiguous_format) if meet(t, out) else t
 
 
 def follow(what: str, *tensors: torch.Tensor) -> bool:
@@ -118,8 +139,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     (heads a multiple of kv_heads; query head h reads kv head h * kv_heads // heads), float16 or bfloat16.  cu_seqlens: int32
     [n + 1] on the device, ascending; rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 are sequence i, up to 2048 of them.  Returns
     [tokens, heads, 128] in q's type; rows of no sequence are zeros, or, in a buffer given as `out` (dense 16-byte aligned
-    rows apart from each other; q itself may be it, and is copied then), left as they are.  max_len: the caller's bound on the
-    lengths (default: all tokens), which the work is split for.  scale: 1 / sqrt(128) by default.
+    rows apart from each other), left as they are.  Inputs that out is written over are copied first.  max_len: the caller's
+    bound on the lengths (default: all tokens), which the work is split for.  scale: 1 / sqrt(128) by default.
 
     Inputs may have any strides (rows that are not dense or not 16-byte aligned are copied).  A token that a query does not
     see has no part in its row, whatever it holds; a NaN in a query gives a row of NaN.  There is no gradient: a backward pass
@@ -156,7 +177,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if follows:
             raise LeanKVError("%s: out= does not support autograd, which follows q, k or v" % what)
         os = out_rows(out, q, what)
-        q = apart(q, out)
+        q, k, v = apart(q, out), apart(k, out), apart(v, out)
     (q, qs), (k, ks), (v, vs) = rows(q), rows(k, apart=True), rows(v, apart=True)
     batch = cu_seqlens.shape[0] - 1
     nbytes = _bytes(n, batch, heads, kv_heads, bound)

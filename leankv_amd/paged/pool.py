@@ -298,14 +298,18 @@ class PagedKV:
         among it): [max_seqs, heads, 128].  An empty sequence gives zeros.  max_len: the caller's bound on lens (default: the
         longest that the table holds), which the work is split for; a longer sequence counts as its first max_len tokens.
         Neighbouring sequences (as far as 16 query heads of a kv head go) that name the same pages read them once.  scale:
-        1 / sqrt(128) by default.  out: a buffer like q, rows dense, 16-byte aligned and apart (q itself may be it)."""
+        1 / sqrt(128) by default.  out: a buffer like q, rows dense, 16-byte aligned and apart (q itself may be it; where it
+        lies over q in another way, q is copied first)."""
         what = "PagedKV.decode_attention"
         self._layer(layer, what)
         heads = self._queries(q, what)
         if q.shape[0] != self.max_seqs:
             raise LeanKVError("%s: q must have a row for each of %d sequences, got %s" % (what, self.max_seqs, tuple(q.shape)))
         bound = self._bound(max_len, what)
+        given = out is not None
         out, os = self._output(q, out, what)
+        if given and (q.data_ptr() != out.data_ptr() or q.stride() != out.stride()):
+            q = apart(q, out)
         q, qs = rows(q)
         nbytes = _decode_bytes(self.max_seqs, heads, self.kv_heads, bound)
         ws = self._workspace(nbytes) if nbytes else None
@@ -318,8 +322,8 @@ class PagedKV:
                           out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention of the newest tokens' queries (after their store), q [rows, heads, 128]: rows cu[s] .. cu[s + 1] - 1
         are those of sequence s (further ones than it holds tokens are zeros), and query i of m sees tokens 0 .. lens[s] - m +
-        i.  Returns [rows, heads, 128]; rows of no sequence are zeros, or, in a buffer given as `out` (q itself may be it, and is
-        copied then), left as they are.
+        i.  Returns [rows, heads, 128]; rows of no sequence are zeros, or, in a buffer given as `out` (queries that it is written
+        over are copied first), left as they are.
         max_new, max_len: the caller's bounds on the rows of a sequence and on lens, which the work is split for.  (A sequence
         that extend refused, taken[s] = 0, has its rows computed as those of the tokens that it holds.)"""
         what = "PagedKV.prefill_attention"
