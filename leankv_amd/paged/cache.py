@@ -169,12 +169,15 @@ class PagedCache(HFCache):
         """Called before tokens that may be cut again (assisted generation); pages need no record of them."""
 
     def reorder_cache(self, beam_idx: torch.LongTensor):
-        """Sequence b goes on from sequence beam_idx[b] (beam search): pages are shared, not copied."""
+        """Sequence b goes on from sequence beam_idx[b] (beam search): pages are shared, not copied.  (Beams on the device are
+        waited for: one out of range would empty its sequence there, while its tokens are counted here.)"""
         self._idle("reorder_cache")
         if self.kv is None:
             return
         if beam_idx.numel() != self.kv.max_seqs:
             raise ValueError("PagedCache.reorder_cache: %d beams of %d sequences" % (beam_idx.numel(), self.kv.max_seqs))
+        if beam_idx.dtype not in (torch.int32, torch.int64) or bool(((beam_idx < 0) | (beam_idx >= self.kv.max_seqs)).any()):
+            raise ValueError("PagedCache.reorder_cache: beams are sequence numbers 0 .. %d" % (self.kv.max_seqs - 1))
         self.kv.fork(beam_idx.reshape(-1).to(device=self.kv.device, dtype=torch.int32).contiguous())
 
     def _chosen(self, index: torch.Tensor):
