@@ -67,15 +67,19 @@ class PagedCache(HFCache):
             cap = max(self._init_cap, tokens)
             self.kv = PagedKV(self.num_layers, H, B * -(-cap // self.page_size), B, cap, self.page_size, t.dtype, t.device)
         kv = self.kv
-        if (kv.max_seqs, kv.kv_heads, kv.dtype) != (B, H, t.dtype):
-            raise ValueError("PagedCache: holds %d sequences of %d heads in %s, got %d of %d in %s"
-                             % (kv.max_seqs, kv.kv_heads, kv.dtype, B, H, t.dtype))
+        self._alike(t)
         if tokens > kv.max_len:
             cap = kv.max_len
             while cap < tokens:
                 cap *= 2
             self.kv = kv = kv.resized(max(kv.num_pages, B * (cap // self.page_size)), cap)
         return kv
+
+    def _alike(self, t: torch.Tensor):
+        kv, (B, H) = self.kv, t.shape[:2]
+        if (kv.max_seqs, kv.kv_heads, kv.dtype, kv.device) != (B, H, t.dtype, t.device):
+            raise ValueError("PagedCache: holds %d sequences of %d heads in %s on %s, got %d of %d in %s on %s"
+                             % (kv.max_seqs, kv.kv_heads, kv.dtype, kv.device, B, H, t.dtype, t.device))
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, cache_kwargs=None):
         if self._fused_pending[layer_idx] or self._prefill_pending[layer_idx]:
@@ -86,6 +90,11 @@ class PagedCache(HFCache):
                 "fused_attention=False" % layer_idx)
         if key_states.dtype not in DTYPES:
             raise ValueError("PagedCache: float16 or bfloat16 keys and values expected, got %s" % key_states.dtype)
+        if key_states.dim() != 4 or key_states.shape[3] != HEAD_DIM or value_states.shape != key_states.shape \
+                or value_states.dtype != key_states.dtype or value_states.device != key_states.device:
+            raise ValueError("PagedCache: keys and values must be [B, heads, tokens, %d] of one type on one device, got %s %s on "
+                             "%s and %s %s on %s" % (HEAD_DIM, tuple(key_states.shape), key_states.dtype, key_states.device,
+                                                     tuple(value_states.shape), value_states.dtype, value_states.device))
         B, H, S, _ = key_states.shape
         p0 = self._seq_lengths[layer_idx]
         T = p0 + S
@@ -94,16 +103,24 @@ class PagedCache(HFCache):
             # (one more token a sequence: extend and store take the rows as they are)
             self._cu = None if S == 1 and p0 else torch.arange(B + 1, dtype=torch.int32, device=kv.device) * S
             kv.extend(self._cu)
-            self._seen_tokens += S
         elif self.kv is None or T != self._seq_lengths[0]:
             raise RuntimeError("PagedCache: layer %d would hold %d tokens, layer 0 holds %d (layers are updated in order)"
                                % (layer_idx, T, self._seq_lengths[0]))
+        else:
+            self._alike(key_states)
         set_active(self)
         kv = self.kv
-        k, v = _packed(key_states), _packed(value_states)
-        if S:
-            kv.store(layer_idx, k, v, self._cu)
+        try:
+            k, v = _packed(key_states), _packed(value_states)
+            if S:
+                kv.store(layer_idx, k, v, self._cu)
+        except Exception:
+            if layer_idx == 0:  # the room that was made for them
+                kv.truncate(torch.full((B,), p0, dtype=torch.int32, device=kv.device))
+            raise
         self._seq_lengths[layer_idx] = T
+        if layer_idx == 0:
+            self._seen_tokens += S
         if self.fused_attention and S:
             (self._fused_pending if S == 1 and p0 else self._prefill_pending)[layer_idx] = True
             self._pending_len[layer_idx] = T

@@ -32,3 +32,46 @@ def test_beams_out_of_range(cuda, where):
     assert torch.equal(cache[1][0], k)
     cache.reorder_cache(torch.tensor([1, 1], device=where))
     assert torch.equal(cache[0][1], v[[1, 1]])
+
+
+def test_refused_updates_leave_the_cache_as_it_was(cuda):
+    cache = _cache(cuda)
+    k, v = _kv(2)
+    for bad in (v.bfloat16(), v[:1], v[:, :1], v[:, :, :4], v[..., :64], v.cpu(), v[0]):
+        with pytest.raises(ValueError, match="of one type on one device"):
+            cache.update(k, bad, 0)
+    with pytest.raises(ValueError, match="of one type on one device"):
+        cache.update(k[..., :64], v[..., :64], 0)
+    assert cache.kv is None and cache.get_seq_length() == 0 and cache.seen_tokens == 0
+    for layer in range(2):
+        cache.update(k, v, layer)
+    for S in (1, 3):
+        k1, v1 = _kv(3 + S, S=S)
+        with pytest.raises(ValueError, match="of one type on one device"):
+            cache.update(k1, v1.bfloat16(), 0)
+        with pytest.raises(ValueError, match="holds 2 sequences"):
+            cache.update(k1.bfloat16(), v1.bfloat16(), 0)
+        n = cache.get_seq_length(0)
+        cache.update(k1, v1, 0)
+        for bad in ((k1[:1], v1[:1]), (k1[:, :1], v1[:, :1]), (k1.bfloat16(), v1.bfloat16())):
+            with pytest.raises(ValueError, match="holds 2 sequences"):
+                cache.update(*bad, 1)
+        cache.update(k1, v1, 1)
+        assert cache.kv.lens.tolist() == [n + S] * 2 and cache.seen_tokens == n + S
+        assert torch.equal(cache[0][0][:, :, n:], k1) and torch.equal(cache[1][1][:, :, n:], v1)
+        assert torch.equal(cache[1][0][:, :, :5], k)
+
+
+def test_a_tangent_takes_no_room(cuda):
+    from leankv_amd._lib import LeanKVError
+    from torch.autograd import forward_ad
+
+    cache = _cache(cuda, layers=1)
+    k, v = _kv(7)
+    cache.update(k, v, 0)
+    with forward_ad.dual_level():
+        with pytest.raises(LeanKVError, match="forward-mode"):
+            cache.update(forward_ad.make_dual(k, torch.ones_like(k)), v, 0)
+    assert cache.kv.lens.tolist() == [5, 5] and cache.get_seq_length() == 5 and cache.seen_tokens == 5
+    cache.update(k, v, 0)
+    assert torch.equal(cache[0][0], torch.cat([k, k], 2))
