@@ -36,6 +36,7 @@ constexpr int kChunk = 32;
 constexpr int kStep = kChunk * kWaves;  // tokens of a workgroup's step
 constexpr int kMaxPages = 1024;         // page ids of a split, staged in LDS
 constexpr int kMaxSplits = 1024;
+constexpr size_t kMostBytes = size_t{1} << 28;  // of records where the plan has the choice
 
 __device__ __forceinline__ float groups_max(float v) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -60,7 +61,7 @@ struct DecodeArgs {
   int Hq, G;
   int g_small;  // c / G = c * g_small >> 16 for columns c of a group
   int tiles;    // column tiles of a kv head: 1, or ceil(G / 16)
-  int group;    // sequences of a group: 32 / G, or 1 where none are shared
+  int group;    // sequences of a group: up to 32 / G, or 1 where none are shared
   int max_len, chunk, splits;  // tokens of a split
   int slots;    // records of a row: splits, or splits (group + 1): a split's own part, and the shared ones
   const int* cu;  // rows of several queries a sequence: where they begin
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(DecodeArgs P) {
   // ---- the split's pages; of the group's sequences where they end and how many pages they begin alike
   const int page0 = t0 >> st.lg, pages = ((t1 - 1) >> st.lg) - page0 + 1;
   const int* row = st.table + static_cast<int64_t>(s) * st.width + page0;
-  for (int i = tid; i < pages; i += kThr) sh.page[i] = page_id(st, row[i]);
+  for (int i = tid; i < min(pages, kMaxPages); i += kThr) sh.page[i] = page_id(st, row[i]);
   const int base = s - s % P.group, members = min(P.group, st.seqs - base);
   if (P.group > 1) {
     for (int j = wave; j < members; j += kWaves) {
@@ -362,13 +363,17 @@ __global__ __launch_bounds__(kThr, 2) void split_kernel(DecodeArgs P) {
     else
       attend<DT, 2, false>(P, sh, h, page0, lo, hi, hi, cols, slot + 1 + rank, where, all, page_at);
   }
-  if (shared < t1)
-    attend<DT, 1, false>(P, sh, h, page0, shared, t1, t1, own_heads, slot, [&](int c, int& seq, int& head) {
-      seq = s;
-      head = own_head + c;
-    }, all, page_at);
-  else
+  auto own = [&](int c, int& seq, int& head) {
+    seq = s;
+    head = own_head + c;
+  };
+  if (shared >= t1)
     empty(slot, 1);
+  else if (pages <= kMaxPages)
+    attend<DT, 1, false>(P, sh, h, page0, shared, t1, t1, own_heads, slot, own, all, page_at);
+  else  // (a plan without groups)
+    attend<DT, 1, false>(P, sh, h, page0, shared, t1, t1, own_heads, slot, own, all,
+                         [&](int i) { return page_id(st, row[i]); });
 }
 
 // The newest queries of every sequence, rows cu[s] .. of q: grid (splits, kv heads, sequences).
@@ -503,8 +508,13 @@ struct DecodePlan {
   int chunk, splits, group, slots;
 };
 
-DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len, bool rows = false) {
-  const int64_t G = Hq / Hkv, tiles = rows ? 1 : (G + 15) / 16, pairs = S * Hkv * tiles;
+size_t record_bytes(int64_t rows, int64_t slots) {
+  return slots == 1 ? 0 : static_cast<size_t>(rows) * slots * (kD + 2) * 4;
+}
+
+// rows: of queries (x query heads), S of them where every sequence has one.
+DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len, int64_t rows, bool few = false) {
+  const int64_t G = Hq / Hkv, tiles = few ? 1 : (G + 15) / 16, pairs = S * Hkv * tiles;
   const int64_t steps = (max_len + kStep - 1) / kStep;
   // Two workgroups a CU, the most that its registers hold at a time (32 x 8192 tokens, 32/8 heads: 186 us, with four 191,
   // 131072 tokens 100 and 108 us).  One split, which needs no join and shares nothing, where a workgroup a CU walks at most 8 steps
@@ -516,15 +526,27 @@ DecodePlan decode_plan(int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len, bool
     splits = splits > steps ? steps : splits;
     splits = splits > kMaxSplits ? kMaxSplits : splits;
   }
-  int64_t chunk = (steps + splits - 1) / splits;
   // page ids of a split fit their place whatever the page size: 16 tokens a page and the one that it begins in
   const int64_t most = (kMaxPages - 1) * 16 / kStep;
-  chunk = chunk > most ? most : (chunk < 1 ? 1 : chunk);
   DecodePlan p;
-  p.splits = static_cast<int>(steps <= chunk ? 1 : (steps + chunk - 1) / chunk);
-  p.chunk = static_cast<int>(chunk * kStep);
-  p.group = !rows && p.splits > 1 && S > 1 && G <= 16 ? static_cast<int>(32 / G) : 1;
-  p.slots = p.group > 1 ? p.splits * (p.group + 1) : p.splits;
+  auto cut = [&](int64_t chunk) {
+    p.splits = static_cast<int>(steps <= chunk ? 1 : (steps + chunk - 1) / chunk);
+    p.chunk = static_cast<int>(chunk * kStep);
+  };
+  const int64_t whole = (steps + splits - 1) / splits;
+  cut(whole > most ? most : (whole < 1 ? 1 : whole));
+  p.group = !few && p.splits > 1 && G <= 16 ? static_cast<int>(32 / G < S ? 32 / G : S) : 1;
+  // Records for every sequence that might share pages, in every split, are bounded: smaller groups, then longer splits, whose
+  // page ids past their place are read from the table (256 sequences of up to 131072 tokens, 32/8 heads: 345 MB with groups
+  // of 8, 192 with 4; 2048 sequences alone 307 MB in 9 splits, 239 in 7).
+  auto slots = [&]() { return static_cast<int64_t>(p.splits) * (p.group > 1 ? p.group + 1 : 1); };
+  while (p.group > 1 && record_bytes(rows * Hq, slots()) > kMostBytes) p.group /= 2;
+  if (p.group == 1 && record_bytes(rows * Hq, slots()) > kMostBytes) {
+    const int64_t fit = static_cast<int64_t>(kMostBytes / (record_bytes(rows * Hq, 2) / 2));
+    const int64_t fewer = fit > splits ? fit : splits;  // (no fewer than the workgroups need)
+    cut((steps + fewer - 1) / fewer);
+  }
+  p.slots = static_cast<int>(slots());
   return p;
 }
 
@@ -553,8 +575,7 @@ int launch_join(const float* part_o, const float* part_ml, int64_t rows, int64_t
 }
 
 size_t few_rows_bytes(int64_t rows, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_len) {
-  const DecodePlan p = decode_plan(S, Hq, Hkv, max_len, true);
-  return p.slots == 1 ? 0 : static_cast<size_t>(rows * Hq) * p.slots * (kD + 2) * 4;
+  return record_bytes(rows * Hq, decode_plan(S, Hq, Hkv, max_len, rows, true).slots);
 }
 
 int launch_few_rows(const lkv_pages* p, int64_t layer, const void* q, const int64_t* q_strides, int64_t rows, int64_t Hq,
@@ -563,7 +584,7 @@ int launch_few_rows(const lkv_pages* p, int64_t layer, const void* q, const int6
   const size_t need = few_rows_bytes(rows, p->seqs, Hq, p->kv_heads, max_len);
   LKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
               "%s: a 16-byte aligned workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
-  const DecodePlan plan = decode_plan(p->seqs, Hq, p->kv_heads, max_len, true);
+  const DecodePlan plan = decode_plan(p->seqs, Hq, p->kv_heads, max_len, rows, true);
   DecodeArgs A{};
   A.st = device_pages(p);
   A.kv = A.st.pool + layer * p->pages * 2 * p->kv_heads * p->page_size * kD;
@@ -603,8 +624,7 @@ using namespace lkv::pages;
 
 extern "C" size_t lkv_pages_decode_attn_workspace_bytes(int64_t seqs, int64_t Hq, int64_t Hkv, int64_t max_len) {
   if (seqs < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || max_len < 0) return 0;
-  const DecodePlan p = decode_plan(seqs, Hq, Hkv, max_len);
-  return p.slots == 1 ? 0 : static_cast<size_t>(seqs * Hq) * p.slots * (kD + 2) * 4;
+  return record_bytes(seqs * Hq, decode_plan(seqs, Hq, Hkv, max_len, seqs).slots);
 }
 
 extern "C" int lkv_pages_decode_attn(const lkv_pages* p, int64_t layer, const void* q, const int64_t* q_strides,
@@ -621,7 +641,7 @@ extern "C" int lkv_pages_decode_attn(const lkv_pages* p, int64_t layer, const vo
   if (int rc = check_rows(out, out_strides, what, "out")) return rc;
   const int64_t G = Hq / p->kv_heads, tiles = (G + 15) / 16;
   LKV_REQUIRE(p->kv_heads * tiles < 65536 && p->seqs * Hq < (1ll << 28), "%s: %lld query heads", what, (long long)Hq);
-  const DecodePlan plan = decode_plan(p->seqs, Hq, p->kv_heads, max_len);
+  const DecodePlan plan = decode_plan(p->seqs, Hq, p->kv_heads, max_len, p->seqs);
   const size_t need = lkv_pages_decode_attn_workspace_bytes(p->seqs, Hq, p->kv_heads, max_len);
   LKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
               "%s: a 16-byte aligned workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
