@@ -151,7 +151,9 @@ class PagedCache(HFCache):
         if not self._fused_pending[layer_idx]:
             raise RuntimeError("PagedCache.decode_attention: no one-token update pending for layer %d" % layer_idx)
         self._take(layer_idx)
-        return self.kv.decode_attention(layer_idx, query.squeeze(2), scale=self._scale(scaling)).unsqueeze(2)
+        # (a bound in whole steps of the work, so that most calls find the workspace's size where it was last looked up)
+        bound = min(-(-self._pending_len[layer_idx] // 128) * 128, self.kv.max_len)
+        return self.kv.decode_attention(layer_idx, query.squeeze(2), max_len=bound, scale=self._scale(scaling)).unsqueeze(2)
 
     def prefill_attention(self, layer_idx: int, query: torch.Tensor, scaling: float | None = None) -> torch.Tensor:
         """Causal attention of the newest S tokens' queries [B, Hq, S, D] over this layer's cache -> [B, Hq, S, D]."""

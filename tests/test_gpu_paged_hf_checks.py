@@ -75,3 +75,33 @@ def test_a_tangent_takes_no_room(cuda):
     assert cache.kv.lens.tolist() == [5, 5] and cache.get_seq_length() == 5 and cache.seen_tokens == 5
     cache.update(k, v, 0)
     assert torch.equal(cache[0][0], torch.cat([k, k], 2))
+
+
+def test_decode_is_divided_by_what_is_held(cuda, monkeypatch):
+    """A cache with room for long sequences: the bound that decode is given holds the tokens and little more."""
+    from leankv_amd.paged import PagedCache, PagedKV
+
+    cache = PagedCache(num_layers=1, device=cuda, max_seq_len=30000, fused_attention=True)
+    k, v = _kv(8, S=254)
+    q = torch.randn(2, 4, 254, 128, generator=torch.Generator().manual_seed(9)).half().cuda()
+    cache.update(k, v, 0)
+    cache.prefill_attention(0, q)
+    bounds, plain = [], PagedKV.decode_attention
+
+    def decode(self, layer, q, max_len=None, **kw):
+        bounds.append(max_len)
+        return plain(self, layer, q, max_len=max_len, **kw)
+
+    monkeypatch.setattr(PagedKV, "decode_attention", decode)
+    for _ in range(4):
+        cache.update(k[:, :, :1], v[:, :, :1], 0)
+        got = cache.decode_attention(0, q[:, :, :1])
+        want = plain(cache.kv, 0, q[:, :, 0].contiguous(), max_len=cache.get_seq_length()).unsqueeze(2)
+        assert torch.equal(got, want)
+    assert bounds == [256, 256, 384, 384]
+    short = PagedCache(num_layers=1, device=cuda, max_seq_len=20, page_size=16, fused_attention=True)
+    short.update(k[:, :, :20], v[:, :, :20], 0)
+    short.prefill_attention(0, q[:, :, :20])
+    short.update(k[:, :, :1], v[:, :, :1], 0)
+    short.decode_attention(0, q[:, :, :1])
+    assert bounds[-1] == 32
