@@ -771,7 +771,8 @@ int lkv_kv8_sparse_attn(const lkv_kv8_store* store, const void* q, const int64_t
  * number of entries that name page p (0: free).  Sequences that were forked
  * name the same pages.  All buffers are device memory of the caller, the pool
  * 16-byte aligned, table -1 and the others 0 before the first use (what lies in
- * free pages does not matter).
+ * free pages does not matter).  width * page_size is below 2^30 and
+ * seqs * (width + 1) below 2^31.
  */
 typedef struct lkv_pages {
   void* pool;     /* [layers][pages][2 (K, V)][kv_heads][page_size][128]     */

@@ -434,6 +434,9 @@ int check_pages(const lkv_pages* p, const char* what) {
   LKV_REQUIRE(p->seqs >= 1 && p->seqs <= kMaxSeqs, "%s: seqs=%lld must be 1 .. %d", what, (long long)p->seqs, kMaxSeqs);
   LKV_REQUIRE(p->width >= 1 && p->width * p->page_size < (1ll << 30), "%s: width=%lld out of range", what,
               (long long)p->width);
+  // (extend counts the pages that all sequences ask for in 32 bits: a row of the table and a copy each at most, whatever cu holds)
+  LKV_REQUIRE(p->seqs * (p->width + 1) < (1ll << 31), "%s: a table of %lld x %lld pages (2^31 are the most)", what,
+              (long long)p->seqs, (long long)p->width);
   LKV_REQUIRE(p->pool && p->table && p->lens && p->refs && p->taken, "%s: null pointer", what);
   LKV_REQUIRE(aligned16(p->pool) && aligned4(p->table) && aligned4(p->lens) && aligned4(p->refs) && aligned4(p->taken),
               "%s: the pool must be 16-byte aligned, table, lens, refs and taken 4-byte", what);

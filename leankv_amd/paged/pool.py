@@ -68,6 +68,8 @@ class PagedKV:
             raise ValueError("PagedKV: max_seqs=%d must be 1 to %d" % (max_seqs, MAX_SEQS))
         if page_size not in PAGE_SIZES:
             raise ValueError("PagedKV: page_size=%s must be one of %s" % (page_size, PAGE_SIZES))
+        if max_seqs * (-(-max_len // page_size) + 1) >= 1 << 31:
+            raise ValueError("PagedKV: a table of %d sequences of up to %d tokens is too large" % (max_seqs, max_len))
         if dtype not in DTYPES:
             raise ValueError("PagedKV: dtype=%s must be float16 or bfloat16" % dtype)
         self.device = torch.device(device)
