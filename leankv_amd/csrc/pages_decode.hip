@@ -397,12 +397,12 @@ __global__ __launch_bounds__(kThr, 2) void rows_kernel(DecodeArgs P) {
   const int t0 = split * P.chunk, t1 = split == P.splits - 1 ? len : min(t0 + P.chunk, len);
   // queries that there are no tokens for, or none in this split
   const int from = t0 < t1 ? qlen : 0;
-  for (int e = tid; e < (m - from) * G * (kD / 8); e += kThr) {
-    const int x = e / (kD / 8), i = from + x / G;
-    const int64_t row = row0 + i, head = h * G + x % G;
+  for (int x = from * G + (tid >> 4); x < m * G; x += kThr / 16) {  // 16 lanes a row
+    const int i = x / G;
+    const int64_t row = row0 + i, head = h * G + x - i * G;
     if (P.slots == 1)
-      *reinterpret_cast<u32x4*>(P.out + row * P.o_ss + head * P.o_sh + 8 * (e % (kD / 8))) = u32x4{};
-    else if (e % (kD / 8) == 0)
+      *reinterpret_cast<u32x4*>(P.out + row * P.o_ss + head * P.o_sh + 8 * (tid & 15)) = u32x4{};
+    else if ((tid & 15) == 0)
       *reinterpret_cast<float2*>(P.part_ml + 2 * ((row * P.Hq + head) * P.slots + split)) = part_record(-INFINITY, 0.f);
   }
   if (t0 >= t1 || !qlen) return;  // uniform
