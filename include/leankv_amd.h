@@ -854,7 +854,8 @@ int lkv_pages_decode_attn(const lkv_pages* st, int64_t layer, const void* q, con
  * Causal attention of packed sequences: rows cu[b] .. cu[b + 1] - 1 of
  * q [rows][Hq][128] and k, v [rows][Hkv][128] (float16 or bfloat16, strides of
  * row and head) are sequence b; query i of it sees its tokens 0 .. i.  cu int32
- * [B + 1] on the device, ascending.  max_len is a bound on the lengths (the work
+ * [B + 1] on the device, ascending (with entries that fall rows hold anything).
+ * max_len is a bound on the lengths (the work
  * is split for it; longer ones are right too).  Rows that belong to no sequence
  * are zeros with fill = 1 and left as they are with fill = 0.  out does not
  * overlap q, k or v.

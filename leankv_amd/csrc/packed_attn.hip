@@ -748,9 +748,21 @@ __global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
   if (tid == 0) s_any = 0;
   __syncthreads();
   int pieces = 0;  // column tiles of all sequences
+  int low = 0, high = 0;  // their rows
   for (int b = lane; b < P.B; b += 64) {
     longest = max(longest, s_len[b]);
     pieces += tiles_over<W>(-1, s_len[b], s_rows[b], G);
+    low += s_rows[b] & 0xffff;
+    high += s_rows[b] >> 16;
+  }
+  // Starts that fall: sequences would lie over each other, and their pieces pass what the launch counted with.  None is taken.
+  low = wave_total(low);
+  high = wave_total(high) + (low >> 16);
+  if (high > P.rows >> 16 || (high == P.rows >> 16 && (low & 0xffff) > (P.rows & 0xffff))) {  // uniform
+    __syncthreads();
+    for (int b = tid; b < P.B; b += kThr) s_rows[b] = 0;
+    __syncthreads();
+    pieces = 0;
   }
 #pragma unroll
   for (int x = 32; x; x >>= 1) longest = max(longest, __shfl_xor(longest, x));
