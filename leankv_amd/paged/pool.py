@@ -223,8 +223,8 @@ class PagedKV:
             parent = torch.arange(self.max_seqs, dtype=torch.int32, device=self.device).masked_fill_(which, -1)
         else:
             which = [which] if isinstance(which, int) else list(which)
-            if not all(isinstance(s, int) and 0 <= s < self.max_seqs for s in which):
-                raise LeanKVError("PagedKV.free: sequences %s outside 0 .. %d" % (which, self.max_seqs - 1))
+            if not all(isinstance(s, int) and not isinstance(s, bool) and 0 <= s < self.max_seqs for s in which):
+                raise LeanKVError("PagedKV.free: sequence numbers 0 .. %d expected, got %s" % (self.max_seqs - 1, which))
             done = set(which)
             parent = torch.tensor([-1 if s in done else s for s in range(self.max_seqs)], dtype=torch.int32,
                                   device=self.device)

@@ -75,3 +75,19 @@ def test_walks_in_full_pools(cuda, pages, seqs, width, page, dtype):
                 both.compare((seed, call))
         except StopIteration:
             pass
+
+
+def test_free_takes_numbers(cuda):
+    """A list of truth values is no list of sequences: [True, False] would be sequences 1 and 0."""
+    from leankv_amd._lib import LeanKVError
+    from leankv_amd.paged import PagedKV
+
+    cache = PagedKV(1, 1, 8, 3, 64, page_size=16)
+    cache.extend(_ints([0, 5, 10, 15]))
+    for bad in ([True, False, True], True, [3], [-1], [0.0]):
+        with pytest.raises(LeanKVError, match="sequence numbers"):
+            cache.free(bad)
+    assert cache.lens.tolist() == [5, 5, 5]
+    cache.free([1, 1])
+    cache.free(2)
+    assert cache.lens.tolist() == [5, 0, 0]
