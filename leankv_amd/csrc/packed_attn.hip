@@ -17,8 +17,8 @@
 // workgroup goes through the piece again with care: values that are no numbers count as 0 in the masked tiles' products, and
 // a second product counts, of each kind, those that a column sees.
 //
-// 8 waves, a CU's whole LDS: a row is staged once for 256 columns, and 212 registers hold a wave's queries, its sums and both
-// operands on their way.  Bound by the products (54 % of the SIMDs' cycles over a prompt of 8192) and the vector work beside them
+// 8 waves, a CU's whole LDS: a row is staged once for 256 columns, and 239 registers (256 over pages) hold a wave's queries, its
+// sums and both operands on their way.  Bound by the products (54 % of the SIMDs' cycles over a prompt of 8192) and the vector work beside them
 // (52 %): 3480 cycles a tile for the two waves of a SIMD, 2048 of them products, and 12 thousand to begin and end a piece.
 // 32/8 heads: a prompt of 8192 tokens 496-606 us by card, 907-1109 TFLOP/s (1.96 GHz under that load where it takes 530; the
 // library's product of 8192^3 reached 1241); 4 x 512 queries over 8192 tokens 260-312 us, up to 1030 TFLOP/s; 16 prompts to 1201
@@ -771,8 +771,10 @@ __global__ __launch_bounds__(Shape<W>::kThr, 2) void prefill_kernel(Args P) {
 
   // ---- into how many parts the longest pieces are cut.  What that takes, in tiles: the longest part, or the workgroups' mean
   // and some of a part (in two rounds what the last of the first and the first of the second take, if that is more), about 4
-  // a round for beginning and ending pieces, and writing and joining the parts' rows.  The waves look at every eighth number
-  // each.
+  // a round for beginning and ending pieces, and writing and joining the parts' rows (a launch is 2.5 tiles' time, 7.6e6 bytes a
+  // tile's time are what the card writes and reads again).  All of it was measured with 32/8 heads, where a tile takes 1.8
+  // us; the shares of a part, 0.15 and 0.3, and the 5 % by which a cut has to gain are not derived but set by times of chunks over
+  // 0.4 to 17 K tokens there.  They choose between divisions that are all right.  The waves look at every eighth number each.
   int cuts = 1, chunk = 1 << 24, less = 0;
   if (P.splits > 1) {
     float work = 0.f;

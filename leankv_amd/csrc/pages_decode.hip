@@ -19,11 +19,11 @@
 // those that do not see the last tokens have weight 0 there.  Where such a token's value is no number, 0 times it is none
 // either: it counts as 0 then, and a second product counts, of each kind, those that a column sees.
 //
-// Bound by memory: a wave's next chunk (16 KB) is on its way while it computes this one, 8 waves a CU (230 registers), so that
-// 128 KB a CU are.  32/8 heads: 32 sequences of 8192 tokens 186 us, 5.8 TB/s; 32 of 1.6-8 K 135 us, 4.8 TB/s (the longest end
-// last); 131072 tokens of one sequence 98 us, of them 95 (5.7 TB/s) reading and 5 joining 64 splits; 32 beams over 4 prompts of
-// 8192 tokens, 152 MB read once, 34 us.  5 drafted tokens of 8 sequences of 4096 29 us, of them 26 (5.1 TB/s) reading; in the
-// prefill kernel, whose waves wait for each other's rows, 37.
+// Bound by memory: a wave's next chunk (16 KB) is on its way while it computes this one, 8 waves a CU (229 registers; 250 with
+// masks), so that 128 KB a CU are.  32/8 heads, by card: 32 sequences of 8192 tokens 186 us, 5.8 TB/s; 32 of 1.6-8 K 135-136 us, 4.8
+// TB/s (the longest end last); 131072 tokens of one sequence 98-99 us, of them 95 (5.7 TB/s) reading and 5 joining 64 splits; 32
+// beams over 4 prompts of 8192 tokens, 152 MB read once, 34-40 us.  5 drafted tokens of 8 sequences of 4096 29-34 us, of them 26
+// (5.1 TB/s) reading; in the prefill kernel, whose waves wait for each other's rows, 37 where it takes 29.
 #include "pages_common.h"
 
 namespace lkv {
