@@ -286,8 +286,10 @@ class PagedKV:
         return self._books.clone()
 
     def rollback(self, snapshot: torch.Tensor) -> None:
-        """The tables as a snapshot of this pool has them.  What the pages hold is not taken back: only tokens that were added
-        since are gone, as long as no page of the snapshot was released and given to another sequence."""
+        """The tables as a snapshot of this pool has them.  What the pages hold is not taken back: tokens that were added since
+        are gone, and those of the snapshot are there as long as, since then, none of its pages was released and taken again or
+        moved by compact, no sequence was cut (truncate, fork with lens) and grew over what was cut off, and sequences that
+        grew on one last page were as long as each other (extend lets the first of them go on in it)."""
         if not isinstance(snapshot, torch.Tensor) or snapshot.shape != self._books.shape \
                 or snapshot.dtype is not torch.int32 or snapshot.device != self.device:
             raise LeanKVError("PagedKV.rollback: a snapshot of this pool expected")
